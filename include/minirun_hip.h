@@ -48,7 +48,8 @@ typedef enum mr_dtype {
     MR_F16 = 1,
     MR_F32 = 2,
     MR_U32 = 3,
-    MR_I32 = 4
+    MR_I32 = 4,
+    MR_U8 = 5
 } mr_dtype;
 
 /* Library version string, e.g. "minirun-hip 0.1.0 gfx950". */
@@ -291,6 +292,93 @@ mr_status mr_tile_upload(void *device_dst, const void *pinned_src, int64_t bytes
 mr_status mr_affine_gather_matmul(const void *x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride,
                                   const mr_affine_weight *w, int64_t experts, const int32_t *rhs_indices,
                                   int32_t experts_per_token, void *y, mr_dtype y_dtype, void *stream);
+
+/* ------------------------------------------------------------------------
+ * MXFP4 matrices (Sources/MLXBridge/MXFP4Weights.swift:36-60): rows of
+ * blocks of 32 values along the columns.  packed: uint32 [rows, cols / 8],
+ * element j of a word in bits 4j .. 4j + 3, each an e2m1 number (sign bit,
+ * then 0, .5, 1, 1.5, 2, 3, 4, 6); scales: one E8M0 byte per block, uint8
+ * [rows, cols / 32]; value = e2m1 * 2^(byte - 127), NaN for the 32 values of a
+ * block whose byte is 255.  No padding between rows; a stack of experts is
+ * laid out back to back.
+ * ------------------------------------------------------------------------ */
+typedef struct mr_mxfp4_matrix {
+    const uint32_t *packed; /* 16-byte aligned */
+    const uint8_t *scales;  /* 4-byte aligned */
+    int64_t rows, cols;     /* cols a multiple of 32 */
+} mr_mxfp4_matrix;
+
+/* The operands' types and shapes, as mr_affine_validate checks affine ones:
+ * packed uint32 and scales uint8 of rank 2, or 3 for a stack of experts, with
+ * 8 values a word and 32 a scale; a matrix may have no rows.  On success fills
+ * the geometry (experts = 0 for a single matrix). */
+mr_status mr_mxfp4_validate(mr_dtype packed_dtype, int32_t packed_rank, const int64_t *packed_shape,
+                            mr_dtype scales_dtype, int32_t scales_rank, const int64_t *scales_shape, int64_t *experts,
+                            int64_t *rows, int64_t *cols);
+
+/* x [rows, cols] (bf16 or f32, row stride x_stride) to packed and scales.
+ * Per block with largest magnitude A: byte = max(0, floor(log2 A) - 2 + 127)
+ * (0 for zeros); each value becomes the e2m1 number nearest to
+ * x / 2^(byte - 127), the even code of two equally near, at most 6 in
+ * magnitude, with the sign of x.  A block with a NaN or an infinity becomes
+ * NaN whole (byte 255, codes 0). */
+mr_status mr_mxfp4_quantize(const void *x, mr_dtype x_dtype, int64_t rows, int64_t cols, int64_t x_stride,
+                            uint32_t *packed, uint8_t *scales, void *stream);
+
+/* The values of a matrix (or of a stack: rows = experts * rows) as f32 or
+ * bf16, out [rows, cols] with row stride out_stride; exact, but infinite where
+ * a value passes the type's largest (byte 253 and 254). */
+mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_dtype, int64_t out_stride,
+                              void *stream);
+
+/* ------------------------------------------------------------------------
+ * The way of tokens to routed experts and back, around products of rows in
+ * expert order.  No counterpart of its own in the reference, whose experts
+ * run token by token (QwenExpertBackends.swift:77-260).
+ *
+ * A pair is (token t, slot j), index t * per_token + j; ids [tokens][per_token]
+ * holds its expert.  Pairs with an id in [0, experts) get a row each: rows are
+ * ordered by expert, inside an expert by pair index.  Other ids (an expert held
+ * elsewhere, a padded token) have no row.
+ *   offsets [experts + 1]: expert e's rows are offsets[e] .. offsets[e + 1] - 1
+ *   pair_of_row [tokens * per_token]: the row's pair; -1 past the last row
+ *   row_of_pair [tokens * per_token]: the pair's row; -1 for none
+ * experts is at most 4096, tokens * per_token at most 2^24.  Workspace:
+ * mr_expert_sort_workspace_size (0 up to 4096 pairs).  The result does not
+ * depend on timing.
+ * ------------------------------------------------------------------------ */
+size_t mr_expert_sort_workspace_size(int32_t tokens, int32_t per_token, int32_t experts);
+mr_status mr_expert_sort(const int32_t *ids, int32_t tokens, int32_t per_token, int32_t experts, int32_t *offsets,
+                         int32_t *pair_of_row, int32_t *row_of_pair, void *workspace, size_t workspace_bytes,
+                         void *stream);
+
+/* rows[row_of_pair[t][j]] = x[t], bit for bit, for every pair that has a row:
+ * x [tokens, dim], rows [tokens * per_token, dim], both of `dtype` (bf16 or
+ * f32).  Rows past the last are left as they were.  An entry of row_of_pair
+ * outside [0, tokens * per_token) counts as -1, here and below. */
+mr_status mr_expert_dispatch(const void *x, mr_dtype dtype, int32_t tokens, int64_t dim, int64_t x_stride,
+                             const int32_t *row_of_pair, int32_t per_token, void *rows, int64_t rows_stride,
+                             void *stream);
+
+/* out[t] = sum over the slots j that have a row, in their order, of
+ * weights[t][j] * rows[row_of_pair[t][j]]: f32 sums, rounded once to `dtype`
+ * (that of rows and out); weights f32 [tokens][per_token], or NULL for ones.  A
+ * token without a row gets zeros.  With weights NULL this is the gradient of
+ * mr_expert_dispatch: rows the gradient of its output, out that of x. */
+mr_status mr_expert_combine(const void *rows, mr_dtype dtype, int64_t rows_stride, int64_t dim,
+                            const int32_t *row_of_pair, const float *weights, int32_t tokens, int32_t per_token,
+                            void *out, int64_t out_stride, void *stream);
+
+/* Gradients of mr_expert_combine for d_out [tokens, dim], the gradient of its
+ * output: d_rows[row_of_pair[t][j]] = weights[t][j] * d_out[t] (rows past the
+ * last are left as they were) and, in f32, d_weights[t][j] = the dot product of
+ * d_out[t] and rows[row_of_pair[t][j]] (0 for a pair without a row).  Either may
+ * be NULL; rows is read for d_weights only.  d_rows must not overlap rows or
+ * d_out. */
+mr_status mr_expert_combine_backward(const void *d_out, mr_dtype dtype, int64_t d_out_stride, int64_t dim,
+                                     const void *rows, int64_t rows_stride, const int32_t *row_of_pair,
+                                     const float *weights, int32_t tokens, int32_t per_token, void *d_rows,
+                                     int64_t d_rows_stride, float *d_weights, void *stream);
 
 /* ------------------------------------------------------------------------
  * Dense projections: k3Linear (Sources/ModelAdapters/Operators/Linear.swift:

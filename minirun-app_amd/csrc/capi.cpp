@@ -42,6 +42,7 @@ const char* dtype_name(mr_dtype d) {
         case MR_F32: return "float32";
         case MR_U32: return "uint32";
         case MR_I32: return "int32";
+        case MR_U8: return "uint8";
     }
     return "unknown";
 }

@@ -71,6 +71,18 @@ __device__ __forceinline__ uint32_t pack_bf16x2_hw(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
+// The eight e2m1 numbers of an MXFP4 word times a power of two, as bf16
+// (exact: e2m1 has two significant bits).  The instruction takes the power
+// from `scale`'s exponent field alone: byte << 23 is 2^(byte - 127) for every
+// E8M0 byte, 0 (2^-127) and 255 (NaN) included.
+__device__ __forceinline__ bf16x8 mxfp4_bf16(uint32_t word, float scale) {
+    const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3))};
+    return __builtin_bit_cast(bf16x8, v);
+}
+
 // sigmoid(g) = 1 / (1 + 2^(-g log2 e)) on the hardware exp2 and reciprocal
 // (each within 1 ulp); 0 and 1 at the extremes.
 __device__ __forceinline__ float sigmoid_f32(float g) {

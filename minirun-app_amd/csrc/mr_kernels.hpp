@@ -504,4 +504,60 @@ hipError_t launch_rope(const RopeParams& p, hipStream_t st);
 hipError_t launch_cache_append(const CacheAppendParams& p, hipStream_t st);
 hipError_t launch_absorb_q(const AbsorbParams& p, hipStream_t st);
 
+// ---------------------------------------------------------------- MXFP4
+struct Mxfp4QuantizeParams {
+    const void* x;  // bf16, or f32 when x_f32
+    int x_f32;
+    int64_t rows, cols, x_stride;
+    uint32_t* packed;  // [rows][cols / 8]
+    uint8_t* scales;   // [rows][cols / 32]
+};
+
+struct Mxfp4DequantizeParams {
+    const uint32_t* packed;
+    const uint8_t* scales;
+    int64_t rows, cols;
+    void* out;  // bf16, or f32 when out_f32
+    int out_f32;
+    int64_t out_stride;
+};
+
+hipError_t launch_mxfp4_quantize(Mxfp4QuantizeParams p, hipStream_t st);
+hipError_t launch_mxfp4_dequantize(Mxfp4DequantizeParams p, hipStream_t st);
+
+// ---------------------------------------------------------------- routed experts
+constexpr int EXPERT_MAX = 4096;          // experts of a sort
+constexpr int EXPERT_SORT_PAIRS = 4096;   // pairs per workgroup of the sort
+
+struct ExpertSortParams {
+    const int32_t* ids;
+    int32_t pairs, experts;
+    int32_t* offsets;      // [experts + 1]
+    int32_t* pair_of_row;  // [pairs]
+    int32_t* row_of_pair;  // [pairs]
+    int32_t* counts;       // workspace [blocks][experts], more than one block only
+};
+
+// rows of `dim` values, bf16 or f32; row r of `src` / `dst` at stride ld_*
+struct ExpertRowsParams {
+    const void* tokens;  // dispatch: x; backward: d_out
+    int64_t ld_tokens;
+    const void* rows;    // combine, backward: the experts' results
+    int64_t ld_rows;
+    void* out;           // dispatch: rows; combine: tokens; backward: d_rows (or null)
+    int64_t ld_out;
+    int f32;
+    int64_t dim;
+    int32_t n_tokens, per_token;
+    const int32_t* row_of_pair;
+    const float* weights;  // null: ones
+    float* d_weights;      // backward (or null)
+};
+
+inline int expert_sort_blocks(int64_t pairs) { return (int)((pairs + EXPERT_SORT_PAIRS - 1) / EXPERT_SORT_PAIRS); }
+hipError_t launch_expert_sort(const ExpertSortParams& p, hipStream_t st);
+hipError_t launch_expert_dispatch(const ExpertRowsParams& p, hipStream_t st);
+hipError_t launch_expert_combine(const ExpertRowsParams& p, hipStream_t st);
+hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, hipStream_t st);
+
 }  // namespace mr

@@ -1,0 +1,205 @@
+// MXFP4 quantisation and its inverse: blocks of 32 values along a row, one
+// power of two (E8M0) and 32 e2m1 numbers each, the storage of
+// MXFP4Weights.swift:36-60 (element j of a word in bits 4j .. 4j + 3).
+//
+// Per block, with A the largest magnitude:
+//   byte = max(0, floor(log2 A) - 2 + 127), so that A / 2^(byte - 127) is in
+//          [4, 8), or below 4 where the byte is clamped (A < 2^-125)
+//   code = the e2m1 number (0, .5, 1, 1.5, 2, 3, 4, 6) nearest to
+//          |x| / 2^(byte - 127), the even code of two equally near ones, 6
+//          above it; the sign is x's
+// floor(log2 A) is A's exponent field, so nothing is computed in floating
+// point before v_cvt_scalef32_pk_fp4, which divides by the power of two and
+// rounds (subnormal values and byte 0 included; pinned against the rule on
+// hardware).  A block with a NaN or an infinity gets byte 255 and codes 0: all
+// of its values are NaN.
+//
+// What bounds it: HBM (2 or 4 bytes read, 17 / 32 of a byte written per
+// value).  A lane owns 8 values (16 or 32 bytes of loads, one word stored), so
+// every load and store of a wave covers whole lines; the four lanes of a block
+// find A by two DPP steps.  Each lane has the loads of MX_U such pieces in
+// flight before it uses the first.
+#include <algorithm>
+
+#include "mr_kernels.hpp"
+
+namespace mr {
+
+namespace {
+
+constexpr int MX_U = 4;      // pieces of 512 values per wave
+constexpr int MX_WAVES = 4;  // waves per workgroup
+
+// eight values of a row as f32 bit patterns (bf16: in the high halves)
+struct MxEight {
+    uint32_t v[8];
+};
+
+template <bool F32, bool VEC>
+__device__ __forceinline__ MxEight mx_load8(const void* p, int64_t i) {
+    MxEight r;
+    if constexpr (F32) {
+        if constexpr (VEC) {
+            const u32x4 a = ((const u32x4*)((const uint32_t*)p + i))[0], b = ((const u32x4*)((const uint32_t*)p + i))[1];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r.v[k] = a[k], r.v[4 + k] = b[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r.v[k] = ((const uint32_t*)p)[i + k];
+        }
+    } else {
+        if constexpr (VEC) {
+            const u32x4 a = *(const u32x4*)((const uint16_t*)p + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r.v[2 * k] = a[k] << 16, r.v[2 * k + 1] = a[k] & 0xffff0000u;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r.v[k] = (uint32_t)((const uint16_t*)p)[i + k] << 16;
+        }
+    }
+    return r;
+}
+
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
+}
+
+// Wave `unit` of the grid takes values 512 MX_U (unit % per_row) .. of row
+// unit / per_row.  cols is a multiple of 32, so the four lanes of a block are
+// all inside the row or all past it.
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_quantize_kernel(Mxfp4QuantizeParams p, int64_t per_row) {
+    const int64_t unit = (int64_t)blockIdx.x * MX_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = p.rows == 1 ? 0 : unit / per_row;
+    if (row >= p.rows) return;
+    const int l = threadIdx.x & 63;
+    const int64_t c0 = (unit - row * per_row) * (512 * MX_U) + 8 * l;
+    const char* x = (const char*)p.x + row * p.x_stride * (F32 ? 4 : 2);
+    MxEight v[MX_U];
+#pragma unroll
+    for (int u = 0; u < MX_U; ++u)
+        if (c0 + 512 * u < p.cols) v[u] = mx_load8<F32, VEC>(x, c0 + 512 * u);
+#pragma unroll
+    for (int u = 0; u < MX_U; ++u) {
+        const int64_t c = c0 + 512 * u;
+        if (c >= p.cols) return;
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, v[u].v[k] & 0x7fffffffu);
+        top = quad_max(top);
+        const bool finite = top < 0x7f800000u;
+        const uint32_t e = top >> 23, byte = finite ? (e > 2 ? e - 2 : 0) : 255u;
+        const float scale = __uint_as_float(finite ? byte << 23 : 0x3f800000u);
+        auto f = [&](int k) { return __uint_as_float(v[u].v[k]); };
+        uint32_t w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(0), f(1), scale, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(2), f(3), scale, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(4), f(5), scale, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(6), f(7), scale, 3);
+        const int64_t o = row * p.cols + c;
+        p.packed[o >> 3] = finite ? w : 0u;
+        if ((l & 3) == 0) p.scales[o >> 5] = (uint8_t)byte;
+    }
+}
+
+// value = (+-) e2m1 * 2^(byte - 127), exact in f32 and bf16 (subnormal there
+// below byte 1 or 2, infinite where it passes the type's largest); NaN at byte
+// 255.  A lane owns a word: 8 values.
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_dequantize_kernel(Mxfp4DequantizeParams p, int64_t per_row) {
+    const int64_t unit = (int64_t)blockIdx.x * MX_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = p.rows == 1 ? 0 : unit / per_row;
+    if (row >= p.rows) return;
+    const int l = threadIdx.x & 63;
+    const int64_t c0 = (unit - row * per_row) * (512 * MX_U) + 8 * l;
+    uint32_t w[MX_U];
+    uint32_t b[MX_U];
+#pragma unroll
+    for (int u = 0; u < MX_U; ++u)
+        if (c0 + 512 * u < p.cols) {
+            const int64_t o = row * p.cols + c0 + 512 * u;
+            w[u] = p.packed[o >> 3];
+            b[u] = p.scales[o >> 5];
+        }
+#pragma unroll
+    for (int u = 0; u < MX_U; ++u) {
+        const int64_t c = c0 + 512 * u;
+        if (c >= p.cols) return;
+        const float scale = __uint_as_float(b[u] << 23);
+        const int64_t o = row * p.out_stride + c;
+        if constexpr (F32) {
+            const f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 0),
+                                __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 1),
+                                __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 2),
+                                __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 3)};
+            float* out = (float*)p.out + o;
+            if constexpr (VEC) {
+                ((f32x4*)out)[0] = f32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+                ((f32x4*)out)[1] = f32x4{v[2][0], v[2][1], v[3][0], v[3][1]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) out[k] = v[k >> 1][k & 1];
+            }
+        } else {
+            const u32x4 v = __builtin_bit_cast(u32x4, mxfp4_bf16(w[u], scale));
+            uint16_t* out = (uint16_t*)p.out + o;
+            if constexpr (VEC) {
+                *(u32x4*)out = v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) out[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+            }
+        }
+    }
+}
+
+// rows laid out without gaps are one long row
+template <typename P>
+int64_t mx_units(P& p, int64_t& stride, int64_t& per_row) {
+    if (stride == p.cols) {
+        p.cols *= p.rows;
+        stride = p.cols;
+        p.rows = 1;
+    }
+    per_row = (p.cols + 512 * MX_U - 1) / (512 * MX_U);
+    return per_row * p.rows;
+}
+
+template <typename K, typename P>
+hipError_t mx_launch(K kern, const P& p, int64_t units, int64_t per_row, hipStream_t st) {
+    const int64_t grid = (units + MX_WAVES - 1) / MX_WAVES;
+    if (grid >= (1ll << 32) / (64 * MX_WAVES)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * MX_WAVES), 0, st, p, per_row);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_mxfp4_quantize(Mxfp4QuantizeParams p, hipStream_t st) {
+    const int size = p.x_f32 ? 4 : 2;
+    const bool vec = ((uintptr_t)p.x & 15) == 0 && (p.rows == 1 || p.x_stride * size % 16 == 0);
+    if (p.rows == 1) p.x_stride = p.cols;
+    int64_t per_row;
+    const int64_t units = mx_units(p, p.x_stride, per_row);
+    if (p.x_f32)
+        return vec ? mx_launch(mxfp4_quantize_kernel<true, true>, p, units, per_row, st)
+                   : mx_launch(mxfp4_quantize_kernel<true, false>, p, units, per_row, st);
+    return vec ? mx_launch(mxfp4_quantize_kernel<false, true>, p, units, per_row, st)
+               : mx_launch(mxfp4_quantize_kernel<false, false>, p, units, per_row, st);
+}
+
+hipError_t launch_mxfp4_dequantize(Mxfp4DequantizeParams p, hipStream_t st) {
+    const int size = p.out_f32 ? 4 : 2;
+    const bool vec = ((uintptr_t)p.out & 15) == 0 && (p.rows == 1 || p.out_stride * size % 16 == 0);
+    if (p.rows == 1) p.out_stride = p.cols;
+    int64_t per_row;
+    const int64_t units = mx_units(p, p.out_stride, per_row);
+    if (p.out_f32)
+        return vec ? mx_launch(mxfp4_dequantize_kernel<true, true>, p, units, per_row, st)
+                   : mx_launch(mxfp4_dequantize_kernel<true, false>, p, units, per_row, st);
+    return vec ? mx_launch(mxfp4_dequantize_kernel<false, true>, p, units, per_row, st)
+               : mx_launch(mxfp4_dequantize_kernel<false, false>, p, units, per_row, st);
+}
+
+}  // namespace mr

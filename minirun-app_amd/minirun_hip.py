@@ -11,6 +11,7 @@ Names follow the reference operators they stand in for:
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 import os
@@ -22,7 +23,7 @@ SELFTEST_PATH = os.path.join(LIB_DIR, "libminirun_selftest.so")
 
 OK, INVALID_SHAPE, INVALID_DTYPE, INDEX_OUT_OF_RANGE, DUPLICATE_INDEX, NONFINITE, HIP_ERROR, \
     INVALID_ARGUMENT, WORKSPACE_TOO_SMALL = range(9)
-BF16, F16, F32, U32, I32 = range(5)
+BF16, F16, F32, U32, I32, U8 = range(6)
 
 DECODE_VALIDATE_INDICES = 1
 DECODE_SPLIT_ONLY = 4
@@ -139,6 +140,10 @@ class TopkArgs(C.Structure):
     ]
 
 
+class MXFP4Desc(C.Structure):
+    _fields_ = [("packed", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64)]
+
+
 TOPK_CHECK = 1
 TOPK_UNCHECKED = 2
 
@@ -197,6 +202,16 @@ SIGNATURES = {
     "mr_indexer_scores": (C.c_int, [_P, C.c_int, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int,
                                     C.c_int32, C.c_int32, C.c_int64, _P, C.c_int, C.c_int32, C.c_int32, C.c_int64,
                                     _P, C.c_int64, _P]),
+    "mr_mxfp4_validate": (C.c_int, [C.c_int, C.c_int32, _I64P, C.c_int, C.c_int32, _I64P, _I64P, _I64P, _I64P]),
+    "mr_mxfp4_quantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int64, _P, _P, _P]),
+    "mr_mxfp4_dequantize": (C.c_int, [C.POINTER(MXFP4Desc), _P, C.c_int, C.c_int64, _P]),
+    "mr_expert_sort_workspace_size": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
+    "mr_expert_sort": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, C.c_size_t, _P]),
+    "mr_expert_dispatch": (C.c_int, [_P, C.c_int, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, _P, C.c_int64, _P]),
+    "mr_expert_combine": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, _P, C.c_int32, C.c_int32, _P, C.c_int64,
+                                    _P]),
+    "mr_expert_combine_backward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, C.c_int64, _P, _P, C.c_int32,
+                                             C.c_int32, _P, C.c_int64, _P, _P]),
     "mr_attention_indices_window": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _P, _I32P, _I32P]),
     "mr_attention_indices_compressed": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _I32P, _I32P]),
 }
@@ -582,6 +597,229 @@ def affine_gather_mm(x, w: AffineWeights, rhs_indices, out_dtype=None, stream=No
                                           C.byref(w.desc()), experts, _ptr(rhs_indices), K, _ptr(y),
                                           _dtype_code(y.dtype), _stream(stream)))
     return y
+
+
+# ------------------------------------------------------------------ MXFP4 and routed experts
+def _call_stream(t, stream):
+    """The stream handle of a call on tensor t's device, and a context in which
+    what the call allocates belongs to that stream (None: the current one on
+    that device)."""
+    torch = _torch()
+    if stream is None:
+        if t.device.index == torch.cuda.current_device():
+            ctx = contextlib.nullcontext()
+        else:
+            ctx = torch.cuda.device(t.device)
+        return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream), ctx
+    if isinstance(stream, torch.cuda.Stream):
+        return C.c_void_p(stream.cuda_stream), torch.cuda.stream(stream)
+    handle = stream.value if isinstance(stream, C.c_void_p) else stream
+    s = torch.cuda.ExternalStream(handle, t.device) if handle else torch.cuda.default_stream(t.device)
+    return C.c_void_p(handle), torch.cuda.stream(s)
+
+
+def _same_device(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {first.device}")
+
+
+def _need_whole(t, name, dtype=None):
+    """A GPU tensor without gaps (axes of one entry may have any stride)."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA (HIP) tensor")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _rows2d(t, name, shape=None):
+    """Row stride of a 2-D tensor with contiguous rows."""
+    if not (isinstance(t, _torch().Tensor) and t.dim() and t.shape[-1] == 1 and t.is_cuda):
+        _need(t, name)
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name} must be {'2-D' if shape is None else list(shape)}, got {list(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+class MXFP4Weights:
+    """MXFP4Weights (MXFP4Weights.swift:36-60) over device tensors: packed
+    uint32 (torch.int32 or uint32 storage) [experts?, rows, cols / 8], scales
+    uint8 (E8M0) [experts?, rows, cols / 32].  Also the form in which
+    activations come out of mxfp4_quantize.  Construction validates through
+    mr_mxfp4_validate."""
+
+    def __init__(self, packed, scales):
+        torch = _torch()
+        pdt = U32 if packed.dtype in (torch.int32, torch.uint32) else 99
+        sdt = U8 if scales.dtype == torch.uint8 else 99
+        ps = (C.c_int64 * packed.dim())(*packed.shape)
+        ss = (C.c_int64 * scales.dim())(*scales.shape)
+        ex, rows, cols = C.c_int64(), C.c_int64(), C.c_int64()
+        _check(load().mr_mxfp4_validate(pdt, packed.dim(), ps, sdt, scales.dim(), ss, C.byref(ex), C.byref(rows),
+                                        C.byref(cols)))
+        _need_whole(packed, "packed")
+        _need_whole(scales, "scales")
+        _same_device(packed, scales=scales)
+        self.packed, self.scales = packed, scales
+        self.experts = ex.value or None
+        self.rows, self.cols = rows.value, cols.value
+        self.out_features, self.in_features = self.rows, self.cols
+
+    def desc(self):
+        """One matrix (one expert of a stack)."""
+        return MXFP4Desc(self.packed.data_ptr(), self.scales.data_ptr(), self.rows, self.cols)
+
+
+def mxfp4_quantize(x, stream=None):
+    """x [rows, cols] (or a vector, one row; or a stack [experts, rows, cols])
+    bf16 or f32 -> MXFP4Weights: per 32 values the power of two that puts the
+    largest magnitude into [4, 8) and the nearest e2m1 numbers (ties to even,
+    at most 6); a block with a NaN or an infinity is NaN whole."""
+    torch = _torch()
+    _need(x, "x")
+    if x.dim() not in (1, 2, 3):
+        raise ValueError(f"x must be [rows, cols], a row or a stack of matrices, got {list(x.shape)}")
+    lead, cols = (1,) if x.dim() == 1 else x.shape[:-1], x.shape[-1]
+    handle, ctx = _call_stream(x, stream)
+    with ctx:
+        x2 = x if x.dim() == 2 else x.reshape(-1, cols)
+        packed = torch.empty(*lead, cols // 8, dtype=torch.int32, device=x.device)
+        scales = torch.empty(*lead, cols // 32, dtype=torch.uint8, device=x.device)
+        _check(load().mr_mxfp4_quantize(_ptr(x2), _dtype_code(x2.dtype), x2.shape[0], cols, _rows2d(x2, "x"),
+                                        _ptr(packed), _ptr(scales), handle))
+    return MXFP4Weights(packed, scales)
+
+
+def mxfp4_dequantize(w: MXFP4Weights, dtype=None, stream=None):
+    """The values that w stands for, f32 by default or bf16, in w's shape."""
+    torch = _torch()
+    handle, ctx = _call_stream(w.packed, stream)
+    with ctx:
+        out = torch.empty(*w.scales.shape[:-1], w.cols, dtype=dtype or torch.float32, device=w.packed.device)
+        d = w.desc()
+        d.rows = w.rows * (w.experts or 1)
+        _check(load().mr_mxfp4_dequantize(C.byref(d), _ptr(out), _dtype_code(out.dtype), w.cols, handle))
+    return out
+
+
+class ExpertOrder:
+    """Pairs (token, slot) in expert order, as expert_sort leaves them: offsets
+    int32 [experts + 1], pair_of_row int32 [tokens * per_token], row_of_pair
+    int32 [tokens, per_token] (-1: no row)."""
+
+    def __init__(self, offsets, pair_of_row, row_of_pair, experts):
+        torch = _torch()
+        for t, n in ((offsets, "offsets"), (pair_of_row, "pair_of_row"), (row_of_pair, "row_of_pair")):
+            _need_whole(t, n, torch.int32)
+        _same_device(offsets, pair_of_row=pair_of_row, row_of_pair=row_of_pair)
+        if row_of_pair.dim() != 2 or offsets.numel() != experts + 1 or pair_of_row.numel() != row_of_pair.numel():
+            raise ValueError("an order is offsets [experts + 1], pair_of_row [tokens * per_token] and row_of_pair "
+                             "[tokens, per_token]")
+        self.offsets, self.pair_of_row, self.row_of_pair, self.experts = offsets, pair_of_row, row_of_pair, experts
+        self.tokens, self.per_token = row_of_pair.shape
+
+
+def expert_sort(ids, experts, stream=None):
+    """ids int32 [tokens, per_token] -> ExpertOrder: the pairs with an id in
+    [0, experts) by expert, inside an expert by pair index; other ids have no
+    row."""
+    torch = _torch()
+    _need_whole(ids, "ids", torch.int32)
+    if ids.dim() != 2:
+        raise ValueError(f"ids must be [tokens, per_token], got {list(ids.shape)}")
+    T, K = ids.shape
+    handle, ctx = _call_stream(ids, stream)
+    with ctx:
+        n = load().mr_expert_sort_workspace_size(T, K, experts)
+        buf = torch.empty(max(experts, 0) + 1 + 2 * T * K, dtype=torch.int32, device=ids.device)
+        offsets, pair, row = buf.split([max(experts, 0) + 1, T * K, T * K])
+        ws = torch.empty(n, dtype=torch.uint8, device=ids.device) if n else None
+        _check(load().mr_expert_sort(_ptr(ids), T, K, experts, _ptr(offsets), _ptr(pair), _ptr(row), _ptr(ws), n,
+                                     handle))
+    return ExpertOrder(offsets, pair, row.view(T, K), experts)
+
+
+def expert_dispatch(x, order: ExpertOrder, out=None, stream=None):
+    """x [tokens, dim] bf16 or f32 -> rows [tokens * per_token, dim] in expert
+    order, bit for bit.  Rows past the last of the order are not written (give
+    `out` to keep what they hold)."""
+    torch = _torch()
+    ld = _rows2d(x, "x")
+    _same_device(x, order=order.offsets, out=out)
+    if x.shape[0] != order.tokens:
+        raise ValueError(f"x has {x.shape[0]} tokens, the order {order.tokens}")
+    shape = (order.tokens * order.per_token, x.shape[1])
+    handle, ctx = _call_stream(x, stream)
+    with ctx:
+        rows = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
+        if rows.dtype != x.dtype:
+            raise TypeError(f"out must be {x.dtype}, got {rows.dtype}")
+        _check(load().mr_expert_dispatch(_ptr(x), _dtype_code(x.dtype), order.tokens, x.shape[1], ld,
+                                         _ptr(order.row_of_pair), order.per_token, _ptr(rows),
+                                         _rows2d(rows, "out", shape), handle))
+    return rows
+
+
+def _expert_weights(weights, order):
+    torch = _torch()
+    if weights is None:
+        return
+    _need_whole(weights, "weights", torch.float32)
+    if tuple(weights.shape) != (order.tokens, order.per_token):
+        raise ValueError(f"weights must be [{order.tokens}, {order.per_token}], got {list(weights.shape)}")
+
+
+def expert_combine(rows, order: ExpertOrder, weights=None, stream=None):
+    """rows [tokens * per_token, dim] in expert order -> [tokens, dim]: per
+    token the sum of its rows times weights f32 [tokens, per_token] (None:
+    ones), in f32, rounded once."""
+    torch = _torch()
+    ld = _rows2d(rows, "rows")
+    _expert_weights(weights, order)
+    _same_device(rows, order=order.offsets, weights=weights)
+    if rows.shape[0] != order.tokens * order.per_token:
+        raise ValueError(f"rows has {rows.shape[0]} rows, the order {order.tokens * order.per_token}")
+    handle, ctx = _call_stream(rows, stream)
+    with ctx:
+        out = torch.empty(order.tokens, rows.shape[1], dtype=rows.dtype, device=rows.device)
+        _check(load().mr_expert_combine(_ptr(rows), _dtype_code(rows.dtype), ld, rows.shape[1],
+                                        _ptr(order.row_of_pair), _ptr(weights), order.tokens, order.per_token,
+                                        _ptr(out), rows.shape[1], handle))
+    return out
+
+
+def expert_combine_backward(d_out, rows, order: ExpertOrder, weights=None, out=None, stream=None):
+    """Gradients of expert_combine for d_out [tokens, dim]: (d_rows, in expert
+    order; d_weights f32 [tokens, per_token], 0 where a pair has no row).  Rows
+    of d_rows past the last of the order are not written (give `out` to keep
+    what they hold); rows and d_out have one dtype."""
+    torch = _torch()
+    ld_g, ld = _rows2d(d_out, "d_out"), _rows2d(rows, "rows")
+    _expert_weights(weights, order)
+    _same_device(d_out, rows=rows, order=order.offsets, weights=weights, out=out)
+    shape = (order.tokens * order.per_token, d_out.shape[1])
+    if d_out.shape[0] != order.tokens or tuple(rows.shape) != shape or rows.dtype != d_out.dtype:
+        raise ValueError(f"d_out must be [{order.tokens}, dim] and rows {list(shape)} of its dtype, got "
+                         f"{list(d_out.shape)} and {list(rows.shape)} {rows.dtype}")
+    handle, ctx = _call_stream(d_out, stream)
+    with ctx:
+        d_rows = torch.empty(shape, dtype=rows.dtype, device=rows.device) if out is None else out
+        if d_rows.dtype != rows.dtype:
+            raise TypeError(f"out must be {rows.dtype}, got {d_rows.dtype}")
+        d_weights = torch.empty(order.tokens, order.per_token, dtype=torch.float32, device=rows.device)
+        _check(load().mr_expert_combine_backward(_ptr(d_out), _dtype_code(d_out.dtype), ld_g, d_out.shape[1],
+                                                 _ptr(rows), ld, _ptr(order.row_of_pair), _ptr(weights),
+                                                 order.tokens, order.per_token, _ptr(d_rows),
+                                                 _rows2d(d_rows, "out", shape), _ptr(d_weights), handle))
+    return d_rows, d_weights
+
+
+def expert_dispatch_backward(d_rows, order: ExpertOrder, stream=None):
+    """Gradient of expert_dispatch: per token the sum of its rows' gradients."""
+    return expert_combine(d_rows, order, None, stream)
 
 
 def rms_norm(x, weight, eps=1e-6, out_dtype=None, stream=None):

@@ -29,7 +29,7 @@ public struct HIPTensor {
     }
 
     public var raw: UnsafeRawPointer { UnsafeRawPointer(pointer) }
-    public func bytes(_ n: Int) -> Int { n * (dtype == MR_F32 || dtype == MR_U32 || dtype == MR_I32 ? 4 : 2) }
+    public func bytes(_ n: Int) -> Int { n * (dtype == MR_U8 ? 1 : dtype == MR_F32 || dtype == MR_U32 || dtype == MR_I32 ? 4 : 2) }
 }
 
 /// A non-OK mr_status with the library's message for it (the reference's

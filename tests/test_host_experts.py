@@ -1,0 +1,136 @@
+"""Argument checks of the MXFP4 and routed-expert entry points on the host:
+every refusal comes before a GPU call, with its status and a message."""
+import ctypes as C
+
+import pytest
+
+import minirun_hip as M
+
+AT = 1 << 32  # an address that no refused call reads
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return M.load()
+
+
+def refused(status, want, *words):
+    assert status == want, (status, M.last_error())
+    assert all(w in M.last_error() for w in words), M.last_error()
+
+
+def shape(*dims):
+    return (C.c_int64 * len(dims))(*dims)
+
+
+def validate(lib, packed, scales, pdt=M.U32, sdt=M.U8):
+    ex, rows, cols = C.c_int64(-1), C.c_int64(-1), C.c_int64(-1)
+    st = lib.mr_mxfp4_validate(pdt, len(packed), shape(*packed), sdt, len(scales), shape(*scales), C.byref(ex),
+                               C.byref(rows), C.byref(cols))
+    return st, (ex.value, rows.value, cols.value)
+
+
+def test_validate(lib):
+    assert validate(lib, (7, 8), (7, 2)) == (M.OK, (0, 7, 64))
+    assert validate(lib, (3, 7, 8), (3, 7, 2)) == (M.OK, (3, 7, 64))
+    assert validate(lib, (0, 4), (0, 1)) == (M.OK, (0, 0, 32))
+    refused(validate(lib, (7, 8), (7, 2), pdt=M.F32)[0], M.INVALID_DTYPE, "uint32")
+    refused(validate(lib, (7, 8), (7, 2), sdt=M.BF16)[0], M.INVALID_DTYPE, "uint8")
+    refused(validate(lib, (8,), (2,))[0], M.INVALID_SHAPE, "rank")
+    refused(validate(lib, (3, 7, 8), (7, 2))[0], M.INVALID_SHAPE, "rank")
+    refused(validate(lib, (7, 8), (6, 2))[0], M.INVALID_SHAPE, "disagree")
+    refused(validate(lib, (3, 7, 8), (2, 7, 2))[0], M.INVALID_SHAPE, "disagree")
+    refused(validate(lib, (7, 8), (7, 1))[0], M.INVALID_SHAPE, "blocks of 32")
+    refused(validate(lib, (7, 6), (7, 1))[0], M.INVALID_SHAPE, "blocks of 32")
+    refused(validate(lib, (0, 7, 8), (0, 7, 2))[0], M.INVALID_SHAPE)
+    refused(validate(lib, (7, 0), (7, 0))[0], M.INVALID_SHAPE)
+    refused(lib.mr_mxfp4_validate(M.U32, 2, None, M.U8, 2, None, None, None, None), M.INVALID_ARGUMENT)
+
+
+def test_quantize_refusals(lib):
+    q = lambda x=AT, dt=M.BF16, rows=4, cols=64, ld=64, p=AT, s=AT: lib.mr_mxfp4_quantize(x, dt, rows, cols, ld, p, s, None)
+    for cols in (0, -32, 33, 48):
+        refused(q(cols=cols, ld=64), M.INVALID_SHAPE, "32")
+    refused(q(rows=-1), M.INVALID_SHAPE)
+    refused(q(rows=2 ** 40), M.INVALID_SHAPE, "2^37")
+    for dt in (M.F16, M.U32, M.U8, 99, -1):
+        refused(q(dt=dt), M.INVALID_DTYPE, "bf16 or f32")
+    for kw in ({"x": None}, {"p": None}, {"s": None}):
+        refused(q(**kw), M.INVALID_ARGUMENT, "non-NULL")
+    refused(q(ld=63), M.INVALID_ARGUMENT, "stride")
+    refused(q(x=AT + 1), M.INVALID_ARGUMENT, "misaligned")
+    refused(q(x=AT + 2, dt=M.F32), M.INVALID_ARGUMENT, "misaligned")
+    refused(q(p=AT + 2), M.INVALID_ARGUMENT, "misaligned")
+    assert q(rows=0, x=None) == M.OK
+
+
+def test_dequantize_refusals(lib):
+    def d(packed=AT, scales=AT, rows=4, cols=64, out=AT, dt=M.BF16, ld=64):
+        return lib.mr_mxfp4_dequantize(C.byref(M.MXFP4Desc(packed, scales, rows, cols)), out, dt, ld, None)
+
+    refused(lib.mr_mxfp4_dequantize(None, AT, M.BF16, 64, None), M.INVALID_ARGUMENT)
+    refused(d(cols=40), M.INVALID_SHAPE)
+    refused(d(rows=-2), M.INVALID_SHAPE)
+    refused(d(dt=M.F16), M.INVALID_DTYPE)
+    for kw in ({"packed": None}, {"scales": None}, {"out": None}, {"ld": 32}, {"packed": AT + 2}, {"out": AT + 1}):
+        refused(d(**kw), M.INVALID_ARGUMENT)
+    assert d(rows=0, out=None) == M.OK
+
+
+def test_sort_sizes_and_refusals(lib):
+    size = lib.mr_expert_sort_workspace_size
+    assert size(512, 8, 128) == 0  # one workgroup
+    assert size(513, 8, 128) == 2 * 128 * 4
+    assert size(1 << 21, 8, 4096) == 4096 * 4096 * 4
+    assert size(0, 8, 16) == 0
+    for bad in ((-1, 1, 1), (1, 0, 1), (1, -3, 1), (1, 1, 0), (1, 1, 4097), ((1 << 21) + 1, 8, 4), (2 ** 31 - 1, 2 ** 31 - 1, 4)):
+        assert size(*bad) == 0
+        refused(lib.mr_expert_sort(AT, *bad, AT, AT, AT, AT, 1 << 40, None), M.INVALID_SHAPE)
+    sort = lambda ids=AT, o=AT, p=AT, r=AT, ws=AT, n=1 << 30, t=600: lib.mr_expert_sort(ids, t, 8, 16, o, p, r, ws, n, None)
+    for kw in ({"ids": None}, {"o": None}, {"p": None}, {"r": None}):
+        refused(sort(**kw), M.INVALID_ARGUMENT, "non-NULL")
+    for kw in ({"ids": AT + 1}, {"o": AT + 2}, {"p": AT + 3}, {"r": AT + 2}, {"ws": AT + 2}):
+        refused(sort(**kw), M.INVALID_ARGUMENT, "misaligned")
+    refused(sort(n=127), M.WORKSPACE_TOO_SMALL, "required")
+    refused(sort(ws=None), M.WORKSPACE_TOO_SMALL)
+
+
+def test_row_refusals(lib):
+    dispatch = lambda x=AT, dt=M.BF16, t=4, dim=64, ld=64, m=AT, k=2, out=AT, lo=64: lib.mr_expert_dispatch(
+        x, dt, t, dim, ld, m, k, out, lo, None)
+    combine = lambda x=AT, dt=M.BF16, t=4, dim=64, ld=64, m=AT, k=2, out=AT, lo=64, w=None: lib.mr_expert_combine(
+        x, dt, ld, dim, m, w, t, k, out, lo, None)
+    backward = lambda x=AT, dt=M.BF16, t=4, dim=64, ld=64, m=AT, k=2, out=AT, lo=64, w=None, y=AT, dw=AT: \
+        lib.mr_expert_combine_backward(x, dt, ld, dim, y, 64, m, w, t, k, out, lo, dw, None)
+    for call in (dispatch, combine, backward):
+        refused(call(t=-1), M.INVALID_SHAPE)
+        refused(call(k=0), M.INVALID_SHAPE)
+        refused(call(t=2 ** 23, k=3), M.INVALID_SHAPE, "2^24")
+        refused(call(dim=0, ld=0, lo=0), M.INVALID_SHAPE)
+        refused(call(dim=2 ** 24 + 1, ld=2 ** 25, lo=2 ** 25), M.INVALID_SHAPE)
+        refused(call(t=2 ** 23, k=1, dim=2 ** 20, ld=2 ** 20, lo=2 ** 20), M.INVALID_SHAPE, "one launch")
+        for dt in (M.F16, M.I32, 99):
+            refused(call(dt=dt), M.INVALID_DTYPE)
+        for kw in ({"x": None}, {"m": None}, {"ld": 63}, {"lo": 63}, {"ld": 2 ** 41}, {"x": AT + 1}, {"out": AT + 1}, {"m": AT + 2}):
+            refused(call(**kw), M.INVALID_ARGUMENT)
+        assert call(t=0, x=None) == M.OK
+    for call in (dispatch, combine):
+        refused(call(out=None), M.INVALID_ARGUMENT)
+    for call in (combine, backward):
+        refused(call(w=AT + 2), M.INVALID_ARGUMENT)
+    refused(backward(y=None), M.INVALID_ARGUMENT)
+    refused(backward(dw=AT + 1), M.INVALID_ARGUMENT)
+    assert backward(out=None, dw=None, x=None) == M.OK  # nothing asked for
+
+
+def test_python_checks_come_before_the_library():
+    import torch
+
+    cpu = torch.zeros(4, 64)
+    for call in (lambda: M.mxfp4_quantize(cpu), lambda: M.expert_sort(torch.zeros(4, 2, dtype=torch.int32), 3),
+                 lambda: M.ExpertOrder(*(torch.zeros(4, dtype=torch.int32),) * 3, experts=3),
+                 lambda: M.MXFP4Weights(torch.zeros(4, 8, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.uint8))):
+        with pytest.raises(TypeError, match="CUDA"):
+            call()
+    with pytest.raises(M.MRError, match="uint8"):
+        M.MXFP4Weights(torch.zeros(4, 8, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32))
