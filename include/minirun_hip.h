@@ -303,9 +303,9 @@ mr_status mr_affine_gather_matmul(const void *x, mr_dtype x_dtype, int32_t token
  * laid out back to back.
  * ------------------------------------------------------------------------ */
 typedef struct mr_mxfp4_matrix {
-    const uint32_t *packed; /* 16-byte aligned */
-    const uint8_t *scales;  /* 4-byte aligned */
-    int64_t rows, cols;     /* cols a multiple of 32 */
+    const uint32_t *packed;
+    const uint8_t *scales;
+    int64_t rows, cols; /* cols a multiple of 32 */
 } mr_mxfp4_matrix;
 
 /* The operands' types and shapes, as mr_affine_validate checks affine ones:
@@ -330,6 +330,22 @@ mr_status mr_mxfp4_quantize(const void *x, mr_dtype x_dtype, int64_t rows, int64
  * a value passes the type's largest (byte 253 and 254). */
 mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_dtype, int64_t out_stride,
                               void *stream);
+
+/* y[t, :] = x[t, :] . W^T for a matrix W [out, in] = w (the MXFP4 sibling of
+ * mr_affine_matmul): x [tokens, in] bf16 or f32 with row stride x_stride; y
+ * [tokens, out] bf16 or f32 with row stride y_stride; f32 sums.  Weights are
+ * taken exactly; f32 activations too (as three bf16 parts).  x is 16-byte
+ * aligned with rows a multiple of 16 bytes apart, w->packed 16-byte aligned;
+ * in is at most 2^24.  The order of a token's sums, and so its last bits,
+ * depends on how many tokens the call has. */
+mr_status mr_mxfp4_matmul(const void *x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride,
+                          const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype, int64_t y_stride, void *stream);
+
+/* The same with x in MXFP4 too (mr_mxfp4_quantize's output; x->cols = w->cols,
+ * x->rows tokens, x->packed 16-byte aligned, x->rows * x->cols at most 2^34):
+ * products of the stored numbers, exact, on the scaled MFMA, in f32 sums. */
+mr_status mr_mxfp4_matmul_quantized(const mr_mxfp4_matrix *x, const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype,
+                                    int64_t y_stride, void *stream);
 
 /* ------------------------------------------------------------------------
  * The way of tokens to routed experts and back, around products of rows in
@@ -359,6 +375,33 @@ mr_status mr_expert_sort(const int32_t *ids, int32_t tokens, int32_t per_token, 
 mr_status mr_expert_dispatch(const void *x, mr_dtype dtype, int32_t tokens, int64_t dim, int64_t x_stride,
                              const int32_t *row_of_pair, int32_t per_token, void *rows, int64_t rows_stride,
                              void *stream);
+
+/* Products of rows in expert order, each expert's rows times its own matrix:
+ * for the rows r of expert e, y[r, :] = x[source(r), :] . W_e^T, as
+ * mr_mxfp4_matmul or (x_scales set) mr_mxfp4_matmul_quantized compute it, with
+ * their alignments.  w describes one expert of a stack laid out back to back.
+ * source(r) is r with pair_of_row NULL (x has `rows` rows), else
+ * pair_of_row[r] / per_token (x has one row per token).  Rows of y past the
+ * last expert's are left as they were.  offsets, pair_of_row: mr_expert_sort's;
+ * values that it does not write give rows of y that are unspecified, never an
+ * access outside the buffers. */
+typedef struct mr_mxfp4_expert_args {
+    const void *x; /* bf16 or f32 rows, or MXFP4 words [x_rows, in / 8] */
+    mr_dtype x_dtype; /* MR_BF16, MR_F32; MR_U32 for MXFP4 */
+    int64_t x_stride; /* elements; not read for MXFP4 */
+    const uint8_t *x_scales; /* MXFP4: [x_rows, in / 32]; else NULL */
+    int32_t x_rows;
+    mr_mxfp4_matrix w;
+    int32_t experts;
+    const int32_t *offsets; /* device [experts + 1] */
+    const int32_t *pair_of_row; /* device [rows], or NULL */
+    int32_t per_token; /* with pair_of_row */
+    int32_t rows; /* of y: tokens * per_token, at most 2^24 */
+    void *y;
+    mr_dtype y_dtype; /* MR_BF16 or MR_F32 */
+    int64_t y_stride;
+} mr_mxfp4_expert_args;
+mr_status mr_mxfp4_expert_matmul(const mr_mxfp4_expert_args *args, void *stream);
 
 /* out[t] = sum over the slots j that have a row, in their order, of
  * weights[t][j] * rows[row_of_pair[t][j]]: f32 sums, rounded once to `dtype`

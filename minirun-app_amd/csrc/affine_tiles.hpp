@@ -1,25 +1,12 @@
 // What the MFMA kernels over 4-bit affine rows share (skinny.hip,
-// affine_gemm.hip): buffer offsets past every row, nibbles as bf16 operands,
-// scales, and outputs from dequantized weights.
+// affine_gemm.hip): nibbles as bf16 operands, scales, and outputs from
+// dequantized weights.
 #pragma once
-#include "mr_kernels.hpp"
+#include "few_tiles.hpp"
 
 namespace mr {
 
 namespace {
-
-// byte offsets outside every buffer (host check: buffers under 2^30 bytes), of
-// a lane's row and of a k-block past the row's end; their sum is outside too
-constexpr uint32_t SK_OOB_ROW = 0x40000000u, SK_OOB_K = 0x80000000u;
-
-// the resource in scalar registers (its inputs are uniform, but may have been
-// computed in vector registers)
-__device__ __forceinline__ i32x4 uniform_rsrc(const void* base, uint32_t bytes) {
-    i32x4 r = buffer_rsrc(base, bytes);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
-    return r;
-}
 
 // eight nibbles of a word as bf16 0..15, in their order
 __device__ __forceinline__ bf16x8 nibbles_bf16(uint32_t w) {
@@ -137,11 +124,6 @@ __device__ float sk_affine_again(uint64_t rows, const uint16_t* x, const char* p
         if (l == j) acc = d;
     }
     return acc;
-}
-
-__device__ __forceinline__ void dma4_buf(i32x4 rsrc, uint32_t voff, const void* lds_dst_wave_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
 }
 
 }  // namespace

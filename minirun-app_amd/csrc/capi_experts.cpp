@@ -107,6 +107,100 @@ mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix* w, void* out, mr_dtype out_
     return done(mr::launch_mxfp4_dequantize(p, (hipStream_t)stream), "MXFP4 dequantization launch");
 }
 
+// what the products ask of x, w and y; fills what they share
+static mr_status gemm_params(const char* what, const void* x, mr_dtype x_dtype, const uint8_t* x_scales, int64_t x_rows,
+                             int64_t x_stride, const mr_mxfp4_matrix* w, int64_t y_rows, void* y, mr_dtype y_dtype,
+                             int64_t y_stride, mr::Mxfp4GemmParams& p) {
+    const mr_status st = check_extent(w->rows, w->cols, what);
+    if (st != MR_OK) return st;
+    const bool mx = x_dtype == MR_U32;
+    if (w->rows == 0 || w->rows > (1 << 30) || w->cols > (1 << 24))
+        return fail(MR_INVALID_SHAPE, "%s: a weight of %lld x %lld (at most 2^30 x 2^24)", what, (long long)w->rows,
+                    (long long)w->cols);
+    if (x_rows < 0 || x_rows > INT32_MAX) return fail(MR_INVALID_SHAPE, "%s: x has %lld rows", what, (long long)x_rows);
+    if ((!mx && !act(x_dtype)) || !act(y_dtype))
+        return fail(MR_INVALID_DTYPE, "%s: x must be bf16, f32 or MXFP4 and y bf16 or f32, got %s and %s", what,
+                    mrc::dtype_name(x_dtype), mrc::dtype_name(y_dtype));
+    // byte offsets of x's scales in 32 bits
+    if (mx && x_rows > (int64_t(1) << 34) / w->cols)
+        return fail(MR_INVALID_SHAPE, "%s: x of %lld x %lld values is more than 2^34", what, (long long)x_rows,
+                    (long long)w->cols);
+    if (x_rows == 0 || y_rows == 0) return MR_OK;
+    if (!x || (mx && !x_scales) || !w->packed || !w->scales || !y)
+        return fail(MR_INVALID_ARGUMENT, "%s: x, w and y must be non-NULL", what);
+    const int size = x_dtype == MR_F32 ? 4 : 2;
+    if (!mrc::aligned16(x) || !mrc::aligned16(w->packed) || (!mx && x_rows > 1 && x_stride * size % 16))
+        return fail(MR_INVALID_ARGUMENT, "%s: x and w->packed must be 16-byte aligned, x's rows a multiple of 16 bytes apart",
+                    what);
+    if ((!mx && x_rows > 1 && !stride_ok(x_stride, w->cols)) || (y_rows > 1 && !stride_ok(y_stride, w->rows)) ||
+        !elem_aligned(y, y_dtype))
+        return fail(MR_INVALID_ARGUMENT, "%s: a stride shorter than the rows, or a misaligned y", what);
+    p.x = x;
+    p.x_scales = x_scales;
+    p.x_kind = mx ? mr::MX_X_MXFP4 : (x_dtype == MR_F32 ? mr::MX_X_F32 : mr::MX_X_BF16);
+    p.ldx = x_stride;
+    p.packed = w->packed;
+    p.scales = w->scales;
+    p.y = y;
+    p.y_f32 = y_dtype == MR_F32;
+    p.ldy = y_stride;
+    p.M = (int)x_rows;
+    p.N = (int)w->rows;
+    p.K = (int)w->cols;
+    return MR_OK;
+}
+
+mr_status mr_mxfp4_matmul(const void* x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride, const mr_mxfp4_matrix* w,
+                          void* y, mr_dtype y_dtype, int64_t y_stride, void* stream) {
+    if (!w) return fail(MR_INVALID_ARGUMENT, "MXFP4 matmul: w is NULL");
+    if (x_dtype == MR_U32)
+        return fail(MR_INVALID_DTYPE, "MXFP4 matmul: x must be bf16 or f32 (mr_mxfp4_matmul_quantized takes MXFP4)");
+    mr::Mxfp4GemmParams p{};
+    const mr_status st = gemm_params("MXFP4 matmul", x, x_dtype, nullptr, tokens, x_stride, w, tokens, y, y_dtype, y_stride, p);
+    if (st != MR_OK || tokens == 0) return st;
+    return done(mr::launch_mxfp4_gemm(p, mrc::cu_count(), (hipStream_t)stream), "MXFP4 matmul launch");
+}
+
+mr_status mr_mxfp4_matmul_quantized(const mr_mxfp4_matrix* x, const mr_mxfp4_matrix* w, void* y, mr_dtype y_dtype,
+                                    int64_t y_stride, void* stream) {
+    if (!x || !w) return fail(MR_INVALID_ARGUMENT, "MXFP4 matmul: x or w is NULL");
+    if (x->cols != w->cols)
+        return fail(MR_INVALID_SHAPE, "MXFP4 matmul: x has %lld columns, w %lld", (long long)x->cols, (long long)w->cols);
+    mr::Mxfp4GemmParams p{};
+    const mr_status st = gemm_params("MXFP4 matmul", x->packed, MR_U32, x->scales, x->rows, 0, w, x->rows, y, y_dtype, y_stride, p);
+    if (st != MR_OK || x->rows == 0) return st;
+    return done(mr::launch_mxfp4_gemm(p, mrc::cu_count(), (hipStream_t)stream), "MXFP4 matmul launch");
+}
+
+mr_status mr_mxfp4_expert_matmul(const mr_mxfp4_expert_args* a, void* stream) {
+    const char* what = "MXFP4 expert matmul";
+    if (!a) return fail(MR_INVALID_ARGUMENT, "mr_mxfp4_expert_matmul: args is NULL");
+    if (a->experts <= 0 || a->experts > mr::EXPERT_MAX)
+        return fail(MR_INVALID_SHAPE, "%s: %d experts (1 to %d)", what, a->experts, mr::EXPERT_MAX);
+    if (a->rows < 0 || a->rows > (1 << 24) || (a->pair_of_row && (a->per_token <= 0 || a->rows % a->per_token)))
+        return fail(MR_INVALID_SHAPE, "%s: %d rows (at most 2^24) of tokens with %d experts each", what, a->rows, a->per_token);
+    const int32_t x_rows = a->pair_of_row ? a->rows / a->per_token : a->rows;
+    if (a->x_rows != x_rows)
+        return fail(MR_INVALID_SHAPE, "%s: x has %d rows, %d are asked for", what, a->x_rows, x_rows);
+    if ((a->x_dtype == MR_U32) != (a->x_scales != nullptr) && a->rows > 0)
+        return fail(MR_INVALID_ARGUMENT, "%s: x_scales goes with MXFP4 words, and only with them", what);
+    mr::Mxfp4GemmParams p{};
+    const mr_status st = gemm_params(what, a->x, a->x_dtype, a->x_scales, a->x_rows, a->x_stride, &a->w, a->rows, a->y,
+                                     a->y_dtype, a->y_stride, p);
+    if (st != MR_OK || a->rows == 0) return st;
+    if (!a->offsets || !mrc::aligned4(a->offsets) || !mrc::aligned4(a->pair_of_row))
+        return fail(MR_INVALID_ARGUMENT, "%s: offsets is NULL, or a misaligned pointer", what);
+    p.offsets = a->offsets;
+    p.experts = a->experts;
+    p.pairs = a->rows;
+    p.pair_of_row = a->pair_of_row;
+    p.per_token = a->per_token;
+    if (!mr::mxfp4_gemm_fits(p))
+        return fail(MR_INVALID_SHAPE, "%s: %d rows of %lld outputs are more than one launch takes", what, a->rows,
+                    (long long)a->w.rows);
+    return done(mr::launch_mxfp4_gemm(p, mrc::cu_count(), (hipStream_t)stream), "MXFP4 expert matmul launch");
+}
+
 static mr_status check_sort(int32_t tokens, int32_t per_token, int32_t experts) {
     if (tokens < 0 || per_token <= 0 || int64_t(tokens) * per_token > (1 << 24))
         return fail(MR_INVALID_SHAPE, "expert sort: %d tokens of %d experts (at most 2^24 pairs)", tokens, per_token);

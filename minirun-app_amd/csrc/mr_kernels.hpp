@@ -525,6 +525,29 @@ struct Mxfp4DequantizeParams {
 hipError_t launch_mxfp4_quantize(Mxfp4QuantizeParams p, hipStream_t st);
 hipError_t launch_mxfp4_dequantize(Mxfp4DequantizeParams p, hipStream_t st);
 
+// y = x . W^T with an MXFP4 weight: tokens of one matrix, or (offsets set)
+// rows in expert order, each expert's times its own matrix of a stack
+enum MxX { MX_X_BF16 = 0, MX_X_F32 = 1, MX_X_MXFP4 = 2 };
+struct Mxfp4GemmParams {
+    const void* x;            // M rows of K values at stride ldx; MXFP4: packed words, no gaps
+    const uint8_t* x_scales;  // MXFP4
+    int x_kind;
+    int64_t ldx;
+    const uint32_t* packed;  // [experts?][N][K / 8]
+    const uint8_t* scales;   // [experts?][N][K / 32]
+    void* y;
+    int y_f32;
+    int64_t ldy;
+    int M, N, K;
+    const int32_t* offsets;      // null: one matrix
+    int experts, pairs;          // pairs: rows of y
+    const int32_t* pair_of_row;  // null: row r of y is row r of x; else row pair / per_token
+    int per_token;
+};
+
+bool mxfp4_gemm_fits(const Mxfp4GemmParams& p);
+hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st);
+
 // ---------------------------------------------------------------- routed experts
 constexpr int EXPERT_MAX = 4096;          // experts of a sort
 constexpr int EXPERT_SORT_PAIRS = 4096;   // pairs per workgroup of the sort

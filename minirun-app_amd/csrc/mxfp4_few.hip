@@ -1,0 +1,332 @@
+// Products with MXFP4 weights for few rows: y[t][o] = sum_i x[t][i] w[o][i],
+// for the tokens of one matrix, or for rows in expert order, each expert's rows
+// times its own matrix of a stack.  x is bf16, f32, or MXFP4 itself.
+//
+// What bounds it: the weights' bytes from HBM, 17 / 32 of a byte each, read
+// once per 16 TT rows of x; then x's bytes from L2.  A workgroup owns 16 RT
+// weight rows and 16 TT rows of x, and its NW waves split K: wave w takes the
+// entries w, w + NW, ... of 128 k.  Each wave streams its entries into a ring
+// of S entries in LDS by DMA and waits for its own loads alone; the waves'
+// sums meet in LDS once, at the end, in a fixed order.
+//
+// A lane of the MFMA holds weight row l % 16 and the block l / 16 of the
+// entry's four: 16 bytes of codes and one scale byte, so nothing is
+// exchanged between lanes.
+//   x in bf16: the block's four words become bf16 with their scale (exact: two
+//     significant bits), one v_mfma_f32_16x16x32_bf16 each, with the eight
+//     values of x that belong to the word.
+//   x in f32: the same with x cut into three bf16 parts by truncation, whose
+//     sum is x exactly.
+//   x in MXFP4: v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands' codes
+//     and scale bytes as they are.
+// Chains start from zero per entry and are added to the running sums in f32.
+//
+// K is a multiple of 32.  In an entry that the row ends in, codes of W and x
+// past the end are loaded as zeros (W through the buffer's bounds, x from a
+// block of zeros), and scale bytes past the end, which may be the next row's,
+// are replaced by that of 1.  Scale rows start on any byte: each row's four
+// bytes come through the two aligned words that hold them.
+#include <algorithm>
+
+#include "few_tiles.hpp"
+#include "mxfp4_tiles.hpp"
+
+namespace mr {
+
+namespace {
+
+template <int XT>
+struct XEntry {  // of 128 k
+    static constexpr int BYTES = XT == MX_X_BF16 ? 256 : (XT == MX_X_F32 ? 512 : 64);
+    static constexpr int CHUNKS = BYTES / 16;     // of 16 bytes per row
+    static constexpr int RPI = 64 / CHUNKS;       // rows per DMA instruction
+    static constexpr int KPC = 128 / CHUNKS;      // values per chunk
+    // chunk c of row r is in slot c ^ swizzle(r), so that the 16 rows of a
+    // read of one chunk lie in 16 bank groups
+    static __device__ __forceinline__ int swizzle(int r) { return XT == MX_X_MXFP4 ? (r >> 2) & 3 : r & 15; }
+};
+
+// the three bf16 parts of eight f32 values, by truncation
+__device__ __forceinline__ void split3(const u32x4& a, const u32x4& b, bf16x8 (&part)[3]) {
+    u32x4 v[3];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint32_t x[2] = {k < 2 ? a[2 * k] : b[2 * k - 4], k < 2 ? a[2 * k + 1] : b[2 * k - 3]};
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            v[n][k] = (x[0] >> 16) | (x[1] & 0xffff0000u);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float f = __uint_as_float(x[h]), top = __uint_as_float(x[h] & 0xffff0000u);
+                x[h] = fabsf(f) == INFINITY ? 0u : __float_as_uint(f - top);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) part[n] = __builtin_bit_cast(bf16x8, v[n]);
+}
+
+template <int XT, int RT, int TT, int XI, int S, int NW>
+struct FewShape {
+    using X = XEntry<XT>;
+    static constexpr int SI = (RT + 1) / 2;                             // DMA instructions of W's scales
+    static constexpr int XS = XT == MX_X_MXFP4 ? (TT + 1) / 2 : 0;      // of x's
+    static constexpr int NI = RT + SI + XI + XS;
+    static constexpr int SOFF = 1024 * RT, XOFF = SOFF + 256 * SI, XSOFF = XOFF + 1024 * XI, ENTRY = XSOFF + 256 * XS;
+    static constexpr int ROWS = XI * X::RPI;                            // rows of x in an entry
+    static constexpr size_t LDS = std::max<size_t>((size_t)NW * S * ENTRY, (size_t)NW * RT * TT * 1024);
+    static_assert((S - 1) * NI < 64, "vmcnt range");
+    static_assert(ROWS >= 16 * TT || TT == 1, "rows of an entry");
+    static_assert(LDS <= 163840, "LDS");
+};
+
+template <int XT, int RT, int TT, int XI, int S, int NW, bool ROUTED>
+__global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, int blocks) {
+    using F = FewShape<XT, RT, TT, XI, S, NW>;
+    using X = XEntry<XT>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int l = threadIdx.x & 63, q = l >> 4, lr = l & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n_tiles = (p.N + 16 * RT - 1) / (16 * RT);
+    int tile, m0, toks;
+    int64_t first_row = 0;  // weight row 0 of the expert
+    if constexpr (ROUTED) {
+        MxTile t;
+        if (!mx_find_tile<16 * TT>(p.offsets, p.experts, p.pairs, n_tiles, t)) return;
+        tile = t.n_tile;
+        m0 = t.row;
+        toks = t.rows;
+        first_row = (int64_t)t.expert * p.N;
+    } else {
+        int tb;
+        sk_tile(blockIdx.x, blocks, tile, tb);
+        if (tile >= n_tiles) return;
+        m0 = tb * 16 * TT;
+        toks = min(16 * TT, p.M - m0);
+    }
+    const int n0 = tile * 16 * RT, rows = min(16 * RT, p.N - n0);
+    const uint32_t wrow = (uint32_t)p.K / 2, srow = (uint32_t)p.K / 32;
+    const i32x4 wres = uniform_rsrc((const char*)p.packed + (first_row + n0) * wrow, (uint32_t)rows * wrow);
+    // scales through aligned words
+    const uint64_t saddr = (uint64_t)(uintptr_t)p.scales + (first_row + n0) * srow;
+    const uint32_t soff0 = (uint32_t)saddr & 3u;
+    const i32x4 sres = uniform_rsrc((const void*)(uintptr_t)(saddr & ~3ull), (soff0 + (uint32_t)rows * srow + 3u) & ~3u);
+    const int nblk = (p.K + 127) / 128;
+    const int n = w < nblk ? (nblk - 1 - w) / NW + 1 : 0;  // this wave's entries
+
+    const uint32_t wch = (l & 3) ^ ((l >> 4) & 3);  // W: lane l fills slot l % 4 of row l / 4
+    uint32_t wo[RT], so[F::SI];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = 16 * r + (l >> 2);
+        wo[r] = row < rows ? (uint32_t)row * wrow + 16u * wch : SK_OOB_ROW;
+    }
+#pragma unroll
+    for (int v = 0; v < F::SI; ++v) {  // lane l: word l % 2 of row 32 v + l / 2
+        const int row = 32 * v + (l >> 1);
+        so[v] = row < rows ? ((soff0 + (uint32_t)row * srow) & ~3u) + 4u * (l & 1) : SK_OOB_ROW;
+    }
+    // x: row of x of row i of this workgroup's (past the last: the last)
+    auto xrow = [&](int i) -> int64_t {
+        i = min(i, toks - 1);
+        if constexpr (ROUTED) {
+            if (p.pair_of_row) return min((uint32_t)p.pair_of_row[m0 + i] / (uint32_t)p.per_token, (uint32_t)(p.M - 1));
+            return min(m0 + i, p.M - 1);
+        }
+        return m0 + i;
+    };
+    const char* xp[XI];
+#pragma unroll
+    for (int u = 0; u < XI; ++u) {
+        const int row = X::RPI * u + l / X::CHUNKS;
+        const int ch = (l % X::CHUNKS) ^ X::swizzle(row);
+        xp[u] = (const char*)p.x + (XT == MX_X_MXFP4 ? xrow(row) * wrow : xrow(row) * p.ldx * (XT == MX_X_F32 ? 4 : 2)) + 16 * ch;
+    }
+    auto x_first = [&](int u) {  // the lane's first value in an entry
+        const int row = X::RPI * u + l / X::CHUNKS;
+        return X::KPC * ((l % X::CHUNKS) ^ X::swizzle(row));
+    };
+    i32x4 xsres{};
+    uint32_t xso[F::XS > 0 ? F::XS : 1], xsh[TT];
+    if constexpr (XT == MX_X_MXFP4) {
+        const uint64_t xa = (uint64_t)(uintptr_t)p.x_scales;
+        xsres = uniform_rsrc((const void*)(uintptr_t)(xa & ~3ull), (((uint32_t)xa & 3u) + (uint32_t)p.M * srow + 3u) & ~3u);
+#pragma unroll
+        for (int v = 0; v < F::XS; ++v)
+            xso[v] = ((((uint32_t)xa & 3u) + (uint32_t)xrow(32 * v + (l >> 1)) * srow) & ~3u) + 4u * (l & 1);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) xsh[t] = (((uint32_t)xa & 3u) + (uint32_t)xrow(16 * t + lr) * srow) & 3u;
+    }
+
+    char* ring = lds + w * S * F::ENTRY;
+    auto issue = [&](int i, int slot) {
+        const int blk = w + NW * i;
+        const bool live = i < n;
+        char* e = ring + slot * F::ENTRY;
+        const uint32_t ko = live && 128u * blk + 32u * wch < (uint32_t)p.K ? 64u * blk : SK_OOB_K;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) dma16_buf(wres, wo[r] + ko, e + 1024 * r);
+#pragma unroll
+        for (int v = 0; v < F::SI; ++v) dma4_buf(sres, so[v] + (live ? 4u * blk : SK_OOB_K), e + F::SOFF + 256 * v);
+#pragma unroll
+        for (int u = 0; u < XI; ++u) {
+            const bool in = live && 128 * blk + x_first(u) < p.K;
+            dma16(in ? xp[u] + (int64_t)blk * X::BYTES : (const char*)mx_zeros, e + F::XOFF + 1024 * u);
+        }
+#pragma unroll
+        for (int v = 0; v < F::XS; ++v) dma4_buf(xsres, xso[v] + (live ? 4u * blk : SK_OOB_K), e + F::XSOFF + 256 * v);
+    };
+    f32x4 tot[RT][TT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) tot[r][t] = f32x4{};
+#pragma unroll
+    for (int s = 0; s < S; ++s) issue(s, s);
+    uint32_t wsh[RT];  // the row's first scale byte in its words
+#pragma unroll
+    for (int r = 0; r < RT; ++r) wsh[r] = (soff0 + (uint32_t)(16 * r + lr) * srow) & 3u;
+    // the scale byte of block q, that of 1 past the row's end
+    auto scale_byte = [&](const u32x2& v, uint32_t sh, bool in) -> uint32_t {
+        const uint32_t d = __builtin_amdgcn_alignbyte(v[1], v[0], sh);
+        return in ? (d >> (8 * q)) & 255u : 127u;
+    };
+    int slot = 0;
+    for (int i = 0; i < n; ++i) {
+        wait_vmcnt<(S - 1) * F::NI>();
+        const char* e = ring + slot * F::ENTRY;
+        u32x4 fw[RT];
+        u32x2 sw[RT], sx[TT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            fw[r] = *(const u32x4*)(e + 1024 * r + 64 * lr + 16 * (q ^ (lr >> 2)));
+            sw[r] = *(const u32x2*)(e + F::SOFF + 128 * r + 8 * lr);
+        }
+        constexpr int XF = XT == MX_X_MXFP4 ? 1 : (XT == MX_X_F32 ? 8 : 4);  // 16-byte pieces per lane
+        u32x4 fx[TT][XF];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int row = (16 * t + lr) % F::ROWS;
+#pragma unroll
+            for (int s = 0; s < XF; ++s)
+                fx[t][s] = *(const u32x4*)(e + F::XOFF + X::BYTES * row + 16 * ((XF * q + s) ^ X::swizzle(row)));
+            if constexpr (XT == MX_X_MXFP4) sx[t] = *(const u32x2*)(e + F::XSOFF + 8 * (16 * t + lr));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // the same, known to the compiler
+        __builtin_amdgcn_sched_barrier(0);
+        issue(i + S, slot);
+        slot = slot + 1 == S ? 0 : slot + 1;
+        const bool in = 128 * (w + NW * i) + 32 * q < p.K;
+        if constexpr (XT == MX_X_MXFP4) {
+            uint32_t bx[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) bx[t] = scale_byte(sx[t], xsh[t], in);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const uint32_t bw = scale_byte(sw[r], wsh[r], in);
+#pragma unroll
+                for (int t = 0; t < TT; ++t) tot[r][t] += mfma16_mxfp4(fx[t][0], bx[t], fw[r], bw, f32x4{});
+            }
+        } else {
+            float sc[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) sc[r] = __uint_as_float(scale_byte(sw[r], wsh[r], in) << 23);
+            f32x4 part[RT][TT];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                bf16x8 wf[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wf[r] = mxfp4_bf16(fw[r][s], sc[r]);
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    if constexpr (XT == MX_X_F32) {
+                        bf16x8 xf[3];
+                        split3(fx[t][2 * s], fx[t][2 * s + 1], xf);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            // small parts first
+                            const f32x4 c = mfma16(xf[2], wf[r], s == 0 ? f32x4{} : part[r][t]);
+                            part[r][t] = mfma16(xf[0], wf[r], mfma16(xf[1], wf[r], c));
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+                            part[r][t] = mfma16(__builtin_bit_cast(bf16x8, fx[t][s]), wf[r], s == 0 ? f32x4{} : part[r][t]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) tot[r][t] += part[r][t];
+        }
+    }
+    wait_vmcnt<0>();
+    sk_reduce<RT, TT, NW>(lds, tot, [&](int r, int t, int lane, f32x4 v) {
+        const int nn = 16 * r + (lane & 15);
+        if (nn >= rows) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int m = 16 * t + 4 * (lane >> 4) + e;
+            if (m >= toks) break;
+            const int64_t o = (int64_t)(m0 + m) * p.ldy + n0 + nn;
+            if (p.y_f32)
+                ((float*)p.y)[o] = v[e];
+            else
+                ((uint16_t*)p.y)[o] = f32_to_bf16_bits(v[e]);
+        }
+    });
+}
+
+template <int XT, int RT, int TT, int XI, int S, int NW>
+hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
+    constexpr size_t lds = FewShape<XT, RT, TT, XI, S, NW>::LDS;
+    const bool routed = p.offsets != nullptr;
+    const auto kern = routed ? mxfp4_few_kernel<XT, RT, TT, XI, S, NW, true> : mxfp4_few_kernel<XT, RT, TT, XI, S, NW, false>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    const int64_t tiles = (p.N + 16 * RT - 1) / (16 * RT), blocks = ((int64_t)p.M + 16 * TT - 1) / (16 * TT);
+    const int64_t grid = routed ? (mx_tile_bound(p, 16 * TT) * tiles + 7) / 8 * 8 : (tiles + 7) / 8 * 8 * blocks;
+    if (grid * 64 * NW >= (1ll << 32)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), lds, st, p, (int)blocks);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+static hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, hipStream_t st) {
+    // rows of x that one workgroup takes: all, or for experts about the mean
+    const int m = p.offsets ? (p.pairs + p.experts - 1) / p.experts : p.M;
+    if (p.x_kind == MX_X_MXFP4) return m <= 16 ? launch_few<2, 2, 1, 1, 2, 8>(p, st) : launch_few<2, 2, 4, 4, 2, 8>(p, st);
+    if (p.x_kind == MX_X_F32) return m <= 16 ? launch_few<1, 2, 1, 8, 1, 8>(p, st) : launch_few<1, 2, 2, 16, 1, 8>(p, st);
+    return m <= 16 ? launch_few<0, 2, 1, 4, 2, 8>(p, st) : launch_few<0, 2, 4, 16, 1, 8>(p, st);
+}
+
+// as many workgroups as a routed call can need in a grid of less than 2^32
+// threads
+bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
+    return !p.offsets || (mx_tile_bound(p, 16) * ((p.N + 31) / 32) + 7) * 512 < (1ll << 32);
+}
+
+// A matrix's tokens in as many launches as grids of less than 2^32 threads
+// take (one, up to 2^23 workgroups of 16 tokens x 32 weight rows).
+hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st) {
+    if (p.offsets) return launch_mxfp4_few(p, st);
+    const int64_t most = (((int64_t)1 << 23) / ((p.N + 31) / 32 + 7) - 1) * 16 / 64 * 64;
+    for (int64_t m = 0; m < p.M; m += most) {
+        Mxfp4GemmParams q = p;
+        q.M = (int)std::min<int64_t>(most, p.M - m);
+        const int64_t row = p.x_kind == MX_X_MXFP4 ? p.K / 2 : p.ldx * (p.x_kind == MX_X_F32 ? 4 : 2);
+        q.x = (const char*)p.x + m * row;
+        if (p.x_scales) q.x_scales = p.x_scales + m * (p.K / 32);
+        q.y = (char*)p.y + m * p.ldy * (p.y_f32 ? 4 : 2);
+        const hipError_t e = launch_mxfp4_few(q, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace mr

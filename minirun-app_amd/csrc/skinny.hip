@@ -45,40 +45,6 @@ namespace mr {
 
 namespace {
 
-// row tile and token block of this workgroup: consecutive workgroups go to
-// the 8 XCDs in turn
-__device__ __forceinline__ void sk_tile(int bid, int blocks, int& tile, int& tb) {
-    const int lo = bid & 7, hi = bid >> 3;
-    tb = hi % blocks;
-    tile = (hi / blocks) * 8 + lo;
-}
-
-// partial sums of the waves -> LDS -> one f32x4 per (tile, lane): emit(r, t,
-// lane, value) of row tile r, token tile t
-template <int RT, int TT, int NW, typename F>
-__device__ __forceinline__ void sk_reduce(char* lds, const f32x4 (&acc)[RT][TT], F emit) {
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
-    constexpr int P = RT * TT * 64;
-    f32x4* d = (f32x4*)lds;
-    __syncthreads();  // every wave is done with its ring
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) d[w * P + (r * TT + t) * 64 + l] = acc[r][t];
-    __syncthreads();
-    for (int i = tid; i < P; i += 64 * NW) {
-        f32x4 v[NW];
-#pragma unroll
-        for (int k = 0; k < NW; ++k) v[k] = d[k * P + i];
-#pragma unroll
-        for (int n = 1; n < NW; n *= 2)
-#pragma unroll
-            for (int k = 0; k + n < NW; k += 2 * n) v[k] += v[k + n];
-        const int rt = __builtin_amdgcn_readfirstlane(i >> 6);
-        emit(rt / TT, rt % TT, i & 63, v[0]);
-    }
-}
-
 // ---------------------------------------------------------------- dense
 // Ring entry: 32 k; W [16 RT rows][64 B], then x [16 TT rows][64 B]; 16-byte
 // chunk c of row r in slot c ^ ((r >> 2) & 3), so the 16 rows of a ds_read_b128

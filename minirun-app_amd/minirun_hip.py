@@ -144,6 +144,15 @@ class MXFP4Desc(C.Structure):
     _fields_ = [("packed", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64)]
 
 
+class MXFP4ExpertArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_dtype", C.c_int), ("x_stride", C.c_int64), ("x_scales", C.c_void_p), ("x_rows", C.c_int32),
+        ("w", MXFP4Desc), ("experts", C.c_int32), ("offsets", C.c_void_p), ("pair_of_row", C.c_void_p),
+        ("per_token", C.c_int32), ("rows", C.c_int32),
+        ("y", C.c_void_p), ("y_dtype", C.c_int), ("y_stride", C.c_int64),
+    ]
+
+
 TOPK_CHECK = 1
 TOPK_UNCHECKED = 2
 
@@ -205,6 +214,9 @@ SIGNATURES = {
     "mr_mxfp4_validate": (C.c_int, [C.c_int, C.c_int32, _I64P, C.c_int, C.c_int32, _I64P, _I64P, _I64P, _I64P]),
     "mr_mxfp4_quantize": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int64, _P, _P, _P]),
     "mr_mxfp4_dequantize": (C.c_int, [C.POINTER(MXFP4Desc), _P, C.c_int, C.c_int64, _P]),
+    "mr_mxfp4_matmul": (C.c_int, [_P, C.c_int, C.c_int32, C.c_int64, C.POINTER(MXFP4Desc), _P, C.c_int, C.c_int64, _P]),
+    "mr_mxfp4_matmul_quantized": (C.c_int, [C.POINTER(MXFP4Desc), C.POINTER(MXFP4Desc), _P, C.c_int, C.c_int64, _P]),
+    "mr_mxfp4_expert_matmul": (C.c_int, [C.POINTER(MXFP4ExpertArgs), _P]),
     "mr_expert_sort_workspace_size": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
     "mr_expert_sort": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, C.c_size_t, _P]),
     "mr_expert_dispatch": (C.c_int, [_P, C.c_int, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, _P, C.c_int64, _P]),
@@ -705,6 +717,36 @@ def mxfp4_dequantize(w: MXFP4Weights, dtype=None, stream=None):
     return out
 
 
+def mxfp4_mm(x, w: MXFP4Weights, out_dtype=None, stream=None):
+    """x [tokens, in] (or one row) -> x . W^T [tokens, out], f32 sums.  x is
+    bf16 or f32 (16-byte aligned rows; y in its dtype unless out_dtype says
+    otherwise), or MXFP4Weights (y in bf16 by default)."""
+    torch = _torch()
+    if w.experts is not None:
+        raise ValueError("mxfp4_mm takes one matrix; mxfp4_expert_mm a stack of experts")
+    if isinstance(x, MXFP4Weights):
+        if x.experts is not None:
+            raise ValueError("x must be one matrix [tokens, in], got a stack")
+        _same_device(w.packed, x=x.packed)
+        handle, ctx = _call_stream(w.packed, stream)
+        with ctx:
+            y = torch.empty(x.rows, w.rows, dtype=out_dtype or torch.bfloat16, device=w.packed.device)
+            _check(load().mr_mxfp4_matmul_quantized(C.byref(x.desc()), C.byref(w.desc()), _ptr(y), _dtype_code(y.dtype),
+                                                    w.rows, handle))
+        return y
+    x2 = x.unsqueeze(0) if x.dim() == 1 else x
+    ld = _rows2d(x2, "x")
+    if x2.shape[1] != w.cols:
+        raise ValueError(f"x has {x2.shape[1]} features, the weight {w.cols}")
+    _same_device(w.packed, x=x)
+    handle, ctx = _call_stream(x, stream)
+    with ctx:
+        y = torch.empty(x2.shape[0], w.rows, dtype=out_dtype or x.dtype, device=x.device)
+        _check(load().mr_mxfp4_matmul(_ptr(x2), _dtype_code(x2.dtype), x2.shape[0], ld, C.byref(w.desc()), _ptr(y),
+                                      _dtype_code(y.dtype), w.rows, handle))
+    return y if x.dim() == 2 else y.reshape(w.rows)
+
+
 class ExpertOrder:
     """Pairs (token, slot) in expert order, as expert_sort leaves them: offsets
     int32 [experts + 1], pair_of_row int32 [tokens * per_token], row_of_pair
@@ -761,6 +803,45 @@ def expert_dispatch(x, order: ExpertOrder, out=None, stream=None):
                                          _ptr(order.row_of_pair), order.per_token, _ptr(rows),
                                          _rows2d(rows, "out", shape), handle))
     return rows
+
+
+def mxfp4_expert_mm(x, w: MXFP4Weights, order: ExpertOrder, sorted_rows=False, out_dtype=None, out=None, stream=None):
+    """Rows in expert order [tokens * per_token, out]: row r is W_e . x of its
+    expert e and its token's x (x [tokens, in]), or with sorted_rows of row r of
+    x [tokens * per_token, in].  x and the result's dtype as for mxfp4_mm; w is
+    a stack.  Rows past the last of the order are not written (give `out` to
+    keep what they hold)."""
+    torch = _torch()
+    if w.experts != order.experts:
+        raise ValueError(f"the weight has {w.experts} experts, the order {order.experts}")
+    rows = order.tokens * order.per_token
+    a = MXFP4ExpertArgs()
+    if isinstance(x, MXFP4Weights):
+        if x.experts is not None:
+            raise ValueError("x must be one matrix, got a stack")
+        dtype, shape = out_dtype or torch.bfloat16, (x.rows, x.cols)
+        a.x, a.x_dtype, a.x_scales = x.packed.data_ptr(), U32, x.scales.data_ptr()
+        _same_device(w.packed, x=x.packed, order=order.offsets, out=out)
+    else:
+        a.x_stride = _rows2d(x, "x")
+        dtype, shape = out_dtype or x.dtype, tuple(x.shape)
+        a.x, a.x_dtype = x.data_ptr(), _dtype_code(x.dtype)
+        _same_device(w.packed, x=x, order=order.offsets, out=out)
+    if shape != (rows if sorted_rows else order.tokens, w.cols):
+        raise ValueError(f"x must be {[rows if sorted_rows else order.tokens, w.cols]}, got {list(shape)}")
+    handle, ctx = _call_stream(w.packed, stream)
+    with ctx:
+        y = torch.empty(rows, w.rows, dtype=dtype, device=w.packed.device) if out is None else out
+        if out is not None and out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError(f"out must be {out_dtype}, got {out.dtype}")
+        a.x_rows, a.w, a.experts, a.offsets = shape[0], w.desc(), order.experts, order.offsets.data_ptr()
+        a.per_token, a.rows = order.per_token, rows
+        if not sorted_rows:
+            a.pair_of_row = order.pair_of_row.data_ptr()
+        a.y_stride = _rows2d(y, "out", (rows, w.rows))
+        a.y, a.y_dtype = y.data_ptr(), _dtype_code(y.dtype)
+        _check(load().mr_mxfp4_expert_matmul(C.byref(a), handle))
+    return y
 
 
 def _expert_weights(weights, order):

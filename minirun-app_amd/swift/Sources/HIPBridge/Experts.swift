@@ -65,3 +65,41 @@ public func hipExpertCombineBackward(_ dOut: HIPTensor, rows: HIPTensor, _ order
                                                   Int32(order.tokens), Int32(order.perToken), dRows?.pointer,
                                                   Int64(dRows?.strides[0] ?? 0), dw, stream))
 }
+
+/// Each expert's rows times its own matrix of the stack `w`
+/// (QwenExpertBackends.swift:143,244 multiply token by token): x is one bf16 or
+/// f32 row per token, or per row of the order with `sortedRows`.
+public func hipMXFP4ExpertMM(_ x: HIPTensor, _ w: HIPMXFP4Weights, _ order: HIPExpertOrder, sortedRows: Bool = false,
+                             into y: HIPTensor, stream: HIPStream = nil) throws {
+    var a = mr_mxfp4_expert_args()
+    a.x = x.raw
+    a.x_dtype = x.dtype
+    a.x_stride = Int64(x.strides[0])
+    a.x_rows = Int32(x.shape[0])
+    try hipExpertMM(&a, w, order, sortedRows: sortedRows, into: y, stream: stream)
+}
+
+/// The same with x in MXFP4 (hipMXFP4Quantize's output).
+public func hipMXFP4ExpertMM(quantized x: HIPMXFP4Weights, _ w: HIPMXFP4Weights, _ order: HIPExpertOrder,
+                             sortedRows: Bool = false, into y: HIPTensor, stream: HIPStream = nil) throws {
+    var a = mr_mxfp4_expert_args()
+    a.x = UnsafeRawPointer(x.desc.packed)
+    a.x_dtype = MR_U32
+    a.x_scales = x.desc.scales
+    a.x_rows = Int32(x.desc.rows)
+    try hipExpertMM(&a, w, order, sortedRows: sortedRows, into: y, stream: stream)
+}
+
+private func hipExpertMM(_ a: inout mr_mxfp4_expert_args, _ w: HIPMXFP4Weights, _ order: HIPExpertOrder,
+                         sortedRows: Bool, into y: HIPTensor, stream: HIPStream) throws {
+    a.w = w.desc
+    a.experts = Int32(order.experts)
+    a.offsets = UnsafePointer(order.offsets.pointer.assumingMemoryBound(to: Int32.self))
+    a.pair_of_row = sortedRows ? nil : UnsafePointer(order.pairOfRow.pointer.assumingMemoryBound(to: Int32.self))
+    a.per_token = Int32(order.perToken)
+    a.rows = Int32(order.tokens * order.perToken)
+    a.y = y.pointer
+    a.y_dtype = y.dtype
+    a.y_stride = Int64(y.strides[0])
+    try HIPError.check(mr_mxfp4_expert_matmul(&a, stream))
+}

@@ -34,3 +34,18 @@ public func hipMXFP4Dequantize(_ w: HIPMXFP4Weights, into out: HIPTensor, stream
     d.rows *= Int64(w.experts ?? 1)
     try HIPError.check(mr_mxfp4_dequantize(&d, out.pointer, out.dtype, Int64(out.strides[out.strides.count - 2]), stream))
 }
+
+/// MXFP4 matmul (MLXBridge/MXFP4Weights.swift:36-60 holds the weight): y =
+/// x . W^T for bf16 or f32 rows.
+public func hipMXFP4MM(_ x: HIPTensor, _ w: HIPMXFP4Weights, into y: HIPTensor, stream: HIPStream = nil) throws {
+    var d = w.desc
+    try HIPError.check(mr_mxfp4_matmul(x.raw, x.dtype, Int32(x.shape[0]), Int64(x.strides[0]), &d, y.pointer, y.dtype,
+                                       Int64(y.strides[0]), stream))
+}
+
+/// The same with x in MXFP4 (hipMXFP4Quantize's output) too.
+public func hipMXFP4MM(quantized x: HIPMXFP4Weights, _ w: HIPMXFP4Weights, into y: HIPTensor,
+                       stream: HIPStream = nil) throws {
+    var dx = x.desc, dw = w.desc
+    try HIPError.check(mr_mxfp4_matmul_quantized(&dx, &dw, y.pointer, y.dtype, Int64(y.strides[0]), stream))
+}

@@ -77,6 +77,69 @@ def test_dequantize_refusals(lib):
     assert d(rows=0, out=None) == M.OK
 
 
+def w_desc(packed=AT, scales=AT, rows=64, cols=96):
+    return C.byref(M.MXFP4Desc(packed, scales, rows, cols))
+
+
+def test_matmul_refusals(lib):
+    def mm(x=AT, dt=M.BF16, t=4, ld=96, y=AT, ydt=M.BF16, ldy=64, **w):
+        return lib.mr_mxfp4_matmul(x, dt, t, ld, w_desc(**w), y, ydt, ldy, None)
+
+    refused(lib.mr_mxfp4_matmul(AT, M.BF16, 4, 96, None, AT, M.BF16, 64, None), M.INVALID_ARGUMENT)
+    for kw in ({"cols": 80}, {"cols": 0}, {"rows": 0}, {"rows": -4}, {"rows": 2 ** 30 + 1}, {"cols": 2 ** 24 + 32}, {"t": -1}):
+        refused(mm(**kw), M.INVALID_SHAPE)
+    for kw in ({"dt": M.F16}, {"dt": M.U8}, {"dt": 77}, {"ydt": M.F16}, {"ydt": M.U32}):
+        refused(mm(**kw), M.INVALID_DTYPE)
+    refused(mm(dt=M.U32), M.INVALID_DTYPE, "mr_mxfp4_matmul_quantized")
+    for kw in ({"x": None}, {"y": None}, {"packed": None}, {"scales": None}):
+        refused(mm(**kw), M.INVALID_ARGUMENT, "non-NULL")
+    for kw in ({"x": AT + 8}, {"packed": AT + 4}, {"ld": 100}, {"ld": 98, "dt": M.F32}):
+        refused(mm(**kw), M.INVALID_ARGUMENT, "16")
+    for kw in ({"ld": 88}, {"ldy": 63}, {"y": AT + 1}, {"y": AT + 2, "ydt": M.F32}, {"ld": 2 ** 41}):
+        refused(mm(**kw), M.INVALID_ARGUMENT)
+    assert mm(t=0, x=None, y=None) == M.OK
+
+
+def test_quantized_matmul_refusals(lib):
+    def mm(y=AT, ydt=M.BF16, ldy=64, x=w_desc(rows=4), **w):
+        return lib.mr_mxfp4_matmul_quantized(x, w_desc(**w), y, ydt, ldy, None)
+
+    refused(mm(x=None), M.INVALID_ARGUMENT)
+    refused(mm(cols=64), M.INVALID_SHAPE, "columns")
+    refused(mm(x=w_desc(rows=2 ** 31)), M.INVALID_SHAPE)
+    refused(mm(x=w_desc(rows=2 ** 28)), M.INVALID_SHAPE, "2^34")
+    refused(mm(ydt=M.F16), M.INVALID_DTYPE)
+    for kw in ({"x": w_desc(packed=None)}, {"x": w_desc(scales=None)}, {"y": None}, {"x": w_desc(packed=AT + 4)}, {"ldy": 63}):
+        refused(mm(**kw), M.INVALID_ARGUMENT)
+    assert mm(x=w_desc(rows=0), y=None) == M.OK
+
+
+def test_expert_matmul_refusals(lib):
+    def mm(w=None, **kw):
+        a = M.MXFP4ExpertArgs()
+        a.x, a.x_dtype, a.x_stride, a.x_rows = AT, M.BF16, 96, 4
+        a.w = M.MXFP4Desc(AT, AT, 64, 96)
+        a.experts, a.offsets, a.pair_of_row, a.per_token, a.rows = 8, AT, AT, 2, 8
+        a.y, a.y_dtype, a.y_stride = AT, M.BF16, 64
+        for k, v in (w or {}).items():
+            setattr(a.w, k, v)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.mr_mxfp4_expert_matmul(C.byref(a), None)
+
+    refused(lib.mr_mxfp4_expert_matmul(None, None), M.INVALID_ARGUMENT)
+    for kw in ({"experts": 0}, {"experts": 4097}, {"rows": -2}, {"rows": 2 ** 24 + 2}, {"rows": 7}, {"per_token": 0},
+               {"x_rows": 8}, {"pair_of_row": None}, {"w": {"cols": 72}}, {"w": {"rows": 0}},
+               {"w": {"rows": 2 ** 29}, "rows": 2 ** 24, "x_rows": 2 ** 23, "y_stride": 2 ** 29}):
+        refused(mm(**kw), M.INVALID_SHAPE)
+    for kw in ({"x_dtype": M.F16}, {"y_dtype": M.U32}):
+        refused(mm(**kw), M.INVALID_DTYPE)
+    for kw in ({"x": None}, {"y": None}, {"offsets": None}, {"offsets": AT + 2}, {"pair_of_row": AT + 1}, {"x": AT + 4},
+               {"x_scales": AT}, {"x_dtype": M.U32}, {"x_stride": 90}, {"y_stride": 60}, {"w": {"packed": None}}):
+        refused(mm(**kw), M.INVALID_ARGUMENT)
+    assert mm(rows=0, x_rows=0, x=None, y=None) == M.OK
+
+
 def test_sort_sizes_and_refusals(lib):
     size = lib.mr_expert_sort_workspace_size
     assert size(512, 8, 128) == 0  # one workgroup
