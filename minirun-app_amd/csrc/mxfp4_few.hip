@@ -297,7 +297,7 @@ hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
 
 }  // namespace
 
-static hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, hipStream_t st) {
+hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, hipStream_t st) {
     // rows of x that one workgroup takes: all, or for experts about the mean
     const int m = p.offsets ? (p.pairs + p.experts - 1) / p.experts : p.M;
     if (p.x_kind == MX_X_MXFP4) return m <= 16 ? launch_few<2, 2, 1, 1, 2, 8>(p, st) : launch_few<2, 2, 4, 4, 2, 8>(p, st);
@@ -311,11 +311,21 @@ bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
     return !p.offsets || (mx_tile_bound(p, 16) * ((p.N + 31) / 32) + 7) * 512 < (1ll << 32);
 }
 
+// Rows per large tile (0: the kernel for few rows).
+static int tile_rows(const Mxfp4GemmParams& p, int cu_count) {
+    if (!mxfp4_tiles_ok(p)) return 0;
+    const int64_t m = p.offsets ? (p.pairs + p.experts - 1) / p.experts : p.M;
+    if (m < 64) return 0;
+    const int64_t n_tiles = (p.N + 255) / 256, m_tiles = (m + 255) / 256 * (p.offsets ? p.experts : 1);
+    return m > 128 && n_tiles * m_tiles >= cu_count ? 256 : 128;
+}
+
 // A matrix's tokens in as many launches as grids of less than 2^32 threads
 // take (one, up to 2^23 workgroups of 16 tokens x 32 weight rows).
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st) {
-    if (p.offsets) return launch_mxfp4_few(p, st);
-    const int64_t most = (((int64_t)1 << 23) / ((p.N + 31) / 32 + 7) - 1) * 16 / 64 * 64;
+    const int tm = tile_rows(p, cu_count);
+    if (p.offsets) return tm ? launch_mxfp4_tiles(p, tm, st) : launch_mxfp4_few(p, st);
+    const int64_t most = (((int64_t)1 << 23) / ((p.N + 31) / 32 + 7) - 1) * 16 / 256 * 256;
     for (int64_t m = 0; m < p.M; m += most) {
         Mxfp4GemmParams q = p;
         q.M = (int)std::min<int64_t>(most, p.M - m);
@@ -323,7 +333,7 @@ hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t
         q.x = (const char*)p.x + m * row;
         if (p.x_scales) q.x_scales = p.x_scales + m * (p.K / 32);
         q.y = (char*)p.y + m * p.ldy * (p.y_f32 ? 4 : 2);
-        const hipError_t e = launch_mxfp4_few(q, st);
+        const hipError_t e = tm ? launch_mxfp4_tiles(q, tm, st) : launch_mxfp4_few(q, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

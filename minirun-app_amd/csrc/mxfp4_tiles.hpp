@@ -24,6 +24,15 @@ __device__ __forceinline__ f32x4 mfma16_mxfp4(const u32x4& a, uint32_t sa, const
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
+// D[32][32] += A . B^T over 64 k: lane l holds row l % 32 and block l / 32, and
+// its scale in byte SEL of the word.  D as v_mfma_f32_32x32x16_bf16's.
+template <int SEL>
+__device__ __forceinline__ f32x16 mfma32_mxfp4(const u32x4& a, uint32_t sa, const u32x4& b, uint32_t sb, const f32x16& c) {
+    const i32x8 va = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i32x8 vb = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, SEL, (int)sa, SEL, (int)sb);
+}
+
 struct MxTile {
     int expert, row, rows;  // rows row .. row + rows - 1 of y are the expert's
     int n_tile;             // of its weight rows
