@@ -335,15 +335,15 @@ mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_
  * mr_affine_matmul): x [tokens, in] bf16 or f32 with row stride x_stride; y
  * [tokens, out] bf16 or f32 with row stride y_stride; f32 sums.  Weights are
  * taken exactly; f32 activations too (as three bf16 parts).  x is 16-byte
- * aligned with rows a multiple of 16 bytes apart, w->packed 16-byte aligned;
- * in is at most 2^24.  The order of a token's sums, and so its last bits,
+ * aligned with rows a multiple of 16 and at most 2^23 bytes apart, w->packed
+ * 16-byte aligned; in is at most 2^20.  The order of a token's sums, and so its last bits,
  * depends on how many tokens the call has. */
 mr_status mr_mxfp4_matmul(const void *x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride,
                           const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype, int64_t y_stride, void *stream);
 
 /* The same with x in MXFP4 too (mr_mxfp4_quantize's output; x->cols = w->cols,
- * x->rows tokens, x->packed 16-byte aligned, x->rows * x->cols at most 2^34):
- * products of the stored numbers, exact, on the scaled MFMA, in f32 sums. */
+ * x->rows tokens, x->packed 16-byte aligned): products of the stored numbers,
+ * exact, on the scaled MFMA, in f32 sums. */
 mr_status mr_mxfp4_matmul_quantized(const mr_mxfp4_matrix *x, const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype,
                                     int64_t y_stride, void *stream);
 
@@ -381,7 +381,8 @@ mr_status mr_expert_dispatch(const void *x, mr_dtype dtype, int32_t tokens, int6
  * mr_mxfp4_matmul or (x_scales set) mr_mxfp4_matmul_quantized compute it, with
  * their alignments.  w describes one expert of a stack laid out back to back.
  * source(r) is r with pair_of_row NULL (x has `rows` rows), else
- * pair_of_row[r] / per_token (x has one row per token).  Rows of y past the
+ * pair_of_row[r] / per_token (x has one row per token, less than 2^32 - 2^16
+ * bytes in all).  Rows of y past the
  * last expert's are left as they were.  offsets, pair_of_row: mr_expert_sort's;
  * values that it does not write give rows of y that are unspecified, never an
  * access outside the buffers. */

@@ -114,17 +114,13 @@ static mr_status gemm_params(const char* what, const void* x, mr_dtype x_dtype, 
     const mr_status st = check_extent(w->rows, w->cols, what);
     if (st != MR_OK) return st;
     const bool mx = x_dtype == MR_U32;
-    if (w->rows == 0 || w->rows > (1 << 30) || w->cols > (1 << 24))
-        return fail(MR_INVALID_SHAPE, "%s: a weight of %lld x %lld (at most 2^30 x 2^24)", what, (long long)w->rows,
+    if (w->rows == 0 || w->rows > (1 << 30) || w->cols > (1 << 20))
+        return fail(MR_INVALID_SHAPE, "%s: a weight of %lld x %lld (at most 2^30 x 2^20)", what, (long long)w->rows,
                     (long long)w->cols);
     if (x_rows < 0 || x_rows > INT32_MAX) return fail(MR_INVALID_SHAPE, "%s: x has %lld rows", what, (long long)x_rows);
     if ((!mx && !act(x_dtype)) || !act(y_dtype))
         return fail(MR_INVALID_DTYPE, "%s: x must be bf16, f32 or MXFP4 and y bf16 or f32, got %s and %s", what,
                     mrc::dtype_name(x_dtype), mrc::dtype_name(y_dtype));
-    // byte offsets of x's scales in 32 bits
-    if (mx && x_rows > (int64_t(1) << 34) / w->cols)
-        return fail(MR_INVALID_SHAPE, "%s: x of %lld x %lld values is more than 2^34", what, (long long)x_rows,
-                    (long long)w->cols);
     if (x_rows == 0 || y_rows == 0) return MR_OK;
     if (!x || (mx && !x_scales) || !w->packed || !w->scales || !y)
         return fail(MR_INVALID_ARGUMENT, "%s: x, w and y must be non-NULL", what);
@@ -132,18 +128,21 @@ static mr_status gemm_params(const char* what, const void* x, mr_dtype x_dtype, 
     if (!mrc::aligned16(x) || !mrc::aligned16(w->packed) || (!mx && x_rows > 1 && x_stride * size % 16))
         return fail(MR_INVALID_ARGUMENT, "%s: x and w->packed must be 16-byte aligned, x's rows a multiple of 16 bytes apart",
                     what);
-    if ((!mx && x_rows > 1 && !stride_ok(x_stride, w->cols)) || (y_rows > 1 && !stride_ok(y_stride, w->rows)) ||
+    // byte offsets of the rows of a tile in 32 bits
+    if (!mx && x_rows > 1 && x_stride > (1 << 23) / size)
+        return fail(MR_INVALID_ARGUMENT, "%s: rows of x more than 2^23 bytes apart", what);
+    if ((!mx && x_rows > 1 && x_stride < w->cols) || (y_rows > 1 && !stride_ok(y_stride, w->rows)) ||
         !elem_aligned(y, y_dtype))
         return fail(MR_INVALID_ARGUMENT, "%s: a stride shorter than the rows, or a misaligned y", what);
     p.x = x;
     p.x_scales = x_scales;
     p.x_kind = mx ? mr::MX_X_MXFP4 : (x_dtype == MR_F32 ? mr::MX_X_F32 : mr::MX_X_BF16);
-    p.ldx = x_stride;
+    p.ldx = x_rows > 1 ? x_stride : w->cols;
     p.packed = w->packed;
     p.scales = w->scales;
     p.y = y;
     p.y_f32 = y_dtype == MR_F32;
-    p.ldy = y_stride;
+    p.ldy = y_rows > 1 ? y_stride : w->rows;
     p.M = (int)x_rows;
     p.N = (int)w->rows;
     p.K = (int)w->cols;
@@ -195,6 +194,10 @@ mr_status mr_mxfp4_expert_matmul(const mr_mxfp4_expert_args* a, void* stream) {
     p.pairs = a->rows;
     p.pair_of_row = a->pair_of_row;
     p.per_token = a->per_token;
+    // byte offsets of all rows of x in 32 bits
+    const int64_t x_row = p.x_kind == mr::MX_X_MXFP4 ? p.K / 2 : p.ldx * (p.x_kind == mr::MX_X_F32 ? 4 : 2);
+    if (a->pair_of_row && p.M * x_row >= 0xffff0000ll)
+        return fail(MR_INVALID_SHAPE, "%s: x of %d rows by token is 2^32 bytes or more; give its rows in expert order", what, p.M);
     if (!mr::mxfp4_gemm_fits(p))
         return fail(MR_INVALID_SHAPE, "%s: %d rows of %lld outputs are more than one launch takes", what, a->rows,
                     (long long)a->w.rows);

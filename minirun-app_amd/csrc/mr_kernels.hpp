@@ -546,7 +546,6 @@ struct Mxfp4GemmParams {
 };
 
 // tiles of tm = 256 or 128 rows of x times 256 weight rows
-bool mxfp4_tiles_ok(const Mxfp4GemmParams& p);
 hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int tm, hipStream_t st);
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p);
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st);

@@ -499,15 +499,6 @@ hipError_t mg_launch_r(const Mxfp4GemmParams& p, hipStream_t st) {
 
 }  // namespace
 
-// What the tiles need: 32-bit byte offsets of a tile's rows, or of all of x
-// where rows come by token, below the offset that stands for zeros
-bool mxfp4_tiles_ok(const Mxfp4GemmParams& p) {
-    if (p.x_kind == MX_X_F32) return false;
-    const int64_t row = p.x_kind == MX_X_MXFP4 ? p.K / 2 : p.ldx * 2;
-    const int64_t x_rows = p.offsets && p.pair_of_row ? p.M : 256;
-    return x_rows * row < 0xffff0000ll && 256ll * (p.K / 2) < 0xffff0000ll;
-}
-
 hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int tm, hipStream_t st) {
     if (p.x_kind == MX_X_MXFP4) return tm == 256 ? mg_launch_r<MX_X_MXFP4, 256>(p, st) : mg_launch_r<MX_X_MXFP4, 128>(p, st);
     return tm == 256 ? mg_launch_r<MX_X_BF16, 256>(p, st) : mg_launch_r<MX_X_BF16, 128>(p, st);

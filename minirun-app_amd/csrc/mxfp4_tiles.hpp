@@ -1,4 +1,4 @@
-// What the MXFP4 products share: the scaled MFMA, a block of zeros, and which
+// What the MXFP4 products share: the scaled MFMA, and which
 // expert, rows and weight rows a workgroup of a routed product has.
 #pragma once
 #include <algorithm>
@@ -11,17 +11,15 @@ namespace {
 
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
-// where DMA takes values past the end of a row from
-__device__ const u32x4 mx_zeros[1] = {};
-
 // D[16][16] += A . B^T over 128 k, both operands e2m1 codes with a scale byte
 // per 32: lane l holds row l % 16 and block l / 16 (16 bytes of codes, element
-// 0 in the low bits of the first word; the scale byte in the low byte).  D as
+// 0 in the low bits of the first word; its scale in byte SEL of the word).  D as
 // v_mfma_f32_16x16x32_bf16's.
+template <int SEL>
 __device__ __forceinline__ f32x4 mfma16_mxfp4(const u32x4& a, uint32_t sa, const u32x4& b, uint32_t sb, const f32x4& c) {
     const i32x8 va = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
     const i32x8 vb = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, 0, (int)sa, 0, (int)sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, SEL, (int)sa, SEL, (int)sb);
 }
 
 // D[32][32] += A . B^T over 64 k: lane l holds row l % 32 and block l / 32, and

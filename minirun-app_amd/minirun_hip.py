@@ -612,34 +612,35 @@ def affine_gather_mm(x, w: AffineWeights, rhs_indices, out_dtype=None, stream=No
 
 
 # ------------------------------------------------------------------ MXFP4 and routed experts
-def _call_stream(t, stream):
-    """The stream handle of a call on tensor t's device, and a context in which
-    what the call allocates belongs to that stream (None: the current one on
-    that device)."""
+_HERE = contextlib.nullcontext()
+
+
+def _call_stream(device, stream):
+    """The stream handle of a call on `device`, and a context in which what the
+    call allocates belongs to that stream (None: the current one there)."""
     torch = _torch()
+    cuda = torch.cuda
     if stream is None:
-        if t.device.index == torch.cuda.current_device():
-            ctx = contextlib.nullcontext()
-        else:
-            ctx = torch.cuda.device(t.device)
-        return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream), ctx
-    if isinstance(stream, torch.cuda.Stream):
-        return C.c_void_p(stream.cuda_stream), torch.cuda.stream(stream)
+        # current_stream(device).cuda_stream without the two Python objects
+        # between, which cost 2 of a small call's 10 us
+        handle = torch._C._cuda_getCurrentRawStream(device.index)
+        return handle, _HERE if device.index == cuda.current_device() else cuda.device(device)
+    if isinstance(stream, cuda.Stream):
+        return stream.cuda_stream, cuda.stream(stream)
     handle = stream.value if isinstance(stream, C.c_void_p) else stream
-    s = torch.cuda.ExternalStream(handle, t.device) if handle else torch.cuda.default_stream(t.device)
-    return C.c_void_p(handle), torch.cuda.stream(s)
+    s = cuda.ExternalStream(handle, device) if handle else cuda.default_stream(device)
+    return handle, cuda.stream(s)
 
 
-def _same_device(first, **others):
-    for name, t in others.items():
+def _same_device(first, *others):
+    for t in others:
         if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, the other tensors on {first.device}")
+            raise ValueError(f"a tensor is on {t.device}, the first on {first.device}")
 
 
 def _need_whole(t, name, dtype=None):
     """A GPU tensor without gaps (axes of one entry may have any stride)."""
-    torch = _torch()
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, _torch().Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA (HIP) tensor")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
@@ -649,11 +650,14 @@ def _need_whole(t, name, dtype=None):
 
 def _rows2d(t, name, shape=None):
     """Row stride of a 2-D tensor with contiguous rows."""
-    if not (isinstance(t, _torch().Tensor) and t.dim() and t.shape[-1] == 1 and t.is_cuda):
-        _need(t, name)
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if not isinstance(t, _torch().Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA (HIP) tensor")
+    if t.dim() != 2 or (shape is not None and t.shape != shape):
         raise ValueError(f"{name} must be {'2-D' if shape is None else list(shape)}, got {list(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    ld, step = t.stride()
+    if step != 1 and t.shape[1] != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return ld if t.shape[0] > 1 and ld > 0 else max(ld, t.shape[1])
 
 
 class MXFP4Weights:
@@ -674,11 +678,19 @@ class MXFP4Weights:
                                         C.byref(cols)))
         _need_whole(packed, "packed")
         _need_whole(scales, "scales")
-        _same_device(packed, scales=scales)
-        self.packed, self.scales = packed, scales
-        self.experts = ex.value or None
-        self.rows, self.cols = rows.value, cols.value
-        self.out_features, self.in_features = self.rows, self.cols
+        _same_device(packed, scales)
+        self._set(packed, scales, ex.value or None, rows.value, cols.value)
+
+    def _set(self, packed, scales, experts, rows, cols):
+        self.packed, self.scales, self.experts, self.rows, self.cols = packed, scales, experts, rows, cols
+        self.out_features, self.in_features = rows, cols
+
+    @classmethod
+    def _made(cls, packed, scales, experts, rows, cols):
+        """Of tensors that this module has just made to fit."""
+        w = cls.__new__(cls)
+        w._set(packed, scales, experts, rows, cols)
+        return w
 
     def desc(self):
         """One matrix (one expert of a stack)."""
@@ -695,25 +707,27 @@ def mxfp4_quantize(x, stream=None):
     if x.dim() not in (1, 2, 3):
         raise ValueError(f"x must be [rows, cols], a row or a stack of matrices, got {list(x.shape)}")
     lead, cols = (1,) if x.dim() == 1 else x.shape[:-1], x.shape[-1]
-    handle, ctx = _call_stream(x, stream)
+    handle, ctx = _call_stream(x.device, stream)
     with ctx:
         x2 = x if x.dim() == 2 else x.reshape(-1, cols)
-        packed = torch.empty(*lead, cols // 8, dtype=torch.int32, device=x.device)
-        scales = torch.empty(*lead, cols // 32, dtype=torch.uint8, device=x.device)
-        _check(load().mr_mxfp4_quantize(_ptr(x2), _dtype_code(x2.dtype), x2.shape[0], cols, _rows2d(x2, "x"),
-                                        _ptr(packed), _ptr(scales), handle))
-    return MXFP4Weights(packed, scales)
+        packed = torch.empty((*lead, cols // 8), dtype=torch.int32, device=x.device)
+        scales = torch.empty((*lead, cols // 32), dtype=torch.uint8, device=x.device)
+        _check(load().mr_mxfp4_quantize(x2.data_ptr(), _dtype_code(x2.dtype), x2.shape[0], cols, _rows2d(x2, "x"),
+                                        packed.data_ptr(), scales.data_ptr(), handle))
+    if x.dim() == 3 and not lead[0]:
+        raise ValueError("a stack needs one matrix at least")
+    return MXFP4Weights._made(packed, scales, lead[0] if x.dim() == 3 else None, lead[-1], cols)
 
 
 def mxfp4_dequantize(w: MXFP4Weights, dtype=None, stream=None):
     """The values that w stands for, f32 by default or bf16, in w's shape."""
     torch = _torch()
-    handle, ctx = _call_stream(w.packed, stream)
+    handle, ctx = _call_stream(w.packed.device, stream)
     with ctx:
-        out = torch.empty(*w.scales.shape[:-1], w.cols, dtype=dtype or torch.float32, device=w.packed.device)
+        out = torch.empty((*w.scales.shape[:-1], w.cols), dtype=dtype or torch.float32, device=w.packed.device)
         d = w.desc()
         d.rows = w.rows * (w.experts or 1)
-        _check(load().mr_mxfp4_dequantize(C.byref(d), _ptr(out), _dtype_code(out.dtype), w.cols, handle))
+        _check(load().mr_mxfp4_dequantize(C.byref(d), out.data_ptr(), _dtype_code(out.dtype), w.cols, handle))
     return out
 
 
@@ -727,22 +741,22 @@ def mxfp4_mm(x, w: MXFP4Weights, out_dtype=None, stream=None):
     if isinstance(x, MXFP4Weights):
         if x.experts is not None:
             raise ValueError("x must be one matrix [tokens, in], got a stack")
-        _same_device(w.packed, x=x.packed)
-        handle, ctx = _call_stream(w.packed, stream)
+        _same_device(w.packed, x.packed)
+        handle, ctx = _call_stream(w.packed.device, stream)
         with ctx:
             y = torch.empty(x.rows, w.rows, dtype=out_dtype or torch.bfloat16, device=w.packed.device)
-            _check(load().mr_mxfp4_matmul_quantized(C.byref(x.desc()), C.byref(w.desc()), _ptr(y), _dtype_code(y.dtype),
+            _check(load().mr_mxfp4_matmul_quantized(C.byref(x.desc()), C.byref(w.desc()), y.data_ptr(), _dtype_code(y.dtype),
                                                     w.rows, handle))
         return y
     x2 = x.unsqueeze(0) if x.dim() == 1 else x
     ld = _rows2d(x2, "x")
     if x2.shape[1] != w.cols:
         raise ValueError(f"x has {x2.shape[1]} features, the weight {w.cols}")
-    _same_device(w.packed, x=x)
-    handle, ctx = _call_stream(x, stream)
+    _same_device(w.packed, x)
+    handle, ctx = _call_stream(x.device, stream)
     with ctx:
         y = torch.empty(x2.shape[0], w.rows, dtype=out_dtype or x.dtype, device=x.device)
-        _check(load().mr_mxfp4_matmul(_ptr(x2), _dtype_code(x2.dtype), x2.shape[0], ld, C.byref(w.desc()), _ptr(y),
+        _check(load().mr_mxfp4_matmul(x2.data_ptr(), _dtype_code(x2.dtype), x2.shape[0], ld, C.byref(w.desc()), y.data_ptr(),
                                       _dtype_code(y.dtype), w.rows, handle))
     return y if x.dim() == 2 else y.reshape(w.rows)
 
@@ -756,12 +770,21 @@ class ExpertOrder:
         torch = _torch()
         for t, n in ((offsets, "offsets"), (pair_of_row, "pair_of_row"), (row_of_pair, "row_of_pair")):
             _need_whole(t, n, torch.int32)
-        _same_device(offsets, pair_of_row=pair_of_row, row_of_pair=row_of_pair)
+        _same_device(offsets, pair_of_row, row_of_pair)
         if row_of_pair.dim() != 2 or offsets.numel() != experts + 1 or pair_of_row.numel() != row_of_pair.numel():
             raise ValueError("an order is offsets [experts + 1], pair_of_row [tokens * per_token] and row_of_pair "
                              "[tokens, per_token]")
+        self._set(offsets, pair_of_row, row_of_pair, experts)
+
+    def _set(self, offsets, pair_of_row, row_of_pair, experts):
         self.offsets, self.pair_of_row, self.row_of_pair, self.experts = offsets, pair_of_row, row_of_pair, experts
         self.tokens, self.per_token = row_of_pair.shape
+
+    @classmethod
+    def _made(cls, offsets, pair_of_row, row_of_pair, experts):
+        o = cls.__new__(cls)
+        o._set(offsets, pair_of_row, row_of_pair, experts)
+        return o
 
 
 def expert_sort(ids, experts, stream=None):
@@ -773,15 +796,17 @@ def expert_sort(ids, experts, stream=None):
     if ids.dim() != 2:
         raise ValueError(f"ids must be [tokens, per_token], got {list(ids.shape)}")
     T, K = ids.shape
-    handle, ctx = _call_stream(ids, stream)
+    handle, ctx = _call_stream(ids.device, stream)
+    lib = load()
     with ctx:
-        n = load().mr_expert_sort_workspace_size(T, K, experts)
-        buf = torch.empty(max(experts, 0) + 1 + 2 * T * K, dtype=torch.int32, device=ids.device)
-        offsets, pair, row = buf.split([max(experts, 0) + 1, T * K, T * K])
+        n = lib.mr_expert_sort_workspace_size(T, K, experts)
+        head, pairs = max(experts, 0) + 1, T * K
+        buf = torch.empty(head + 2 * pairs, dtype=torch.int32, device=ids.device)
         ws = torch.empty(n, dtype=torch.uint8, device=ids.device) if n else None
-        _check(load().mr_expert_sort(_ptr(ids), T, K, experts, _ptr(offsets), _ptr(pair), _ptr(row), _ptr(ws), n,
-                                     handle))
-    return ExpertOrder(offsets, pair, row.view(T, K), experts)
+        at = buf.data_ptr()
+        _check(lib.mr_expert_sort(ids.data_ptr(), T, K, experts, at, at + 4 * head, at + 4 * (head + pairs),
+                                  ws.data_ptr() if n else None, n, handle))
+    return ExpertOrder._made(buf[:head], buf[head:head + pairs], buf[head + pairs:].view(T, K), experts)
 
 
 def expert_dispatch(x, order: ExpertOrder, out=None, stream=None):
@@ -790,17 +815,17 @@ def expert_dispatch(x, order: ExpertOrder, out=None, stream=None):
     `out` to keep what they hold)."""
     torch = _torch()
     ld = _rows2d(x, "x")
-    _same_device(x, order=order.offsets, out=out)
+    _same_device(x, order.offsets, out)
     if x.shape[0] != order.tokens:
         raise ValueError(f"x has {x.shape[0]} tokens, the order {order.tokens}")
     shape = (order.tokens * order.per_token, x.shape[1])
-    handle, ctx = _call_stream(x, stream)
+    handle, ctx = _call_stream(x.device, stream)
     with ctx:
         rows = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
         if rows.dtype != x.dtype:
             raise TypeError(f"out must be {x.dtype}, got {rows.dtype}")
-        _check(load().mr_expert_dispatch(_ptr(x), _dtype_code(x.dtype), order.tokens, x.shape[1], ld,
-                                         _ptr(order.row_of_pair), order.per_token, _ptr(rows),
+        _check(load().mr_expert_dispatch(x.data_ptr(), _dtype_code(x.dtype), order.tokens, x.shape[1], ld,
+                                         order.row_of_pair.data_ptr(), order.per_token, rows.data_ptr(),
                                          _rows2d(rows, "out", shape), handle))
     return rows
 
@@ -821,15 +846,15 @@ def mxfp4_expert_mm(x, w: MXFP4Weights, order: ExpertOrder, sorted_rows=False, o
             raise ValueError("x must be one matrix, got a stack")
         dtype, shape = out_dtype or torch.bfloat16, (x.rows, x.cols)
         a.x, a.x_dtype, a.x_scales = x.packed.data_ptr(), U32, x.scales.data_ptr()
-        _same_device(w.packed, x=x.packed, order=order.offsets, out=out)
+        _same_device(w.packed, x.packed, order.offsets, out)
     else:
         a.x_stride = _rows2d(x, "x")
         dtype, shape = out_dtype or x.dtype, tuple(x.shape)
         a.x, a.x_dtype = x.data_ptr(), _dtype_code(x.dtype)
-        _same_device(w.packed, x=x, order=order.offsets, out=out)
+        _same_device(w.packed, x, order.offsets, out)
     if shape != (rows if sorted_rows else order.tokens, w.cols):
         raise ValueError(f"x must be {[rows if sorted_rows else order.tokens, w.cols]}, got {list(shape)}")
-    handle, ctx = _call_stream(w.packed, stream)
+    handle, ctx = _call_stream(w.packed.device, stream)
     with ctx:
         y = torch.empty(rows, w.rows, dtype=dtype, device=w.packed.device) if out is None else out
         if out is not None and out_dtype is not None and out.dtype != out_dtype:
@@ -860,15 +885,15 @@ def expert_combine(rows, order: ExpertOrder, weights=None, stream=None):
     torch = _torch()
     ld = _rows2d(rows, "rows")
     _expert_weights(weights, order)
-    _same_device(rows, order=order.offsets, weights=weights)
+    _same_device(rows, order.offsets, weights)
     if rows.shape[0] != order.tokens * order.per_token:
         raise ValueError(f"rows has {rows.shape[0]} rows, the order {order.tokens * order.per_token}")
-    handle, ctx = _call_stream(rows, stream)
+    handle, ctx = _call_stream(rows.device, stream)
     with ctx:
         out = torch.empty(order.tokens, rows.shape[1], dtype=rows.dtype, device=rows.device)
-        _check(load().mr_expert_combine(_ptr(rows), _dtype_code(rows.dtype), ld, rows.shape[1],
-                                        _ptr(order.row_of_pair), _ptr(weights), order.tokens, order.per_token,
-                                        _ptr(out), rows.shape[1], handle))
+        _check(load().mr_expert_combine(rows.data_ptr(), _dtype_code(rows.dtype), ld, rows.shape[1],
+                                        order.row_of_pair.data_ptr(), (None if weights is None else weights.data_ptr()), order.tokens, order.per_token,
+                                        out.data_ptr(), rows.shape[1], handle))
     return out
 
 
@@ -880,21 +905,21 @@ def expert_combine_backward(d_out, rows, order: ExpertOrder, weights=None, out=N
     torch = _torch()
     ld_g, ld = _rows2d(d_out, "d_out"), _rows2d(rows, "rows")
     _expert_weights(weights, order)
-    _same_device(d_out, rows=rows, order=order.offsets, weights=weights, out=out)
+    _same_device(d_out, rows, order.offsets, weights, out)
     shape = (order.tokens * order.per_token, d_out.shape[1])
     if d_out.shape[0] != order.tokens or tuple(rows.shape) != shape or rows.dtype != d_out.dtype:
         raise ValueError(f"d_out must be [{order.tokens}, dim] and rows {list(shape)} of its dtype, got "
                          f"{list(d_out.shape)} and {list(rows.shape)} {rows.dtype}")
-    handle, ctx = _call_stream(d_out, stream)
+    handle, ctx = _call_stream(d_out.device, stream)
     with ctx:
         d_rows = torch.empty(shape, dtype=rows.dtype, device=rows.device) if out is None else out
         if d_rows.dtype != rows.dtype:
             raise TypeError(f"out must be {rows.dtype}, got {d_rows.dtype}")
         d_weights = torch.empty(order.tokens, order.per_token, dtype=torch.float32, device=rows.device)
-        _check(load().mr_expert_combine_backward(_ptr(d_out), _dtype_code(d_out.dtype), ld_g, d_out.shape[1],
-                                                 _ptr(rows), ld, _ptr(order.row_of_pair), _ptr(weights),
-                                                 order.tokens, order.per_token, _ptr(d_rows),
-                                                 _rows2d(d_rows, "out", shape), _ptr(d_weights), handle))
+        _check(load().mr_expert_combine_backward(d_out.data_ptr(), _dtype_code(d_out.dtype), ld_g, d_out.shape[1],
+                                                 rows.data_ptr(), ld, order.row_of_pair.data_ptr(), (None if weights is None else weights.data_ptr()),
+                                                 order.tokens, order.per_token, d_rows.data_ptr(),
+                                                 _rows2d(d_rows, "out", shape), d_weights.data_ptr(), handle))
     return d_rows, d_weights
 
 

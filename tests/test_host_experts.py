@@ -86,7 +86,7 @@ def test_matmul_refusals(lib):
         return lib.mr_mxfp4_matmul(x, dt, t, ld, w_desc(**w), y, ydt, ldy, None)
 
     refused(lib.mr_mxfp4_matmul(AT, M.BF16, 4, 96, None, AT, M.BF16, 64, None), M.INVALID_ARGUMENT)
-    for kw in ({"cols": 80}, {"cols": 0}, {"rows": 0}, {"rows": -4}, {"rows": 2 ** 30 + 1}, {"cols": 2 ** 24 + 32}, {"t": -1}):
+    for kw in ({"cols": 80}, {"cols": 0}, {"rows": 0}, {"rows": -4}, {"rows": 2 ** 30 + 1}, {"cols": 2 ** 20 + 32}, {"t": -1}):
         refused(mm(**kw), M.INVALID_SHAPE)
     for kw in ({"dt": M.F16}, {"dt": M.U8}, {"dt": 77}, {"ydt": M.F16}, {"ydt": M.U32}):
         refused(mm(**kw), M.INVALID_DTYPE)
@@ -95,7 +95,7 @@ def test_matmul_refusals(lib):
         refused(mm(**kw), M.INVALID_ARGUMENT, "non-NULL")
     for kw in ({"x": AT + 8}, {"packed": AT + 4}, {"ld": 100}, {"ld": 98, "dt": M.F32}):
         refused(mm(**kw), M.INVALID_ARGUMENT, "16")
-    for kw in ({"ld": 88}, {"ldy": 63}, {"y": AT + 1}, {"y": AT + 2, "ydt": M.F32}, {"ld": 2 ** 41}):
+    for kw in ({"ld": 88}, {"ldy": 63}, {"y": AT + 1}, {"y": AT + 2, "ydt": M.F32}, {"ld": 2 ** 22 + 8}, {"ld": 2 ** 41}, {"ldy": 2 ** 41}):
         refused(mm(**kw), M.INVALID_ARGUMENT)
     assert mm(t=0, x=None, y=None) == M.OK
 
@@ -107,7 +107,6 @@ def test_quantized_matmul_refusals(lib):
     refused(mm(x=None), M.INVALID_ARGUMENT)
     refused(mm(cols=64), M.INVALID_SHAPE, "columns")
     refused(mm(x=w_desc(rows=2 ** 31)), M.INVALID_SHAPE)
-    refused(mm(x=w_desc(rows=2 ** 28)), M.INVALID_SHAPE, "2^34")
     refused(mm(ydt=M.F16), M.INVALID_DTYPE)
     for kw in ({"x": w_desc(packed=None)}, {"x": w_desc(scales=None)}, {"y": None}, {"x": w_desc(packed=AT + 4)}, {"ldy": 63}):
         refused(mm(**kw), M.INVALID_ARGUMENT)
@@ -130,6 +129,7 @@ def test_expert_matmul_refusals(lib):
     refused(lib.mr_mxfp4_expert_matmul(None, None), M.INVALID_ARGUMENT)
     for kw in ({"experts": 0}, {"experts": 4097}, {"rows": -2}, {"rows": 2 ** 24 + 2}, {"rows": 7}, {"per_token": 0},
                {"x_rows": 8}, {"pair_of_row": None}, {"w": {"cols": 72}}, {"w": {"rows": 0}},
+               {"rows": 2 ** 23, "x_rows": 2 ** 22, "w": {"cols": 512}, "x_stride": 512},
                {"w": {"rows": 2 ** 29}, "rows": 2 ** 24, "x_rows": 2 ** 23, "y_stride": 2 ** 29}):
         refused(mm(**kw), M.INVALID_SHAPE)
     for kw in ({"x_dtype": M.F16}, {"y_dtype": M.U32}):
