@@ -336,7 +336,7 @@ mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_
  * [tokens, out] bf16 or f32 with row stride y_stride; f32 sums.  Weights are
  * taken exactly; f32 activations too (as three bf16 parts).  x is 16-byte
  * aligned with rows a multiple of 16 and at most 2^23 bytes apart, w->packed
- * 16-byte aligned; in is at most 2^20.  The order of a token's sums, and so its last bits,
+ * 16-byte aligned; out is at most 2^22, in 2^20.  The order of a token's sums, and so its last bits,
  * depends on how many tokens the call has. */
 mr_status mr_mxfp4_matmul(const void *x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride,
                           const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype, int64_t y_stride, void *stream);

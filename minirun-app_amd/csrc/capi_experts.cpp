@@ -114,8 +114,8 @@ static mr_status gemm_params(const char* what, const void* x, mr_dtype x_dtype, 
     const mr_status st = check_extent(w->rows, w->cols, what);
     if (st != MR_OK) return st;
     const bool mx = x_dtype == MR_U32;
-    if (w->rows == 0 || w->rows > (1 << 30) || w->cols > (1 << 20))
-        return fail(MR_INVALID_SHAPE, "%s: a weight of %lld x %lld (at most 2^30 x 2^20)", what, (long long)w->rows,
+    if (w->rows == 0 || w->rows > mr::MXFP4_MAX_OUT || w->cols > (1 << 20))
+        return fail(MR_INVALID_SHAPE, "%s: a weight of %lld x %lld (at most 2^22 x 2^20)", what, (long long)w->rows,
                     (long long)w->cols);
     if (x_rows < 0 || x_rows > INT32_MAX) return fail(MR_INVALID_SHAPE, "%s: x has %lld rows", what, (long long)x_rows);
     if ((!mx && !act(x_dtype)) || !act(y_dtype))

@@ -545,6 +545,7 @@ struct Mxfp4GemmParams {
     int per_token;
 };
 
+constexpr int MXFP4_MAX_OUT = 1 << 22;  // weight rows of a product
 // tiles of tm = 256 or 128 rows of x times 256 weight rows
 hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int tm, hipStream_t st);
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p);

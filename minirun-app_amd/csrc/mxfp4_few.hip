@@ -158,15 +158,15 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
 #pragma unroll
         for (int c = 0; c < 2 * RT; ++c) {
             const bool in = live && 256u * ent + 32u * (ch8 ^ (4 * (c & 1))) < K;
-            dma16_buf(wres, wo[c] + (in ? 128u * ent : SK_OOB_K), e + 1024 * c);
+            mx_dma16(wres, wo[c] + (in ? 128u * ent : SK_OOB_K), e + 1024 * c);
         }
-        dma16_buf(sres, so + (live ? 8u * ent : SK_OOB_K), e + F::SOFF);
+        mx_dma16(sres, so + (live ? 8u * ent : SK_OOB_K), e + F::SOFF);
 #pragma unroll
         for (int u = 0; u < XI; ++u) {
             const bool in = live && 256u * ent + X::KPC * x_chunk(u) < K && X::RPI * u + l / X::CHUNKS < toks;
-            dma16_buf(xres, in ? xo[u] + (uint32_t)X::BYTES * ent : PAST, e + F::XOFF + 1024 * u);
+            mx_dma16(xres, in ? xo[u] + (uint32_t)X::BYTES * ent : PAST, e + F::XOFF + 1024 * u);
         }
-        if constexpr (XT == MX_X_MXFP4) dma16_buf(xsres, live && l < toks ? xso + 8u * ent : PAST, e + F::XSOFF);
+        if constexpr (XT == MX_X_MXFP4) mx_dma16(xsres, live && l < toks ? xso + 8u * ent : PAST, e + F::XSOFF);
     };
     f32x4 tot[RT][TT];
 #pragma unroll
@@ -284,6 +284,254 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
     });
 }
 
+// The same products for more rows of x, where reading x once per 16 or 32 weight
+// rows would cost more than the weights: the NW waves of a workgroup own 16 RT
+// weight rows each and share the 16 TT rows of x.  K streams through a ring of S
+// stages of 256 k (x once, W and its scales per wave), one barrier per stage: it
+// says that every wave's part of the stage has landed and that the slot of the
+// last one is free, into which stage s + S - 1 then goes.  Up to S - 1 stages are
+// in flight.  No sum crosses a wave.
+template <int XT, int RT, int TT, int S, int NW>
+struct MidShape {
+    using X = XEntry<XT>;
+    static constexpr int XI = 16 * TT / X::RPI;           // DMA instructions of x
+    static constexpr int XPW = (XI + NW - 1) / NW;        // of a wave
+    static constexpr int XS = XT == MX_X_MXFP4 ? 1 : 0;   // of x's scales: a copy per wave
+    static constexpr int NI = XPW + 2 * RT + 1 + XS;
+    static constexpr int WAVE = 2048 * RT + 1024 + 1024 * XS;  // bytes of a wave's part
+    static constexpr int STAGE = 1024 * XI + NW * WAVE;
+    static constexpr size_t LDS = (size_t)S * STAGE;
+    static_assert(S >= 2 && (S - 1) * NI < 64 && LDS <= 163840 && RT <= 4 && TT <= 4, "stages");
+};
+
+template <int XT, int RT, int TT, int S, int NW, bool ROUTED>
+__global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, int blocks) {
+    using F = MidShape<XT, RT, TT, S, NW>;
+    using X = XEntry<XT>;
+    constexpr int BM = 16 * TT, BN = 16 * RT * NW;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int l = threadIdx.x & 63, q = l >> 4, lr = l & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n_tiles = (p.N + BN - 1) / BN;
+    int tile, m0, toks;
+    int64_t first_row = 0;  // weight row 0 of the expert
+    if constexpr (ROUTED) {
+        MxTile t;
+        if (!mx_find_tile<BM>(p.offsets, p.experts, p.pairs, n_tiles, t)) return;
+        tile = t.n_tile;
+        m0 = t.row;
+        toks = t.rows;
+        first_row = (int64_t)t.expert * p.N;
+    } else {
+        int tb;
+        sk_tile(blockIdx.x, blocks, tile, tb);
+        if (tile >= n_tiles) return;
+        m0 = tb * BM;
+        toks = min(BM, p.M - m0);
+    }
+    // this wave's rows; none for a wave past N, which still loads its part of x
+    const int n0 = tile * BN + 16 * RT * w, rows = min(16 * RT, p.N - n0);
+    const uint32_t K = (uint32_t)p.K, wrow = K / 2, srow = K / 32;
+    const int64_t xrow = XT == MX_X_MXFP4 ? wrow : p.ldx * (XT == MX_X_F32 ? 4 : 2);
+    const int64_t w_first = first_row + min(n0, p.N - 1);
+    const uint32_t wrows = (uint32_t)max(rows, 0);
+    const i32x4 wres = uniform_rsrc((const char*)p.packed + w_first * wrow, wrows * wrow);
+    const uint64_t wsa = (uint64_t)(uintptr_t)p.scales + w_first * srow;
+    const uint32_t ws0 = (uint32_t)wsa & 3u;
+    const i32x4 sres = uniform_rsrc((const void*)(uintptr_t)(wsa & ~3ull), wrows ? (ws0 + wrows * srow + 3u) & ~3u : 0u);
+    const bool by_token = ROUTED && p.pair_of_row != nullptr;
+    const int64_t x_from = by_token ? 0 : m0, x_rows = by_token ? p.M : toks;
+    const i32x4 xres = uniform_rsrc((const char*)p.x + x_from * xrow,
+                                    (uint32_t)((x_rows - 1) * xrow + X::BYTES * (int64_t)K / 256));
+    auto x_index = [&](int r) -> uint32_t {
+        r = min(r, toks - 1);
+        if (by_token) return min((uint32_t)p.pair_of_row[m0 + r] / (uint32_t)p.per_token, (uint32_t)(p.M - 1));
+        return (uint32_t)r;
+    };
+    const int nst = (int)((K + 255) / 256);
+
+    constexpr uint32_t PAST = 0xfffffff0u;  // an offset that reads zeros
+    const uint32_t ch8 = (l & 7) ^ (l >> 4);
+    uint32_t wo[2 * RT], xo[F::XPW], xso = 0, xsh[TT];
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) {
+        const int r = 8 * i + (l >> 3);
+        wo[i] = r < rows ? (uint32_t)r * wrow + 16u * (ch8 ^ (4 * (i & 1))) : SK_OOB_ROW;
+    }
+    const uint32_t so = l < rows ? (ws0 + (uint32_t)l * srow) & ~3u : SK_OOB_ROW;
+    // x: this wave's instruction u of XPW (the last waves may repeat one)
+    auto x_instr = [&](int u) { return min(F::XPW * w + u, F::XI - 1); };
+    auto x_row = [&](int u) { return X::RPI * x_instr(u) + l / X::CHUNKS; };
+    auto x_chunk = [&](int u) { return (uint32_t)((l % X::CHUNKS) ^ X::swizzle(x_row(u))); };
+#pragma unroll
+    for (int u = 0; u < F::XPW; ++u) xo[u] = x_index(x_row(u)) * (uint32_t)xrow + 16u * x_chunk(u);
+    i32x4 xsres{};
+    if constexpr (XT == MX_X_MXFP4) {
+        const uint64_t xa = (uint64_t)(uintptr_t)p.x_scales + x_from * srow;
+        const uint32_t xs0 = (uint32_t)xa & 3u;
+        xsres = uniform_rsrc((const void*)(uintptr_t)(xa & ~3ull), (xs0 + (uint32_t)x_rows * srow + 3u) & ~3u);
+        xso = (xs0 + x_index(l) * srow) & ~3u;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) xsh[t] = ((xs0 + x_index(16 * t + lr) * srow) & 3u) + 2u * q;
+    }
+    const int woff = 1024 * F::XI + w * F::WAVE;  // of the wave's part in a stage
+    auto issue = [&](int s, int slot) {
+        const uint32_t st = s;
+        const bool live = s < nst;
+        char* e = lds + slot * F::STAGE;
+#pragma unroll
+        for (int u = 0; u < F::XPW; ++u) {
+            const bool in = live && 256u * st + X::KPC * x_chunk(u) < K && x_row(u) < toks;
+            mx_dma16(xres, in ? xo[u] + (uint32_t)X::BYTES * st : PAST, e + 1024 * x_instr(u));
+        }
+        e += woff;
+#pragma unroll
+        for (int c = 0; c < 2 * RT; ++c) {
+            const bool in = live && 256u * st + 32u * (ch8 ^ (4 * (c & 1))) < K;
+            mx_dma16(wres, wo[c] + (in ? 128u * st : SK_OOB_K), e + 1024 * c);
+        }
+        mx_dma16(sres, so + (live ? 8u * st : SK_OOB_K), e + 2048 * RT);
+        if constexpr (XT == MX_X_MXFP4) mx_dma16(xsres, live && l < toks ? xso + 8u * st : PAST, e + 2048 * RT + 1024);
+    };
+    f32x4 tot[RT][TT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) tot[r][t] = f32x4{};
+    uint32_t wsh[RT];  // byte of the lane's first block in its row's 16
+#pragma unroll
+    for (int r = 0; r < RT; ++r) wsh[r] = ((ws0 + (uint32_t)(16 * r + lr) * srow) & 3u) + 2u * q;
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) issue(s, s);
+    auto scale_bytes = [&](const char* row, uint32_t at, bool in0, bool in1) -> uint32_t {
+        const uint32_t* v = (const uint32_t*)row + (at >> 2);
+        const uint32_t d = __builtin_amdgcn_alignbyte(v[1], v[0], at & 3u);
+        return in1 ? d : (in0 ? (d & 0xffu) | 0x7f00u : 0x7f7fu);
+    };
+    int slot = 0;
+#pragma unroll 1
+    for (int s = 0; s < nst; ++s) {
+        wait_vmcnt<(S - 2) * F::NI>();
+        lds_barrier();
+        issue(s + S - 1, slot ? slot - 1 : S - 1);
+        const char* e = lds + slot * F::STAGE;
+        const char* ew = e + woff;
+        const uint32_t k0 = 256u * s + 64u * q;
+        const bool in0 = k0 < K, in1 = k0 + 32 < K;
+        u32x4 fw[RT][2];
+        uint32_t bw[RT], bx[TT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) fw[r][u] = *(const u32x4*)(ew + 2048 * r + 128 * lr + 16 * ((2 * q + u) ^ (lr >> 1)));
+            bw[r] = scale_bytes(ew + 2048 * RT + 16 * (16 * r + lr), wsh[r], in0, in1);
+        }
+        if constexpr (XT == MX_X_MXFP4) {
+#pragma unroll
+            for (int t = 0; t < TT; ++t) bx[t] = scale_bytes(ew + 2048 * RT + 1024 + 16 * (16 * t + lr), xsh[t], in0, in1);
+        }
+        constexpr int XF = XT == MX_X_MXFP4 ? 1 : (XT == MX_X_F32 ? 8 : 4);  // 16-byte pieces per block
+        f32x4 part[RT][TT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) part[r][t] = f32x4{};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            u32x4 fx[TT][XF];
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+#pragma unroll
+                for (int c = 0; c < XF; ++c)
+                    fx[t][c] = *(const u32x4*)(e + X::BYTES * (16 * t + lr) + 16 * ((XF * (2 * q + u) + c) ^ X::swizzle(16 * t + lr)));
+            // W is the first operand: a lane then holds four outputs of one row of y
+            if constexpr (XT == MX_X_MXFP4) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t)
+                        part[r][t] = u ? mfma16_mxfp4<1>(fw[r][1], bw[r], fx[t][0], bx[t], part[r][t])
+                                       : mfma16_mxfp4<0>(fw[r][0], bw[r], fx[t][0], bx[t], part[r][t]);
+            } else {
+                float sc[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) sc[r] = __uint_as_float(((bw[r] >> (8 * u)) & 255u) << 23);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    bf16x8 wf[RT];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) wf[r] = mxfp4_bf16(fw[r][u][c], sc[r]);
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) {
+                        if constexpr (XT == MX_X_F32) {
+                            bf16x8 xf[3];
+                            split3(fx[t][2 * c], fx[t][2 * c + 1], xf);
+#pragma unroll
+                            for (int r = 0; r < RT; ++r)  // small parts first
+                                part[r][t] = mfma16(wf[r], xf[0], mfma16(wf[r], xf[1], mfma16(wf[r], xf[2], part[r][t])));
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < RT; ++r) part[r][t] = mfma16(wf[r], __builtin_bit_cast(bf16x8, fx[t][c]), part[r][t]);
+                        }
+                    }
+                }
+            }
+        }
+        slot = slot + 1 == S ? 0 : slot + 1;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) tot[r][t] += part[r][t];
+    }
+    wait_vmcnt<0>();  // (loads of zeros past the last stage)
+    // tot[r][t][e]: y row m0 + 16 t + l % 16, column n0 + 16 r + 4 (l / 16) + e
+    const int size = p.y_f32 ? 4 : 2;
+    const bool vec = ((uintptr_t)p.y & (4 * size - 1)) == 0 && (p.ldy & 3) == 0;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        const int m = 16 * t + lr;
+        if (m >= toks) continue;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int c = 16 * r + 4 * q;
+            const int64_t o = (int64_t)(m0 + m) * p.ldy + n0 + c;
+            const f32x4 v = tot[r][t];
+            if (vec && c + 4 <= rows) {
+                if (p.y_f32)
+                    *(f32x4*)((float*)p.y + o) = v;
+                else
+                    *(u32x2*)((uint16_t*)p.y + o) = u32x2{pack_bf16x2_hw(v[0], v[1]), pack_bf16x2_hw(v[2], v[3])};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < rows) {
+                        if (p.y_f32)
+                            ((float*)p.y)[o + e] = v[e];
+                        else
+                            ((uint16_t*)p.y)[o + e] = f32_to_bf16_bits(v[e]);
+                    }
+            }
+        }
+    }
+}
+
+template <int XT, int RT, int TT, int S, int NW>
+hipError_t launch_mid(const Mxfp4GemmParams& p, hipStream_t st) {
+    using F = MidShape<XT, RT, TT, S, NW>;
+    constexpr int BM = 16 * TT, BN = 16 * RT * NW;
+    const bool routed = p.offsets != nullptr;
+    const auto kern = routed ? mxfp4_mid_kernel<XT, RT, TT, S, NW, true> : mxfp4_mid_kernel<XT, RT, TT, S, NW, false>;
+    if (F::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)F::LDS);
+        if (e != hipSuccess) return e;
+    }
+    const int64_t tiles = (p.N + BN - 1) / BN, blocks = ((int64_t)p.M + BM - 1) / BM;
+    const int64_t grid = routed ? (mx_tile_bound(p, BM) * tiles + 7) / 8 * 8 : (tiles + 7) / 8 * 8 * blocks;
+    if (grid * 64 * NW >= (1ll << 32)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), F::LDS, st, p, (int)blocks);
+    return hipGetLastError();
+}
+
 template <int XT, int RT, int TT, int XI, int S, int NW>
 hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
     using F = FewShape<XT, RT, TT, XI, S, NW>;
@@ -301,38 +549,105 @@ hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Which kernel and tile.  Both split a call into workgroups of some weight rows
+// x some rows of x; small ones fill the GPU, large ones read less.  In us, one
+// call among others, weights in turn:
+//   matrix, x in bf16: 576 x 7168, 96 tokens, 16 x 16 with 8 waves 7.4, 32 x 16
+//     8.4, mid 128 x 32 over 20; 1536 x 7168, 64 tokens, 32 x 16 with 8 waves
+//     8.5, 4 waves 10.9, 16 x 16 12.3; 128 tokens, 4 waves 12.5, 8 waves 14.7;
+//     7168 x 16384, 64 tokens, 64 x 16 with 4 waves 33, 32 x 16 43, mid 46; 24576
+//     x 1536, 40 tokens, mid 11.5, 64 x 16 17 (19 rows of x each read by 1536
+//     workgroups of 16 rows before)
+//   x in MXFP4, which costs a quarter to read: 7168 x 16384, 64 tokens, 64 x 32
+//     with 8 waves 18.7, 64 x 64 24.4, 32 x 16 28; 128 tokens, 64 x 64 23.8, 64 x
+//     32 31; 24576 x 1536, 40 tokens, mid 64 x 32 8.0, 128 x 32 8.3
+//   experts by their mean rows (128 of 768 x 2048): 6 rows, mid 128 x 16 25.6,
+//     128 x 32 28.1; 19 rows, 36.5 and 32.0; MXFP4, 31 rows, mid 128 x 64 34.4,
+//     128 x 32 37.7; one token, 8 of 128, two rows of x staged 4.8, 16 rows 6.0
+bool few_pairs(const Mxfp4GemmParams& p) { return p.pairs <= 4096 && (int64_t)p.pairs * ((p.N + 15) / 16) < (1 << 23); }
+
+hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+    const int entries = (p.K + 255) / 256;
+    if (p.offsets) {
+        if (p.pairs <= 2 * p.experts && few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4>(p, st);
+        return p.pairs <= 12 * p.experts ? launch_mid<0, 2, 1, 2, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
+    }
+    if (p.M <= 2) {
+        if (entries >= 16) return launch_few<0, 1, 1, 1, 1, 8>(p, st);
+        return entries >= 8 ? launch_few<0, 1, 1, 1, 1, 4>(p, st) : launch_few<0, 1, 1, 1, 1, 2>(p, st);
+    }
+    const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
+    if (n16 * b <= cus) return launch_few<0, 1, 1, 8, 1, 8>(p, st);
+    if (n32 * b <= cus) return launch_few<0, 2, 1, 8, 1, 8>(p, st);
+    if (n32 * b <= 2 * cus) return launch_few<0, 2, 1, 8, 1, 4>(p, st);
+    if (n64 * b <= 2 * cus) return launch_few<0, 4, 1, 8, 1, 4>(p, st);
+    return b == 1 ? launch_mid<0, 2, 1, 2, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
+}
+
+hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+    if (p.offsets) {
+        if (p.pairs <= 2 * p.experts && few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4>(p, st);
+        if (p.pairs <= 8 * p.experts) return launch_mid<2, 2, 1, 2, 4>(p, st);
+        return p.pairs <= 24 * p.experts ? launch_mid<2, 2, 2, 2, 4>(p, st) : launch_mid<2, 2, 4, 2, 4>(p, st);
+    }
+    const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
+    if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 1, 8>(p, st);
+    if (b == 1 && n16 <= 2 * cus) return launch_few<2, 1, 1, 2, 2, 4>(p, st);
+    if (n32 * b <= cus) return launch_few<2, 2, 1, 2, 1, 8>(p, st);
+    if (n64 * ((b + 1) / 2) <= cus) return launch_few<2, 4, 2, 4, 1, 8>(p, st);
+    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 8>(p, st);
+    return b <= 4 ? launch_mid<2, 1, 2, 2, 4>(p, st) : launch_mid<2, 2, 4, 2, 4>(p, st);
+}
+
+// f32: the cuts of x cost more than its bytes, so a cut serves 32 or 64 weight
+// rows (24576 x 1536: one token 16 us with 16 rows; 16 tokens, mid 128 x 16
+// 17.6, 64 x 16 21.4; 1536 x 7168, 64 tokens, 32 x 16 with 4 waves 23, mid 66)
+hipError_t launch_few_f32(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+    if (!p.offsets && p.M == 1) return launch_few<1, 4, 1, 1, 1, 4>(p, st);
+    if (!p.offsets && p.K > 4096 && (int64_t)((p.N + 31) / 32) * ((p.M + 15) / 16) <= 2 * cus) return launch_few<1, 2, 1, 16, 1, 4>(p, st);
+    return launch_mid<1, 2, 1, 2, 4>(p, st);
+}
+
+hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+    if (p.x_kind == MX_X_MXFP4) return launch_few_mxfp4(p, cus, st);
+    return p.x_kind == MX_X_F32 ? launch_few_f32(p, cus, st) : launch_few_bf16(p, cus, st);
+}
+
+// Rows per large tile (mxfp4_gemm.hip), or 0.  They pay once they cover the
+// GPU for the larger part: bf16, 24576 x 1536, 192 tokens (192 tiles of 128) 23.8
+// us, few rows 26.5, 128 tokens 22.2 and 18.3; 7168 x 16384, 400 tokens (112) 173
+// and 135.  MXFP4 at 112 tiles 62 and 63.  Tiles of 256 rows likewise (24576 x
+// 1536, 400 tokens: 39.8, of 128 45.5; 256 tokens: 36.5 and 24.6).  Experts by
+// their mean rows: bf16 100 rows 91 us, few rows 85; MXFP4 50 rows 38 and 42, 31
+// rows 36 and 34.
+int tile_rows(const Mxfp4GemmParams& p, int cus) {
+    if (p.x_kind == MX_X_F32) return 0;
+    const bool mx = p.x_kind == MX_X_MXFP4;
+    const int64_t n = (p.N + 255) / 256;
+    if (p.offsets) {
+        const int64_t rows = p.pairs / p.experts;
+        return rows < (mx ? 40 : 128) ? 0 : 128;
+    }
+    if (n * (((int64_t)p.M + 255) / 256) * 8 >= 5 * cus) return 256;
+    return n * (((int64_t)p.M + 127) / 128) * 8 >= (mx ? 3 : 5) * cus ? 128 : 0;
+}
+
 }  // namespace
 
-hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, hipStream_t st) {
-    // rows of x that one workgroup takes: all, or for experts about the mean
-    const int m = p.offsets ? (p.pairs + p.experts - 1) / p.experts : p.M;
-    if (p.x_kind == MX_X_MXFP4) return m <= 16 ? launch_few<2, 2, 1, 2, 2, 8>(p, st) : launch_few<2, 2, 4, 8, 1, 8>(p, st);
-    if (p.x_kind == MX_X_F32) return m <= 16 ? launch_few<1, 2, 1, 16, 1, 4>(p, st) : launch_few<1, 2, 2, 32, 1, 4>(p, st);
-    if (m <= 2 && (!p.offsets || p.pairs <= 4096)) return launch_few<0, 2, 1, 1, 3, 8>(p, st);
-    return m <= 16 ? launch_few<0, 2, 1, 8, 1, 8>(p, st) : launch_few<0, 2, 4, 32, 1, 4>(p, st);
-}
-
-// as many workgroups as a routed call can need in a grid of less than 2^32
-// threads
+// as many workgroups as a routed call can need (of 256 threads, 16 rows of x and
+// 128 weight rows, or as many threads on fewer rows of few pairs) in a grid of
+// less than 2^32 threads
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
-    return !p.offsets || (mx_tile_bound(p, 16) * ((p.N + 31) / 32) + 7) * 512 < (1ll << 32);
+    return !p.offsets || (mx_tile_bound(p, 16) * ((p.N + 127) / 128) + 7) * 256 < (1ll << 32);
 }
 
-// Rows per large tile (0: the kernel for few rows).
-static int tile_rows(const Mxfp4GemmParams& p, int cu_count) {
-    if (p.x_kind == MX_X_F32) return 0;
-    const int64_t m = p.offsets ? (p.pairs + p.experts - 1) / p.experts : p.M;
-    if (m < 64) return 0;
-    const int64_t n_tiles = (p.N + 255) / 256, m_tiles = (m + 255) / 256 * (p.offsets ? p.experts : 1);
-    return m > 128 && n_tiles * m_tiles >= cu_count ? 256 : 128;
-}
-
-// A matrix's tokens in as many launches as grids of less than 2^32 threads
-// take (one, up to 2^23 workgroups of 16 tokens x 32 weight rows).
+// A matrix's tokens in as many launches as grids of less than 2^32 threads take:
+// one, up to 2^23 workgroups of 16 tokens x 16 weight rows (MXFP4_MAX_OUT weight
+// rows leave 256 tokens each).
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st) {
     const int tm = tile_rows(p, cu_count);
-    if (p.offsets) return tm ? launch_mxfp4_tiles(p, tm, st) : launch_mxfp4_few(p, st);
-    const int64_t most = (((int64_t)1 << 23) / ((p.N + 31) / 32 + 7) - 1) * 16 / 256 * 256;
+    if (p.offsets) return tm ? launch_mxfp4_tiles(p, tm, st) : launch_mxfp4_few(p, cu_count, st);
+    const int64_t most = ((int64_t)1 << 23) / ((p.N + 15) / 16 + 8) * 16 / 256 * 256;
     for (int64_t m = 0; m < p.M; m += most) {
         Mxfp4GemmParams q = p;
         q.M = (int)std::min<int64_t>(most, p.M - m);
@@ -340,7 +655,7 @@ hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t
         q.x = (const char*)p.x + m * row;
         if (p.x_scales) q.x_scales = p.x_scales + m * (p.K / 32);
         q.y = (char*)p.y + m * p.ldy * (p.y_f32 ? 4 : 2);
-        const hipError_t e = tm ? launch_mxfp4_tiles(q, tm, st) : launch_mxfp4_few(q, st);
+        const hipError_t e = tm ? launch_mxfp4_tiles(q, tm, st) : launch_mxfp4_few(q, cu_count, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
         t = min(t, AT - 1);
         const uint32_t ch = ch8 ^ (4 * (q & 1));
         const bool past = RAGGED && (MX ? 256u * t + 32u * ch : 64u * t + 8u * ch) >= K;
-        dma16_buf(xres, past ? PAST : ao[q] + 128u * t, st + 1024 * (DA * w + q));
+        mx_dma16(xres, past ? PAST : ao[q] + 128u * t, st + 1024 * (DA * w + q));
     };
     // instruction q of W's piece t (MXFP4: stage t)
     const int BT = MX ? AT : AT / 2;
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
         t = min(t, BT - 1);
         const uint32_t ch = MX ? ch8 ^ (4 * (q & 1)) : ch4;
         const bool past = RAGGED && (MX ? 256u : 128u) * t + 32u * ch >= K;
-        dma16_buf(wres, past ? PAST : bo[q] + (MX ? 128u : 64u) * t, st + 1024 * (DB * w + q));
+        mx_dma16(wres, past ? PAST : bo[q] + (MX ? 128u : 64u) * t, st + 1024 * (DB * w + q));
     };
     // instruction q of scale group t (of 512 or 128 k)
     const int ST = (p.K + (MX ? 511 : 127)) / (MX ? 512 : 128);
@@ -181,11 +181,11 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
         t = min(t, ST - 1);
         if constexpr (MX) {
             if (q < 2)
-                dma16_buf(sres[q], so[q] + 16u * t, st + 2048 * w + 1024 * q);
+                mx_dma16(sres[q], so[q] + 16u * t, st + 2048 * w + 1024 * q);
             else
-                dma4_buf(sres[q - 2], so[q - 2] + 16u * t + 16u, st + 16 * S::SROWS + 512 * w + 256 * (q - 2));
+                mx_dma4(sres[q - 2], so[q - 2] + 16u * t + 16u, st + 16 * S::SROWS + 512 * w + 256 * (q - 2));
         } else {
-            dma4_buf(sres[0], so[0] + 4u * t + 4u * q, st + 1024 * q + 256 * w);
+            mx_dma4(sres[0], so[0] + 4u * t + 4u * q, st + 1024 * q + 256 * w);
         }
     };
 

@@ -79,6 +79,29 @@ def test_whole_numbers_are_exact(M, out, inp, kind):
         assert torch.equal(yb, y.bfloat16())
 
 
+# token and output counts on both sides of every change of kernel or tile (a few
+# outputs to most of the GPU's workgroups, one token to tiles of 256), K with and
+# without a remainder
+WIDE = [(1, 300, 544), (2, 300, 4128), (20, 300, 288), (10, 4104, 288), (40, 2056, 544), (100, 2056, 160), (100, 4000, 288),
+        (100, 4104, 256), (40, 16392, 96), (10, 33000, 96), (100, 8200, 2080), (20, 300, 4128), (100, 16392, 288),
+        (200, 16392, 288), (300, 16392, 512), (600, 16392, 256), (600, 16385, 288), (700, 16390, 32), (1100, 8190, 416)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens,out,inp", WIDE)
+def test_whole_numbers_are_exact_in_every_kernel(M, tokens, out, inp, kind):
+    import torch
+
+    rng = np.random.default_rng(tokens + out)
+    w, w64 = weights(M, rng, out, inp, lo=126, hi=129)
+    x, x64 = whole(rng, kind, tokens, inp)
+    want = (x64.astype(np.float32) @ w64.astype(np.float32).T).astype(np.float64)  # exact: see above
+    assert np.abs(want).max() < 2 ** 21
+    y = M.mxfp4_mm(operand(M, x), w, out_dtype=torch.float32)
+    assert np.array_equal(X.host(y), want), np.abs(X.host(y) - want).max()
+    assert torch.equal(M.mxfp4_mm(operand(M, x), w, out_dtype=torch.bfloat16), y.bfloat16())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("tokens,out,inp", [(1, 1536, 7168), (13, 576, 7168), (37, 1536, 1536), (200, 768, 2048),
                                             (1000, 512, 512), (300, 2048, 7168)])
@@ -226,7 +249,8 @@ def test_offsets_past_32_bits(M):
 
 
 EXPERTS = [(1, 1, 1, 7, 32), (1, 8, 128, 96, 256), (5, 2, 3, 33, 96), (40, 3, 9, 160, 160), (200, 8, 32, 264, 512),
-           (700, 4, 5, 512, 288), (64, 6, 257, 48, 64), (1500, 2, 4, 300, 1024)]
+           (700, 4, 5, 512, 288), (64, 6, 257, 48, 64), (1500, 2, 4, 300, 1024), (40, 4, 40, 136, 544), (90, 8, 60, 520, 288),
+           (260, 8, 60, 264, 96)]
 
 
 @pytest.mark.parametrize("ids", ["spread", "hot", "one", "dropped", "none", "twice"])
