@@ -360,7 +360,7 @@ mr_status mr_mxfp4_matmul_quantized(const mr_mxfp4_matrix *x, const mr_mxfp4_mat
  *   pair_of_row [tokens * per_token]: the row's pair; -1 past the last row
  *   row_of_pair [tokens * per_token]: the pair's row; -1 for none
  * experts is at most 4096, tokens * per_token at most 2^24.  Workspace:
- * mr_expert_sort_workspace_size (0 up to 4096 pairs).  The result does not
+ * mr_expert_sort_workspace_size (0 up to 2048 pairs).  The result does not
  * depend on timing.
  * ------------------------------------------------------------------------ */
 size_t mr_expert_sort_workspace_size(int32_t tokens, int32_t per_token, int32_t experts);

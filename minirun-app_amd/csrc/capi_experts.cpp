@@ -32,8 +32,8 @@ mr_status check_rows(int32_t tokens, int32_t per_token, int64_t dim, mr_dtype dt
         return fail(MR_INVALID_SHAPE, "%s: %d tokens of %d experts (at most 2^24 pairs)", what, tokens, per_token);
     if (dim <= 0 || dim > (1 << 24)) return fail(MR_INVALID_SHAPE, "%s: rows of %lld values", what, (long long)dim);
     if (!act(dtype)) return fail(MR_INVALID_DTYPE, "%s: rows must be bf16 or f32, got %s", what, mrc::dtype_name(dtype));
-    // workgroups of at least 64 threads in a grid of less than 2^32
-    if (double(tokens) * (double(dim) / 8 + 256) >= 4294967296.0)
+    // a thread per 8 or 16 values, in whole waves, in a grid of less than 2^32
+    if (double(tokens) * (double(dim) / 8 + 1024) >= 4294967296.0)
         return fail(MR_INVALID_SHAPE, "%s: %d tokens of %lld values are more than one launch takes", what, tokens,
                     (long long)dim);
     return MR_OK;
@@ -260,7 +260,7 @@ mr_status mr_expert_dispatch(const void* x, mr_dtype dtype, int32_t tokens, int6
     p.n_tokens = tokens;
     p.per_token = per_token;
     p.row_of_pair = row_of_pair;
-    return done(mr::launch_expert_dispatch(p, (hipStream_t)stream), "expert dispatch launch");
+    return done(mr::launch_expert_dispatch(p, mrc::cu_count(), (hipStream_t)stream), "expert dispatch launch");
 }
 
 mr_status mr_expert_combine(const void* rows, mr_dtype dtype, int64_t rows_stride, int64_t dim,
@@ -285,7 +285,7 @@ mr_status mr_expert_combine(const void* rows, mr_dtype dtype, int64_t rows_strid
     p.per_token = per_token;
     p.row_of_pair = row_of_pair;
     p.weights = weights;
-    return done(mr::launch_expert_combine(p, (hipStream_t)stream), "expert combine launch");
+    return done(mr::launch_expert_combine(p, mrc::cu_count(), (hipStream_t)stream), "expert combine launch");
 }
 
 mr_status mr_expert_combine_backward(const void* d_out, mr_dtype dtype, int64_t d_out_stride, int64_t dim,
@@ -316,7 +316,7 @@ mr_status mr_expert_combine_backward(const void* d_out, mr_dtype dtype, int64_t 
     p.row_of_pair = row_of_pair;
     p.weights = weights;
     p.d_weights = d_weights;
-    return done(mr::launch_expert_combine_backward(p, (hipStream_t)stream), "expert combine backward launch");
+    return done(mr::launch_expert_combine_backward(p, mrc::cu_count(), (hipStream_t)stream), "expert combine backward launch");
 }
 
 }  // extern "C"

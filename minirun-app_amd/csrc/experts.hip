@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(ES_THREADS) expert_count_kernel(ExpertSortPara
     for (int e = threadIdx.x; e < p.experts; e += ES_THREADS) out[e] = bins[e];
 }
 
-// One workgroup places 4096 pairs.  LDS: cursor[wave][expert], at first the
+// One workgroup places 2048 pairs (4096: 2 us more at 32768 pairs).  LDS: cursor[wave][expert], at first the
 // wave's count of the expert, then the row that the wave's next pair of it
 // gets: the expert's first row, plus its pairs in earlier workgroups, plus
 // those in earlier waves.  A wave then takes its pairs in order, 64 at a time;
@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(ES_THREADS) expert_count_kernel(ExpertSortPara
 __global__ void __launch_bounds__(ES_THREADS) expert_place_kernel(ExpertSortParams p) {
     extern __shared__ int32_t cursor[];
     __shared__ int32_t sums[ES_WAVES];
+    __shared__ int32_t group_sums[2][ES_THREADS];
     const int tid = threadIdx.x, l = tid & 63, E = p.experts;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int blocks = gridDim.x, first = blockIdx.x * EXPERT_SORT_PAIRS;
@@ -82,17 +83,30 @@ __global__ void __launch_bounds__(ES_THREADS) expert_place_kernel(ExpertSortPara
     for (int e0 = 0; e0 < E; e0 += ES_THREADS) {
         const int e = e0 + tid;
         int before = 0, total = 0;  // of the expert: in earlier workgroups, in all
-        if (e < E) {
-            if (blocks == 1) {
+        if (blocks == 1) {
+            if (e < E) {
 #pragma unroll
                 for (int k = 0; k < ES_WAVES; ++k) total += cursor[k * E + e];
-            } else {
+            }
+        } else {
+            // `groups` threads per expert share the workgroups' counts
+            const int left = min(E - e0, ES_THREADS), groups = ES_THREADS / left;
+            const int g = tid / left, own = e0 + tid - g * left;
+            if (g < groups) {
 #pragma unroll 8
-                for (int b = 0; b < blocks; ++b) {
-                    const int c = p.counts[(int64_t)b * E + e];
+                for (int b = g; b < blocks; b += groups) {
+                    const int c = p.counts[(int64_t)b * E + own];
                     total += c;
                     before += b < (int)blockIdx.x ? c : 0;
                 }
+            }
+            group_sums[0][tid] = total;
+            group_sums[1][tid] = before;
+            __syncthreads();
+            total = before = 0;
+            for (int k = 0; e < E && k < groups; ++k) {
+                total += group_sums[0][k * left + tid];
+                before += group_sums[1][k * left + tid];
             }
         }
         const int incl = (int)wave_scan_incl((uint32_t)total);
@@ -149,49 +163,60 @@ __global__ void __launch_bounds__(ES_THREADS) expert_place_kernel(ExpertSortPara
 }
 
 // ---------------------------------------------------------------- rows
-// Eight values of a row per thread: VEC, 8 next to each other (16 or 32
-// bytes, rows 16-byte aligned); otherwise 8 at a distance of the workgroup's
-// threads, so that a wave still reads whole lines.
+// Eight values of a row as stored: VEC, 8 next to each other (16 or 32 bytes,
+// rows 16-byte aligned); otherwise 8 at a distance of the workgroup's threads,
+// so that a wave still reads whole lines.
 template <bool F32, bool VEC>
 struct Eight {
-    float v[8];
-    __device__ __forceinline__ void load(const void* p, int64_t c, int step, int64_t dim) {
-        if constexpr (VEC) {
-            if constexpr (F32) {
-                const f32x4 a = *(const f32x4*)((const float*)p + c), b = *(const f32x4*)((const float*)p + c + 4);
+    using Elem = std::conditional_t<F32, uint32_t, uint16_t>;
+    static constexpr int N16 = F32 ? 2 : 1;
+    std::conditional_t<VEC, u32x4[N16], Elem[8]> v;
+    __device__ __forceinline__ void load(const void* row, int64_t c, int64_t dim) {
+        const Elem* p = (const Elem*)row + c;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
-            } else {
-                const u32x4 a = *(const u32x4*)((const uint16_t*)p + c);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[2 * k] = __uint_as_float(a[k] << 16), v[2 * k + 1] = __uint_as_float(a[k] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t i = c + (int64_t)k * step;
-                v[k] = i >= dim ? 0.f : (F32 ? ((const float*)p)[i] : bf16_bits_to_f32(((const uint16_t*)p)[i]));
-            }
+        for (int k = 0; k < (VEC ? N16 : 8); ++k) {
+            if constexpr (VEC)
+                v[k] = ((const u32x4*)p)[k];
+            else
+                v[k] = c + (int64_t)k * blockDim.x < dim ? p[(int64_t)k * blockDim.x] : (Elem)0;
         }
     }
-    __device__ __forceinline__ void store(void* p, int64_t c, int step, int64_t dim) const {
-        if constexpr (VEC) {
-            if constexpr (F32) {
-                *(f32x4*)((float*)p + c) = f32x4{v[0], v[1], v[2], v[3]};
-                *(f32x4*)((float*)p + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
-            } else {
-                *(u32x4*)((uint16_t*)p + c) = u32x4{pack_bf16x2_hw(v[0], v[1]), pack_bf16x2_hw(v[2], v[3]),
-                                                    pack_bf16x2_hw(v[4], v[5]), pack_bf16x2_hw(v[6], v[7])};
-            }
-        } else {
+    __device__ __forceinline__ void store(void* row, int64_t c, int64_t dim) const {
+        Elem* p = (Elem*)row + c;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t i = c + (int64_t)k * step;
-                if (i < dim) {
-                    if (F32)
-                        ((float*)p)[i] = v[k];
-                    else
-                        ((uint16_t*)p)[i] = f32_to_bf16_bits(v[k]);
+        for (int k = 0; k < (VEC ? N16 : 8); ++k) {
+            if constexpr (VEC)
+                ((u32x4*)p)[k] = v[k];
+            else if (c + (int64_t)k * blockDim.x < dim)
+                p[(int64_t)k * blockDim.x] = v[k];
+        }
+    }
+    __device__ __forceinline__ float get(int k) const {
+        if constexpr (VEC) {
+            if constexpr (F32) return __uint_as_float(v[k >> 2][k & 3]);
+            return __uint_as_float(k & 1 ? v[0][k >> 1] & 0xffff0000u : v[0][k >> 1] << 16);
+        } else {
+            return F32 ? __uint_as_float(v[k]) : __uint_as_float((uint32_t)v[k] << 16);
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+            if constexpr (F32) {
+                if constexpr (VEC) {
+                    v[k >> 2][k & 3] = __float_as_uint(f[k]);
+                    v[k >> 2][(k & 3) + 1] = __float_as_uint(f[k + 1]);
+                } else {
+                    v[k] = __float_as_uint(f[k]);
+                    v[k + 1] = __float_as_uint(f[k + 1]);
+                }
+            } else {
+                const uint32_t two = pack_bf16x2_hw(f[k], f[k + 1]);
+                if constexpr (VEC) {
+                    v[0][k >> 1] = two;
+                } else {
+                    v[k] = (uint16_t)two;
+                    v[k + 1] = (uint16_t)(two >> 16);
                 }
             }
         }
@@ -199,188 +224,254 @@ struct Eight {
 };
 
 template <bool F32>
-__device__ __forceinline__ const char* row_at(const void* p, int64_t row, int64_t ld) {
-    return (const char*)p + row * ld * (F32 ? 4 : 2);
+__device__ __forceinline__ char* row_at(const void* p, int64_t row, int64_t ld) {
+    return (char*)p + row * ld * (F32 ? 4 : 2);
 }
 
-// the first value of this thread's eight in span `s` of 8 blockDim.x values
+// the first value of this thread's piece `i` of a row (of 8 blockDim.x values)
 template <bool VEC>
-__device__ __forceinline__ int64_t span_col(int64_t s) {
-    return 8 * s * blockDim.x + (VEC ? 8 : 1) * (int64_t)threadIdx.x;
+__device__ __forceinline__ int64_t piece_col(int64_t i) {
+    return 8 * i * blockDim.x + (VEC ? 8 : 1) * (int64_t)threadIdx.x;
 }
 
-// row of pair i, -1 for none (and for what no sort writes)
-__device__ __forceinline__ int pair_row(const ExpertRowsParams& p, int64_t i) {
-    const int r = p.row_of_pair[i];
-    return (int64_t)(uint32_t)r < (int64_t)p.n_tokens * p.per_token ? r : -1;
-}
-
-// One workgroup per token and span: the token's piece is read once and stored
-// per_token times, bit for bit.
-template <bool F32, bool VEC>
-__global__ void __launch_bounds__(256) expert_dispatch_kernel(ExpertRowsParams p, int spans) {
-    using Elem = std::conditional_t<F32, uint32_t, uint16_t>;
-    const int64_t t = blockIdx.x / (unsigned)spans;
-    const int64_t c = span_col<VEC>(blockIdx.x - t * spans);
-    if (c >= p.dim) return;
-    const Elem* x = (const Elem*)row_at<F32>(p.tokens, t, p.ld_tokens) + c;
-    const int n = VEC ? 8 : (int)std::min<int64_t>(8, (p.dim - c + blockDim.x - 1) / blockDim.x);
-    u32x4 v[F32 ? 2 : 1];
-    Elem e[8];
-    if constexpr (VEC) {
-#pragma unroll
-        for (int k = 0; k < (F32 ? 2 : 1); ++k) v[k] = ((const u32x4*)x)[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < n) e[k] = x[(int64_t)k * blockDim.x];
+// The rows of a token's slots j0 .. j0 + 63: lane j has that of slot j0 + j
+// (-1: none, and for what no sort writes), and its weight.  `has`: the slots
+// that have one.  Batches of rows are read off with readlane, so that their
+// addresses and the branches round them are scalar.
+struct Slots {
+    int row;
+    float weight;
+    uint64_t has;
+    __device__ __forceinline__ void load(const ExpertRowsParams& p, int64_t t, int j0) {
+        const int j = j0 + (threadIdx.x & 63);
+        const int64_t i = t * p.per_token + j;
+        row = -1;
+        weight = 1.f;
+        if (j < p.per_token) {
+            row = p.row_of_pair[i];
+            if ((int64_t)(uint32_t)row >= (int64_t)p.n_tokens * p.per_token) row = -1;
+            if (p.weights) weight = p.weights[i];
+        }
+        has = __ballot(row >= 0);
     }
-    for (int j = 0; j < p.per_token; ++j) {
-        const int r = pair_row(p, t * p.per_token + j);
-        if (r < 0) continue;
-        Elem* y = (Elem*)row_at<F32>(p.out, r, p.ld_out) + c;
-        if constexpr (VEC) {
+    __device__ __forceinline__ int row_of(int j) const { return __builtin_amdgcn_readlane(row, j); }
+    __device__ __forceinline__ float weight_of(int j) const {
+        return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j));
+    }
+};
+
+// One workgroup per token and span of a row: the piece is read once and stored
+// once per slot that has a row, bit for bit.  Bound by its stores (4096 tokens of
+// 7168, 4 rows each: 294 MB in 50 us).
+template <bool F32, bool VEC, int U>
+__global__ void __launch_bounds__(512) expert_dispatch_kernel(ExpertRowsParams p, int spans) {
+    const int64_t t = blockIdx.x / (unsigned)spans, s = blockIdx.x - t * spans;
+    Eight<F32, VEC> x[U];
 #pragma unroll
-            for (int k = 0; k < (F32 ? 2 : 1); ++k) ((u32x4*)y)[k] = v[k];
-        } else {
+    for (int u = 0; u < U; ++u) {
+        const int64_t c = piece_col<VEC>(s * U + u);
+        if (c < p.dim) x[u].load(row_at<F32>(p.tokens, t, p.ld_tokens), c, p.dim);
+    }
+    for (int j0 = 0; j0 < p.per_token; j0 += 64) {
+        Slots sl;
+        sl.load(p, t, j0);
+        for (uint64_t m = sl.has; m; m &= m - 1) {
+            char* row = row_at<F32>(p.out, sl.row_of(__builtin_ctzll(m)), p.ld_out);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k < n) y[(int64_t)k * blockDim.x] = e[k];
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = piece_col<VEC>(s * U + u);
+                if (c < p.dim) x[u].store(row, c, p.dim);
+            }
         }
     }
 }
 
-constexpr int EC_U = 8;  // slots whose rows are in flight together
+constexpr int EC_ROWS = 8;  // rows of a token in flight together
 
 // One workgroup per token and span; sums in f32, in slot order.
-template <bool F32, bool VEC>
-__global__ void __launch_bounds__(256) expert_combine_kernel(ExpertRowsParams p, int spans) {
-    const int64_t t = blockIdx.x / (unsigned)spans;
-    const int64_t c = span_col<VEC>(blockIdx.x - t * spans);
-    if (c >= p.dim) return;
-    Eight<F32, VEC> sum;
+template <bool F32, bool VEC, int U>
+__global__ void __launch_bounds__(512) expert_combine_kernel(ExpertRowsParams p, int spans) {
+    const int64_t t = blockIdx.x / (unsigned)spans, s = blockIdx.x - t * spans;
+    float sum[U][8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum.v[k] = 0.f;
-    for (int j0 = 0; j0 < p.per_token; j0 += EC_U) {
-        Eight<F32, VEC> y[EC_U];
-        int r[EC_U];
-        float w[EC_U];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < EC_U; ++j) {
-            const int64_t i = t * p.per_token + j0 + j;
-            r[j] = j0 + j < p.per_token ? pair_row(p, i) : -1;
-            w[j] = r[j] >= 0 && p.weights ? p.weights[i] : 1.f;
-        }
+        for (int k = 0; k < 8; ++k) sum[u][k] = 0.f;
+    for (int j0 = 0; j0 < p.per_token; j0 += 64) {
+        Slots sl;
+        sl.load(p, t, j0);
+        uint64_t m = sl.has;
+        while (m) {
+            Eight<F32, VEC> y[EC_ROWS][U];
+            float w[EC_ROWS];
+            const int n = min(__popcll(m), EC_ROWS);
 #pragma unroll
-        for (int j = 0; j < EC_U; ++j)
-            if (r[j] >= 0) y[j].load(row_at<F32>(p.rows, r[j], p.ld_rows), c, blockDim.x, p.dim);
+            for (int b = 0; b < EC_ROWS; ++b) {
+                if (b >= n) continue;
+                const int j = __builtin_ctzll(m);
+                m &= m - 1;
+                w[b] = sl.weight_of(j);
+                const char* row = row_at<F32>(p.rows, sl.row_of(j), p.ld_rows);
 #pragma unroll
-        for (int j = 0; j < EC_U; ++j)
-            if (r[j] >= 0) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum.v[k] = fmaf(w[j], y[j].v[k], sum.v[k]);
+                for (int u = 0; u < U; ++u) {
+                    const int64_t c = piece_col<VEC>(s * U + u);
+                    if (c < p.dim) y[b][u].load(row, c, p.dim);
+                }
             }
+#pragma unroll
+            for (int b = 0; b < EC_ROWS; ++b) {
+                if (b >= n) continue;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum[u][k] = fmaf(w[b], y[b][u].get(k), sum[u][k]);
+            }
+        }
     }
-    sum.store((char*)row_at<F32>(p.out, t, p.ld_out), c, blockDim.x, p.dim);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t c = piece_col<VEC>(s * U + u);
+        Eight<F32, VEC> o;
+        o.set(sum[u]);
+        if (c < p.dim) o.store(row_at<F32>(p.out, t, p.ld_out), c, p.dim);
+    }
 }
 
-// One workgroup per token, all spans: d_out[t] is read once per EC_U slots,
-// each slot's row once, each d_row written once; the dot products are summed
-// per thread over the spans, then over the workgroup in a fixed order.
-template <bool F32, bool VEC>
-__global__ void __launch_bounds__(256) expert_combine_backward_kernel(ExpertRowsParams p, int spans) {
-    __shared__ float part[4][EC_U];
+// One workgroup per token, all spans: d_out[t] is read once per batch of rows,
+// each row once, each d_row written once; the dot products are summed per thread
+// over the spans, then over the workgroup in a fixed order.
+template <bool F32, bool VEC, int U>
+__global__ void __launch_bounds__(512) expert_combine_backward_kernel(ExpertRowsParams p, int spans) {
+    __shared__ float part[8][EC_ROWS];
     const int64_t t = blockIdx.x;
-    const int tid = threadIdx.x, w = tid >> 6, waves = blockDim.x >> 6;
-    for (int j0 = 0; j0 < p.per_token; j0 += EC_U) {
-        int r[EC_U];
-        float wt[EC_U], dot[EC_U];
+    const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, waves = blockDim.x >> 6;
+    for (int j0 = 0; j0 < p.per_token; j0 += 64) {
+        Slots sl;
+        sl.load(p, t, j0);
+        if (p.d_weights && w == 0 && j0 + l < p.per_token && sl.row < 0) p.d_weights[t * p.per_token + j0 + l] = 0.f;
+        uint64_t m = sl.has;
+        while (m) {
+            const int n = min(__popcll(m), EC_ROWS);
+            float wt[EC_ROWS], dot[EC_ROWS];
+            int r[EC_ROWS], slot[EC_ROWS];
 #pragma unroll
-        for (int j = 0; j < EC_U; ++j) {
-            const int64_t i = t * p.per_token + j0 + j;
-            r[j] = j0 + j < p.per_token ? pair_row(p, i) : -1;
-            wt[j] = r[j] >= 0 && p.weights ? p.weights[i] : 1.f;
-            dot[j] = 0.f;
-        }
-        for (int s = 0; s < spans; ++s) {
-            const int64_t c = span_col<VEC>(s);
-            if (c >= p.dim) break;
-            Eight<F32, VEC> g, y[EC_U];
-            g.load(row_at<F32>(p.tokens, t, p.ld_tokens), c, blockDim.x, p.dim);
+            for (int b = 0; b < EC_ROWS; ++b) {
+                dot[b] = 0.f;
+                wt[b] = 0.f;
+                r[b] = slot[b] = 0;
+                if (b >= n) continue;
+                slot[b] = __builtin_ctzll(m);
+                m &= m - 1;
+                r[b] = sl.row_of(slot[b]);
+                wt[b] = sl.weight_of(slot[b]);
+            }
+            for (int s = 0; s < spans; ++s) {
+                Eight<F32, VEC> g[U], y[EC_ROWS][U];
+                int64_t c[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    c[u] = piece_col<VEC>((int64_t)s * U + u);
+                    if (c[u] < p.dim) g[u].load(row_at<F32>(p.tokens, t, p.ld_tokens), c[u], p.dim);
+                }
+                if (p.d_weights) {
+#pragma unroll
+                    for (int b = 0; b < EC_ROWS; ++b) {
+                        if (b >= n) continue;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (c[u] < p.dim) y[b][u].load(row_at<F32>(p.rows, r[b], p.ld_rows), c[u], p.dim);
+                    }
+                }
+                if (p.out) {
+#pragma unroll
+                    for (int b = 0; b < EC_ROWS; ++b) {
+                        if (b >= n) continue;
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            float d[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) d[k] = wt[b] * g[u].get(k);
+                            Eight<F32, VEC> o;
+                            o.set(d);
+                            if (c[u] < p.dim) o.store(row_at<F32>(p.out, r[b], p.ld_out), c[u], p.dim);
+                        }
+                    }
+                }
+                if (p.d_weights) {
+#pragma unroll
+                    for (int b = 0; b < EC_ROWS; ++b) {
+                        if (b >= n) continue;
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            if (c[u] >= p.dim) continue;
+                            float d = 0.f;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) d = fmaf(g[u].get(k), y[b][u].get(k), d);
+                            dot[b] += d;
+                        }
+                    }
+                }
+            }
             if (p.d_weights) {
 #pragma unroll
-                for (int j = 0; j < EC_U; ++j)
-                    if (r[j] >= 0) y[j].load(row_at<F32>(p.rows, r[j], p.ld_rows), c, blockDim.x, p.dim);
+                for (int b = 0; b < EC_ROWS; ++b) dot[b] = wave_sum(dot[b]);
+                if (l == 0) {
 #pragma unroll
-                for (int j = 0; j < EC_U; ++j)
-                    if (r[j] >= 0) {
+                    for (int b = 0; b < EC_ROWS; ++b) part[w][b] = dot[b];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int b = 0; b < EC_ROWS; ++b)
+                    if (tid == b && b < n) {
                         float d = 0.f;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) d = fmaf(g.v[k], y[j].v[k], d);
-                        dot[j] += d;
+                        for (int k = 0; k < waves; ++k) d += part[k][b];
+                        p.d_weights[t * p.per_token + j0 + slot[b]] = d;
                     }
+                __syncthreads();  // the parts are read before they are written again
             }
-            if (p.out) {
-#pragma unroll
-                for (int j = 0; j < EC_U; ++j)
-                    if (r[j] >= 0) {
-                        Eight<F32, VEC> d;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) d.v[k] = wt[j] * g.v[k];
-                        d.store((char*)row_at<F32>(p.out, r[j], p.ld_out), c, blockDim.x, p.dim);
-                    }
-            }
-        }
-        if (p.d_weights) {
-#pragma unroll
-            for (int j = 0; j < EC_U; ++j) dot[j] = wave_sum(dot[j]);
-            if ((tid & 63) == 0) {
-#pragma unroll
-                for (int j = 0; j < EC_U; ++j) part[w][j] = dot[j];
-            }
-            __syncthreads();
-            if (tid < EC_U && j0 + tid < p.per_token) {
-                float d = 0.f;
-                for (int k = 0; k < waves; ++k) d += part[k][tid];
-                p.d_weights[t * p.per_token + j0 + tid] = d;
-            }
-            __syncthreads();  // the parts are read before they are written again
         }
     }
 }
 
-// threads of a workgroup: eight values each, no more waves than the row has
-// work for
-int row_threads(int64_t dim) { return (int)std::min<int64_t>(256, (dim + 511) / 512 * 64); }
+bool row_aligned(const void* p, int64_t ld, int size) { return !p || (((uintptr_t)p & 15) == 0 && ld * size % 16 == 0); }
 
-bool row_aligned(const void* p, int64_t ld, int64_t rows, int size) {
-    return !p || (((uintptr_t)p & 15) == 0 && (rows == 1 || ld * size % 16 == 0));
-}
-
-template <typename L>
-hipError_t row_launch(const ExpertRowsParams& p, bool per_span, L launch) {
-    const int size = p.f32 ? 4 : 2, threads = row_threads(p.dim);
-    const bool vec = p.dim % 8 == 0 && row_aligned(p.tokens, p.ld_tokens, 2, size) &&
-                     row_aligned(p.rows, p.ld_rows, 2, size) && row_aligned(p.out, p.ld_out, 2, size);
-    const int64_t spans = (p.dim + 8 * threads - 1) / (8 * threads), grid = p.n_tokens * (per_span ? spans : 1);
-    if (grid * threads >= (1ll << 32)) return hipErrorInvalidValue;
-    launch(vec, dim3((unsigned)grid), dim3((unsigned)threads), (int)spans);
-    return hipGetLastError();
+// Threads of a workgroup and pieces of 8 values per thread (U): two pieces and
+// up to 512 threads, so that most rows are one workgroup's; where there are few
+// tokens, one piece and a wave each, to have the work on many CUs (per_span)
+struct RowLaunch {
+    bool vec, two;
+    int threads, spans;
+};
+RowLaunch row_launch(const ExpertRowsParams& p, bool per_span, int cus) {
+    const int size = p.f32 ? 4 : 2;
+    RowLaunch r;
+    r.vec = p.dim % 8 == 0 && row_aligned(p.tokens, p.ld_tokens, size) && row_aligned(p.rows, p.ld_rows, size) &&
+            row_aligned(p.out, p.ld_out, size);
+    const int64_t pieces = (p.dim + 7) / 8;
+    const bool few = per_span && p.n_tokens < cus;
+    r.two = !few && pieces > 64;
+    const int u = r.two ? 2 : 1;
+    r.threads = few ? 64 : (int)std::min<int64_t>(512, (pieces + 64 * u - 1) / (64 * u) * 64);
+    r.spans = (int)((pieces + (int64_t)r.threads * u - 1) / ((int64_t)r.threads * u));
+    return r;
 }
 
 }  // namespace
 
-#define MR_ROW_KERNEL(KERNEL, PER_SPAN)                                                                      \
-    return row_launch(p, PER_SPAN, [&](bool vec, dim3 g, dim3 b, int spans) {                                \
-        if (p.f32)                                                                                           \
-            vec ? KERNEL<true, true><<<g, b, 0, st>>>(p, spans) : KERNEL<true, false><<<g, b, 0, st>>>(p, spans);   \
-        else                                                                                                 \
-            vec ? KERNEL<false, true><<<g, b, 0, st>>>(p, spans) : KERNEL<false, false><<<g, b, 0, st>>>(p, spans); \
-    })
+#define MR_ROW_KERNEL(KERNEL, PER_SPAN)                                                          \
+    const RowLaunch r = row_launch(p, PER_SPAN, cu_count);                                       \
+    const int64_t grid = (int64_t)p.n_tokens * (PER_SPAN ? r.spans : 1);                         \
+    if (grid * r.threads >= (1ll << 32)) return hipErrorInvalidValue;                            \
+    const auto kern = p.f32 ? (r.vec ? (r.two ? KERNEL<true, true, 2> : KERNEL<true, true, 1>)   \
+                                     : (r.two ? KERNEL<true, false, 2> : KERNEL<true, false, 1>)) \
+                            : (r.vec ? (r.two ? KERNEL<false, true, 2> : KERNEL<false, true, 1>) \
+                                     : (r.two ? KERNEL<false, false, 2> : KERNEL<false, false, 1>)); \
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(r.threads), 0, st, p, r.spans);          \
+    return hipGetLastError()
 
-hipError_t launch_expert_dispatch(const ExpertRowsParams& p, hipStream_t st) { MR_ROW_KERNEL(expert_dispatch_kernel, true); }
-hipError_t launch_expert_combine(const ExpertRowsParams& p, hipStream_t st) { MR_ROW_KERNEL(expert_combine_kernel, true); }
-hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, hipStream_t st) {
+hipError_t launch_expert_dispatch(const ExpertRowsParams& p, int cu_count, hipStream_t st) { MR_ROW_KERNEL(expert_dispatch_kernel, true); }
+hipError_t launch_expert_combine(const ExpertRowsParams& p, int cu_count, hipStream_t st) { MR_ROW_KERNEL(expert_combine_kernel, true); }
+hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, int cu_count, hipStream_t st) {
     MR_ROW_KERNEL(expert_combine_backward_kernel, false);
 }
 

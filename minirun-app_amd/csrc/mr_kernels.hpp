@@ -553,7 +553,7 @@ hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t
 
 // ---------------------------------------------------------------- routed experts
 constexpr int EXPERT_MAX = 4096;          // experts of a sort
-constexpr int EXPERT_SORT_PAIRS = 4096;   // pairs per workgroup of the sort
+constexpr int EXPERT_SORT_PAIRS = 2048;   // pairs per workgroup of the sort
 
 struct ExpertSortParams {
     const int32_t* ids;
@@ -582,8 +582,8 @@ struct ExpertRowsParams {
 
 inline int expert_sort_blocks(int64_t pairs) { return (int)((pairs + EXPERT_SORT_PAIRS - 1) / EXPERT_SORT_PAIRS); }
 hipError_t launch_expert_sort(const ExpertSortParams& p, hipStream_t st);
-hipError_t launch_expert_dispatch(const ExpertRowsParams& p, hipStream_t st);
-hipError_t launch_expert_combine(const ExpertRowsParams& p, hipStream_t st);
-hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, hipStream_t st);
+hipError_t launch_expert_dispatch(const ExpertRowsParams& p, int cu_count, hipStream_t st);
+hipError_t launch_expert_combine(const ExpertRowsParams& p, int cu_count, hipStream_t st);
+hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, int cu_count, hipStream_t st);
 
 }  // namespace mr

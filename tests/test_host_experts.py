@@ -142,9 +142,9 @@ def test_expert_matmul_refusals(lib):
 
 def test_sort_sizes_and_refusals(lib):
     size = lib.mr_expert_sort_workspace_size
-    assert size(512, 8, 128) == 0  # one workgroup
-    assert size(513, 8, 128) == 2 * 128 * 4
-    assert size(1 << 21, 8, 4096) == 4096 * 4096 * 4
+    assert size(256, 8, 128) == 0  # one workgroup
+    assert size(257, 8, 128) == 2 * 128 * 4
+    assert size(1 << 21, 8, 4096) == 8192 * 4096 * 4
     assert size(0, 8, 16) == 0
     for bad in ((-1, 1, 1), (1, 0, 1), (1, -3, 1), (1, 1, 0), (1, 1, 4097), ((1 << 21) + 1, 8, 4), (2 ** 31 - 1, 2 ** 31 - 1, 4)):
         assert size(*bad) == 0
