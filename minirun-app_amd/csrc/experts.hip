@@ -163,31 +163,44 @@ __global__ void __launch_bounds__(ES_THREADS) expert_place_kernel(ExpertSortPara
 }
 
 // ---------------------------------------------------------------- rows
-// Eight values of a row as stored: VEC, 8 next to each other (16 or 32 bytes,
-// rows 16-byte aligned); otherwise 8 at a distance of the workgroup's threads,
-// so that a wave still reads whole lines.
+// Eight values of a row as stored: VEC, 16 bytes next to each other (f32: twice,
+// at a distance of the workgroup's), rows 16-byte aligned; otherwise 8 at a
+// distance of the workgroup's threads.  Every instruction of a wave covers whole
+// lines.  Loads are streaming (a row is read
+// once), and so are the stores of results; dispatched rows, which the experts'
+// products read next, are not (4096 tokens of 7168, 4 rows each, all three calls:
+// 142 -> 127 us; rows stored past the caches as well 125, but then the products
+// after them take 20 of 480 us more).
 template <bool F32, bool VEC>
 struct Eight {
     using Elem = std::conditional_t<F32, uint32_t, uint16_t>;
-    static constexpr int N16 = F32 ? 2 : 1;
+    static constexpr int N16 = F32 ? 2 : 1, E16 = F32 ? 4 : 8;  // 16-byte units, values of one
     std::conditional_t<VEC, u32x4[N16], Elem[8]> v;
     __device__ __forceinline__ void load(const void* row, int64_t c, int64_t dim) {
         const Elem* p = (const Elem*)row + c;
 #pragma unroll
         for (int k = 0; k < (VEC ? N16 : 8); ++k) {
             if constexpr (VEC)
-                v[k] = ((const u32x4*)p)[k];
+                v[k] = k == 0 || c + (int64_t)k * E16 * blockDim.x < dim
+                           ? __builtin_nontemporal_load((const u32x4*)(p + (int64_t)k * E16 * blockDim.x))
+                           : u32x4{};
             else
                 v[k] = c + (int64_t)k * blockDim.x < dim ? p[(int64_t)k * blockDim.x] : (Elem)0;
         }
     }
+    template <bool STREAM>
     __device__ __forceinline__ void store(void* row, int64_t c, int64_t dim) const {
         Elem* p = (Elem*)row + c;
 #pragma unroll
         for (int k = 0; k < (VEC ? N16 : 8); ++k) {
-            if constexpr (VEC)
-                ((u32x4*)p)[k] = v[k];
-            else if (c + (int64_t)k * blockDim.x < dim)
+            if constexpr (VEC) {
+                u32x4* const to = (u32x4*)(p + (int64_t)k * E16 * blockDim.x);
+                if (k > 0 && c + (int64_t)k * E16 * blockDim.x >= dim) continue;
+                if constexpr (STREAM)
+                    __builtin_nontemporal_store(v[k], to);
+                else
+                    *to = v[k];
+            } else if (c + (int64_t)k * blockDim.x < dim)
                 p[(int64_t)k * blockDim.x] = v[k];
         }
     }
@@ -229,9 +242,9 @@ __device__ __forceinline__ char* row_at(const void* p, int64_t row, int64_t ld) 
 }
 
 // the first value of this thread's piece `i` of a row (of 8 blockDim.x values)
-template <bool VEC>
+template <bool F32, bool VEC>
 __device__ __forceinline__ int64_t piece_col(int64_t i) {
-    return 8 * i * blockDim.x + (VEC ? 8 : 1) * (int64_t)threadIdx.x;
+    return 8 * i * blockDim.x + (VEC ? Eight<F32, VEC>::E16 : 1) * (int64_t)threadIdx.x;
 }
 
 // The rows of a token's slots j0 .. j0 + 63: lane j has that of slot j0 + j
@@ -262,14 +275,14 @@ struct Slots {
 
 // One workgroup per token and span of a row: the piece is read once and stored
 // once per slot that has a row, bit for bit.  Bound by its stores (4096 tokens of
-// 7168, 4 rows each: 294 MB in 50 us).
+// 7168, 4 rows each: 294 MB in 47 us).
 template <bool F32, bool VEC, int U>
 __global__ void __launch_bounds__(512) expert_dispatch_kernel(ExpertRowsParams p, int spans) {
     const int64_t t = blockIdx.x / (unsigned)spans, s = blockIdx.x - t * spans;
     Eight<F32, VEC> x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int64_t c = piece_col<VEC>(s * U + u);
+        const int64_t c = piece_col<F32, VEC>(s * U + u);
         if (c < p.dim) x[u].load(row_at<F32>(p.tokens, t, p.ld_tokens), c, p.dim);
     }
     for (int j0 = 0; j0 < p.per_token; j0 += 64) {
@@ -279,8 +292,8 @@ __global__ void __launch_bounds__(512) expert_dispatch_kernel(ExpertRowsParams p
             char* row = row_at<F32>(p.out, sl.row_of(__builtin_ctzll(m)), p.ld_out);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t c = piece_col<VEC>(s * U + u);
-                if (c < p.dim) x[u].store(row, c, p.dim);
+                const int64_t c = piece_col<F32, VEC>(s * U + u);
+                if (c < p.dim) x[u].template store<false>(row, c, p.dim);
             }
         }
     }
@@ -314,7 +327,7 @@ __global__ void __launch_bounds__(512) expert_combine_kernel(ExpertRowsParams p,
                 const char* row = row_at<F32>(p.rows, sl.row_of(j), p.ld_rows);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int64_t c = piece_col<VEC>(s * U + u);
+                    const int64_t c = piece_col<F32, VEC>(s * U + u);
                     if (c < p.dim) y[b][u].load(row, c, p.dim);
                 }
             }
@@ -330,10 +343,10 @@ __global__ void __launch_bounds__(512) expert_combine_kernel(ExpertRowsParams p,
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int64_t c = piece_col<VEC>(s * U + u);
+        const int64_t c = piece_col<F32, VEC>(s * U + u);
         Eight<F32, VEC> o;
         o.set(sum[u]);
-        if (c < p.dim) o.store(row_at<F32>(p.out, t, p.ld_out), c, p.dim);
+        if (c < p.dim) o.template store<true>(row_at<F32>(p.out, t, p.ld_out), c, p.dim);
     }
 }
 
@@ -370,7 +383,7 @@ __global__ void __launch_bounds__(512) expert_combine_backward_kernel(ExpertRows
                 int64_t c[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    c[u] = piece_col<VEC>((int64_t)s * U + u);
+                    c[u] = piece_col<F32, VEC>((int64_t)s * U + u);
                     if (c[u] < p.dim) g[u].load(row_at<F32>(p.tokens, t, p.ld_tokens), c[u], p.dim);
                 }
                 if (p.d_weights) {
@@ -393,7 +406,7 @@ __global__ void __launch_bounds__(512) expert_combine_backward_kernel(ExpertRows
                             for (int k = 0; k < 8; ++k) d[k] = wt[b] * g[u].get(k);
                             Eight<F32, VEC> o;
                             o.set(d);
-                            if (c[u] < p.dim) o.store(row_at<F32>(p.out, r[b], p.ld_out), c[u], p.dim);
+                            if (c[u] < p.dim) o.template store<true>(row_at<F32>(p.out, r[b], p.ld_out), c[u], p.dim);
                         }
                     }
                 }
