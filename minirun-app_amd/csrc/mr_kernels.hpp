@@ -546,8 +546,8 @@ struct Mxfp4GemmParams {
 };
 
 constexpr int MXFP4_MAX_OUT = 1 << 22;  // weight rows of a product
-// tiles of tm = 256 or 128 rows of x times 256 weight rows
-hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int tm, hipStream_t st);
+// tiles of 256 or 128 rows of x times as many weight rows (experts' rows: 128)
+hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int size, hipStream_t st);
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p);
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st);
 

@@ -118,11 +118,13 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
     const int64_t x_from = by_token ? 0 : m0, x_rows = by_token ? p.M : toks;
     const i32x4 xres = uniform_rsrc((const char*)p.x + x_from * xrow,
                                     (uint32_t)((x_rows - 1) * xrow + X::BYTES * (int64_t)K / 256));
-    auto x_index = [&](int r) -> uint32_t {  // of this workgroup's -> row of the buffer
-        r = min(r, toks - 1);
-        if (by_token) return min((uint32_t)p.pair_of_row[m0 + r] / (uint32_t)p.per_token, (uint32_t)(p.M - 1));
-        return (uint32_t)r;
-    };
+    // rows of x that this lane loads from, then (MXFP4) whose scales it loads and
+    // that its fragments are of
+    constexpr int NX = XI + (XT == MX_X_MXFP4 ? 1 + TT : 0);
+    uint32_t xr[NX];
+    mx_x_rows<NX>(p, by_token, m0, toks, xr, [&](int u) {
+        return u < XI ? X::RPI * u + l / X::CHUNKS : (u == XI ? l : 16 * (u - XI - 1) + lr);
+    });
     const int nent = (int)((K + 255) / 256);
     const int n = w < nent ? (nent - 1 - w) / NW + 1 : 0;  // this wave's entries
 
@@ -139,15 +141,15 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
     const uint32_t so = l < rows ? (ws0 + (uint32_t)l * srow) & ~3u : SK_OOB_ROW;
     auto x_chunk = [&](int u) { return (uint32_t)((l % X::CHUNKS) ^ X::swizzle(X::RPI * u + l / X::CHUNKS)); };
 #pragma unroll
-    for (int u = 0; u < XI; ++u) xo[u] = x_index(X::RPI * u + l / X::CHUNKS) * (uint32_t)xrow + 16u * x_chunk(u);
+    for (int u = 0; u < XI; ++u) xo[u] = xr[u] * (uint32_t)xrow + 16u * x_chunk(u);
     i32x4 xsres{};
     if constexpr (XT == MX_X_MXFP4) {
         const uint64_t xa = (uint64_t)(uintptr_t)p.x_scales + x_from * srow;
         const uint32_t xs0 = (uint32_t)xa & 3u;
         xsres = uniform_rsrc((const void*)(uintptr_t)(xa & ~3ull), (xs0 + (uint32_t)x_rows * srow + 3u) & ~3u);
-        xso = (xs0 + x_index(l) * srow) & ~3u;
+        xso = (xs0 + xr[XI] * srow) & ~3u;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) xsh[t] = ((xs0 + x_index(16 * t + lr) * srow) & 3u) + 2u * q;
+        for (int t = 0; t < TT; ++t) xsh[t] = ((xs0 + xr[XI + 1 + t] * srow) & 3u) + 2u * q;
     }
 
     char* ring = lds + w * S * F::ENTRY;
@@ -343,11 +345,6 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
     const int64_t x_from = by_token ? 0 : m0, x_rows = by_token ? p.M : toks;
     const i32x4 xres = uniform_rsrc((const char*)p.x + x_from * xrow,
                                     (uint32_t)((x_rows - 1) * xrow + X::BYTES * (int64_t)K / 256));
-    auto x_index = [&](int r) -> uint32_t {
-        r = min(r, toks - 1);
-        if (by_token) return min((uint32_t)p.pair_of_row[m0 + r] / (uint32_t)p.per_token, (uint32_t)(p.M - 1));
-        return (uint32_t)r;
-    };
     const int nst = (int)((K + 255) / 256);
 
     constexpr uint32_t PAST = 0xfffffff0u;  // an offset that reads zeros
@@ -363,16 +360,20 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
     auto x_instr = [&](int u) { return min(F::XPW * w + u, F::XI - 1); };
     auto x_row = [&](int u) { return X::RPI * x_instr(u) + l / X::CHUNKS; };
     auto x_chunk = [&](int u) { return (uint32_t)((l % X::CHUNKS) ^ X::swizzle(x_row(u))); };
+    constexpr int NX = F::XPW + (XT == MX_X_MXFP4 ? 1 + TT : 0);
+    uint32_t xr[NX];
+    mx_x_rows<NX>(p, by_token, m0, toks, xr,
+                  [&](int u) { return u < F::XPW ? x_row(u) : (u == F::XPW ? l : 16 * (u - F::XPW - 1) + lr); });
 #pragma unroll
-    for (int u = 0; u < F::XPW; ++u) xo[u] = x_index(x_row(u)) * (uint32_t)xrow + 16u * x_chunk(u);
+    for (int u = 0; u < F::XPW; ++u) xo[u] = xr[u] * (uint32_t)xrow + 16u * x_chunk(u);
     i32x4 xsres{};
     if constexpr (XT == MX_X_MXFP4) {
         const uint64_t xa = (uint64_t)(uintptr_t)p.x_scales + x_from * srow;
         const uint32_t xs0 = (uint32_t)xa & 3u;
         xsres = uniform_rsrc((const void*)(uintptr_t)(xa & ~3ull), (xs0 + (uint32_t)x_rows * srow + 3u) & ~3u);
-        xso = (xs0 + x_index(l) * srow) & ~3u;
+        xso = (xs0 + xr[F::XPW] * srow) & ~3u;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) xsh[t] = ((xs0 + x_index(16 * t + lr) * srow) & 3u) + 2u * q;
+        for (int t = 0; t < TT; ++t) xsh[t] = ((xs0 + xr[F::XPW + 1 + t] * srow) & 3u) + 2u * q;
     }
     const int woff = 1024 * F::XI + w * F::WAVE;  // of the wave's part in a stage
     auto issue = [&](int s, int slot) {
@@ -613,23 +614,29 @@ hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     return p.x_kind == MX_X_F32 ? launch_few_f32(p, cus, st) : launch_few_bf16(p, cus, st);
 }
 
-// Rows per large tile (mxfp4_gemm.hip), or 0.  They pay once they cover the
-// GPU for the larger part: bf16, 24576 x 1536, 192 tokens (192 tiles of 128) 23.8
-// us, few rows 26.5, 128 tokens 22.2 and 18.3; 7168 x 16384, 400 tokens (112) 173
-// and 135.  MXFP4 at 112 tiles 62 and 63.  Tiles of 256 rows likewise (24576 x
-// 1536, 400 tokens: 39.8, of 128 45.5; 256 tokens: 36.5 and 24.6).  Experts by
-// their mean rows: bf16 100 rows 91 us, few rows 85; MXFP4 50 rows 38 and 42, 31
-// rows 36 and 34.
-int tile_rows(const Mxfp4GemmParams& p, int cus) {
+// Rows and columns of a large tile (mxfp4_gemm.hip): 256, 128, or 0 for none.
+// One matrix: tiles of 128 (two workgroups a CU) pay once they cover the larger
+// part of the GPU and the kernels of few rows would read W more than once (bf16:
+// 24576 x 1536, 65 tokens, 192 tiles, 14 us and few rows 17, 64 tokens 14 and 11;
+// 7168 x 16384, 300 tokens, 168 tiles, 108 and 138, 200 tokens, 112 tiles, 107 and
+// 83; 16384 x 4096, 65 tokens, 128 tiles, 31 and 25; MXFP4: there 15 and 17, 64
+// tokens 15 and 11; 24576 x 1536, 37 tokens, 6.7 and 7.7; 1536 x 7168, 1000
+// tokens, 96 tiles, 19 and 24, 600 tokens, 60 tiles, 24 and 12).  A full round of
+// them takes 4/7 of one of 256 x 256, which read half as much: bf16, 24576 x 1536,
+// 600 tokens, 2 rounds 47 us, 2 of 256 74; 1000 tokens, 3 72, 2 of 256 77; 16384 x
+// 4096, 1000 tokens, 2 123, 1 of 256 106, MXFP4 46 and 40.
+// Experts (128 of 768 x 2048) by their mean rows: bf16 100 rows, 128 80, few rows
+// 86; 50 rows 63 and 55; MXFP4 50 rows 37 and 41, 31 rows 35 and 35; 256 rows 67,
+// 256 x 256 77.
+int tile_size(const Mxfp4GemmParams& p, int cus) {
     if (p.x_kind == MX_X_F32) return 0;
     const bool mx = p.x_kind == MX_X_MXFP4;
-    const int64_t n = (p.N + 255) / 256;
-    if (p.offsets) {
-        const int64_t rows = p.pairs / p.experts;
-        return rows < (mx ? 40 : 128) ? 0 : 128;
-    }
-    if (n * (((int64_t)p.M + 255) / 256) * 8 >= 5 * cus) return 256;
-    return n * (((int64_t)p.M + 127) / 128) * 8 >= (mx ? 3 : 5) * cus ? 128 : 0;
+    if (p.offsets) return p.pairs / p.experts < (mx ? 28 : 80) ? 0 : 128;
+    if (p.M <= (mx ? 32 : 64)) return 0;
+    auto tiles = [&](int size) { return (((int64_t)p.N + size - 1) / size) * (((int64_t)p.M + size - 1) / size); };
+    if (tiles(128) * 8 < (mx ? (p.M <= 64 ? 6 : 4) : 5) * cus) return 0;
+    const int64_t rounds128 = (tiles(128) + 2 * cus - 1) / (2 * cus), rounds256 = (tiles(256) + cus - 1) / cus;
+    return 7 * rounds256 <= 4 * rounds128 ? 256 : 128;
 }
 
 }  // namespace
@@ -645,8 +652,8 @@ bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
 // one, up to 2^23 workgroups of 16 tokens x 16 weight rows (MXFP4_MAX_OUT weight
 // rows leave 256 tokens each).
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st) {
-    const int tm = tile_rows(p, cu_count);
-    if (p.offsets) return tm ? launch_mxfp4_tiles(p, tm, st) : launch_mxfp4_few(p, cu_count, st);
+    const int tile = tile_size(p, cu_count);
+    if (p.offsets) return tile ? launch_mxfp4_tiles(p, tile, st) : launch_mxfp4_few(p, cu_count, st);
     const int64_t most = ((int64_t)1 << 23) / ((p.N + 15) / 16 + 8) * 16 / 256 * 256;
     for (int64_t m = 0; m < p.M; m += most) {
         Mxfp4GemmParams q = p;
@@ -655,7 +662,7 @@ hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t
         q.x = (const char*)p.x + m * row;
         if (p.x_scales) q.x_scales = p.x_scales + m * (p.K / 32);
         q.y = (char*)p.y + m * p.ldy * (p.y_f32 ? 4 : 2);
-        const hipError_t e = tm ? launch_mxfp4_tiles(q, tm, st) : launch_mxfp4_few(q, cu_count, st);
+        const hipError_t e = tile ? launch_mxfp4_tiles(q, tile, st) : launch_mxfp4_few(q, cu_count, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -1,17 +1,23 @@
 // Products with MXFP4 weights for many rows: y[t][o] = sum_i x[t][i] w[o][i]
-// in tiles of TM = 256 or 128 rows of x times 256 weight rows, for the tokens of
-// one matrix or for rows in expert order (a tile then has rows of one expert).
+// in tiles of TM x TN rows of x and W, 256 x 256 or 128 x 128, for the tokens of
+// one matrix or for rows in expert order (tiles of 128, each of one expert's rows).
 // x is bf16, or MXFP4 itself; y bf16 or f32.
 //
 // What bounds it: the matrix pipe, and the way of the operands to it.  One
-// workgroup of 4 waves computes a tile, each wave a (TM / 2) x 128 block of
-// 32x32 MFMA tiles, whose accumulators fill half of its registers; each operand
-// fragment serves MI or 4 of them.  Operands come by global -> LDS DMA, issued
-// between the MFMAs.  A load costs by the lines it touches, about two clocks
-// each, whether it takes 4 or 128 bytes of a line, so rows come in whole lines
-// of 128 bytes and scales 16 bytes of a row at a time (64-byte pieces and four
-// scale bytes per load kept the matrix pipe waiting: 4096 x 7168 x 16384 in
-// MXFP4 took 312 us, its loads alone 264).
+// workgroup of 4 waves computes a tile, each wave a quarter of it in 32x32 MFMA
+// tiles; each operand fragment serves MI or JN of them.  With 256 x 256 (the
+// accumulators are half of the registers, one workgroup a CU) a prompt of 4096
+// tokens runs at 1.2 PFLOP/s in bf16 (24576 x 1536, 255 us) and 3.9 PFLOP/s in
+// MXFP4 (7168 x 16384, 245 us).  128 x 128 reads twice as much per operation, but
+// two workgroups a CU cover each other's waits, ends of tiles and starts: 4096
+// tokens to 8 of 128 experts of 768 x 2048, MXFP4, 67 us, with 128 x 256 and one
+// workgroup a CU 78 (of this, 31 us is the time of the bytes: eight stages a tile
+// leave the loads' and the barriers' latency in view).
+// Operands come by global -> LDS DMA, issued between the MFMAs.  A load costs by
+// the lines it touches, about two clocks each, whether it takes 4 or 128 bytes of
+// a line, so rows come in whole lines of 128 bytes and scales 16 bytes of a row
+// at a time (64-byte pieces and four scale bytes per load kept the matrix pipe
+// waiting: 4096 x 7168 x 16384 in MXFP4 took 312 us, its loads alone 264).
 //
 //   x in MXFP4: v_mfma_scale_f32_32x32x64_f8f6f4 on the codes and scale bytes
 //     as stored.  A stage is 256 k: a line of each row of x and W, in a ring of
@@ -48,40 +54,40 @@ namespace mr {
 
 namespace {
 
-constexpr int MG_TN = 256, MG_THREADS = 256;
+constexpr int MG_THREADS = 256;
 
 __device__ __forceinline__ int slot128(int r, int c) { return 8 * r + (c ^ ((r >> 1) & 7)); }
 __device__ __forceinline__ int slot64(int r, int c) { return 4 * r + (c ^ ((r >> 2) & 3)); }
 
-template <int XT, int TM, bool RAGGED>
+template <int XT, int TM, int TN, bool RAGGED>
 struct MgShape {
     static constexpr bool MX = XT == MX_X_MXFP4;
     static constexpr int A = TM * 128;                // bytes of x in a stage
-    static constexpr int B = MG_TN * (MX ? 128 : 64);  // of W in its pieces
+    static constexpr int B = TN * (MX ? 128 : 64);    // of W in its pieces
     static constexpr int NA = MX ? 2 : 3;             // stages of x in the ring; W and scales: 2
-    // scales: 16 bytes (MXFP4: of 512 rows, x's first) or 4 per row, and RAGGED
-    // the word after them
-    static constexpr int SROWS = MX ? 512 : 256, SROW = MX ? 16 : 4;
+    // scales: 16 bytes (MXFP4: x's rows first) or 4 per row, and RAGGED the word
+    // after them; rows in whole instructions of the four waves
+    static constexpr int SROWS = MX ? (TM + TN + 255) / 256 * 256 : TN, SROW = MX ? 16 : 4;
     static constexpr int S = SROWS * (SROW + (RAGGED ? 4 : 0));
     static constexpr int RING = NA * A + 2 * B + 2 * S;
     // DMA instructions per wave: x and W of a stage or piece, scales
-    static constexpr int DA = A / 4096, DB = B / 4096, DS = (MX ? 2 : 1) * (RAGGED ? 2 : 1);
-    static constexpr size_t LDS_BF16 = std::max<size_t>(RING, (size_t)TM * MG_TN * 2);
-    static constexpr size_t LDS_F32 = std::max<size_t>(RING, (size_t)TM / 2 * MG_TN * 4);
+    static constexpr int DA = A / 4096, DB = B / 4096, SQ = MX ? SROWS / 256 : 1, DS = SQ * (RAGGED ? 2 : 1);
+    static constexpr size_t LDS_BF16 = std::max<size_t>(RING, (size_t)TM * TN * 2);
+    static constexpr size_t LDS_F32 = std::max<size_t>(RING, (size_t)TM / 2 * TN * 4);
     static_assert(LDS_BF16 <= 163840 && LDS_F32 <= 163840, "LDS");
 };
 
-template <int XT, int TM, bool ROUTED, bool YF32, bool RAGGED>
-__global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmParams p) {
-    using S = MgShape<XT, TM, RAGGED>;
+template <int XT, int TM, int TN, bool ROUTED, bool YF32, bool RAGGED>
+__global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kernel(Mxfp4GemmParams p) {
+    using S = MgShape<XT, TM, TN, RAGGED>;
     constexpr bool MX = S::MX;
-    constexpr int DA = S::DA, DB = S::DB, DS = S::DS;
+    constexpr int DA = S::DA, DB = S::DB, DS = S::DS, SQ = S::SQ;
     constexpr int WM = TM / 2, MI = WM / 32;  // rows and 32-row MFMA tiles per wave
-    constexpr int WN = MG_TN / 2, JN = WN / 32;  // columns and 32-column ones
+    constexpr int WN = TN / 2, JN = WN / 32;  // columns and 32-column ones
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n_tiles = (p.N + MG_TN - 1) / MG_TN;
+    const int n_tiles = (p.N + TN - 1) / TN;
     int m0, rows, nt;
     int64_t first = 0;  // weight row 0 of the expert
     if constexpr (ROUTED) {
@@ -106,10 +112,10 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
         nt = (bid % (GM * n_tiles)) / gsize;
         rows = min(TM, p.M - m0);
     }
-    const int n0 = nt * MG_TN;
+    const int n0 = nt * TN;
     const uint32_t wrow = (uint32_t)p.K / 2, srow = (uint32_t)p.K / 32;
     const uint32_t xrow = MX ? wrow : (uint32_t)p.ldx * 2u;
-    const int wrows = min(MG_TN, p.N - n0);
+    const int wrows = min(TN, p.N - n0);
 
     // x: from the tile's first row, or (rows by token) from row 0 with the
     // token's offset; a byte offset past the buffer reads zeros
@@ -119,11 +125,16 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
     const uint32_t x_bytes = (uint32_t)((x_rows - 1) * (MX ? wrow : p.ldx * 2) + (MX ? wrow : 2 * p.K));
     const i32x4 xres = uniform_rsrc((const char*)p.x + x_from * (MX ? wrow : p.ldx * 2), x_bytes);
     const i32x4 wres = uniform_rsrc((const char*)p.packed + (first + n0) * wrow, (uint32_t)wrows * wrow);
-    auto x_index = [&](int r) -> uint32_t {  // row of the tile -> row of the buffer
-        r = min(r, rows - 1);
-        if (by_token) return min((uint32_t)p.pair_of_row[m0 + r] / (uint32_t)p.per_token, (uint32_t)(p.M - 1));
-        return (uint32_t)r;
-    };
+    // rows of x that this lane loads from, and (q >= DA) whose scales it loads, or
+    // (RAGGED) that its fragments are of
+    constexpr int NX = DA + (MX ? SQ + (RAGGED ? MI : 0) : 0);
+    const int wm = w >> 1, wn = w & 1;
+    uint32_t xr[NX];
+    mx_x_rows<NX>(p, by_token, m0, rows, xr, [&](int u) {
+        if (u < DA) return 8 * (DA * w + u) + (l >> 3);
+        if (u < DA + SQ) return 64 * (SQ * w + u - DA) + l;
+        return wm * WM + (u - DA - SQ) * 32 + (l & 31);
+    });
     // scales: through aligned words
     const uint64_t wsa = (uint64_t)(uintptr_t)p.scales + (first + n0) * srow;
     const uint32_t ws0 = (uint32_t)wsa & 3u;
@@ -140,22 +151,22 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
     // lane l of a DMA instruction over 128-byte rows fills slot l % 8 of row 8 i
     // + l / 8 (odd i: chunk ^ 4), over 64-byte rows slot l % 4 of row 16 i + l / 4
     const uint32_t ch8 = (l & 7) ^ (l >> 4), ch4 = (l & 3) ^ ((l >> 4) & 3);
-    uint32_t ao[DA], bo[DB], so[MX ? 2 : 1];
-    i32x4 sres[MX ? 2 : 1];
+    uint32_t ao[DA], bo[DB], so[SQ];
+    i32x4 sres[SQ];
 #pragma unroll
-    for (int q = 0; q < DA; ++q) ao[q] = x_index(8 * (DA * w + q) + (l >> 3)) * xrow + 16u * (ch8 ^ (4 * (q & 1)));
+    for (int q = 0; q < DA; ++q) ao[q] = xr[q] * xrow + 16u * (ch8 ^ (4 * (q & 1)));
 #pragma unroll
     for (int q = 0; q < DB; ++q) {
         const int r = MX ? 8 * (DB * w + q) + (l >> 3) : 16 * (DB * w + q) + (l >> 2);
         bo[q] = (uint32_t)min(r, wrows - 1) * wrow + 16u * (MX ? ch8 ^ (4 * (q & 1)) : ch4);
     }
 #pragma unroll
-    for (int q = 0; q < (MX ? 2 : 1); ++q) {  // scales: a row per lane, x's rows first
-        const int first_r = MX ? 128 * w + 64 * q : 64 * w;
+    for (int q = 0; q < SQ; ++q) {  // scales: a row per lane, x's rows first
+        const int first_r = MX ? 64 * (SQ * w + q) : 64 * (w % (TN / 64));
         const bool of_x = MX && first_r < TM;
         const int r = first_r + l - (MX && !of_x ? TM : 0);
         sres[q] = of_x ? xsres : wsres;
-        so[q] = (of_x ? xs0 + x_index(r) * srow : ws0 + (uint32_t)min(r, wrows - 1) * srow) & ~3u;
+        so[q] = (of_x ? xs0 + xr[MX ? DA + q : 0] * srow : ws0 + (uint32_t)min(r, wrows - 1) * srow) & ~3u;
     }
     const uint32_t K = (uint32_t)p.K;
     constexpr uint32_t PAST = 0xfffffff0u;  // an offset that reads zeros
@@ -180,16 +191,15 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
     auto dma_s = [&](int t, char* st, int q) {
         t = min(t, ST - 1);
         if constexpr (MX) {
-            if (q < 2)
-                mx_dma16(sres[q], so[q] + 16u * t, st + 2048 * w + 1024 * q);
+            if (q < SQ)
+                mx_dma16(sres[q], so[q] + 16u * t, st + 1024 * (SQ * w + q));
             else
-                mx_dma4(sres[q - 2], so[q - 2] + 16u * t + 16u, st + 16 * S::SROWS + 512 * w + 256 * (q - 2));
+                mx_dma4(sres[q - SQ], so[q - SQ] + 16u * t + 16u, st + 16 * S::SROWS + 256 * (SQ * w + q - SQ));
         } else {
-            mx_dma4(sres[0], so[0] + 4u * t + 4u * q, st + 1024 * q + 256 * w);
+            mx_dma4(sres[0], so[0] + 4u * t + 4u * q, st + 4 * TN * q + 256 * (w % (TN / 64)));
         }
     };
 
-    const int wm = w >> 1, wn = w & 1;
     f32x16 acc[MI][JN];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -199,7 +209,7 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
     uint32_t ash[MI], bsh[JN];
     if constexpr (RAGGED) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) ash[i] = MX ? (xs0 + x_index(wm * WM + i * 32 + (l & 31)) * srow) & 3u : 0u;
+        for (int i = 0; i < MI; ++i) ash[i] = MX ? (xs0 + xr[MX ? DA + SQ + i : 0] * srow) & 3u : 0u;
 #pragma unroll
         for (int j = 0; j < JN; ++j) bsh[j] = (ws0 + (uint32_t)min(wn * WN + j * 32 + (l & 31), wrows - 1) * srow) & 3u;
     }
@@ -324,7 +334,7 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
                 const int r = wn * WN + j * 32 + (l & 31);
                 v.b[j] = *(const u32x4*)(st + 16 * slot64(r, c));
                 uint32_t d = *(const uint32_t*)(ss + 4 * r);
-                if constexpr (RAGGED) d = __builtin_amdgcn_alignbyte(*(const uint32_t*)(ss + 1024 + 4 * r), d, bsh[j]);
+                if constexpr (RAGGED) d = __builtin_amdgcn_alignbyte(*(const uint32_t*)(ss + 4 * TN + 4 * r), d, bsh[j]);
                 const bool past = RAGGED && 64u * (uint32_t)min(t, AT - 1) + 32u * h >= K;
                 v.s[j] = __uint_as_float(past ? 127u << 23 : ((d >> (8 * c)) & 255u) << 23);
             }
@@ -408,18 +418,18 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
                             const int q = (wn * WN + j * 32 + 8 * g + 4 * h) >> 2;
-                            *(f32x4*)(ly + row * MG_TN + 4 * (q ^ (row & 15))) =
+                            *(f32x4*)(ly + row * TN + 4 * (q ^ (row & 15))) =
                                 f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
                         }
                 }
             }
             __syncthreads();
             float* yf = (float*)p.y + (int64_t)(m0 + half * WM) * p.ldy + n0;
-            constexpr int PER = WM * MG_TN / 4 / MG_THREADS;
+            constexpr int PER = WM * TN / 4 / MG_THREADS;
 #pragma unroll 4
             for (int it = 0; it < PER; ++it) {
-                const int idx = tid + MG_THREADS * it, row = idx >> 6, q = idx & 63;
-                const f32x4 v = *(const f32x4*)(ly + row * MG_TN + 4 * (q ^ (row & 15)));
+                const int idx = tid + MG_THREADS * it, row = idx / (TN / 4), q = idx % (TN / 4);
+                const f32x4 v = *(const f32x4*)(ly + row * TN + 4 * (q ^ (row & 15)));
                 if (half * WM + row >= rows) continue;
                 float* o = yf + (int64_t)row * p.ldy + 4 * q;
                 if (vec && n0 + 4 * q + 4 <= p.N) {
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
             __syncthreads();
         }
     } else {
-        // 16-byte chunk q of row r at q ^ (r & 31)
+        // 16-byte chunk q of row r at q ^ r
         uint16_t* ly = (uint16_t*)lds;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -443,21 +453,21 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int col = wn * WN + j * 32 + 8 * g + 4 * h;
-                    const int q = (col >> 3) ^ (row & 31);
+                    const int q = (col >> 3) ^ (row & (TN / 8 - 1));
                     u32x2 v;
                     v[0] = pack_bf16x2_hw(acc[i][j][4 * g], acc[i][j][4 * g + 1]);
                     v[1] = pack_bf16x2_hw(acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-                    *(u32x2*)(ly + row * MG_TN + 8 * q + (col & 7)) = v;
+                    *(u32x2*)(ly + row * TN + 8 * q + (col & 7)) = v;
                     __builtin_amdgcn_sched_barrier(0);  // (registers)
                 }
         }
         __syncthreads();
         uint16_t* yb = (uint16_t*)p.y + (int64_t)m0 * p.ldy + n0;
-        constexpr int PER = TM * MG_TN / 8 / MG_THREADS;
+        constexpr int PER = TM * TN / 8 / MG_THREADS;
 #pragma unroll 4
         for (int it = 0; it < PER; ++it) {
-            const int idx = tid + MG_THREADS * it, row = idx >> 5, q = idx & 31;
-            const u32x4 v = *(const u32x4*)(ly + row * MG_TN + 8 * (q ^ (row & 31)));
+            const int idx = tid + MG_THREADS * it, row = idx / (TN / 8), q = idx % (TN / 8);
+            const u32x4 v = *(const u32x4*)(ly + row * TN + 8 * (q ^ (row & (TN / 8 - 1))));
             if (row >= rows) continue;
             uint16_t* o = yb + (int64_t)row * p.ldy + 8 * q;
             if (vec && n0 + 8 * q + 8 <= p.N) {
@@ -471,37 +481,40 @@ __global__ void __launch_bounds__(MG_THREADS, 1) mxfp4_gemm_kernel(Mxfp4GemmPara
     }
 }
 
-template <int XT, int TM, bool ROUTED, bool YF32, bool RAGGED>
+template <int XT, int TM, int TN, bool ROUTED, bool YF32, bool RAGGED>
 hipError_t mg_launch(const Mxfp4GemmParams& p, hipStream_t st) {
-    using S = MgShape<XT, TM, RAGGED>;
+    using S = MgShape<XT, TM, TN, RAGGED>;
     constexpr size_t lds = YF32 ? S::LDS_F32 : S::LDS_BF16;
-    const auto kern = mxfp4_gemm_kernel<XT, TM, ROUTED, YF32, RAGGED>;
+    const auto kern = mxfp4_gemm_kernel<XT, TM, TN, ROUTED, YF32, RAGGED>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
-    const int64_t n_tiles = (p.N + MG_TN - 1) / MG_TN;
+    const int64_t n_tiles = (p.N + TN - 1) / TN;
     const int64_t grid = ROUTED ? (mx_tile_bound(p, TM) * n_tiles + 7) / 8 * 8 : (p.M + (int64_t)TM - 1) / TM * n_tiles;
     if (grid * MG_THREADS >= (1ll << 32)) return hipErrorInvalidValue;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(MG_THREADS), lds, st, p);
     return hipGetLastError();
 }
 
-template <int XT, int TM, bool ROUTED>
+template <int XT, int TM, int TN, bool ROUTED>
 hipError_t mg_launch_y(const Mxfp4GemmParams& p, hipStream_t st) {
     const bool ragged = p.K % (XT == MX_X_MXFP4 ? 256 : 128) || ((uintptr_t)p.scales & 3) || ((uintptr_t)p.x_scales & 3);
-    if (p.y_f32) return ragged ? mg_launch<XT, TM, ROUTED, true, true>(p, st) : mg_launch<XT, TM, ROUTED, true, false>(p, st);
-    return ragged ? mg_launch<XT, TM, ROUTED, false, true>(p, st) : mg_launch<XT, TM, ROUTED, false, false>(p, st);
+    if (p.y_f32) return ragged ? mg_launch<XT, TM, TN, ROUTED, true, true>(p, st) : mg_launch<XT, TM, TN, ROUTED, true, false>(p, st);
+    return ragged ? mg_launch<XT, TM, TN, ROUTED, false, true>(p, st) : mg_launch<XT, TM, TN, ROUTED, false, false>(p, st);
 }
 
-template <int XT, int TM>
+template <int XT, int TM, int TN>
 hipError_t mg_launch_r(const Mxfp4GemmParams& p, hipStream_t st) {
-    return p.offsets ? mg_launch_y<XT, TM, true>(p, st) : mg_launch_y<XT, TM, false>(p, st);
+    if constexpr (TM == 128) {  // experts' rows run in small tiles only
+        if (p.offsets) return mg_launch_y<XT, TM, TN, true>(p, st);
+    }
+    return mg_launch_y<XT, TM, TN, false>(p, st);
 }
 
 }  // namespace
 
-hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int tm, hipStream_t st) {
-    if (p.x_kind == MX_X_MXFP4) return tm == 256 ? mg_launch_r<MX_X_MXFP4, 256>(p, st) : mg_launch_r<MX_X_MXFP4, 128>(p, st);
-    return tm == 256 ? mg_launch_r<MX_X_BF16, 256>(p, st) : mg_launch_r<MX_X_BF16, 128>(p, st);
+hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int size, hipStream_t st) {
+    if (p.x_kind == MX_X_MXFP4) return size == 256 ? mg_launch_r<MX_X_MXFP4, 256, 256>(p, st) : mg_launch_r<MX_X_MXFP4, 128, 128>(p, st);
+    return size == 256 ? mg_launch_r<MX_X_BF16, 256, 256>(p, st) : mg_launch_r<MX_X_BF16, 128, 128>(p, st);
 }
 
 }  // namespace mr

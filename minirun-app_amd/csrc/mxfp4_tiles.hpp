@@ -61,11 +61,16 @@ struct MxTile {
 // no tile leaves [0, pairs).
 template <int BM>
 __device__ __forceinline__ bool mx_find_tile(const int32_t* offsets, int experts, int pairs, int n_tiles, MxTile& t) {
+    constexpr int R = 4;  // experts per lane whose offsets stay in registers
     const int l = threadIdx.x & 63, run = (experts + 63) / 64;
     auto at = [&](int e) { return min(max(offsets[min(e, experts)], 0), pairs); };
     auto count = [](int lo, int hi) { return hi > lo ? (hi - lo + BM - 1) / BM : 0; };
-    int lo = at(l * run), mine = 0;
-    for (int k = 0; k < run; ++k) {
+    int off[R + 1], mine = 0;
+#pragma unroll
+    for (int k = 0; k <= R; ++k) off[k] = at(l * run + min(k, run));  // (in flight together)
+#pragma unroll
+    for (int k = 0; k < R; ++k) mine += count(off[k], off[k + 1]);
+    for (int k = R, lo = off[R]; k < run; ++k) {
         const int hi = at(l * run + k + 1);
         mine += count(lo, hi);
         lo = hi;
@@ -78,16 +83,20 @@ __device__ __forceinline__ bool mx_find_tile(const int32_t* offsets, int experts
     int e = -1, row = 0, rows = 0;
     if (i >= incl - mine && i < incl) {
         int left = i - (incl - mine);
-        lo = at(l * run);
-        for (int k = 0; k < run; ++k) {
-            const int hi = at(l * run + k + 1), c = count(lo, hi);
-            if (left < c) {
+        auto look = [&](int k, int lo, int hi) {
+            const int c = count(lo, hi);
+            if (e < 0 && left < c) {
                 e = l * run + k;
                 row = lo + left * BM;
                 rows = min(BM, hi - row);
-                break;
             }
             left -= c;
+        };
+#pragma unroll
+        for (int k = 0; k < R; ++k) look(k, off[k], off[k + 1]);
+        for (int k = R, lo = off[R]; k < run && e < 0; ++k) {
+            const int hi = at(l * run + k + 1);
+            look(k, lo, hi);
             lo = hi;
         }
     }
@@ -99,6 +108,22 @@ __device__ __forceinline__ bool mx_find_tile(const int32_t* offsets, int experts
     t.rows = __builtin_amdgcn_readlane(rows, from);
     t.n_tile = __builtin_amdgcn_readfirstlane((int)(id - (int64_t)i * n_tiles));
     return true;
+}
+
+// Rows of x for N rows of a tile that starts at row m0 of y and has `rows`
+// (row_of(u): row u's place in the tile; past the last, the last): the place
+// itself, or where rows come by token, the token's row.  The pairs' loads are in
+// flight together: one after the other they were a third of a small call.
+template <int N, typename F>
+__device__ __forceinline__ void mx_x_rows(const Mxfp4GemmParams& p, bool by_token, int m0, int rows, uint32_t (&out)[N], F row_of) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) out[u] = (uint32_t)min(row_of(u), rows - 1);
+    if (by_token) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) out[u] = (uint32_t)p.pair_of_row[m0 + (int)out[u]];
+#pragma unroll
+        for (int u = 0; u < N; ++u) out[u] = min(out[u] / (uint32_t)p.per_token, (uint32_t)(p.M - 1));
+    }
 }
 
 // the most tiles of bm rows that `pairs` rows of `experts` experts can make
