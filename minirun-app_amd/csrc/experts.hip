@@ -56,12 +56,43 @@ __global__ void __launch_bounds__(ES_THREADS) expert_count_kernel(ExpertSortPara
     for (int e = threadIdx.x; e < p.experts; e += ES_THREADS) out[e] = bins[e];
 }
 
-// One workgroup places 2048 pairs (4096: 2 us more at 32768 pairs).  LDS: cursor[wave][expert], at first the
-// wave's count of the expert, then the row that the wave's next pair of it
-// gets: the expert's first row, plus its pairs in earlier workgroups, plus
-// those in earlier waves.  A wave then takes its pairs in order, 64 at a time;
+// counts[block][expert] becomes the expert's pairs up to and in the workgroup
+// that counted it.  A workgroup has 64 experts (or what is
+// left): `groups` threads per expert share the workgroups' counts in runs.
+constexpr int EX_THREADS = 1024;
+__global__ void __launch_bounds__(EX_THREADS) expert_scan_kernel(ExpertSortParams p, int blocks) {
+    __shared__ int32_t part[EX_THREADS];
+    const int tid = threadIdx.x, e0 = 64 * blockIdx.x, left = min(p.experts - e0, 64), groups = EX_THREADS / left;
+    const int g = tid / left, e = tid - g * left, run = (blocks + groups - 1) / groups;
+    const int lo = min(g * run, blocks), hi = g < groups ? min(lo + run, blocks) : lo;
+    int32_t* at = p.counts + e0 + e;
+    int sum = 0;
+#pragma unroll 8
+    for (int b = lo; b < hi; ++b) sum += at[(int64_t)b * p.experts];
+    part[tid] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int k = 0; k < g; ++k) before += part[k * left + e];
+    for (int b = lo; b < hi; b += 8) {
+        int c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = b + k < hi ? at[(int64_t)(b + k) * p.experts] : 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            before += c[k];
+            if (b + k < hi) at[(int64_t)(b + k) * p.experts] = before;
+        }
+    }
+}
+
+// One workgroup places 2048 pairs (4096: 2 us more at 32768 pairs).  LDS:
+// cursor[wave][expert], at first the wave's count of the expert, then the row
+// that the wave's next pair of it gets: the expert's first row, plus its pairs in
+// earlier workgroups (SCANNED: read; else summed over their counts), plus those
+// in earlier waves.  A wave then takes its pairs in order, 64 at a time;
 // lanes of one expert find each other by one ballot per bit of the id, so a
 // lane's rank among them is a count of bits.
+template <bool SCANNED>
 __global__ void __launch_bounds__(ES_THREADS) expert_place_kernel(ExpertSortParams p) {
     extern __shared__ int32_t cursor[];
     __shared__ int32_t sums[ES_WAVES];
@@ -83,7 +114,12 @@ __global__ void __launch_bounds__(ES_THREADS) expert_place_kernel(ExpertSortPara
     for (int e0 = 0; e0 < E; e0 += ES_THREADS) {
         const int e = e0 + tid;
         int before = 0, total = 0;  // of the expert: in earlier workgroups, in all
-        if (blocks == 1) {
+        if (SCANNED) {
+            if (e < E) {
+                if (blockIdx.x > 0) before = p.counts[((int64_t)blockIdx.x - 1) * E + e];
+                total = p.counts[((int64_t)blocks - 1) * E + e];
+            }
+        } else if (blocks == 1) {
             if (e < E) {
 #pragma unroll
                 for (int k = 0; k < ES_WAVES; ++k) total += cursor[k * E + e];
@@ -490,11 +526,19 @@ hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, int cu_coun
 
 #undef MR_ROW_KERNEL
 
+// Every workgroup of the placement reads all counts, unless they are scanned
+// first, in a launch more (a call in us: 2^20 pairs of 1024 experts 94 -> 27, 2^24
+// pairs of 128 2135 -> 161, of 8 210 -> 80; 32768 pairs of 4096 26 -> 21; 2^17
+// pairs of 256 15 without)
+bool scan_counts(int64_t blocks, int64_t experts) { return blocks > 512 || blocks * experts >= 1 << 16; }
+
 hipError_t launch_expert_sort(const ExpertSortParams& p, hipStream_t st) {
     const int blocks = std::max(1, expert_sort_blocks(p.pairs));
     const size_t lds = (size_t)ES_WAVES * p.experts * 4;
+    const bool scan = scan_counts(blocks, p.experts);
+    const auto place = scan ? expert_place_kernel<true> : expert_place_kernel<false>;
     if (lds > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void*)expert_place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        const hipError_t e = hipFuncSetAttribute((const void*)place, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
     if (blocks > 1) {
@@ -502,7 +546,12 @@ hipError_t launch_expert_sort(const ExpertSortParams& p, hipStream_t st) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(expert_place_kernel, dim3(blocks), dim3(ES_THREADS), lds, st, p);
+    if (scan) {
+        hipLaunchKernelGGL(expert_scan_kernel, dim3((p.experts + 63) / 64), dim3(EX_THREADS), 0, st, p, blocks);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(place, dim3(blocks), dim3(ES_THREADS), lds, st, p);
     return hipGetLastError();
 }
 

@@ -48,6 +48,12 @@ def test_sort_is_the_stable_order(M, tokens, per_token, experts, kind):
         assert np.array_equal(got.cpu().numpy(), ref), name
 
 
+@pytest.mark.parametrize("kind", ["spread", "hot", "dropped", "none"])
+@pytest.mark.parametrize("tokens,per_token,experts", [(9001, 8, 4096), (150001, 7, 3), (131073, 8, 130)])
+def test_sort_of_many_pairs(M, tokens, per_token, experts, kind):
+    test_sort_is_the_stable_order(M, tokens, per_token, experts, kind)
+
+
 def test_sort_of_no_tokens(M):
     import torch
 
