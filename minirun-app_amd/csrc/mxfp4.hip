@@ -65,12 +65,12 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
 }
 
-// Wave `unit` of the grid takes values 512 MX_U (unit % per_row) .. of row
+// Wave `unit` (of this launch's from `first` on) takes values 512 MX_U (unit % per_row) .. of row
 // unit / per_row.  cols is a multiple of 32, so the four lanes of a block are
 // all inside the row or all past it.
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_quantize_kernel(Mxfp4QuantizeParams p, int64_t per_row) {
-    const int64_t unit = (int64_t)blockIdx.x * MX_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_quantize_kernel(Mxfp4QuantizeParams p, int64_t first, int64_t per_row) {
+    const int64_t unit = first + (int64_t)blockIdx.x * MX_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = p.rows == 1 ? 0 : unit / per_row;
     if (row >= p.rows) return;
     const int l = threadIdx.x & 63;
@@ -107,8 +107,8 @@ __global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_quantize_kernel(Mxfp4Quan
 // below byte 1 or 2, infinite where it passes the type's largest); NaN at byte
 // 255.  A lane owns a word: 8 values.
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_dequantize_kernel(Mxfp4DequantizeParams p, int64_t per_row) {
-    const int64_t unit = (int64_t)blockIdx.x * MX_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_dequantize_kernel(Mxfp4DequantizeParams p, int64_t first, int64_t per_row) {
+    const int64_t unit = first + (int64_t)blockIdx.x * MX_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = p.rows == 1 ? 0 : unit / per_row;
     if (row >= p.rows) return;
     const int l = threadIdx.x & 63;
@@ -168,10 +168,15 @@ int64_t mx_units(P& p, int64_t& stride, int64_t& per_row) {
 
 template <typename K, typename P>
 hipError_t mx_launch(K kern, const P& p, int64_t units, int64_t per_row, hipStream_t st) {
-    const int64_t grid = (units + MX_WAVES - 1) / MX_WAVES;
-    if (grid >= (1ll << 32) / (64 * MX_WAVES)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * MX_WAVES), 0, st, p, per_row);
-    return hipGetLastError();
+    // grids of less than 2^32 threads
+    constexpr int64_t MOST = (1ll << 23) * MX_WAVES;
+    for (int64_t first = 0; first < units; first += MOST) {
+        const int64_t grid = (std::min(MOST, units - first) + MX_WAVES - 1) / MX_WAVES;
+        hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * MX_WAVES), 0, st, p, first, per_row);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
