@@ -92,6 +92,10 @@ public func hipMXFP4ExpertMM(quantized x: HIPMXFP4Weights, _ w: HIPMXFP4Weights,
 
 private func hipExpertMM(_ a: inout mr_mxfp4_expert_args, _ w: HIPMXFP4Weights, _ order: HIPExpertOrder,
                          sortedRows: Bool, into y: HIPTensor, stream: HIPStream) throws {
+    guard w.experts == order.experts else {
+        throw HIPError(status: MR_INVALID_SHAPE,
+                       description: "the weight has \(w.experts ?? 0) experts, the order \(order.experts)")
+    }
     a.w = w.desc
     a.experts = Int32(order.experts)
     a.offsets = UnsafePointer(order.offsets.pointer.assumingMemoryBound(to: Int32.self))
