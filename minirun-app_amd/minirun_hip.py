@@ -626,6 +626,8 @@ def _call_stream(device, stream):
         handle = torch._C._cuda_getCurrentRawStream(device.index)
         return handle, _HERE if device.index == cuda.current_device() else cuda.device(device)
     if isinstance(stream, cuda.Stream):
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
         return stream.cuda_stream, cuda.stream(stream)
     handle = stream.value if isinstance(stream, C.c_void_p) else stream
     s = cuda.ExternalStream(handle, device) if handle else cuda.default_stream(device)
@@ -657,7 +659,7 @@ def _rows2d(t, name, shape=None):
     ld, step = t.stride()
     if step != 1 and t.shape[1] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    return ld if t.shape[0] > 1 and ld > 0 else max(ld, t.shape[1])
+    return ld if t.shape[0] > 1 else max(ld, t.shape[1])
 
 
 class MXFP4Weights:
@@ -796,6 +798,8 @@ def expert_sort(ids, experts, stream=None):
     if ids.dim() != 2:
         raise ValueError(f"ids must be [tokens, per_token], got {list(ids.shape)}")
     T, K = ids.shape
+    if max(T, K, abs(experts)) > 1 << 30:
+        raise ValueError(f"{T} tokens of {K} experts of {experts}")
     handle, ctx = _call_stream(ids.device, stream)
     lib = load()
     with ctx:

@@ -197,3 +197,23 @@ def test_python_checks_come_before_the_library():
             call()
     with pytest.raises(M.MRError, match="uint8"):
         M.MXFP4Weights(torch.zeros(4, 8, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32))
+
+
+def test_rows_of_a_tensor_need_a_stride():
+    """Repeated rows (stride 0) have no row stride that the library takes: it is
+    passed on as it is, and refused; one row may have any."""
+    import torch
+
+    class OnGPU(torch.Tensor):
+        is_cuda = True
+
+    def stride(t):
+        return M._rows2d(t.as_subclass(OnGPU), "x")
+
+    assert stride(torch.zeros(1, 64).expand(3, 64)) == 0
+    assert stride(torch.zeros(1, 64)) == 64
+    assert stride(torch.zeros(5, 64)[::5]) == 320
+    assert stride(torch.zeros(64).as_strided((1, 64), (0, 1))) == 64
+    assert stride(torch.zeros(3, 80)[:, :64]) == 80
+    with pytest.raises(ValueError):
+        stride(torch.zeros(3, 1).expand(3, 64))
