@@ -546,8 +546,10 @@ struct Mxfp4GemmParams {
 };
 
 constexpr int MXFP4_MAX_OUT = 1 << 22;  // weight rows of a product
-// tiles of 256 or 128 rows of x times as many weight rows (experts' rows: 128)
-hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int size, hipStream_t st);
+// tiles of 256 or 128 rows of x times as many weight rows (experts' rows: 128),
+// of 128 with two or (x in MXFP4) three workgroups a CU
+enum MxTiles { MX_TILES_NONE, MX_TILES_128x2, MX_TILES_128x3, MX_TILES_256 };
+hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, MxTiles kind, hipStream_t st);
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p);
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st);
 

@@ -562,15 +562,20 @@ hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
 //   x in MXFP4, which costs a quarter to read: 7168 x 16384, 64 tokens, 64 x 32
 //     with 8 waves 18.7, 64 x 64 24.4, 32 x 16 28; 128 tokens, 64 x 64 23.8, 64 x
 //     32 31; 24576 x 1536, 40 tokens, mid 64 x 32 8.0, 128 x 32 8.3
-//   experts by their mean rows (128 of 768 x 2048): 6 rows, mid 128 x 16 25.6,
-//     128 x 32 28.1; 19 rows, 36.5 and 32.0; MXFP4, 31 rows, mid 128 x 64 34.4,
-//     128 x 32 37.7; one token, 8 of 128, two rows of x staged 4.8, 16 rows 6.0
-bool few_pairs(const Mxfp4GemmParams& p) { return p.pairs <= 4096 && (int64_t)p.pairs * ((p.N + 15) / 16) < (1 << 23); }
+//   experts by their mean rows (128 of 768 x 2048, bf16): 6 rows, mid 128 x 16
+//     25.6, 128 x 32 28.1; 19 rows, 36.5 and 32.0
+// and few pairs, two rows of x staged per 16 weight rows, 8 of 128 experts 4.8,
+// mid 8.3; 64 pairs 10.9 and 11.5, 96 13.4 and 12.1; 2048 x 768, 4 pairs 4.3 and
+// 5.2, 16 pairs 6.6 and 5.4; 32 of 1536 x 7168, 24 pairs 20.8 and 23.5, 64 pairs 35
+// and 30; 192 x 1024, 64 pairs 5.0 and 6.0, 192 pairs 7.6 and 6.2.
+bool few_pairs(const Mxfp4GemmParams& p) {
+    return p.pairs <= 2 * p.experts && (int64_t)p.pairs * ((p.N + 15) / 16) * 4 <= 3 * (int64_t)p.K;
+}
 
 hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     const int entries = (p.K + 255) / 256;
     if (p.offsets) {
-        if (p.pairs <= 2 * p.experts && few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4>(p, st);
+        if (few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4>(p, st);
         return p.pairs <= 12 * p.experts ? launch_mid<0, 2, 1, 2, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
     }
     if (p.M <= 2) {
@@ -587,9 +592,8 @@ hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
 
 hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (p.offsets) {
-        if (p.pairs <= 2 * p.experts && few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4>(p, st);
-        if (p.pairs <= 8 * p.experts) return launch_mid<2, 2, 1, 2, 4>(p, st);
-        return p.pairs <= 24 * p.experts ? launch_mid<2, 2, 2, 2, 4>(p, st) : launch_mid<2, 2, 4, 2, 4>(p, st);
+        if (few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4>(p, st);
+        return p.pairs <= 8 * p.experts ? launch_mid<2, 2, 1, 2, 4>(p, st) : launch_mid<2, 2, 2, 2, 4>(p, st);
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
     if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 1, 8>(p, st);
@@ -614,36 +618,52 @@ hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     return p.x_kind == MX_X_F32 ? launch_few_f32(p, cus, st) : launch_few_bf16(p, cus, st);
 }
 
-// Rows and columns of a large tile (mxfp4_gemm.hip): 256, 128, or 0 for none.
-// One matrix: tiles of 128 (two workgroups a CU) pay once they cover the larger
-// part of the GPU and the kernels of few rows would read W more than once (bf16:
-// 24576 x 1536, 65 tokens, 192 tiles, 14 us and few rows 17, 64 tokens 14 and 11;
-// 7168 x 16384, 300 tokens, 168 tiles, 108 and 138, 200 tokens, 112 tiles, 107 and
-// 83; 16384 x 4096, 65 tokens, 128 tiles, 31 and 25; MXFP4: there 15 and 17, 64
-// tokens 15 and 11; 24576 x 1536, 37 tokens, 6.7 and 7.7; 1536 x 7168, 1000
-// tokens, 96 tiles, 19 and 24, 600 tokens, 60 tiles, 24 and 12).  A full round of
-// them takes 4/7 of one of 256 x 256, which read half as much: bf16, 24576 x 1536,
-// 600 tokens, 2 rounds 47 us, 2 of 256 74; 1000 tokens, 3 72, 2 of 256 77; 16384 x
-// 4096, 1000 tokens, 2 123, 1 of 256 106, MXFP4 46 and 40.
-// Experts (128 of 768 x 2048) by their mean rows: bf16 100 rows, 128 80, few rows
-// 86; 50 rows 63 and 55; MXFP4 50 rows 37 and 41, 31 rows 35 and 35; 256 rows 67,
-// 256 x 256 77.
-int tile_size(const Mxfp4GemmParams& p, int cus) {
-    if (p.x_kind == MX_X_F32) return 0;
+// Large tiles (mxfp4_gemm.hip), or none.  Those of 128 x 128 pay once they cover
+// the larger part of the GPU and the kernels of few rows would read W more than
+// once (us, 128 and few rows: bf16, 24576 x 1536, 65 tokens, 192 tiles, 14 and 17,
+// 64 tokens 14 and 11; 7168 x 16384, 300 tokens, 168 tiles, 107 and 135, 200
+// tokens, 112 tiles, 107 and 81; 16384 x 4096, 65 tokens, 128 tiles, 31 and 24;
+// MXFP4: there 15.5 and 16.6, 64 tokens 15.5 and 11.4; 24576 x 1536, 37 tokens,
+// 6.7 and 7.7; 1536 x 7168, 1000 tokens, 96 tiles, 19 and 24, 600 tokens, 60
+// tiles, 24 and 12), and for experts from some rows each (128 of 768 x 2048: bf16,
+// 62 rows, 45 and 50, 50 rows 44 and 45, 31 rows 42 and 35; 32 of 1536 x 7168, 88
+// rows, 85 and 98, 62 rows 82 and 76; MXFP4: 12 rows, 20 and 22).
+// Between the tiles, by rounds of workgroups, in units of a sixth of the time of a
+// round of two a CU (bf16: a last round of at most one a CU takes 4):
+// three a CU 8, 256 x 256 12 (MXFP4) or 10.5 (bf16).  MXFP4, three, two, 256:
+// 24576 x 1536, 300 tokens, 13.5, 16.2 and 16.7 us, 4096 tokens 96, 107 and 103;
+// 16384 x 4096, 1000 tokens, 46, 44 and 38; 4096 tokens to 8 of 128 experts of 768
+// x 2048 45 and 50; 1024 to 8 of 32 of 1536 x 7168 77 and 69.  bf16, two and 256:
+// 24576 x 1536, 600 tokens, 45 and 72, 4096 tokens 260 and 247; 16384 x 4096, 1000
+// tokens, 116 and 101.
+MxTiles tiles_of(const Mxfp4GemmParams& p, int cus) {
+    if (p.x_kind == MX_X_F32) return MX_TILES_NONE;
     const bool mx = p.x_kind == MX_X_MXFP4;
-    if (p.offsets) return p.pairs / p.experts < (mx ? 28 : 80) ? 0 : 128;
-    if (p.M <= (mx ? 32 : 64)) return 0;
-    auto tiles = [&](int size) { return (((int64_t)p.N + size - 1) / size) * (((int64_t)p.M + size - 1) / size); };
-    if (tiles(128) * 8 < (mx ? (p.M <= 64 ? 6 : 4) : 5) * cus) return 0;
-    const int64_t rounds128 = (tiles(128) + 2 * cus - 1) / (2 * cus), rounds256 = (tiles(256) + cus - 1) / cus;
-    return 7 * rounds256 <= 4 * rounds128 ? 256 : 128;
+    auto cols = [&](int size) { return ((int64_t)p.N + size - 1) / size; };
+    int64_t small;  // tiles of 128 (experts: about)
+    if (p.offsets) {
+        if (p.pairs < (mx ? 12 : 60) * (int64_t)p.experts) return MX_TILES_NONE;
+        small = cols(128) * (p.pairs <= 96 * p.experts ? std::min(p.experts, p.pairs) : p.pairs / 128 + p.experts / 2);
+    } else {
+        if (p.M <= (mx ? 32 : 64)) return MX_TILES_NONE;
+        small = cols(128) * (((int64_t)p.M + 127) / 128);
+    }
+    if (small * 8 < (!mx ? 5 : !p.offsets && p.M <= 64 ? 6 : 4) * cus) return MX_TILES_NONE;
+    const int64_t left = small % (2 * cus);
+    const int64_t two = small / (2 * cus) * 6 + (left == 0 ? 0 : left <= cus && !mx ? 4 : 6);
+    const int64_t three = mx ? (small + 3 * cus - 1) / (3 * cus) * 8 : INT64_MAX;
+    if (!p.offsets) {
+        const int64_t rounds = (cols(256) * (((int64_t)p.M + 255) / 256) + cus - 1) / cus;
+        if (mx ? 12 * rounds <= std::min(two, three) : 21 * rounds <= 2 * two) return MX_TILES_256;
+    }
+    return three <= two ? MX_TILES_128x3 : MX_TILES_128x2;
 }
 
 }  // namespace
 
 // as many workgroups as a routed call can need (of 256 threads, 16 rows of x and
-// 128 weight rows, or as many threads on fewer rows of few pairs) in a grid of
-// less than 2^32 threads
+// 128 weight rows; of few pairs no more than 2^20) in a grid of less than 2^32
+// threads
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
     return !p.offsets || (mx_tile_bound(p, 16) * ((p.N + 127) / 128) + 7) * 256 < (1ll << 32);
 }
@@ -652,7 +672,7 @@ bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
 // one, up to 2^23 workgroups of 16 tokens x 16 weight rows (MXFP4_MAX_OUT weight
 // rows leave 256 tokens each).
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st) {
-    const int tile = tile_size(p, cu_count);
+    const MxTiles tile = tiles_of(p, cu_count);
     if (p.offsets) return tile ? launch_mxfp4_tiles(p, tile, st) : launch_mxfp4_few(p, cu_count, st);
     const int64_t most = ((int64_t)1 << 23) / ((p.N + 15) / 16 + 8) * 16 / 256 * 256;
     for (int64_t m = 0; m < p.M; m += most) {

@@ -8,11 +8,13 @@
 // tiles; each operand fragment serves MI or JN of them.  With 256 x 256 (the
 // accumulators are half of the registers, one workgroup a CU) a prompt of 4096
 // tokens runs at 1.2 PFLOP/s in bf16 (24576 x 1536, 255 us) and 3.9 PFLOP/s in
-// MXFP4 (7168 x 16384, 245 us).  128 x 128 reads twice as much per operation, but
-// two workgroups a CU cover each other's waits, ends of tiles and starts: 4096
-// tokens to 8 of 128 experts of 768 x 2048, MXFP4, 67 us, with 128 x 256 and one
-// workgroup a CU 78 (of this, 31 us is the time of the bytes: eight stages a tile
-// leave the loads' and the barriers' latency in view).
+// MXFP4 (7168 x 16384, 245 us; 4.3 with the weights in the caches).  128 x 128
+// reads twice as much per operation, but two or three workgroups a CU cover each
+// other's waits, ends of tiles and starts: 4096 tokens to 8 of 128 experts of 768 x
+// 2048, MXFP4, three 62 us, two 67, with 128 x 256 and one workgroup 78 (31 us is
+// the time of the bytes; eight stages a tile leave latency in view: of the 30000
+// clocks of a tile with two workgroups 19000 were its stages', whose matrix
+// instructions take 5800, 7500 its start and 3500 its end).
 // Operands come by global -> LDS DMA, issued between the MFMAs.  A load costs by
 // the lines it touches, about two clocks each, whether it takes 4 or 128 bytes of
 // a line, so rows come in whole lines of 128 bytes and scales 16 bytes of a row
@@ -26,14 +28,20 @@
 //     The barrier that ends stage t, before its last step, frees its buffer:
 //     half of stage t + 2 is issued in that step, half in the next one, and two
 //     steps are left for it to land.  Scales come for two stages together.
+//     ONE: a ring of one.  The barrier after the reads of a stage's last step
+//     frees it, the next stage is issued at once, and what the MFMAs that follow
+//     leave of its way is the other workgroups' time.  It takes less LDS and fewer
+//     registers, which makes room for a third workgroup; where there are not that
+//     many, or for bf16 (a third one gained nothing there: 112 and 111 us), the
+//     ring of two is faster (7168 x 16384, 400 tokens, 49 and 57 us).
 //   x in bf16: a stage is 64 k: a line of each row of x, in a ring of three; W's
 //     rows come 64 bytes (two stages) at a time, in a ring of two.  Lane half h
 //     has block h of the stage's two: the block's four words, one per 16-deep
 //     step, become bf16 with their scale (exact) beside the MFMAs; for x, step s
 //     of half h takes the chunk 4 h + s.
-// Each step's fragments are read a step ahead; one barrier per stage.  Past the
-// last stage the issues repeat it into stages that are not read, or load zeros,
-// so that the waits are constants.  Chunk c of a 128-byte row r is in slot c ^
+// Each step's fragments are read a step ahead; one barrier per stage (ONE: two).
+// Past the last stage the issues repeat it into stages that are not read, or load
+// zeros, so that the waits are constants.  Chunk c of a 128-byte row r is in slot c ^
 // ((r >> 1) & 7), of a 64-byte one in c ^ ((r >> 2) & 3): the 16 lanes of a read
 // (16 neighbouring rows, one chunk) hit 16 bank groups.
 //
@@ -59,27 +67,29 @@ constexpr int MG_THREADS = 256;
 __device__ __forceinline__ int slot128(int r, int c) { return 8 * r + (c ^ ((r >> 1) & 7)); }
 __device__ __forceinline__ int slot64(int r, int c) { return 4 * r + (c ^ ((r >> 2) & 3)); }
 
-template <int XT, int TM, int TN, bool RAGGED>
+template <int XT, int TM, int TN, bool ONE, bool RAGGED>
 struct MgShape {
     static constexpr bool MX = XT == MX_X_MXFP4;
     static constexpr int A = TM * 128;                // bytes of x in a stage
     static constexpr int B = TN * (MX ? 128 : 64);    // of W in its pieces
-    static constexpr int NA = MX ? 2 : 3;             // stages of x in the ring; W and scales: 2
+    static constexpr int NA = MX ? (ONE ? 1 : 2) : 3, NB = ONE ? 1 : 2;  // stages of x in the ring, of W and the scales
+    static_assert(MX || !ONE, "one stage: MXFP4");
     // scales: 16 bytes (MXFP4: x's rows first) or 4 per row, and RAGGED the word
     // after them; rows in whole instructions of the four waves
     static constexpr int SROWS = MX ? (TM + TN + 255) / 256 * 256 : TN, SROW = MX ? 16 : 4;
     static constexpr int S = SROWS * (SROW + (RAGGED ? 4 : 0));
-    static constexpr int RING = NA * A + 2 * B + 2 * S;
+    static constexpr int RING = NA * A + NB * B + NB * S;
     // DMA instructions per wave: x and W of a stage or piece, scales
     static constexpr int DA = A / 4096, DB = B / 4096, SQ = MX ? SROWS / 256 : 1, DS = SQ * (RAGGED ? 2 : 1);
     static constexpr size_t LDS_BF16 = std::max<size_t>(RING, (size_t)TM * TN * 2);
     static constexpr size_t LDS_F32 = std::max<size_t>(RING, (size_t)TM / 2 * TN * 4);
-    static_assert(LDS_BF16 <= 163840 && LDS_F32 <= 163840, "LDS");
+    static constexpr int PER_CU = TN == 256 ? 1 : (ONE ? 3 : 2);  // workgroups
+    static_assert(PER_CU * LDS_BF16 <= 163840 && PER_CU * LDS_F32 <= 163840, "LDS");
 };
 
-template <int XT, int TM, int TN, bool ROUTED, bool YF32, bool RAGGED>
-__global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kernel(Mxfp4GemmParams p) {
-    using S = MgShape<XT, TM, TN, RAGGED>;
+template <int XT, int TM, int TN, bool ONE, bool ROUTED, bool YF32, bool RAGGED>
+__global__ void __launch_bounds__(MG_THREADS, (MgShape<XT, TM, TN, ONE, RAGGED>::PER_CU)) mxfp4_gemm_kernel(Mxfp4GemmParams p) {
+    using S = MgShape<XT, TM, TN, ONE, RAGGED>;
     constexpr bool MX = S::MX;
     constexpr int DA = S::DA, DB = S::DB, DS = S::DS, SQ = S::SQ;
     constexpr int WM = TM / 2, MI = WM / 32;  // rows and 32-row MFMA tiles per wave
@@ -221,7 +231,7 @@ __global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kern
         uint32_t a[MX ? MI : 1], b[JN];
     };
     char* const ring_b = lds + S::NA * S::A;
-    char* const ring_s = ring_b + 2 * S::B;
+    char* const ring_s = ring_b + S::NB * S::B;
     auto read_a = [&](const char* st, int ks, Frag& f) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) f.a[i] = *(const u32x4*)(st + 16 * slot128(wm * WM + i * 32 + (l & 31), 4 * h + ks));
@@ -246,7 +256,7 @@ __global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kern
         };
         // stage t's word of row r: of the group's four, number 2 (t % 2) + h
         auto word = [&](int t, int r, uint32_t sh) -> uint32_t {
-            const char* st = ring_s + ((t >> 1) & 1) * S::S;
+            const char* st = ring_s + (ONE ? 0 : (t >> 1) & 1) * S::S;
             const int d = 2 * (t & 1) + h;
             const uint32_t v = *(const uint32_t*)(st + 16 * r + 4 * d);
             if constexpr (!RAGGED) return v;
@@ -265,9 +275,9 @@ __global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kern
         constexpr int NQ = DA + DB, H0 = NQ / 2;  // instructions of a stage; those that go with its predecessor's last step
         auto dma = [&](int t, int q) {
             if (q < DA)
-                dma_a(t, lds + (t & 1) * S::A, q);
+                dma_a(t, lds + (ONE ? 0 : t & 1) * S::A, q);
             else
-                dma_b(t, ring_b + (t & 1) * S::B, q - DA);
+                dma_b(t, ring_b + (ONE ? 0 : t & 1) * S::B, q - DA);
         };
         auto step = [&](const Frag& f, const Scales& s, auto ks_, int n, auto issue) {
             constexpr int ks = decltype(ks_)::value;
@@ -279,6 +289,39 @@ __global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kern
             }
         };
         auto none = [](int) {};
+        if constexpr (ONE) {
+            auto load = [&](int t) {
+                if (!(t & 1)) {
+#pragma unroll
+                    for (int q = 0; q < DS; ++q) dma_s(t >> 1, ring_s, q);
+                }
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) dma(t, q);
+            };
+            load(0);
+#pragma unroll 1
+            for (int t = 0; t < AT; ++t) {
+                wait_vmcnt<0>();
+                lds_barrier();  // the stage has landed
+                Scales& now = sg[0];
+                read_scales(t, now);
+                auto read = [&](int ks) {
+                    read_a(lds, ks, fr[0]);
+                    read_b(ring_b, ks, fr[0]);
+                };
+                read(0);
+                step(fr[0], now, std::integral_constant<int, 0>{}, 0, none);
+                read(1);
+                step(fr[0], now, std::integral_constant<int, 1>{}, 0, none);
+                read(2);
+                step(fr[0], now, std::integral_constant<int, 2>{}, 0, none);
+                read(3);
+                lds_barrier();  // every wave has read it
+                if (t + 1 < AT) load(t + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                step(fr[0], now, std::integral_constant<int, 3>{}, 0, none);
+            }
+        } else {
 #pragma unroll
         for (int q = 0; q < DS; ++q) dma_s(0, ring_s, q);
 #pragma unroll
@@ -319,6 +362,7 @@ __global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kern
             stage(t + 1, sg[1], sg[0]);
         }
         if (t < AT) stage(t, sg[0], sg[1]);
+        }
     } else {
         struct Weights {
             u32x4 b[JN];
@@ -481,11 +525,11 @@ __global__ void __launch_bounds__(MG_THREADS, TN == 256 ? 1 : 2) mxfp4_gemm_kern
     }
 }
 
-template <int XT, int TM, int TN, bool ROUTED, bool YF32, bool RAGGED>
+template <int XT, int TM, int TN, bool ONE, bool ROUTED, bool YF32, bool RAGGED>
 hipError_t mg_launch(const Mxfp4GemmParams& p, hipStream_t st) {
-    using S = MgShape<XT, TM, TN, RAGGED>;
+    using S = MgShape<XT, TM, TN, ONE, RAGGED>;
     constexpr size_t lds = YF32 ? S::LDS_F32 : S::LDS_BF16;
-    const auto kern = mxfp4_gemm_kernel<XT, TM, TN, ROUTED, YF32, RAGGED>;
+    const auto kern = mxfp4_gemm_kernel<XT, TM, TN, ONE, ROUTED, YF32, RAGGED>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
     const int64_t n_tiles = (p.N + TN - 1) / TN;
@@ -495,26 +539,27 @@ hipError_t mg_launch(const Mxfp4GemmParams& p, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <int XT, int TM, int TN, bool ROUTED>
+template <int XT, int TM, int TN, bool ONE, bool ROUTED>
 hipError_t mg_launch_y(const Mxfp4GemmParams& p, hipStream_t st) {
     const bool ragged = p.K % (XT == MX_X_MXFP4 ? 256 : 128) || ((uintptr_t)p.scales & 3) || ((uintptr_t)p.x_scales & 3);
-    if (p.y_f32) return ragged ? mg_launch<XT, TM, TN, ROUTED, true, true>(p, st) : mg_launch<XT, TM, TN, ROUTED, true, false>(p, st);
-    return ragged ? mg_launch<XT, TM, TN, ROUTED, false, true>(p, st) : mg_launch<XT, TM, TN, ROUTED, false, false>(p, st);
+    if (p.y_f32)
+        return ragged ? mg_launch<XT, TM, TN, ONE, ROUTED, true, true>(p, st) : mg_launch<XT, TM, TN, ONE, ROUTED, true, false>(p, st);
+    return ragged ? mg_launch<XT, TM, TN, ONE, ROUTED, false, true>(p, st) : mg_launch<XT, TM, TN, ONE, ROUTED, false, false>(p, st);
 }
 
-template <int XT, int TM, int TN>
-hipError_t mg_launch_r(const Mxfp4GemmParams& p, hipStream_t st) {
-    if constexpr (TM == 128) {  // experts' rows run in small tiles only
-        if (p.offsets) return mg_launch_y<XT, TM, TN, true>(p, st);
-    }
-    return mg_launch_y<XT, TM, TN, false>(p, st);
+template <int XT, bool ONE>
+hipError_t mg_launch_128(const Mxfp4GemmParams& p, hipStream_t st) {
+    return p.offsets ? mg_launch_y<XT, 128, 128, ONE, true>(p, st) : mg_launch_y<XT, 128, 128, ONE, false>(p, st);
 }
 
 }  // namespace
 
-hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, int size, hipStream_t st) {
-    if (p.x_kind == MX_X_MXFP4) return size == 256 ? mg_launch_r<MX_X_MXFP4, 256, 256>(p, st) : mg_launch_r<MX_X_MXFP4, 128, 128>(p, st);
-    return size == 256 ? mg_launch_r<MX_X_BF16, 256, 256>(p, st) : mg_launch_r<MX_X_BF16, 128, 128>(p, st);
+hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, MxTiles kind, hipStream_t st) {
+    if (p.x_kind == MX_X_MXFP4) {
+        if (kind == MX_TILES_256) return mg_launch_y<MX_X_MXFP4, 256, 256, false, false>(p, st);
+        return kind == MX_TILES_128x3 ? mg_launch_128<MX_X_MXFP4, true>(p, st) : mg_launch_128<MX_X_MXFP4, false>(p, st);
+    }
+    return kind == MX_TILES_256 ? mg_launch_y<MX_X_BF16, 256, 256, false, false>(p, st) : mg_launch_128<MX_X_BF16, false>(p, st);
 }
 
 }  // namespace mr
