@@ -292,7 +292,8 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
 // stages of 256 k (x once, W and its scales per wave), one barrier per stage: it
 // says that every wave's part of the stage has landed and that the slot of the
 // last one is free, into which stage s + S - 1 then goes.  Up to S - 1 stages are
-// in flight.  No sum crosses a wave.
+// in flight.  S = 1: a second barrier, after the reads of a stage, frees it for the
+// next, and the workgroups of a CU cover each other's waits.  No sum crosses a wave.
 template <int XT, int RT, int TT, int S, int NW>
 struct MidShape {
     using X = XEntry<XT>;
@@ -303,7 +304,7 @@ struct MidShape {
     static constexpr int WAVE = 2048 * RT + 1024 + 1024 * XS;  // bytes of a wave's part
     static constexpr int STAGE = 1024 * XI + NW * WAVE;
     static constexpr size_t LDS = (size_t)S * STAGE;
-    static_assert(S >= 2 && (S - 1) * NI < 64 && LDS <= 163840 && RT <= 4 && TT <= 4, "stages");
+    static_assert((S - 1) * NI < 64 && LDS <= 163840 && RT <= 4 && TT <= 4, "stages");
 };
 
 template <int XT, int RT, int TT, int S, int NW, bool ROUTED>
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
 #pragma unroll
     for (int r = 0; r < RT; ++r) wsh[r] = ((ws0 + (uint32_t)(16 * r + lr) * srow) & 3u) + 2u * q;
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue(s, s);
+    for (int s = 0; s < (S == 1 ? 1 : S - 1); ++s) issue(s, s);
     auto scale_bytes = [&](const char* row, uint32_t at, bool in0, bool in1) -> uint32_t {
         const uint32_t* v = (const uint32_t*)row + (at >> 2);
         const uint32_t d = __builtin_amdgcn_alignbyte(v[1], v[0], at & 3u);
@@ -412,9 +413,9 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
     int slot = 0;
 #pragma unroll 1
     for (int s = 0; s < nst; ++s) {
-        wait_vmcnt<(S - 2) * F::NI>();
+        wait_vmcnt<(S == 1 ? 0 : S - 2) * F::NI>();
         lds_barrier();
-        issue(s + S - 1, slot ? slot - 1 : S - 1);
+        if constexpr (S > 1) issue(s + S - 1, slot ? slot - 1 : S - 1);
         const char* e = lds + slot * F::STAGE;
         const char* ew = e + woff;
         const uint32_t k0 = 256u * s + 64u * q;
@@ -445,6 +446,11 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
 #pragma unroll
                 for (int c = 0; c < XF; ++c)
                     fx[t][c] = *(const u32x4*)(e + X::BYTES * (16 * t + lr) + 16 * ((XF * (2 * q + u) + c) ^ X::swizzle(16 * t + lr)));
+            if (S == 1 && u == 1) {
+                lds_barrier();  // every wave has read the stage
+                if (s + 1 < nst) issue(s + 1, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             // W is the first operand: a lane then holds four outputs of one row of y
             if constexpr (XT == MX_X_MXFP4) {
 #pragma unroll
@@ -557,13 +563,18 @@ hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
 //     8.4, mid 128 x 32 over 20; 1536 x 7168, 64 tokens, 32 x 16 with 8 waves
 //     8.5, 4 waves 10.9, 16 x 16 12.3; 128 tokens, 4 waves 12.5, 8 waves 14.7;
 //     7168 x 16384, 64 tokens, 64 x 16 with 4 waves 33, 32 x 16 43, mid 46; 24576
-//     x 1536, 40 tokens, mid 11.5, 64 x 16 17 (19 rows of x each read by 1536
-//     workgroups of 16 rows before)
+//     x 1536, 37 tokens, mid 64 x 48 10.5, 128 x 32 11.3, 64 x 16 17
 //   x in MXFP4, which costs a quarter to read: 7168 x 16384, 64 tokens, 64 x 32
 //     with 8 waves 18.7, 64 x 64 24.4, 32 x 16 28; 128 tokens, 64 x 64 23.8, 64 x
-//     32 31; 24576 x 1536, 40 tokens, mid 64 x 32 8.0, 128 x 32 8.3
-//   experts by their mean rows (128 of 768 x 2048, bf16): 6 rows, mid 128 x 16
-//     25.6, 128 x 32 28.1; 19 rows, 36.5 and 32.0
+//     32 31; 12000 x 1024, 100 tokens, mid 128 x 32 6.0, 128 x 64 6.9
+//   experts by their mean rows, x in bf16: 128 of 2048 x 768, 6 rows, mid 128 x 16
+//     20.2, 128 x 32 22.4, 12 rows 21.2 and 22.9, 19 rows 25.5 and 24.0; one stage
+//     in the ring, which leaves room for four or five workgroups a CU, where there
+//     are more than two a CU: these, with two stages 24.1, 28.1 (12 rows, 128 x
+//     32) and 29.3; 32 of 1536 x 7168, 6 rows, 384 workgroups, 34.0 and 31.0
+//   MXFP4, with two waves: 128 of 2048 x 768, 9 rows, 64 x 16 18.9, 128 x 16 19.3
+//     (two stages 23.9), 16 rows, 64 x 32 20.9, 64 x 16 21.1; 32 of 1536 x 7168, 12
+//     rows, 29.3 and 34.4; 24576 x 1536, 16 tokens, 64 x 16 5.5, 64 x 32 6.4
 // and few pairs, two rows of x staged per 16 weight rows, 8 of 128 experts 4.8,
 // mid 8.3; 64 pairs 10.9 and 11.5, 96 13.4 and 12.1; 2048 x 768, 4 pairs 4.3 and
 // 5.2, 16 pairs 6.6 and 5.4; 32 of 1536 x 7168, 24 pairs 20.8 and 23.5, 64 pairs 35
@@ -572,11 +583,17 @@ bool few_pairs(const Mxfp4GemmParams& p) {
     return p.pairs <= 2 * p.experts && (int64_t)p.pairs * ((p.N + 15) / 16) * 4 <= 3 * (int64_t)p.K;
 }
 
+// about how many tiles of 128 weight rows x `bm` rows of x a routed call has
+int64_t routed_tiles(const Mxfp4GemmParams& p, int bm) {
+    return ((int64_t)p.N + 127) / 128 * (p.pairs * 4ll <= p.experts * 3ll * bm ? std::min(p.experts, p.pairs) : p.pairs / bm + p.experts / 2);
+}
+
 hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     const int entries = (p.K + 255) / 256;
     if (p.offsets) {
         if (few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4>(p, st);
-        return p.pairs <= 12 * p.experts ? launch_mid<0, 2, 1, 2, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
+        if (p.pairs <= 12 * p.experts) return routed_tiles(p, 16) > 2 * cus ? launch_mid<0, 2, 1, 1, 4>(p, st) : launch_mid<0, 2, 1, 2, 4>(p, st);
+        return routed_tiles(p, 32) > 2 * cus ? launch_mid<0, 2, 2, 1, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
     }
     if (p.M <= 2) {
         if (entries >= 16) return launch_few<0, 1, 1, 1, 1, 8>(p, st);
@@ -587,13 +604,14 @@ hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (n32 * b <= cus) return launch_few<0, 2, 1, 8, 1, 8>(p, st);
     if (n32 * b <= 2 * cus) return launch_few<0, 2, 1, 8, 1, 4>(p, st);
     if (n64 * b <= 2 * cus) return launch_few<0, 4, 1, 8, 1, 4>(p, st);
-    return b == 1 ? launch_mid<0, 2, 1, 2, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
+    if (b == 1) return launch_mid<0, 2, 1, 2, 4>(p, st);
+    return b == 3 && p.K <= 2048 ? launch_mid<0, 1, 3, 1, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
 }
 
 hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (p.offsets) {
         if (few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4>(p, st);
-        return p.pairs <= 8 * p.experts ? launch_mid<2, 2, 1, 2, 4>(p, st) : launch_mid<2, 2, 2, 2, 4>(p, st);
+        return p.pairs <= 10 * p.experts ? launch_mid<2, 2, 1, 1, 2>(p, st) : launch_mid<2, 2, 2, 1, 2>(p, st);
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
     if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 1, 8>(p, st);
@@ -601,16 +619,22 @@ hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (n32 * b <= cus) return launch_few<2, 2, 1, 2, 1, 8>(p, st);
     if (n64 * ((b + 1) / 2) <= cus) return launch_few<2, 4, 2, 4, 1, 8>(p, st);
     if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 8>(p, st);
-    return b <= 4 ? launch_mid<2, 1, 2, 2, 4>(p, st) : launch_mid<2, 2, 4, 2, 4>(p, st);
+    return b <= 4 ? launch_mid<2, 2, 1, 1, 2>(p, st) : launch_mid<2, 2, 2, 1, 4>(p, st);
 }
 
 // f32: the cuts of x cost more than its bytes, so a cut serves 32 or 64 weight
-// rows (24576 x 1536: one token 16 us with 16 rows; 16 tokens, mid 128 x 16
-// 17.6, 64 x 16 21.4; 1536 x 7168, 64 tokens, 32 x 16 with 4 waves 23, mid 66)
+// rows where there are workgroups enough (mid 64 and 32 rows a wave: 24576 x 1536,
+// 37 tokens, 576 tiles of 128, 29 and 32 us, 5 tokens 19 and 16.6; 128 experts of
+// 768 x 2048, 12 rows, 40 and 53; 64 of 512 x 512, one row, 9.0 and 8.1); few of
+// them split K instead: 1536 x 7168, 64 tokens, 32 x 16 with 4 waves 23, mid 62,
+// 2048 x 2048 9 and 20
 hipError_t launch_few_f32(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (!p.offsets && p.M == 1) return launch_few<1, 4, 1, 1, 1, 4>(p, st);
-    if (!p.offsets && p.K > 4096 && (int64_t)((p.N + 31) / 32) * ((p.M + 15) / 16) <= 2 * cus) return launch_few<1, 2, 1, 16, 1, 4>(p, st);
-    return launch_mid<1, 2, 1, 2, 4>(p, st);
+    const int64_t b = ((int64_t)p.M + 15) / 16;
+    if (!p.offsets && (p.N + 31) / 32 * b <= 2 * cus) return launch_few<1, 2, 1, 16, 1, 4>(p, st);
+    const int64_t tiles = p.offsets ? routed_tiles(p, 16) : (p.N + 127) / 128 * b;
+    if (2 * tiles <= cus) return launch_mid<1, 1, 1, 1, 4>(p, st);
+    return tiles <= cus ? launch_mid<1, 2, 1, 1, 4>(p, st) : launch_mid<1, 4, 1, 1, 4>(p, st);
 }
 
 hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
@@ -626,8 +650,9 @@ hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
 // MXFP4: there 15.5 and 16.6, 64 tokens 15.5 and 11.4; 24576 x 1536, 37 tokens,
 // 6.7 and 7.7; 1536 x 7168, 1000 tokens, 96 tiles, 19 and 24, 600 tokens, 60
 // tiles, 24 and 12), and for experts from some rows each (128 of 768 x 2048: bf16,
-// 62 rows, 45 and 50, 50 rows 44 and 45, 31 rows 42 and 35; 32 of 1536 x 7168, 88
-// rows, 85 and 98, 62 rows 82 and 76; MXFP4: 12 rows, 20 and 22).
+// 62 rows, 45 and 46, 50 rows 44 and 38, 31 rows 42 and 31; 32 of 1536 x 7168, 88
+// rows, 85 and 98, 62 rows 82 and 76; MXFP4: 31 rows, 22.0 and 23.9, 19 rows 20.5
+// and 19.6).
 // Between the tiles, by rounds of workgroups, in units of a sixth of the time of a
 // round of two a CU (bf16: a last round of at most one a CU takes 4):
 // three a CU 8, 256 x 256 12 (MXFP4) or 10.5 (bf16).  MXFP4, three, two, 256:
@@ -640,10 +665,10 @@ MxTiles tiles_of(const Mxfp4GemmParams& p, int cus) {
     if (p.x_kind == MX_X_F32) return MX_TILES_NONE;
     const bool mx = p.x_kind == MX_X_MXFP4;
     auto cols = [&](int size) { return ((int64_t)p.N + size - 1) / size; };
-    int64_t small;  // tiles of 128 (experts: about)
+    int64_t small;  // tiles of 128
     if (p.offsets) {
-        if (p.pairs < (mx ? 12 : 60) * (int64_t)p.experts) return MX_TILES_NONE;
-        small = cols(128) * (p.pairs <= 96 * p.experts ? std::min(p.experts, p.pairs) : p.pairs / 128 + p.experts / 2);
+        if (p.pairs < (mx ? 24 : 60) * (int64_t)p.experts) return MX_TILES_NONE;
+        small = routed_tiles(p, 128);
     } else {
         if (p.M <= (mx ? 32 : 64)) return MX_TILES_NONE;
         small = cols(128) * (((int64_t)p.M + 127) / 128);

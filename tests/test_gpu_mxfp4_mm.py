@@ -85,7 +85,7 @@ def test_whole_numbers_are_exact(M, out, inp, kind):
 WIDE = [(1, 300, 544), (2, 300, 4128), (20, 300, 288), (10, 4104, 288), (40, 2056, 544), (100, 2056, 160), (100, 4000, 288),
         (100, 4104, 256), (40, 16392, 96), (10, 33000, 96), (100, 8200, 2080), (20, 300, 4128), (100, 16392, 288),
         (200, 16392, 288), (300, 16392, 512), (600, 16392, 256), (600, 16385, 288), (700, 16390, 32), (1100, 8190, 416),
-        (1000, 16384, 512), (1000, 16300, 288)]
+        (1000, 16384, 512), (1000, 16300, 288), (100, 8200, 544), (20, 8200, 96)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -252,7 +252,8 @@ def test_offsets_past_32_bits(M):
 EXPERTS = [(1, 1, 1, 7, 32), (1, 8, 128, 96, 256), (5, 2, 3, 33, 96), (40, 3, 9, 160, 160), (200, 8, 32, 264, 512),
            (700, 4, 5, 512, 288), (64, 6, 257, 48, 64), (1500, 2, 4, 300, 1024), (40, 4, 40, 136, 544), (90, 8, 60, 520, 288),
            (260, 8, 60, 264, 96), (300, 8, 60, 600, 544), (500, 8, 60, 392, 512), (500, 8, 60, 520, 288),
-           (260, 8, 100, 700, 256), (260, 8, 100, 700, 288), (3, 2, 9, 48, 1024), (7, 4, 14, 40, 544)]
+           (260, 8, 100, 700, 256), (260, 8, 100, 700, 288), (3, 2, 9, 48, 1024), (7, 4, 14, 40, 544),
+           (100, 4, 150, 500, 160), (30, 4, 60, 340, 96)]
 
 
 @pytest.mark.parametrize("ids", ["spread", "hot", "one", "dropped", "none", "twice"])
