@@ -20,6 +20,7 @@
 // find A by two DPP steps.  Each lane has the loads of MX_U such pieces in
 // flight before it uses the first.
 #include <algorithm>
+#include <type_traits>
 
 #include "mr_kernels.hpp"
 
@@ -30,34 +31,49 @@ namespace {
 constexpr int MX_U = 4;      // pieces of 512 values per wave
 constexpr int MX_WAVES = 4;  // waves per workgroup
 
-// eight values of a row as f32 bit patterns (bf16: in the high halves)
-struct MxEight {
-    uint32_t v[8];
-};
-
+// Eight values of a row as stored, from or to a buffer at a byte offset.  What lies
+// past the end of a buffer is zeros or is not stored, without a branch, behind
+// which the compiler would wait for the loads before it.
 template <bool F32, bool VEC>
-__device__ __forceinline__ MxEight mx_load8(const void* p, int64_t i) {
-    MxEight r;
-    if constexpr (F32) {
-        if constexpr (VEC) {
-            const u32x4 a = ((const u32x4*)((const uint32_t*)p + i))[0], b = ((const u32x4*)((const uint32_t*)p + i))[1];
+struct MxEight {
+    using Elem = std::conditional_t<F32, uint32_t, uint16_t>;
+    static constexpr int N16 = F32 ? 2 : 1, SIZE = F32 ? 4 : 2;
+    std::conditional_t<VEC, u32x4[N16], Elem[8]> v;
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t row, int at) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) r.v[k] = a[k], r.v[4 + k] = b[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) r.v[k] = ((const uint32_t*)p)[i + k];
-        }
-    } else {
-        if constexpr (VEC) {
-            const u32x4 a = *(const u32x4*)((const uint16_t*)p + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) r.v[2 * k] = a[k] << 16, r.v[2 * k + 1] = a[k] & 0xffff0000u;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) r.v[k] = (uint32_t)((const uint16_t*)p)[i + k] << 16;
+        for (int k = 0; k < (VEC ? N16 : 8); ++k) {
+            if constexpr (VEC)
+                v[k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(row, at + 16 * k, 0, 0));
+            else if constexpr (F32)
+                v[k] = __builtin_amdgcn_raw_buffer_load_b32(row, at + 4 * k, 0, 0);
+            else
+                v[k] = __builtin_amdgcn_raw_buffer_load_b16(row, at + 2 * k, 0, 0);
         }
     }
-    return r;
+    // value k's bits as those of an f32
+    __device__ __forceinline__ uint32_t bits(int k) const {
+        if constexpr (!VEC)
+            return F32 ? (uint32_t)v[k] : (uint32_t)v[k] << 16;
+        else if constexpr (F32)
+            return v[k >> 2][k & 3];
+        else
+            return k & 1 ? v[0][k >> 1] & 0xffff0000u : v[0][k >> 1] << 16;
+    }
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, int at) const {
+#pragma unroll
+        for (int k = 0; k < (VEC ? N16 : 8); ++k) {
+            if constexpr (VEC)
+                __builtin_amdgcn_raw_buffer_store_b128(v[k], row, at + 16 * k, 0, 0);
+            else if constexpr (F32)
+                __builtin_amdgcn_raw_buffer_store_b32(v[k], row, at + 4 * k, 0, 0);
+            else
+                __builtin_amdgcn_raw_buffer_store_b16(v[k], row, at + 2 * k, 0, 0);
+        }
+    }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, int64_t bytes_before, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((char*)p + bytes_before, 0, bytes, 0x00020000);
 }
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
@@ -74,32 +90,33 @@ __global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_quantize_kernel(Mxfp4Quan
     const int64_t row = p.rows == 1 ? 0 : unit / per_row;
     if (row >= p.rows) return;
     const int l = threadIdx.x & 63;
-    const int64_t c0 = (unit - row * per_row) * (512 * MX_U) + 8 * l;
-    const char* x = (const char*)p.x + row * p.x_stride * (F32 ? 4 : 2);
-    MxEight v[MX_U];
+    const int64_t c0 = (unit - row * per_row) * (512 * MX_U), o = row * p.cols + c0;
+    if (c0 >= p.cols) return;  // (one long row: a wave past its end)
+    const int n = (int)min(p.cols - c0, (int64_t)512 * MX_U);  // of this wave
+    using E = MxEight<F32, VEC>;
+    const __amdgpu_buffer_rsrc_t x = mx_buffer(p.x, (row * p.x_stride + c0) * E::SIZE, n * E::SIZE);
+    const __amdgpu_buffer_rsrc_t packed = mx_buffer(p.packed, o / 2, n / 2), scales = mx_buffer(p.scales, o / 32, n / 32);
+    E v[MX_U];
 #pragma unroll
-    for (int u = 0; u < MX_U; ++u)
-        if (c0 + 512 * u < p.cols) v[u] = mx_load8<F32, VEC>(x, c0 + 512 * u);
+    for (int u = 0; u < MX_U; ++u) v[u].load(x, (512 * u + 8 * l) * E::SIZE);
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
-        const int64_t c = c0 + 512 * u;
-        if (c >= p.cols) return;
         uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, v[u].v[k] & 0x7fffffffu);
+        for (int k = 0; k < 8; ++k) top = max(top, v[u].bits(k) & 0x7fffffffu);
         top = quad_max(top);
         const bool finite = top < 0x7f800000u;
         const uint32_t e = top >> 23, byte = finite ? (e > 2 ? e - 2 : 0) : 255u;
         const float scale = __uint_as_float(finite ? byte << 23 : 0x3f800000u);
-        auto f = [&](int k) { return __uint_as_float(v[u].v[k]); };
+        auto f = [&](int k) { return __uint_as_float(v[u].bits(k)); };
         uint32_t w = 0;
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(0), f(1), scale, 0);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(2), f(3), scale, 1);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(4), f(5), scale, 2);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f(6), f(7), scale, 3);
-        const int64_t o = row * p.cols + c;
-        p.packed[o >> 3] = finite ? w : 0u;
-        if ((l & 3) == 0) p.scales[o >> 5] = (uint8_t)byte;
+        __builtin_amdgcn_raw_buffer_store_b32(finite ? w : 0u, packed, 256 * u + 4 * l, 0, 0);
+        // (one lane of a block's four; the others' offset is past the end)
+        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, scales, l & 3 ? 64 * MX_U : 16 * u + l / 4, 0, 0);
     }
 }
 
@@ -112,45 +129,45 @@ __global__ void __launch_bounds__(64 * MX_WAVES) mxfp4_dequantize_kernel(Mxfp4De
     const int64_t row = p.rows == 1 ? 0 : unit / per_row;
     if (row >= p.rows) return;
     const int l = threadIdx.x & 63;
-    const int64_t c0 = (unit - row * per_row) * (512 * MX_U) + 8 * l;
+    const int64_t c0 = (unit - row * per_row) * (512 * MX_U), o = row * p.cols + c0;
+    if (c0 >= p.cols) return;  // (one long row: a wave past its end)
+    const int n = (int)min(p.cols - c0, (int64_t)512 * MX_U);  // of this wave
+    using E = MxEight<F32, VEC>;
+    const __amdgpu_buffer_rsrc_t out = mx_buffer(p.out, (row * p.out_stride + c0) * E::SIZE, n * E::SIZE);
+    const __amdgpu_buffer_rsrc_t packed = mx_buffer(p.packed, o / 2, n / 2), scales = mx_buffer(p.scales, o / 32, n / 32);
     uint32_t w[MX_U];
     uint32_t b[MX_U];
 #pragma unroll
-    for (int u = 0; u < MX_U; ++u)
-        if (c0 + 512 * u < p.cols) {
-            const int64_t o = row * p.cols + c0 + 512 * u;
-            w[u] = p.packed[o >> 3];
-            b[u] = p.scales[o >> 5];
-        }
+    for (int u = 0; u < MX_U; ++u) {
+        w[u] = __builtin_amdgcn_raw_buffer_load_b32(packed, 256 * u + 4 * l, 0, 0);
+        b[u] = __builtin_amdgcn_raw_buffer_load_b8(scales, 16 * u + l / 4, 0, 0);
+    }
 #pragma unroll
     for (int u = 0; u < MX_U; ++u) {
-        const int64_t c = c0 + 512 * u;
-        if (c >= p.cols) return;
         const float scale = __uint_as_float(b[u] << 23);
-        const int64_t o = row * p.out_stride + c;
+        E y;
         if constexpr (F32) {
             const f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 0),
                                 __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 1),
                                 __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 2),
                                 __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 3)};
-            float* out = (float*)p.out + o;
-            if constexpr (VEC) {
-                ((f32x4*)out)[0] = f32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
-                ((f32x4*)out)[1] = f32x4{v[2][0], v[2][1], v[3][0], v[3][1]};
-            } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) out[k] = v[k >> 1][k & 1];
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (VEC)
+                    y.v[k >> 2][k & 3] = __float_as_uint(v[k >> 1][k & 1]);
+                else
+                    y.v[k] = __float_as_uint(v[k >> 1][k & 1]);
             }
         } else {
             const u32x4 v = __builtin_bit_cast(u32x4, mxfp4_bf16(w[u], scale));
-            uint16_t* out = (uint16_t*)p.out + o;
             if constexpr (VEC) {
-                *(u32x4*)out = v;
+                y.v[0] = v;
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) out[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+                for (int k = 0; k < 8; ++k) y.v[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
             }
         }
+        y.store(out, (512 * u + 8 * l) * E::SIZE);
     }
 }
 
