@@ -334,10 +334,12 @@ mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_
 /* y[t, :] = x[t, :] . W^T for a matrix W [out, in] = w (the MXFP4 sibling of
  * mr_affine_matmul): x [tokens, in] bf16 or f32 with row stride x_stride; y
  * [tokens, out] bf16 or f32 with row stride y_stride; f32 sums.  Weights are
- * taken exactly; f32 activations too (as three bf16 parts).  x is 16-byte
- * aligned with rows a multiple of 16 and at most 2^23 bytes apart, w->packed
- * 16-byte aligned; out is at most 2^22, in 2^20.  The order of a token's sums, and so its last bits,
- * depends on how many tokens the call has. */
+ * taken as mr_mxfp4_dequantize gives them in bf16 (exact but for infinities at
+ * bytes 253 and 254); f32 activations exactly too (as three bf16 parts, but for
+ * parts below 2^-133).  x is 16-byte aligned with rows a multiple of 16 and at
+ * most 2^23 bytes apart, w->packed 16-byte aligned; out is at most 2^22, in
+ * 2^20.  The order of a token's sums, and so its last bits, depends on how many
+ * tokens the call has. */
 mr_status mr_mxfp4_matmul(const void *x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride,
                           const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype, int64_t y_stride, void *stream);
 
@@ -382,10 +384,9 @@ mr_status mr_expert_dispatch(const void *x, mr_dtype dtype, int32_t tokens, int6
  * their alignments.  w describes one expert of a stack laid out back to back.
  * source(r) is r with pair_of_row NULL (x has `rows` rows), else
  * pair_of_row[r] / per_token (x has one row per token, less than 2^32 - 2^16
- * bytes in all).  Rows of y past the
- * last expert's are left as they were.  offsets, pair_of_row: mr_expert_sort's;
- * values that it does not write give rows of y that are unspecified, never an
- * access outside the buffers. */
+ * bytes in all).  Rows of y past the last expert's are left as they were.
+ * offsets, pair_of_row: mr_expert_sort's; values that it does not write give
+ * rows of y that are unspecified, never an access outside the buffers. */
 typedef struct mr_mxfp4_expert_args {
     const void *x; /* bf16 or f32 rows, or MXFP4 words [x_rows, in / 8] */
     mr_dtype x_dtype; /* MR_BF16, MR_F32; MR_U32 for MXFP4 */

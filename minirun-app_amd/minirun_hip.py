@@ -8,6 +8,10 @@ Names follow the reference operators they stand in for:
   mla_decode            K3MLA absorbed attention core (MLA.swift:174-197)
   sparse_attention      DeepSeekV4SparseAttention.forward (DeepSeekV4Attention.swift:747-770)
   validate_indices      its index checks (DeepSeekV4Attention.swift:884-895)
+  MXFP4Weights          the MXFP4 storage (MXFP4Weights.swift:36-60); mxfp4_quantize,
+                        mxfp4_dequantize, mxfp4_mm, mxfp4_expert_mm
+  expert_sort           tokens by expert and back, for QwenExpertBackends.swift:77-260;
+                        expert_dispatch, expert_combine and their gradients
 """
 from __future__ import annotations
 
