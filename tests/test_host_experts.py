@@ -3,10 +3,13 @@ every refusal comes before a GPU call, with its status and a message."""
 import ctypes as C
 
 import pytest
+from hypothesis import HealthCheck, given, settings
+from hypothesis import strategies as st
 
 import minirun_hip as M
 
 AT = 1 << 32  # an address that no refused call reads
+REFUSED = {M.INVALID_SHAPE, M.INVALID_ARGUMENT, M.INVALID_DTYPE, M.WORKSPACE_TOO_SMALL}
 
 
 @pytest.fixture(scope="module")
@@ -217,3 +220,48 @@ def test_rows_of_a_tensor_need_a_stride():
     assert stride(torch.zeros(3, 80)[:, :64]) == 80
     with pytest.raises(ValueError):
         stride(torch.zeros(3, 1).expand(3, 64))
+
+
+# ---------------------------------------------------------------- random arguments
+dim = st.one_of(st.integers(-5, 4200), st.sampled_from([0, 1, 32, 64, 4096, 2 ** 24, 2 ** 31 - 1, -2 ** 31]))
+wide = st.one_of(st.integers(-5, 70000), st.sampled_from([0, 32, 2 ** 20, 2 ** 22, 2 ** 37, 2 ** 62, -2 ** 63, 2 ** 63 - 1]))
+dtype = st.integers(-1, 7)
+RANDOM = settings(max_examples=300, deadline=None, derandomize=True, suppress_health_check=[HealthCheck.too_slow])
+
+
+def nothing_or_refused(status, nothing):
+    """With NULL buffers: refused with a message, or there was nothing to do."""
+    assert status == M.OK and nothing or status in REFUSED and M.last_error(), status
+
+
+@RANDOM
+@given(rows=wide, cols=wide, dt=dtype, ld=wide, experts=dim, tokens=dim)
+def test_mxfp4_checks_of_random_arguments(lib, rows, cols, dt, ld, experts, tokens):
+    w = M.MXFP4Desc(None, None, rows, cols)
+    x = M.MXFP4Desc(None, None, tokens, cols)
+    nothing_or_refused(lib.mr_mxfp4_quantize(None, dt, rows, cols, ld, None, None, None), rows == 0)
+    nothing_or_refused(lib.mr_mxfp4_dequantize(C.byref(w), None, dt, ld, None), rows == 0)
+    nothing_or_refused(lib.mr_mxfp4_matmul(None, dt, tokens, ld, C.byref(w), None, M.F32, ld, None), tokens == 0)
+    nothing_or_refused(lib.mr_mxfp4_matmul_quantized(C.byref(x), C.byref(w), None, dt, ld, None), tokens == 0)
+    a = M.MXFP4ExpertArgs()
+    a.x_dtype, a.x_stride, a.x_rows, a.w, a.experts, a.per_token, a.rows = dt, ld, tokens, w, experts, 1, tokens
+    a.y_dtype, a.y_stride = M.BF16, ld
+    nothing_or_refused(lib.mr_mxfp4_expert_matmul(C.byref(a), None), tokens == 0)
+    ps, ss = shape(rows, cols), shape(rows, experts)
+    status = lib.mr_mxfp4_validate(M.U32, 2, ps, M.U8, 2, ss, None, None, None)
+    nothing_or_refused(status, 0 <= rows and 8 * cols == 32 * experts)
+
+
+@RANDOM
+@given(tokens=dim, per_token=dim, experts=dim, width=wide, dt=dtype, ld=wide)
+def test_routing_checks_of_random_arguments(lib, tokens, per_token, experts, width, dt, ld):
+    size = lib.mr_expert_sort_workspace_size(tokens, per_token, experts)
+    assert 0 <= size <= 2 ** 24 // 2048 * 4096 * 4
+    refused(lib.mr_expert_sort(None, tokens, per_token, experts, None, None, None, None, 0, None),
+            M.INVALID_SHAPE if size == 0 and not (tokens >= 0 and per_token > 0 and tokens * per_token <= 2 ** 24
+                                                  and 0 < experts <= 4096) else M.INVALID_ARGUMENT)
+    none = tokens == 0
+    nothing_or_refused(lib.mr_expert_dispatch(None, dt, tokens, width, ld, None, per_token, None, ld, None), none)
+    nothing_or_refused(lib.mr_expert_combine(None, dt, ld, width, None, None, tokens, per_token, None, ld, None), none)
+    nothing_or_refused(lib.mr_expert_combine_backward(None, dt, ld, width, None, ld, None, None, tokens, per_token, AT, ld,
+                                                      None, None), none)
