@@ -67,6 +67,19 @@ __device__ __forceinline__ void split3(const u32x4& a, const u32x4& b, bf16x8 (&
     for (int n = 0; n < 3; ++n) part[n] = __builtin_bit_cast(bf16x8, v[n]);
 }
 
+// Weight tile and block of x's rows of this workgroup: neighbours, which share a
+// weight tile, on one XCD (consecutive workgroups go to the 8 XCDs in turn), and
+// as many on each (whole weight tiles per XCD left some with half of the work
+// again: 273 x 4096, 200 tokens, 18 tiles, 8.6 us).
+__device__ __forceinline__ bool mx_tile(int n_tiles, int blocks, int& tile, int& tb) {
+    const uint32_t total = (uint32_t)n_tiles * (uint32_t)blocks, per = (total + 7) / 8, j = blockIdx.x >> 3;
+    const uint32_t id = (blockIdx.x & 7) * per + j;
+    if (j >= per || id >= total) return false;
+    tile = (int)(id / (uint32_t)blocks);
+    tb = (int)(id - (uint32_t)tile * (uint32_t)blocks);
+    return true;
+}
+
 template <int XT, int RT, int TT, int XI, int S, int NW>
 struct FewShape {
     using X = XEntry<XT>;
@@ -100,8 +113,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
         first_row = (int64_t)t.expert * p.N;
     } else {
         int tb;
-        sk_tile(blockIdx.x, blocks, tile, tb);
-        if (tile >= n_tiles) return;
+        if (!mx_tile(n_tiles, blocks, tile, tb)) return;
         m0 = tb * F::BM;
         toks = min(F::BM, p.M - m0);
     }
@@ -327,8 +339,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
         first_row = (int64_t)t.expert * p.N;
     } else {
         int tb;
-        sk_tile(blockIdx.x, blocks, tile, tb);
-        if (tile >= n_tiles) return;
+        if (!mx_tile(n_tiles, blocks, tile, tb)) return;
         m0 = tb * BM;
         toks = min(BM, p.M - m0);
     }
@@ -522,51 +533,56 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
     }
 }
 
-template <int XT, int RT, int TT, int S, int NW>
+template <int XT, int RT, int TT, int S, int NW, bool ROUTED = false>
 hipError_t launch_mid(const Mxfp4GemmParams& p, hipStream_t st) {
     using F = MidShape<XT, RT, TT, S, NW>;
     constexpr int BM = 16 * TT, BN = 16 * RT * NW;
-    const bool routed = p.offsets != nullptr;
-    const auto kern = routed ? mxfp4_mid_kernel<XT, RT, TT, S, NW, true> : mxfp4_mid_kernel<XT, RT, TT, S, NW, false>;
+    const auto kern = mxfp4_mid_kernel<XT, RT, TT, S, NW, ROUTED>;
     if (F::LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)F::LDS);
         if (e != hipSuccess) return e;
     }
     const int64_t tiles = (p.N + BN - 1) / BN, blocks = ((int64_t)p.M + BM - 1) / BM;
-    const int64_t grid = routed ? (mx_tile_bound(p, BM) * tiles + 7) / 8 * 8 : (tiles + 7) / 8 * 8 * blocks;
+    const int64_t grid = ROUTED ? (mx_tile_bound(p, BM) * tiles + 7) / 8 * 8 : (tiles * blocks + 7) / 8 * 8;
     if (grid * 64 * NW >= (1ll << 32)) return hipErrorInvalidValue;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), F::LDS, st, p, (int)blocks);
     return hipGetLastError();
 }
 
-template <int XT, int RT, int TT, int XI, int S, int NW>
+template <int XT, int RT, int TT, int XI, int S, int NW, bool ROUTED = false>
 hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
     using F = FewShape<XT, RT, TT, XI, S, NW>;
     constexpr size_t lds = F::LDS;
-    const bool routed = p.offsets != nullptr;
-    const auto kern = routed ? mxfp4_few_kernel<XT, RT, TT, XI, S, NW, true> : mxfp4_few_kernel<XT, RT, TT, XI, S, NW, false>;
+    const auto kern = mxfp4_few_kernel<XT, RT, TT, XI, S, NW, ROUTED>;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
     const int64_t tiles = (p.N + 16 * RT - 1) / (16 * RT), blocks = ((int64_t)p.M + F::BM - 1) / F::BM;
-    const int64_t grid = routed ? (mx_tile_bound(p, F::BM) * tiles + 7) / 8 * 8 : (tiles + 7) / 8 * 8 * blocks;
+    const int64_t grid = ROUTED ? (mx_tile_bound(p, F::BM) * tiles + 7) / 8 * 8 : (tiles * blocks + 7) / 8 * 8;
     if (grid * 64 * NW >= (1ll << 32)) return hipErrorInvalidValue;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), lds, st, p, (int)blocks);
     return hipGetLastError();
 }
 
 // Which kernel and tile.  Both split a call into workgroups of some weight rows
-// x some rows of x; small ones fill the GPU, large ones read less.  In us, one
-// call among others, weights in turn:
-//   matrix, x in bf16: 576 x 7168, 96 tokens, 16 x 16 with 8 waves 7.4, 32 x 16
-//     8.4, mid 128 x 32 over 20; 1536 x 7168, 64 tokens, 32 x 16 with 8 waves
-//     8.5, 4 waves 10.9, 16 x 16 12.3; 128 tokens, 4 waves 12.5, 8 waves 14.7;
-//     7168 x 16384, 64 tokens, 64 x 16 with 4 waves 33, 32 x 16 43, mid 46; 24576
-//     x 1536, 37 tokens, mid 64 x 48 10.5, 128 x 32 11.3, 64 x 16 17
-//   x in MXFP4, which costs a quarter to read: 7168 x 16384, 64 tokens, 64 x 32
-//     with 8 waves 18.7, 64 x 64 24.4, 32 x 16 28; 128 tokens, 64 x 64 23.8, 64 x
-//     32 31; 12000 x 1024, 100 tokens, mid 128 x 32 6.0, 128 x 64 6.9
+// x some rows of x; small ones fill the GPU, large ones read less, and rows that
+// are short leave waves that split them idle.  In us, one call among others:
+//   matrix, x in bf16, one round of workgroups of the smallest tile that gives no
+//     more than one a CU, with 8 waves: 576 x 7168, 96 tokens, 16 x 16 7.4, 32 x
+//     16 8.4; 1536 x 7168, 64 tokens, 32 x 16 8.5, 16 x 16 12.3; 2048 x 12608, 100
+//     tokens, 64 x 16 16.5, 32 x 16 with 4 waves 20.4; with 4 waves where a row is
+//     short: 273 x 1024, 300 tokens, 4.8 and 6.9.  Then one round of 64 x 48 (4096 x
+//     4096, 150 tokens, 14.6, mid 18) or, for long rows, of 64 x 64 with 3 waves
+//     (1536 x 12608, 600 tokens, 51 and 67), else mid: 24576 x 1536, 37 tokens, mid
+//     64 x 48 10.5, 128 x 32 11.3, 64 x 16 17
+//   x in MXFP4, which costs a quarter to read: 7168 x 4096, 16 tokens, 32 x 16 with
+//     8 waves 4.8, 16 x 16 5.8, 64 x 16 5.7; 1024 x 4096, 200 tokens, 64 x 16 with 8
+//     waves 5.9, 64 x 32 6.5, x 1024 32 x 16 with 4 4.1, 64 x 32 4.9; 1024 x 2048,
+//     600 tokens, 64 x 32 with 4 waves 6.6, mid 7.9 (24576 x 1536, 16 tokens, 6.5
+//     and mid 5.5); 7168 x 16384, 64 tokens, 64 x
+//     32 with 8 waves 18.7, 64 x 64 24.4; 2048 x 12608, 600 tokens, 64 x 64 with 4
+//     waves 33, with 8 42; 12000 x 1024, 100 tokens, mid 128 x 32 6.0, 128 x 64 6.9
 //   experts by their mean rows, x in bf16: 128 of 2048 x 768, 6 rows, mid 128 x 16
 //     20.2, 128 x 32 22.4, 12 rows 21.2 and 22.9, 19 rows 25.5 and 24.0; one stage
 //     in the ring, which leaves room for four or five workgroups a CU, where there
@@ -591,34 +607,40 @@ int64_t routed_tiles(const Mxfp4GemmParams& p, int bm) {
 hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     const int entries = (p.K + 255) / 256;
     if (p.offsets) {
-        if (few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4>(p, st);
-        if (p.pairs <= 12 * p.experts) return routed_tiles(p, 16) > 2 * cus ? launch_mid<0, 2, 1, 1, 4>(p, st) : launch_mid<0, 2, 1, 2, 4>(p, st);
-        return routed_tiles(p, 32) > 2 * cus ? launch_mid<0, 2, 2, 1, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
+        if (few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4, true>(p, st);
+        if (p.pairs <= 12 * p.experts) return routed_tiles(p, 16) > 2 * cus ? launch_mid<0, 2, 1, 1, 4, true>(p, st) : launch_mid<0, 2, 1, 2, 4, true>(p, st);
+        return routed_tiles(p, 32) > 2 * cus ? launch_mid<0, 2, 2, 1, 4, true>(p, st) : launch_mid<0, 2, 2, 2, 4, true>(p, st);
     }
     if (p.M <= 2) {
         if (entries >= 16) return launch_few<0, 1, 1, 1, 1, 8>(p, st);
         return entries >= 8 ? launch_few<0, 1, 1, 1, 1, 4>(p, st) : launch_few<0, 1, 1, 1, 1, 2>(p, st);
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
-    if (n16 * b <= cus) return launch_few<0, 1, 1, 8, 1, 8>(p, st);
-    if (n32 * b <= cus) return launch_few<0, 2, 1, 8, 1, 8>(p, st);
+    if (n16 * b <= cus) return entries > 4 ? launch_few<0, 1, 1, 8, 1, 8>(p, st) : launch_few<0, 1, 1, 8, 1, 4>(p, st);
+    if (n32 * b <= cus && entries > 4) return launch_few<0, 2, 1, 8, 1, 8>(p, st);
+    if (n64 * b <= cus && entries >= 8) return launch_few<0, 4, 1, 8, 1, 8>(p, st);
     if (n32 * b <= 2 * cus) return launch_few<0, 2, 1, 8, 1, 4>(p, st);
     if (n64 * b <= 2 * cus) return launch_few<0, 4, 1, 8, 1, 4>(p, st);
+    if (n64 * (((int64_t)p.M + 47) / 48) <= cus) return launch_few<0, 4, 3, 24, 1, 4>(p, st);
+    if (n64 * (((int64_t)p.M + 63) / 64) <= cus && p.K > 4096) return launch_few<0, 4, 4, 32, 1, 3>(p, st);
     if (b == 1) return launch_mid<0, 2, 1, 2, 4>(p, st);
     return b == 3 && p.K <= 2048 ? launch_mid<0, 1, 3, 1, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
 }
 
 hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (p.offsets) {
-        if (few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4>(p, st);
-        return p.pairs <= 10 * p.experts ? launch_mid<2, 2, 1, 1, 2>(p, st) : launch_mid<2, 2, 2, 1, 2>(p, st);
+        if (few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4, true>(p, st);
+        return p.pairs <= 10 * p.experts ? launch_mid<2, 2, 1, 1, 2, true>(p, st) : launch_mid<2, 2, 2, 1, 2, true>(p, st);
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
     if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 1, 8>(p, st);
-    if (b == 1 && n16 <= 2 * cus) return launch_few<2, 1, 1, 2, 2, 4>(p, st);
     if (n32 * b <= cus) return launch_few<2, 2, 1, 2, 1, 8>(p, st);
+    if (n64 * b <= cus && p.K > 2048) return launch_few<2, 4, 1, 2, 1, 8>(p, st);
+    if (n32 * b <= 2 * cus && p.K <= 2048) return launch_few<2, 2, 1, 2, 1, 4>(p, st);
     if (n64 * ((b + 1) / 2) <= cus) return launch_few<2, 4, 2, 4, 1, 8>(p, st);
-    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 8>(p, st);
+    if (b > 4 && n64 * ((b + 1) / 2) <= 2 * cus && p.K <= 2048) return launch_few<2, 4, 2, 4, 1, 4>(p, st);
+    if (n64 * ((b + 3) / 4) <= cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 8>(p, st);
+    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 4>(p, st);
     return b <= 4 ? launch_mid<2, 2, 1, 1, 2>(p, st) : launch_mid<2, 2, 2, 1, 4>(p, st);
 }
 
@@ -629,12 +651,15 @@ hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
 // them split K instead: 1536 x 7168, 64 tokens, 32 x 16 with 4 waves 23, mid 62,
 // 2048 x 2048 9 and 20
 hipError_t launch_few_f32(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
-    if (!p.offsets && p.M == 1) return launch_few<1, 4, 1, 1, 1, 4>(p, st);
+    if (p.offsets) {
+        const int64_t tiles = routed_tiles(p, 16);
+        if (2 * tiles <= cus) return launch_mid<1, 1, 1, 1, 4, true>(p, st);
+        return tiles <= cus ? launch_mid<1, 2, 1, 1, 4, true>(p, st) : launch_mid<1, 4, 1, 1, 4, true>(p, st);
+    }
+    if (p.M == 1) return launch_few<1, 4, 1, 1, 1, 4>(p, st);
     const int64_t b = ((int64_t)p.M + 15) / 16;
-    if (!p.offsets && (p.N + 31) / 32 * b <= 2 * cus) return launch_few<1, 2, 1, 16, 1, 4>(p, st);
-    const int64_t tiles = p.offsets ? routed_tiles(p, 16) : (p.N + 127) / 128 * b;
-    if (2 * tiles <= cus) return launch_mid<1, 1, 1, 1, 4>(p, st);
-    return tiles <= cus ? launch_mid<1, 2, 1, 1, 4>(p, st) : launch_mid<1, 4, 1, 1, 4>(p, st);
+    if ((p.N + 31) / 32 * b <= 2 * cus) return launch_few<1, 2, 1, 16, 1, 4>(p, st);
+    return (p.N + 127) / 128 * b <= cus ? launch_mid<1, 2, 1, 1, 4>(p, st) : launch_mid<1, 4, 1, 1, 4>(p, st);
 }
 
 hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
@@ -648,8 +673,7 @@ hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
 // 64 tokens 14 and 11; 7168 x 16384, 300 tokens, 168 tiles, 107 and 135, 200
 // tokens, 112 tiles, 107 and 81; 16384 x 4096, 65 tokens, 128 tiles, 31 and 24;
 // MXFP4: there 15.5 and 16.6, 64 tokens 15.5 and 11.4; 24576 x 1536, 37 tokens,
-// 6.7 and 7.7; 1536 x 7168, 1000 tokens, 96 tiles, 19 and 24, 600 tokens, 60
-// tiles, 24 and 12), and for experts from some rows each (128 of 768 x 2048: bf16,
+// 6.7 and 7.7; 4096 x 12608, 400 tokens, 128 tiles, 55 and 36), and for experts from some rows each (128 of 768 x 2048: bf16,
 // 62 rows, 45 and 46, 50 rows 44 and 38, 31 rows 42 and 31; 32 of 1536 x 7168, 88
 // rows, 85 and 98, 62 rows 82 and 76; MXFP4: 31 rows, 22.0 and 23.9, 19 rows 20.5
 // and 19.6).
@@ -673,7 +697,7 @@ MxTiles tiles_of(const Mxfp4GemmParams& p, int cus) {
         if (p.M <= (mx ? 32 : 64)) return MX_TILES_NONE;
         small = cols(128) * (((int64_t)p.M + 127) / 128);
     }
-    if (small * 8 < (!mx ? 5 : !p.offsets && p.M <= 64 ? 6 : 4) * cus) return MX_TILES_NONE;
+    if (small * 8 < (!mx || p.K > 4096 ? 5 : !p.offsets && p.M <= 64 ? 6 : 4) * cus) return MX_TILES_NONE;
     const int64_t left = small % (2 * cus);
     const int64_t two = small / (2 * cus) * 6 + (left == 0 ? 0 : left <= cus && !mx ? 4 : 6);
     const int64_t three = mx ? (small + 3 * cus - 1) / (3 * cus) * 8 : INT64_MAX;

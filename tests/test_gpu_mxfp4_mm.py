@@ -85,7 +85,8 @@ def test_whole_numbers_are_exact(M, out, inp, kind):
 WIDE = [(1, 300, 544), (2, 300, 4128), (20, 300, 288), (10, 4104, 288), (40, 2056, 544), (100, 2056, 160), (100, 4000, 288),
         (100, 4104, 256), (40, 16392, 96), (10, 33000, 96), (100, 8200, 2080), (20, 300, 4128), (100, 16392, 288),
         (200, 16392, 288), (300, 16392, 512), (600, 16392, 256), (600, 16385, 288), (700, 16390, 32), (1100, 8190, 416),
-        (1000, 16384, 512), (1000, 16300, 288), (100, 8200, 544), (20, 8200, 96)]
+        (1000, 16384, 512), (1000, 16300, 288), (100, 8200, 544), (20, 8200, 96),
+        (100, 2056, 2080), (300, 2056, 96), (400, 2056, 4128), (100, 264, 544)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
