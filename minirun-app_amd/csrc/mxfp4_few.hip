@@ -42,9 +42,14 @@ struct XEntry {  // of 256 k
     static constexpr int CHUNKS = BYTES / 16;  // of 16 bytes per row
     static constexpr int RPI = 64 / CHUNKS;    // rows per DMA instruction
     static constexpr int KPC = 256 / CHUNKS;   // values per chunk
-    // chunk c of row r is in slot c ^ swizzle(r), so that the 16 rows of a
-    // read of one chunk lie in 16 bank groups
+    // Chunk c of row r is in slot c ^ swizzle(r), so that the 16 rows of a read of
+    // one chunk lie in 16 bank groups.  bf16: with bits 3 and 4 of c exchanged, so
+    // that lanes of the first two of a read's four blocks, which it takes together,
+    // have the same groups for the same rows (four clocks less a read).
     static __device__ __forceinline__ int swizzle(int r) { return XT == MX_X_MXFP4 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int swap(int c) { return XT == MX_X_BF16 ? (c & 7) | (c & 8) << 1 | (c & 16) >> 1 : c; }
+    static __device__ __forceinline__ int slot(int c, int r) { return swap(c) ^ swizzle(r); }
+    static __device__ __forceinline__ int chunk(int slot, int r) { return swap(slot ^ swizzle(r)); }
 };
 
 // the three bf16 parts of eight f32 values, by truncation
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
         wo[i] = r < rows ? (uint32_t)r * wrow + 16u * (ch8 ^ (4 * (i & 1))) : SK_OOB_ROW;
     }
     const uint32_t so = l < rows ? (ws0 + (uint32_t)l * srow) & ~3u : SK_OOB_ROW;
-    auto x_chunk = [&](int u) { return (uint32_t)((l % X::CHUNKS) ^ X::swizzle(X::RPI * u + l / X::CHUNKS)); };
+    auto x_chunk = [&](int u) { return (uint32_t)X::chunk(l % X::CHUNKS, X::RPI * u + l / X::CHUNKS); };
 #pragma unroll
     for (int u = 0; u < XI; ++u) xo[u] = xr[u] * (uint32_t)xrow + 16u * x_chunk(u);
     i32x4 xsres{};
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
                 const int row = (16 * t + lr) % F::ROWS;
 #pragma unroll
                 for (int s = 0; s < XF; ++s)
-                    fx[t][s] = *(const u32x4*)(e + F::XOFF + X::BYTES * row + 16 * ((XF * (2 * q + u) + s) ^ X::swizzle(row)));
+                    fx[t][s] = *(const u32x4*)(e + F::XOFF + X::BYTES * row + 16 * X::slot(XF * (2 * q + u) + s, row));
             }
         };
         if constexpr (XT == MX_X_MXFP4) {
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
     // x: this wave's instruction u of XPW (the last waves may repeat one)
     auto x_instr = [&](int u) { return min(F::XPW * w + u, F::XI - 1); };
     auto x_row = [&](int u) { return X::RPI * x_instr(u) + l / X::CHUNKS; };
-    auto x_chunk = [&](int u) { return (uint32_t)((l % X::CHUNKS) ^ X::swizzle(x_row(u))); };
+    auto x_chunk = [&](int u) { return (uint32_t)X::chunk(l % X::CHUNKS, x_row(u)); };
     constexpr int NX = F::XPW + (XT == MX_X_MXFP4 ? 1 + TT : 0);
     uint32_t xr[NX];
     mx_x_rows<NX>(p, by_token, m0, toks, xr,
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
             for (int t = 0; t < TT; ++t)
 #pragma unroll
                 for (int c = 0; c < XF; ++c)
-                    fx[t][c] = *(const u32x4*)(e + X::BYTES * (16 * t + lr) + 16 * ((XF * (2 * q + u) + c) ^ X::swizzle(16 * t + lr)));
+                    fx[t][c] = *(const u32x4*)(e + X::BYTES * (16 * t + lr) + 16 * X::slot(XF * (2 * q + u) + c, 16 * t + lr));
             if (S == 1 && u == 1) {
                 lds_barrier();  // every wave has read the stage
                 if (s + 1 < nst) issue(s + 1, 0);
