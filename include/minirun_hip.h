@@ -335,7 +335,8 @@ mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_
  * mr_affine_matmul): x [tokens, in] bf16 or f32 with row stride x_stride; y
  * [tokens, out] bf16 or f32 with row stride y_stride; f32 sums.  Weights are
  * taken as mr_mxfp4_dequantize gives them in bf16 (exact but for infinities at
- * bytes 253 and 254); f32 activations exactly too (as three bf16 parts, but for
+ * bytes 253 and 254, which meet activations as in IEEE arithmetic: an infinity,
+ * or NaN with a zero); f32 activations exactly too (as three bf16 parts, but for
  * parts below 2^-133).  x is 16-byte aligned with rows a multiple of 16 and at
  * most 2^23 bytes apart, w->packed 16-byte aligned; out is at most 2^22, in
  * 2^20.  The order of a token's sums, and so its last bits, depends on how many

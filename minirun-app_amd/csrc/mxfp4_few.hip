@@ -18,7 +18,9 @@
 //     significant bits), one v_mfma_f32_16x16x32_bf16 each, with the eight
 //     values of x that belong to the word.
 //   x in f32: the same with x cut into three bf16 parts by truncation, whose
-//     sum is x exactly.
+//     sum is x exactly.  Against an infinite weight (scale bytes 253 and 254) a
+//     part that is zero makes the sum NaN: outputs that are NaN are computed
+//     again, x uncut.
 //   x in MXFP4: v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands' codes
 //     and scale bytes as they are.
 // Chains start from zero per entry and are added to the running sums in f32.
@@ -70,6 +72,51 @@ __device__ __forceinline__ void split3(const u32x4& a, const u32x4& b, bf16x8 (&
     }
 #pragma unroll
     for (int n = 0; n < 3; ++n) part[n] = __builtin_bit_cast(bf16x8, v[n]);
+}
+
+// One output of f32 activations again, by a whole wave: the sum over a row of x
+// and one of W, weights as bf16.  It ends at the first NaN.
+__device__ __forceinline__ float mx_f32_again(const float* x, const uint32_t* packed, const uint8_t* scales, int K) {
+    float d = 0.f;
+#pragma unroll 1
+    for (int k = 8 * (threadIdx.x & 63); k < (K + 511) / 512 * 512; k += 512) {
+        if (k < K) {
+            const u32x4 v[2] = {*(const u32x4*)(x + k), *(const u32x4*)(x + k + 4)};
+            const u32x4 wv = __builtin_bit_cast(u32x4, mxfp4_bf16(packed[k >> 3], __uint_as_float((uint32_t)scales[k >> 5] << 23)));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                d = fmaf(__uint_as_float(v[i >> 2][i & 3]), __uint_as_float(i & 1 ? wv[i >> 1] & 0xffff0000u : wv[i >> 1] << 16), d);
+        }
+        if (__ballot(d != d)) return NAN;
+    }
+    return wave_sum(d);
+}
+
+// Those that are NaN of a wave's outputs again: of lane l, bit i of `again`, in
+// row m of the tile from m0 on and weight row n of the expert, m and n from
+// at(l, i); stored by that lane through store(m, n, value).
+template <typename At, typename Store>
+__device__ __forceinline__ void mx_f32_nans(const Mxfp4GemmParams& p, bool by_token, int64_t first_row, int m0, uint32_t again,
+                                            At at, Store store) {
+    const int l = threadIdx.x & 63;
+    uint64_t lanes = __ballot(again != 0);
+#pragma unroll 1
+    while (__builtin_expect(lanes != 0, 0)) {
+        const int from = __builtin_ctzll(lanes);
+        lanes &= lanes - 1;
+        uint32_t bits = __builtin_amdgcn_readlane(again, from);
+#pragma unroll 1
+        for (; bits; bits &= bits - 1) {
+            int m, n;
+            at(from, __builtin_ctz(bits), m, n);
+            uint32_t row[1];
+            mx_x_rows<1>(p, by_token, m0, m + 1, row, [&](int) { return m; });
+            const int64_t x_row = by_token ? row[0] : m0 + m, w_row = first_row + n;
+            const float y = mx_f32_again((const float*)p.x + x_row * p.ldx, p.packed + w_row * (p.K / 8),
+                                         p.scales + w_row * (p.K / 32), p.K);
+            if (l == from) store(m, n, y);
+        }
+    }
 }
 
 // Weight tile and block of x's rows of this workgroup: neighbours, which share a
@@ -287,18 +334,40 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
             for (int t = 0; t < TT; ++t) tot[r][t] += part[r][t];
     }
     wait_vmcnt<0>();
+    auto store = [&](int m, int n, float y) {
+        const int64_t o = (int64_t)(m0 + m) * p.ldy + n;
+        if (p.y_f32)
+            ((float*)p.y)[o] = y;
+        else
+            ((uint16_t*)p.y)[o] = f32_to_bf16_bits(y);
+    };
     sk_reduce<RT, TT, NW>(lds, tot, [&](int r, int t, int lane, f32x4 v) {
         const int nn = 16 * r + (lane & 15);
-        if (nn >= rows) return;
+        if constexpr (XT == MX_X_F32) {
+            uint32_t again = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int m = 16 * t + 4 * (lane >> 4) + e;
-            if (m >= toks) break;
-            const int64_t o = (int64_t)(m0 + m) * p.ldy + n0 + nn;
-            if (p.y_f32)
-                ((float*)p.y)[o] = v[e];
-            else
-                ((uint16_t*)p.y)[o] = f32_to_bf16_bits(v[e]);
+            for (int e = 0; e < 4; ++e) {
+                const int m = 16 * t + 4 * (lane >> 4) + e;
+                if (nn >= rows || m >= toks) continue;
+                if (v[e] == v[e])
+                    store(m, n0 + nn, v[e]);
+                else
+                    again |= 1u << e;
+            }
+            mx_f32_nans(p, by_token, first_row, m0, again,
+                        [&](int from, int e, int& m, int& n) {
+                            m = 16 * t + 4 * (from >> 4) + e;
+                            n = n0 + 16 * r + (from & 15);
+                        },
+                        store);
+        } else {
+            if (nn >= rows) return;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int m = 16 * t + 4 * (lane >> 4) + e;
+                if (m >= toks) break;
+                store(m, n0 + nn, v[e]);
+            }
         }
     });
 }
@@ -510,6 +579,7 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
     // tot[r][t][e]: y row m0 + 16 t + l % 16, column n0 + 16 r + 4 (l / 16) + e
     const int size = p.y_f32 ? 4 : 2;
     const bool vec = ((uintptr_t)p.y & (4 * size - 1)) == 0 && (p.ldy & 3) == 0;
+    uint32_t again = 0;  // x in f32: which are NaN
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
         const int m = 16 * t + lr;
@@ -519,6 +589,12 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
             const int c = 16 * r + 4 * q;
             const int64_t o = (int64_t)(m0 + m) * p.ldy + n0 + c;
             const f32x4 v = tot[r][t];
+            if constexpr (XT == MX_X_F32) {
+                static_assert(4 * RT * TT <= 32, "a bit per output");
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < rows && v[e] != v[e]) again |= 1u << (4 * (RT * t + r) + e);
+            }
             if (vec && c + 4 <= rows) {
                 if (p.y_f32)
                     *(f32x4*)((float*)p.y + o) = v;
@@ -536,6 +612,19 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
             }
         }
     }
+    if constexpr (XT == MX_X_F32)
+        mx_f32_nans(p, by_token, first_row, m0, again,
+                    [&](int from, int i, int& m, int& n) {
+                        m = 16 * (i / (4 * RT)) + (from & 15);
+                        n = n0 + 16 * (i / 4 % RT) + 4 * (from >> 4) + i % 4;
+                    },
+                    [&](int m, int n, float y) {
+                        const int64_t o = (int64_t)(m0 + m) * p.ldy + n;
+                        if (p.y_f32)
+                            ((float*)p.y)[o] = y;
+                        else
+                            ((uint16_t*)p.y)[o] = f32_to_bf16_bits(y);
+                    });
 }
 
 template <int XT, int RT, int TT, int S, int NW, bool ROUTED = false>
