@@ -374,7 +374,9 @@ mr_status mr_expert_sort(const int32_t *ids, int32_t tokens, int32_t per_token, 
 /* rows[row_of_pair[t][j]] = x[t], bit for bit, for every pair that has a row:
  * x [tokens, dim], rows [tokens * per_token, dim], both of `dtype` (bf16 or
  * f32).  Rows past the last are left as they were.  An entry of row_of_pair
- * outside [0, tokens * per_token) counts as -1, here and below. */
+ * outside [0, tokens * per_token) counts as -1, here and below; where two entries
+ * name one row, which of them is written is not defined.  dim is at most 2^24 and
+ * tokens * max(64, (dim + 7) / 8) less than 2^32, here and below. */
 mr_status mr_expert_dispatch(const void *x, mr_dtype dtype, int32_t tokens, int64_t dim, int64_t x_stride,
                              const int32_t *row_of_pair, int32_t per_token, void *rows, int64_t rows_stride,
                              void *stream);

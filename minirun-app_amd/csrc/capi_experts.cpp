@@ -32,8 +32,9 @@ mr_status check_rows(int32_t tokens, int32_t per_token, int64_t dim, mr_dtype dt
         return fail(MR_INVALID_SHAPE, "%s: %d tokens of %d experts (at most 2^24 pairs)", what, tokens, per_token);
     if (dim <= 0 || dim > (1 << 24)) return fail(MR_INVALID_SHAPE, "%s: rows of %lld values", what, (long long)dim);
     if (!act(dtype)) return fail(MR_INVALID_DTYPE, "%s: rows must be bf16 or f32, got %s", what, mrc::dtype_name(dtype));
-    // a thread per 8 or 16 values, in whole waves, in a grid of less than 2^32
-    if (double(tokens) * (double(dim) / 8 + 1024) >= 4294967296.0)
+    // at most a thread per 8 values, and a wave, for a token (row_launch in
+    // experts.hip), in a grid of less than 2^32
+    if (int64_t(tokens) * std::max<int64_t>(64, (dim + 7) / 8) >= (int64_t(1) << 32))
         return fail(MR_INVALID_SHAPE, "%s: %d tokens of %lld values are more than one launch takes", what, tokens,
                     (long long)dim);
     return MR_OK;
