@@ -21,11 +21,6 @@ __device__ __forceinline__ i32x4 uniform_rsrc(const void* base, uint32_t bytes) 
     return r;
 }
 
-__device__ __forceinline__ void dma4_buf(i32x4 rsrc, uint32_t voff, const void* lds_dst_wave_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
-}
-
 // row tile and token block of this workgroup: consecutive workgroups go to
 // the 8 XCDs in turn
 __device__ __forceinline__ void sk_tile(int bid, int blocks, int& tile, int& tb) {

@@ -172,23 +172,31 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // wait_vmcnt and issues no other vector-memory load after its first DMA,
 // which keeps those counts exact.  (Extra loads the compiler does not see
 // can only make its own waits stricter.)
+//
+// Nor does the compiler look into asm for the wait states that the hardware
+// asks of software: one between a scalar write of m0 and the load, five between
+// a vector instruction's write of a scalar register and a load that reads it.
+// v_readfirstlane makes such registers, and v_readlane brings spilled ones back,
+// right in front of a load, which then reads from anywhere.  So each of these
+// loads has them in front of it (s_nop n: n + 1 states), whatever the allocation
+// and the order of registers come to be.
 __device__ __forceinline__ void dma16(const void* src, const void* lds_dst_wave_base) {
     const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;  // LDS offset (low 32 bits)
-    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
 }
 
 // Same DMA with a wave-uniform 64-bit base in SGPRs and a 32-bit per-lane
 // byte offset: one VGPR per load instead of two.
 __device__ __forceinline__ void dma16_off(const void* sbase, uint32_t voff, const void* lds_dst_wave_base) {
     const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 
 // DMA of 4 bytes per lane (lane i lands at lds_dst_wave_base + 4 i); the
 // same wait rules as dma16_off
 __device__ __forceinline__ void dma4_off(const void* sbase, uint32_t voff, const void* lds_dst_wave_base) {
     const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("global_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 
 // Raw (stride 0) buffer resource over `bytes` bytes from `base`: a load at a
@@ -205,7 +213,13 @@ __device__ __forceinline__ i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
 // a lane whose offset is out of range writes zeros.  Same wait rules as dma16.
 __device__ __forceinline__ void dma16_buf(i32x4 rsrc, uint32_t voff, const void* lds_dst_wave_base) {
     const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
+}
+
+// The same of 4 bytes per lane: lane i lands at lds_dst_wave_base + 4 i
+__device__ __forceinline__ void dma4_buf(i32x4 rsrc, uint32_t voff, const void* lds_dst_wave_base) {
+    const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
+    asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
 }
 
 template <int N>

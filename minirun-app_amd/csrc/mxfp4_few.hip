@@ -224,15 +224,15 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
 #pragma unroll
         for (int c = 0; c < 2 * RT; ++c) {
             const bool in = live && 256u * ent + 32u * (ch8 ^ (4 * (c & 1))) < K;
-            mx_dma16(wres, wo[c] + (in ? 128u * ent : SK_OOB_K), e + 1024 * c);
+            dma16_buf(wres, wo[c] + (in ? 128u * ent : SK_OOB_K), e + 1024 * c);
         }
-        mx_dma16(sres, so + (live ? 8u * ent : SK_OOB_K), e + F::SOFF);
+        dma16_buf(sres, so + (live ? 8u * ent : SK_OOB_K), e + F::SOFF);
 #pragma unroll
         for (int u = 0; u < XI; ++u) {
             const bool in = live && 256u * ent + X::KPC * x_chunk(u) < K && X::RPI * u + l / X::CHUNKS < toks;
-            mx_dma16(xres, in ? xo[u] + (uint32_t)X::BYTES * ent : PAST, e + F::XOFF + 1024 * u);
+            dma16_buf(xres, in ? xo[u] + (uint32_t)X::BYTES * ent : PAST, e + F::XOFF + 1024 * u);
         }
-        if constexpr (XT == MX_X_MXFP4) mx_dma16(xsres, live && l < toks ? xso + 8u * ent : PAST, e + F::XSOFF);
+        if constexpr (XT == MX_X_MXFP4) dma16_buf(xsres, live && l < toks ? xso + 8u * ent : PAST, e + F::XSOFF);
     };
     f32x4 tot[RT][TT];
 #pragma unroll
@@ -469,16 +469,16 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
 #pragma unroll
         for (int u = 0; u < F::XPW; ++u) {
             const bool in = live && 256u * st + X::KPC * x_chunk(u) < K && x_row(u) < toks;
-            mx_dma16(xres, in ? xo[u] + (uint32_t)X::BYTES * st : PAST, e + 1024 * x_instr(u));
+            dma16_buf(xres, in ? xo[u] + (uint32_t)X::BYTES * st : PAST, e + 1024 * x_instr(u));
         }
         e += woff;
 #pragma unroll
         for (int c = 0; c < 2 * RT; ++c) {
             const bool in = live && 256u * st + 32u * (ch8 ^ (4 * (c & 1))) < K;
-            mx_dma16(wres, wo[c] + (in ? 128u * st : SK_OOB_K), e + 1024 * c);
+            dma16_buf(wres, wo[c] + (in ? 128u * st : SK_OOB_K), e + 1024 * c);
         }
-        mx_dma16(sres, so + (live ? 8u * st : SK_OOB_K), e + 2048 * RT);
-        if constexpr (XT == MX_X_MXFP4) mx_dma16(xsres, live && l < toks ? xso + 8u * st : PAST, e + 2048 * RT + 1024);
+        dma16_buf(sres, so + (live ? 8u * st : SK_OOB_K), e + 2048 * RT);
+        if constexpr (XT == MX_X_MXFP4) dma16_buf(xsres, live && l < toks ? xso + 8u * st : PAST, e + 2048 * RT + 1024);
     };
     f32x4 tot[RT][TT];
 #pragma unroll

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(MG_THREADS, (MgShape<XT, TM, TN, ONE, RAGGED>:
         t = min(t, AT - 1);
         const uint32_t ch = ch8 ^ (4 * (q & 1));
         const bool past = RAGGED && (MX ? 256u * t + 32u * ch : 64u * t + 8u * ch) >= K;
-        mx_dma16(xres, past ? PAST : ao[q] + 128u * t, st + 1024 * (DA * w + q));
+        dma16_buf(xres, past ? PAST : ao[q] + 128u * t, st + 1024 * (DA * w + q));
     };
     // instruction q of W's piece t (MXFP4: stage t)
     const int BT = MX ? AT : AT / 2;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(MG_THREADS, (MgShape<XT, TM, TN, ONE, RAGGED>:
         t = min(t, BT - 1);
         const uint32_t ch = MX ? ch8 ^ (4 * (q & 1)) : ch4;
         const bool past = RAGGED && (MX ? 256u : 128u) * t + 32u * ch >= K;
-        mx_dma16(wres, past ? PAST : bo[q] + (MX ? 128u : 64u) * t, st + 1024 * (DB * w + q));
+        dma16_buf(wres, past ? PAST : bo[q] + (MX ? 128u : 64u) * t, st + 1024 * (DB * w + q));
     };
     // instruction q of scale group t (of 512 or 128 k)
     const int ST = (p.K + (MX ? 511 : 127)) / (MX ? 512 : 128);
@@ -202,11 +202,11 @@ __global__ void __launch_bounds__(MG_THREADS, (MgShape<XT, TM, TN, ONE, RAGGED>:
         t = min(t, ST - 1);
         if constexpr (MX) {
             if (q < SQ)
-                mx_dma16(sres[q], so[q] + 16u * t, st + 1024 * (SQ * w + q));
+                dma16_buf(sres[q], so[q] + 16u * t, st + 1024 * (SQ * w + q));
             else
-                mx_dma4(sres[q - SQ], so[q - SQ] + 16u * t + 16u, st + 16 * S::SROWS + 256 * (SQ * w + q - SQ));
+                dma4_buf(sres[q - SQ], so[q - SQ] + 16u * t + 16u, st + 16 * S::SROWS + 256 * (SQ * w + q - SQ));
         } else {
-            mx_dma4(sres[0], so[0] + 4u * t + 4u * q, st + 4 * TN * q + 256 * (w % (TN / 64)));
+            dma4_buf(sres[0], so[0] + 4u * t + 4u * q, st + 4 * TN * q + 256 * (w % (TN / 64)));
         }
     };
 

@@ -11,22 +11,6 @@ namespace {
 
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
-// DMA of 16 or 4 bytes per lane from a buffer resource to LDS, as dma16_buf and
-// dma4_buf, behind five wait states: that many belong between a VALU write of a
-// scalar register and a vector-memory instruction that reads it (one between a
-// write of m0 and its use), and the compiler, which keeps them in front of its
-// own instructions, does not look into asm.  It matters where the resource has
-// been spilled and v_readlane brings it back right in front of the load, which
-// then reads from anywhere.
-__device__ __forceinline__ void mx_dma16(i32x4 rsrc, uint32_t voff, const void* lds_dst_wave_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
-}
-__device__ __forceinline__ void mx_dma4(i32x4 rsrc, uint32_t voff, const void* lds_dst_wave_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)lds_dst_wave_base;
-    asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
-}
-
 // D[16][16] += A . B^T over 128 k, both operands e2m1 codes with a scale byte
 // per 32: lane l holds row l % 16 and block l / 16 (16 bytes of codes, element
 // 0 in the low bits of the first word; its scale in byte SEL of the word).  D as
