@@ -32,6 +32,47 @@ public struct HIPTensor {
     public func bytes(_ n: Int) -> Int { n * (dtype == MR_U8 ? 1 : dtype == MR_F32 || dtype == MR_U32 || dtype == MR_I32 ? 4 : 2) }
 }
 
+/// What a C call cannot see of its pointers, checked before it.
+extension HIPTensor {
+    /// [rows, cols] (nil: any) with the values of a row next to each other.
+    func needRows(_ name: String, _ rows: Int?, _ cols: Int?, dtype want: mr_dtype? = nil) throws {
+        guard shape.count == 2, strides.count == 2, shape[0] == rows ?? shape[0], shape[1] == cols ?? shape[1] else {
+            let size = { (n: Int?) in n.map { "\($0)" } ?? "any" }
+            throw HIPError(status: MR_INVALID_SHAPE,
+                           description: "\(name) must be [\(size(rows)), \(size(cols))], got \(shape)")
+        }
+        guard strides[1] == 1 || shape[1] == 1 else {
+            throw HIPError(status: MR_INVALID_ARGUMENT, description: "\(name) must be contiguous in its last dimension")
+        }
+        try needType(name, want)
+    }
+
+    /// Of this shape (nil: any), without gaps.
+    func needWhole(_ name: String, _ size: [Int]?, dtype want: mr_dtype? = nil) throws {
+        guard shape == size ?? shape, strides.count == shape.count else {
+            throw HIPError(status: MR_INVALID_SHAPE, description: "\(name) must be \(size ?? shape), got \(shape)")
+        }
+        var next = 1
+        for axis in shape.indices.reversed() where !shape.contains(0) {
+            guard strides[axis] == next || shape[axis] == 1 else {
+                throw HIPError(status: MR_INVALID_ARGUMENT, description: "\(name) must be contiguous")
+            }
+            next *= shape[axis]
+        }
+        try needType(name, want)
+    }
+
+    private func needType(_ name: String, _ want: mr_dtype?) throws {
+        guard dtype == want ?? dtype else {
+            throw HIPError(status: MR_INVALID_DTYPE,
+                           description: "\(name) has mr_dtype \(dtype.rawValue), not \(want?.rawValue ?? 0)")
+        }
+    }
+
+    /// Row stride of a 2-D tensor; one row may have any.
+    var rowStride: Int64 { Int64(shape[0] > 1 ? strides[0] : max(strides[0], shape[1])) }
+}
+
 /// A non-OK mr_status with the library's message for it (the reference's
 /// wording where it has one: AffineBridgeError, DeepSeekV4Error).
 public struct HIPError: Error, CustomStringConvertible {
