@@ -1,6 +1,5 @@
 // What the MFMA kernels for few tokens share (skinny.hip, affine_gemm.hip,
-// mxfp4_few.hip): buffer offsets past every row, the order of workgroups, and
-// the sum of the waves' parts.
+// mxfp4_few.hip): buffer offsets past every row, and the sum of the waves' parts.
 #pragma once
 #include "mr_kernels.hpp"
 
@@ -19,14 +18,6 @@ __device__ __forceinline__ i32x4 uniform_rsrc(const void* base, uint32_t bytes) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
     return r;
-}
-
-// row tile and token block of this workgroup: consecutive workgroups go to
-// the 8 XCDs in turn
-__device__ __forceinline__ void sk_tile(int bid, int blocks, int& tile, int& tb) {
-    const int lo = bid & 7, hi = bid >> 3;
-    tb = hi % blocks;
-    tile = (hi / blocks) * 8 + lo;
 }
 
 // partial sums of the waves -> LDS -> one f32x4 per (tile, lane): emit(r, t,

@@ -6,9 +6,11 @@
 // once per 16 TT rows of x; then x's lines from L2, about two clocks each; and
 // for small matrices the chain of a workgroup (find the tile, load, sum).  A
 // workgroup owns 16 RT weight rows and 16 TT rows of x, and its NW waves split
-// K: wave w takes the entries w, w + NW, ... of 256 k.  Each wave streams its
-// entries into a ring of S entries in LDS by DMA and waits for its own loads
-// alone; the waves' sums meet in LDS once, at the end, in a fixed order.
+// K: wave w takes the entries w, w + NW, ... of 256 k.  Each wave has room for one
+// entry in LDS, filled by DMA: once it is in registers the next one goes out, and
+// the products of this one, the other waves and the other workgroups of the CU
+// cover its way.  A wave waits for its own loads alone; the waves' sums meet in LDS
+// once, at the end, in a fixed order.
 //
 // An entry is one 128-byte line of each weight row, the 16 bytes with the row's
 // eight scale bytes, and 256 values of each row of x.  A lane of the MFMA holds
@@ -132,23 +134,21 @@ __device__ __forceinline__ bool mx_tile(int n_tiles, int blocks, int& tile, int&
     return true;
 }
 
-template <int XT, int RT, int TT, int XI, int S, int NW>
+template <int XT, int RT, int TT, int XI, int NW>
 struct FewShape {
     using X = XEntry<XT>;
     static constexpr int XS = XT == MX_X_MXFP4 ? 1 : 0;  // DMA instructions of x's scales (W's: one)
-    static constexpr int NI = 2 * RT + 1 + XI + XS;
     static constexpr int SOFF = 2048 * RT, XOFF = SOFF + 1024, XSOFF = XOFF + 1024 * XI, ENTRY = XSOFF + 1024 * XS;
     static constexpr int ROWS = XI * X::RPI;             // rows of x in an entry
     static constexpr int BM = ROWS < 16 * TT ? ROWS : 16 * TT;  // rows of x per workgroup
-    static constexpr size_t LDS = std::max<size_t>((size_t)NW * S * ENTRY, (size_t)NW * RT * TT * 1024);
-    static_assert((S - 1) * NI < 64, "vmcnt range");
+    static constexpr size_t LDS = std::max<size_t>((size_t)NW * ENTRY, (size_t)NW * RT * TT * 1024);
     static_assert(RT <= 4 && TT <= 4 && (ROWS >= 16 * TT || (TT == 1 && (ROWS & (ROWS - 1)) == 0)), "rows of an entry");
     static_assert(LDS <= 163840, "LDS");
 };
 
-template <int XT, int RT, int TT, int XI, int S, int NW, bool ROUTED>
+template <int XT, int RT, int TT, int XI, int NW, bool ROUTED>
 __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, int blocks) {
-    using F = FewShape<XT, RT, TT, XI, S, NW>;
+    using F = FewShape<XT, RT, TT, XI, NW>;
     using X = XEntry<XT>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int l = threadIdx.x & 63, q = l >> 4, lr = l & 15;
@@ -216,11 +216,10 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
         for (int t = 0; t < TT; ++t) xsh[t] = ((xs0 + xr[XI + 1 + t] * srow) & 3u) + 2u * q;
     }
 
-    char* ring = lds + w * S * F::ENTRY;
-    auto issue = [&](int i, int slot) {
+    char* const e = lds + w * F::ENTRY;
+    auto issue = [&](int i) {
         const uint32_t ent = w + NW * i;
         const bool live = i < n;
-        char* e = ring + slot * F::ENTRY;
 #pragma unroll
         for (int c = 0; c < 2 * RT; ++c) {
             const bool in = live && 256u * ent + 32u * (ch8 ^ (4 * (c & 1))) < K;
@@ -242,18 +241,15 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
     uint32_t wsh[RT];  // byte of the lane's first block in its row's 16
 #pragma unroll
     for (int r = 0; r < RT; ++r) wsh[r] = ((ws0 + (uint32_t)(16 * r + lr) * srow) & 3u) + 2u * q;
-#pragma unroll
-    for (int s = 0; s < S; ++s) issue(s, s);
+    issue(0);
     // scale bytes of the lane's two blocks, those of 1 past the row's end
     auto scale_bytes = [&](const char* row, uint32_t at, bool in0, bool in1) -> uint32_t {
         const uint32_t* v = (const uint32_t*)row + (at >> 2);
         const uint32_t d = __builtin_amdgcn_alignbyte(v[1], v[0], at & 3u);
         return in1 ? d : (in0 ? (d & 0xffu) | 0x7f00u : 0x7f7fu);
     };
-    int slot = 0;
     for (int i = 0; i < n; ++i) {
-        wait_vmcnt<(S - 1) * F::NI>();
-        const char* e = ring + slot * F::ENTRY;
+        wait_vmcnt<0>();
         const uint32_t k0 = 256u * (w + NW * i) + 64u * q;
         const bool in0 = k0 < K, in1 = k0 + 32 < K;
         u32x4 fw[RT][2];
@@ -279,12 +275,12 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
 #pragma unroll
             for (int t = 0; t < TT; ++t) bx[t] = scale_bytes(e + F::XSOFF + 16 * (16 * t + lr), xsh[t], in0, in1);
         }
-        // the slot is free once everything is in registers
+        // the entry's place is free once everything is in registers
         auto refill = [&] {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_waitcnt(0xc07f);  // the same, known to the compiler
             __builtin_amdgcn_sched_barrier(0);
-            issue(i + S, slot);
+            issue(i + 1);
         };
         f32x4 part[RT][TT];
 #pragma unroll
@@ -327,7 +323,6 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
                 }
             }
         }
-        slot = slot + 1 == S ? 0 : slot + 1;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -643,11 +638,11 @@ hipError_t launch_mid(const Mxfp4GemmParams& p, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <int XT, int RT, int TT, int XI, int S, int NW, bool ROUTED = false>
+template <int XT, int RT, int TT, int XI, int NW, bool ROUTED = false>
 hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
-    using F = FewShape<XT, RT, TT, XI, S, NW>;
+    using F = FewShape<XT, RT, TT, XI, NW>;
     constexpr size_t lds = F::LDS;
-    const auto kern = mxfp4_few_kernel<XT, RT, TT, XI, S, NW, ROUTED>;
+    const auto kern = mxfp4_few_kernel<XT, RT, TT, XI, NW, ROUTED>;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
@@ -701,40 +696,40 @@ int64_t routed_tiles(const Mxfp4GemmParams& p, int bm) {
 hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     const int entries = (p.K + 255) / 256;
     if (p.offsets) {
-        if (few_pairs(p)) return launch_few<0, 1, 1, 1, 1, 4, true>(p, st);
+        if (few_pairs(p)) return launch_few<0, 1, 1, 1, 4, true>(p, st);
         if (p.pairs <= 12 * p.experts) return routed_tiles(p, 16) > 2 * cus ? launch_mid<0, 2, 1, 1, 4, true>(p, st) : launch_mid<0, 2, 1, 2, 4, true>(p, st);
         return routed_tiles(p, 32) > 2 * cus ? launch_mid<0, 2, 2, 1, 4, true>(p, st) : launch_mid<0, 2, 2, 2, 4, true>(p, st);
     }
     if (p.M <= 2) {
-        if (entries >= 16) return launch_few<0, 1, 1, 1, 1, 8>(p, st);
-        return entries >= 8 ? launch_few<0, 1, 1, 1, 1, 4>(p, st) : launch_few<0, 1, 1, 1, 1, 2>(p, st);
+        if (entries >= 16) return launch_few<0, 1, 1, 1, 8>(p, st);
+        return entries >= 8 ? launch_few<0, 1, 1, 1, 4>(p, st) : launch_few<0, 1, 1, 1, 2>(p, st);
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
-    if (n16 * b <= cus) return entries > 4 ? launch_few<0, 1, 1, 8, 1, 8>(p, st) : launch_few<0, 1, 1, 8, 1, 4>(p, st);
-    if (n32 * b <= cus && entries > 4) return launch_few<0, 2, 1, 8, 1, 8>(p, st);
-    if (n64 * b <= cus && entries >= 8) return launch_few<0, 4, 1, 8, 1, 8>(p, st);
-    if (n32 * b <= 2 * cus) return launch_few<0, 2, 1, 8, 1, 4>(p, st);
-    if (n64 * b <= 2 * cus) return launch_few<0, 4, 1, 8, 1, 4>(p, st);
-    if (n64 * (((int64_t)p.M + 47) / 48) <= cus) return launch_few<0, 4, 3, 24, 1, 4>(p, st);
-    if (n64 * (((int64_t)p.M + 63) / 64) <= cus && p.K > 4096) return launch_few<0, 4, 4, 32, 1, 3>(p, st);
+    if (n16 * b <= cus) return entries > 4 ? launch_few<0, 1, 1, 8, 8>(p, st) : launch_few<0, 1, 1, 8, 4>(p, st);
+    if (n32 * b <= cus && entries > 4) return launch_few<0, 2, 1, 8, 8>(p, st);
+    if (n64 * b <= cus && entries >= 8) return launch_few<0, 4, 1, 8, 8>(p, st);
+    if (n32 * b <= 2 * cus) return launch_few<0, 2, 1, 8, 4>(p, st);
+    if (n64 * b <= 2 * cus) return launch_few<0, 4, 1, 8, 4>(p, st);
+    if (n64 * (((int64_t)p.M + 47) / 48) <= cus) return launch_few<0, 4, 3, 24, 4>(p, st);
+    if (n64 * (((int64_t)p.M + 63) / 64) <= cus && p.K > 4096) return launch_few<0, 4, 4, 32, 3>(p, st);
     if (b == 1) return launch_mid<0, 2, 1, 2, 4>(p, st);
     return b == 3 && p.K <= 2048 ? launch_mid<0, 1, 3, 1, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
 }
 
 hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
     if (p.offsets) {
-        if (few_pairs(p)) return launch_few<2, 1, 1, 2, 1, 4, true>(p, st);
+        if (few_pairs(p)) return launch_few<2, 1, 1, 2, 4, true>(p, st);
         return p.pairs <= 10 * p.experts ? launch_mid<2, 2, 1, 1, 2, true>(p, st) : launch_mid<2, 2, 2, 1, 2, true>(p, st);
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
-    if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 1, 8>(p, st);
-    if (n32 * b <= cus) return launch_few<2, 2, 1, 2, 1, 8>(p, st);
-    if (n64 * b <= cus && p.K > 2048) return launch_few<2, 4, 1, 2, 1, 8>(p, st);
-    if (n32 * b <= 2 * cus && p.K <= 2048) return launch_few<2, 2, 1, 2, 1, 4>(p, st);
-    if (n64 * ((b + 1) / 2) <= cus) return launch_few<2, 4, 2, 4, 1, 8>(p, st);
-    if (b > 4 && n64 * ((b + 1) / 2) <= 2 * cus && p.K <= 2048) return launch_few<2, 4, 2, 4, 1, 4>(p, st);
-    if (n64 * ((b + 3) / 4) <= cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 8>(p, st);
-    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 1, 4>(p, st);
+    if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 8>(p, st);
+    if (n32 * b <= cus) return launch_few<2, 2, 1, 2, 8>(p, st);
+    if (n64 * b <= cus && p.K > 2048) return launch_few<2, 4, 1, 2, 8>(p, st);
+    if (n32 * b <= 2 * cus && p.K <= 2048) return launch_few<2, 2, 1, 2, 4>(p, st);
+    if (n64 * ((b + 1) / 2) <= cus) return launch_few<2, 4, 2, 4, 8>(p, st);
+    if (b > 4 && n64 * ((b + 1) / 2) <= 2 * cus && p.K <= 2048) return launch_few<2, 4, 2, 4, 4>(p, st);
+    if (n64 * ((b + 3) / 4) <= cus && p.K > 2048) return launch_few<2, 4, 4, 8, 8>(p, st);
+    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 4>(p, st);
     return b <= 4 ? launch_mid<2, 2, 1, 1, 2>(p, st) : launch_mid<2, 2, 2, 1, 4>(p, st);
 }
 
@@ -750,9 +745,9 @@ hipError_t launch_few_f32(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
         if (2 * tiles <= cus) return launch_mid<1, 1, 1, 1, 4, true>(p, st);
         return tiles <= cus ? launch_mid<1, 2, 1, 1, 4, true>(p, st) : launch_mid<1, 4, 1, 1, 4, true>(p, st);
     }
-    if (p.M == 1) return launch_few<1, 4, 1, 1, 1, 4>(p, st);
+    if (p.M == 1) return launch_few<1, 4, 1, 1, 4>(p, st);
     const int64_t b = ((int64_t)p.M + 15) / 16;
-    if ((p.N + 31) / 32 * b <= 2 * cus) return launch_few<1, 2, 1, 16, 1, 4>(p, st);
+    if ((p.N + 31) / 32 * b <= 2 * cus) return launch_few<1, 2, 1, 16, 4>(p, st);
     return (p.N + 127) / 128 * b <= cus ? launch_mid<1, 2, 1, 1, 4>(p, st) : launch_mid<1, 4, 1, 1, 4>(p, st);
 }
 

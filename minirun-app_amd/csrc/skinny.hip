@@ -45,6 +45,14 @@ namespace mr {
 
 namespace {
 
+// row tile and token block of this workgroup: consecutive workgroups go to
+// the 8 XCDs in turn
+__device__ __forceinline__ void sk_tile(int bid, int blocks, int& tile, int& tb) {
+    const int lo = bid & 7, hi = bid >> 3;
+    tb = hi % blocks;
+    tile = (hi / blocks) * 8 + lo;
+}
+
 // ---------------------------------------------------------------- dense
 // Ring entry: 32 k; W [16 RT rows][64 B], then x [16 TT rows][64 B]; 16-byte
 // chunk c of row r in slot c ^ ((r >> 2) & 3), so the 16 rows of a ds_read_b128
