@@ -549,6 +549,15 @@ constexpr int MXFP4_MAX_OUT = 1 << 22;  // weight rows of a product
 // tiles of 256 or 128 rows of x times as many weight rows (experts' rows: 128),
 // of 128 with two or (x in MXFP4) three workgroups a CU
 enum MxTiles { MX_TILES_NONE, MX_TILES_128x2, MX_TILES_128x3, MX_TILES_256 };
+// Which kernel a call takes: waves that split K and meet at the end (MX_FEW), waves
+// that share the rows of x (MX_MID), or large tiles; `out` weight rows x `rows` rows
+// of x per workgroup
+enum MxKernel { MX_FEW, MX_MID, MX_TILES };
+struct Mxfp4Route {
+    MxKernel kernel;
+    int out, rows, waves, stages;
+};
+Mxfp4Route mxfp4_route(const Mxfp4GemmParams& p, int cu_count);
 hipError_t launch_mxfp4_tiles(const Mxfp4GemmParams& p, MxTiles kind, hipStream_t st);
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p);
 hipError_t launch_mxfp4_gemm(const Mxfp4GemmParams& p, int cu_count, hipStream_t st);

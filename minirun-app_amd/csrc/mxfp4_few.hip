@@ -622,35 +622,36 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
                     });
 }
 
-template <int XT, int RT, int TT, int S, int NW, bool ROUTED = false>
-hipError_t launch_mid(const Mxfp4GemmParams& p, hipStream_t st) {
-    using F = MidShape<XT, RT, TT, S, NW>;
-    constexpr int BM = 16 * TT, BN = 16 * RT * NW;
-    const auto kern = mxfp4_mid_kernel<XT, RT, TT, S, NW, ROUTED>;
-    if (F::LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)F::LDS);
-        if (e != hipSuccess) return e;
-    }
-    const int64_t tiles = (p.N + BN - 1) / BN, blocks = ((int64_t)p.M + BM - 1) / BM;
-    const int64_t grid = ROUTED ? (mx_tile_bound(p, BM) * tiles + 7) / 8 * 8 : (tiles * blocks + 7) / 8 * 8;
-    if (grid * 64 * NW >= (1ll << 32)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), F::LDS, st, p, (int)blocks);
-    return hipGetLastError();
-}
-
+// The kernels as a call chooses among them: launch, or say which it is
 template <int XT, int RT, int TT, int XI, int NW, bool ROUTED = false>
-hipError_t launch_few(const Mxfp4GemmParams& p, hipStream_t st) {
+struct Few {
     using F = FewShape<XT, RT, TT, XI, NW>;
-    constexpr size_t lds = F::LDS;
-    const auto kern = mxfp4_few_kernel<XT, RT, TT, XI, NW, ROUTED>;
-    if (lds > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    static constexpr Mxfp4Route ROUTE = {MX_FEW, 16 * RT, F::BM, NW, 1};
+    static constexpr int BN = 16 * RT, BM = F::BM, THREADS = 64 * NW;
+    static constexpr size_t LDS = F::LDS;
+    static constexpr auto KERNEL = mxfp4_few_kernel<XT, RT, TT, XI, NW, ROUTED>;
+    static constexpr bool BY_EXPERT = ROUTED;
+};
+template <int XT, int RT, int TT, int S, int NW, bool ROUTED = false>
+struct Mid {
+    using F = MidShape<XT, RT, TT, S, NW>;
+    static constexpr Mxfp4Route ROUTE = {MX_MID, 16 * RT * NW, 16 * TT, NW, S};
+    static constexpr int BN = 16 * RT * NW, BM = 16 * TT, THREADS = 64 * NW;
+    static constexpr size_t LDS = F::LDS;
+    static constexpr auto KERNEL = mxfp4_mid_kernel<XT, RT, TT, S, NW, ROUTED>;
+    static constexpr bool BY_EXPERT = ROUTED;
+};
+
+template <typename C>
+hipError_t launch(const Mxfp4GemmParams& p, hipStream_t st) {
+    if (C::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)C::KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS);
         if (e != hipSuccess) return e;
     }
-    const int64_t tiles = (p.N + 16 * RT - 1) / (16 * RT), blocks = ((int64_t)p.M + F::BM - 1) / F::BM;
-    const int64_t grid = ROUTED ? (mx_tile_bound(p, F::BM) * tiles + 7) / 8 * 8 : (tiles * blocks + 7) / 8 * 8;
-    if (grid * 64 * NW >= (1ll << 32)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), lds, st, p, (int)blocks);
+    const int64_t tiles = (p.N + C::BN - 1) / C::BN, blocks = ((int64_t)p.M + C::BM - 1) / C::BM;
+    const int64_t grid = C::BY_EXPERT ? (mx_tile_bound(p, C::BM) * tiles + 7) / 8 * 8 : (tiles * blocks + 7) / 8 * 8;
+    if (grid * C::THREADS >= (1ll << 32)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(C::KERNEL, dim3((unsigned)grid), dim3(C::THREADS), C::LDS, st, p, (int)blocks);
     return hipGetLastError();
 }
 
@@ -693,44 +694,46 @@ int64_t routed_tiles(const Mxfp4GemmParams& p, int bm) {
     return ((int64_t)p.N + 127) / 128 * (p.pairs * 4ll <= p.experts * 3ll * bm ? std::min(p.experts, p.pairs) : p.pairs / bm + p.experts / 2);
 }
 
-hipError_t launch_few_bf16(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+template <typename Go>
+auto choose_bf16(const Mxfp4GemmParams& p, int cus, Go go) {
     const int entries = (p.K + 255) / 256;
     if (p.offsets) {
-        if (few_pairs(p)) return launch_few<0, 1, 1, 1, 4, true>(p, st);
-        if (p.pairs <= 12 * p.experts) return routed_tiles(p, 16) > 2 * cus ? launch_mid<0, 2, 1, 1, 4, true>(p, st) : launch_mid<0, 2, 1, 2, 4, true>(p, st);
-        return routed_tiles(p, 32) > 2 * cus ? launch_mid<0, 2, 2, 1, 4, true>(p, st) : launch_mid<0, 2, 2, 2, 4, true>(p, st);
+        if (few_pairs(p)) return go(Few<0, 1, 1, 1, 4, true>{});
+        if (p.pairs <= 12 * p.experts) return routed_tiles(p, 16) > 2 * cus ? go(Mid<0, 2, 1, 1, 4, true>{}) : go(Mid<0, 2, 1, 2, 4, true>{});
+        return routed_tiles(p, 32) > 2 * cus ? go(Mid<0, 2, 2, 1, 4, true>{}) : go(Mid<0, 2, 2, 2, 4, true>{});
     }
     if (p.M <= 2) {
-        if (entries >= 16) return launch_few<0, 1, 1, 1, 8>(p, st);
-        return entries >= 8 ? launch_few<0, 1, 1, 1, 4>(p, st) : launch_few<0, 1, 1, 1, 2>(p, st);
+        if (entries >= 16) return go(Few<0, 1, 1, 1, 8>{});
+        return entries >= 8 ? go(Few<0, 1, 1, 1, 4>{}) : go(Few<0, 1, 1, 1, 2>{});
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
-    if (n16 * b <= cus) return entries > 4 ? launch_few<0, 1, 1, 8, 8>(p, st) : launch_few<0, 1, 1, 8, 4>(p, st);
-    if (n32 * b <= cus && entries > 4) return launch_few<0, 2, 1, 8, 8>(p, st);
-    if (n64 * b <= cus && entries >= 8) return launch_few<0, 4, 1, 8, 8>(p, st);
-    if (n32 * b <= 2 * cus) return launch_few<0, 2, 1, 8, 4>(p, st);
-    if (n64 * b <= 2 * cus) return launch_few<0, 4, 1, 8, 4>(p, st);
-    if (n64 * (((int64_t)p.M + 47) / 48) <= cus) return launch_few<0, 4, 3, 24, 4>(p, st);
-    if (n64 * (((int64_t)p.M + 63) / 64) <= cus && p.K > 4096) return launch_few<0, 4, 4, 32, 3>(p, st);
-    if (b == 1) return launch_mid<0, 2, 1, 2, 4>(p, st);
-    return b == 3 && p.K <= 2048 ? launch_mid<0, 1, 3, 1, 4>(p, st) : launch_mid<0, 2, 2, 2, 4>(p, st);
+    if (n16 * b <= cus) return entries > 4 ? go(Few<0, 1, 1, 8, 8>{}) : go(Few<0, 1, 1, 8, 4>{});
+    if (n32 * b <= cus && entries > 4) return go(Few<0, 2, 1, 8, 8>{});
+    if (n64 * b <= cus && entries >= 8) return go(Few<0, 4, 1, 8, 8>{});
+    if (n32 * b <= 2 * cus) return go(Few<0, 2, 1, 8, 4>{});
+    if (n64 * b <= 2 * cus) return go(Few<0, 4, 1, 8, 4>{});
+    if (n64 * (((int64_t)p.M + 47) / 48) <= cus) return go(Few<0, 4, 3, 24, 4>{});
+    if (n64 * (((int64_t)p.M + 63) / 64) <= cus && p.K > 4096) return go(Few<0, 4, 4, 32, 3>{});
+    if (b == 1) return go(Mid<0, 2, 1, 2, 4>{});
+    return b == 3 && p.K <= 2048 ? go(Mid<0, 1, 3, 1, 4>{}) : go(Mid<0, 2, 2, 2, 4>{});
 }
 
-hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+template <typename Go>
+auto choose_mxfp4(const Mxfp4GemmParams& p, int cus, Go go) {
     if (p.offsets) {
-        if (few_pairs(p)) return launch_few<2, 1, 1, 2, 4, true>(p, st);
-        return p.pairs <= 10 * p.experts ? launch_mid<2, 2, 1, 1, 2, true>(p, st) : launch_mid<2, 2, 2, 1, 2, true>(p, st);
+        if (few_pairs(p)) return go(Few<2, 1, 1, 2, 4, true>{});
+        return p.pairs <= 10 * p.experts ? go(Mid<2, 2, 1, 1, 2, true>{}) : go(Mid<2, 2, 2, 1, 2, true>{});
     }
     const int64_t b = ((int64_t)p.M + 15) / 16, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32, n64 = (p.N + 63) / 64;
-    if (n16 * b <= cus) return launch_few<2, 1, 1, 2, 8>(p, st);
-    if (n32 * b <= cus) return launch_few<2, 2, 1, 2, 8>(p, st);
-    if (n64 * b <= cus && p.K > 2048) return launch_few<2, 4, 1, 2, 8>(p, st);
-    if (n32 * b <= 2 * cus && p.K <= 2048) return launch_few<2, 2, 1, 2, 4>(p, st);
-    if (n64 * ((b + 1) / 2) <= cus) return launch_few<2, 4, 2, 4, 8>(p, st);
-    if (b > 4 && n64 * ((b + 1) / 2) <= 2 * cus && p.K <= 2048) return launch_few<2, 4, 2, 4, 4>(p, st);
-    if (n64 * ((b + 3) / 4) <= cus && p.K > 2048) return launch_few<2, 4, 4, 8, 8>(p, st);
-    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return launch_few<2, 4, 4, 8, 4>(p, st);
-    return b <= 4 ? launch_mid<2, 2, 1, 1, 2>(p, st) : launch_mid<2, 2, 2, 1, 4>(p, st);
+    if (n16 * b <= cus) return go(Few<2, 1, 1, 2, 8>{});
+    if (n32 * b <= cus) return go(Few<2, 2, 1, 2, 8>{});
+    if (n64 * b <= cus && p.K > 2048) return go(Few<2, 4, 1, 2, 8>{});
+    if (n32 * b <= 2 * cus && p.K <= 2048) return go(Few<2, 2, 1, 2, 4>{});
+    if (n64 * ((b + 1) / 2) <= cus) return go(Few<2, 4, 2, 4, 8>{});
+    if (b > 4 && n64 * ((b + 1) / 2) <= 2 * cus && p.K <= 2048) return go(Few<2, 4, 2, 4, 4>{});
+    if (n64 * ((b + 3) / 4) <= cus && p.K > 2048) return go(Few<2, 4, 4, 8, 8>{});
+    if (n64 * ((b + 3) / 4) <= 2 * cus && p.K > 2048) return go(Few<2, 4, 4, 8, 4>{});
+    return b <= 4 ? go(Mid<2, 2, 1, 1, 2>{}) : go(Mid<2, 2, 2, 1, 4>{});
 }
 
 // f32: the cuts of x cost more than its bytes, so a cut serves 32 or 64 weight
@@ -739,21 +742,27 @@ hipError_t launch_few_mxfp4(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
 // 768 x 2048, 12 rows, 40 and 53; 64 of 512 x 512, one row, 9.0 and 8.1); few of
 // them split K instead: 1536 x 7168, 64 tokens, 32 x 16 with 4 waves 23, mid 62,
 // 2048 x 2048 9 and 20
-hipError_t launch_few_f32(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
+template <typename Go>
+auto choose_f32(const Mxfp4GemmParams& p, int cus, Go go) {
     if (p.offsets) {
         const int64_t tiles = routed_tiles(p, 16);
-        if (2 * tiles <= cus) return launch_mid<1, 1, 1, 1, 4, true>(p, st);
-        return tiles <= cus ? launch_mid<1, 2, 1, 1, 4, true>(p, st) : launch_mid<1, 4, 1, 1, 4, true>(p, st);
+        if (2 * tiles <= cus) return go(Mid<1, 1, 1, 1, 4, true>{});
+        return tiles <= cus ? go(Mid<1, 2, 1, 1, 4, true>{}) : go(Mid<1, 4, 1, 1, 4, true>{});
     }
-    if (p.M == 1) return launch_few<1, 4, 1, 1, 4>(p, st);
+    if (p.M == 1) return go(Few<1, 4, 1, 1, 4>{});
     const int64_t b = ((int64_t)p.M + 15) / 16;
-    if ((p.N + 31) / 32 * b <= 2 * cus) return launch_few<1, 2, 1, 16, 4>(p, st);
-    return (p.N + 127) / 128 * b <= cus ? launch_mid<1, 2, 1, 1, 4>(p, st) : launch_mid<1, 4, 1, 1, 4>(p, st);
+    if ((p.N + 31) / 32 * b <= 2 * cus) return go(Few<1, 2, 1, 16, 4>{});
+    return (p.N + 127) / 128 * b <= cus ? go(Mid<1, 2, 1, 1, 4>{}) : go(Mid<1, 4, 1, 1, 4>{});
+}
+
+template <typename Go>
+auto choose(const Mxfp4GemmParams& p, int cus, Go go) {
+    if (p.x_kind == MX_X_MXFP4) return choose_mxfp4(p, cus, go);
+    return p.x_kind == MX_X_F32 ? choose_f32(p, cus, go) : choose_bf16(p, cus, go);
 }
 
 hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
-    if (p.x_kind == MX_X_MXFP4) return launch_few_mxfp4(p, cus, st);
-    return p.x_kind == MX_X_F32 ? launch_few_f32(p, cus, st) : launch_few_bf16(p, cus, st);
+    return choose(p, cus, [&](auto c) { return launch<decltype(c)>(p, st); });
 }
 
 // Large tiles (mxfp4_gemm.hip), or none.  Those of 128 x 128 pay once they cover
@@ -804,6 +813,13 @@ MxTiles tiles_of(const Mxfp4GemmParams& p, int cus) {
 // threads
 bool mxfp4_gemm_fits(const Mxfp4GemmParams& p) {
     return !p.offsets || (mx_tile_bound(p, 16) * ((p.N + 127) / 128) + 7) * 256 < (1ll << 32);
+}
+
+Mxfp4Route mxfp4_route(const Mxfp4GemmParams& p, int cu_count) {
+    const MxTiles tile = tiles_of(p, cu_count);
+    if (tile == MX_TILES_NONE) return choose(p, cu_count, [](auto c) { return decltype(c)::ROUTE; });
+    const int size = tile == MX_TILES_256 ? 256 : 128;
+    return {MX_TILES, size, size, 4, tile == MX_TILES_128x3 ? 1 : 2};
 }
 
 // A matrix's tokens in as many launches as grids of less than 2^32 threads take:
