@@ -379,13 +379,13 @@ template <int XT, int RT, int TT, int S, int NW>
 struct MidShape {
     using X = XEntry<XT>;
     static constexpr int XI = 16 * TT / X::RPI;           // DMA instructions of x
-    static constexpr int XPW = (XI + NW - 1) / NW;        // of a wave
+    static constexpr int XPW = XI / NW;                   // of a wave
     static constexpr int XS = XT == MX_X_MXFP4 ? 1 : 0;   // of x's scales: a copy per wave
     static constexpr int NI = XPW + 2 * RT + 1 + XS;
     static constexpr int WAVE = 2048 * RT + 1024 + 1024 * XS;  // bytes of a wave's part
     static constexpr int STAGE = 1024 * XI + NW * WAVE;
     static constexpr size_t LDS = (size_t)S * STAGE;
-    static_assert((S - 1) * NI < 64 && LDS <= 163840 && RT <= 4 && TT <= 4, "stages");
+    static_assert(XI % NW == 0 && (S - 1) * NI < 64 && LDS <= 163840 && RT <= 4 && TT <= 4, "stages");
 };
 
 template <int XT, int RT, int TT, int S, int NW, bool ROUTED>
@@ -437,8 +437,8 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
         wo[i] = r < rows ? (uint32_t)r * wrow + 16u * (ch8 ^ (4 * (i & 1))) : SK_OOB_ROW;
     }
     const uint32_t so = l < rows ? (ws0 + (uint32_t)l * srow) & ~3u : SK_OOB_ROW;
-    // x: this wave's instruction u of XPW (the last waves may repeat one)
-    auto x_instr = [&](int u) { return min(F::XPW * w + u, F::XI - 1); };
+    // x: this wave's instruction u of XPW
+    auto x_instr = [&](int u) { return F::XPW * w + u; };
     auto x_row = [&](int u) { return X::RPI * x_instr(u) + l / X::CHUNKS; };
     auto x_chunk = [&](int u) { return (uint32_t)X::chunk(l % X::CHUNKS, x_row(u)); };
     constexpr int NX = F::XPW + (XT == MX_X_MXFP4 ? 1 + TT : 0);
@@ -664,8 +664,10 @@ hipError_t launch(const Mxfp4GemmParams& p, hipStream_t st) {
 //     tokens, 64 x 16 16.5, 32 x 16 with 4 waves 20.4; with 4 waves where a row is
 //     short: 273 x 1024, 300 tokens, 4.8 and 6.9.  Then one round of 64 x 48 (4096 x
 //     4096, 150 tokens, 14.6, mid 18) or, for long rows, of 64 x 64 with 3 waves
-//     (1536 x 12608, 600 tokens, 51 and 67), else mid: 24576 x 1536, 37 tokens, mid
-//     64 x 48 10.5, 128 x 32 11.3, 64 x 16 17
+//     (1536 x 12608, 600 tokens, 51 and 67), else mid, 128 x 32: 24576 x 1536, 37
+//     tokens, 10.5, 64 x 16 17 (64 x 48, which fits 33 to 48 tokens: 10.3, but with
+//     the weights from HBM 12.7 and 128 x 32 12.3; 65536 x 2048, 48 tokens, 34.9
+//     and 30.1; 20000 x 1536, 34 tokens, 12.5 and 11.8)
 //   x in MXFP4, which costs a quarter to read: 7168 x 4096, 16 tokens, 32 x 16 with
 //     8 waves 4.8, 16 x 16 5.8, 64 x 16 5.7; 1024 x 4096, 200 tokens, 64 x 16 with 8
 //     waves 5.9, 64 x 32 6.5, x 1024 32 x 16 with 4 4.1, 64 x 32 4.9; 1024 x 2048,
@@ -715,7 +717,7 @@ auto choose_bf16(const Mxfp4GemmParams& p, int cus, Go go) {
     if (n64 * (((int64_t)p.M + 47) / 48) <= cus) return go(Few<0, 4, 3, 24, 4>{});
     if (n64 * (((int64_t)p.M + 63) / 64) <= cus && p.K > 4096) return go(Few<0, 4, 4, 32, 3>{});
     if (b == 1) return go(Mid<0, 2, 1, 2, 4>{});
-    return b == 3 && p.K <= 2048 ? go(Mid<0, 1, 3, 1, 4>{}) : go(Mid<0, 2, 2, 2, 4>{});
+    return go(Mid<0, 2, 2, 2, 4>{});
 }
 
 template <typename Go>

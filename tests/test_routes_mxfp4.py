@@ -64,6 +64,16 @@ MATRIX = {
         (300, 24576, 1536, (TILES, 128, 128, 4, 1)), (4096, 7168, 16384, (TILES, 256, 256, 4, 2)),
     ],
 }
+
+
+def test_neighbouring_sizes_take_the_same_kernel(route):
+    """17 to 64 tokens of bf16 on weights of more than 16384 rows: one kernel, whatever
+    the number of tokens or the row's length."""
+    took = {route("bf16", t, n, k) for t in range(17, 65) for n in (16400, 20480, 24576, 33000, 65536)
+            for k in (512, 1536, 2016, 2048, 2080, 4096, 7168)}
+    assert took == {(MID, 128, 32, 4, 2)}
+
+
 EXPERTS = {
     "bf16": [
         (8, 8, 128, 768, 2048, (FEW, 16, 2, 4, 1)), (768, 8, 128, 2048, 768, (MID, 128, 16, 4, 1)),
