@@ -338,9 +338,9 @@ mr_status mr_mxfp4_dequantize(const mr_mxfp4_matrix *w, void *out, mr_dtype out_
  * bytes 253 and 254, which meet activations as in IEEE arithmetic: an infinity,
  * or NaN with a zero); f32 activations exactly too (as three bf16 parts, but for
  * parts below 2^-133).  x is 16-byte aligned with rows a multiple of 16 and at
- * most 2^23 bytes apart, w->packed 16-byte aligned; out is at most 2^22, in
+ * most 2^23 bytes apart, w->packed 16-byte aligned; out is 1 to 2^22, in at most
  * 2^20.  The order of a token's sums, and so its last bits, depends on how many
- * tokens the call has. */
+ * tokens the call has.  Here and below, outputs overlap no input. */
 mr_status mr_mxfp4_matmul(const void *x, mr_dtype x_dtype, int32_t tokens, int64_t x_stride,
                           const mr_mxfp4_matrix *w, void *y, mr_dtype y_dtype, int64_t y_stride, void *stream);
 
@@ -388,6 +388,8 @@ mr_status mr_expert_dispatch(const void *x, mr_dtype dtype, int32_t tokens, int6
  * source(r) is r with pair_of_row NULL (x has `rows` rows), else
  * pair_of_row[r] / per_token (x has one row per token, less than 2^32 - 2^16
  * bytes in all).  Rows of y past the last expert's are left as they were.
+ * One launch takes (rows + 15 min(experts, rows)) / 16 tiles of rows times
+ * (out + 127) / 128 of weight rows, at most 2^24 - 8 in all; more are refused.
  * offsets, pair_of_row: mr_expert_sort's; values that it does not write give
  * rows of y that are unspecified, never an access outside the buffers. */
 typedef struct mr_mxfp4_expert_args {

@@ -49,7 +49,8 @@ struct XEntry {  // of 256 k
     // Chunk c of row r is in slot c ^ swizzle(r), so that the 16 rows of a read of
     // one chunk lie in 16 bank groups.  bf16: with bits 3 and 4 of c exchanged, so
     // that lanes of the first two of a read's four blocks, which it takes together,
-    // have the same groups for the same rows (four clocks less a read).
+    // have the same groups for the same rows (four clocks less a read; with the two
+    // rows of one token's kernels four more, beside a wait for the weights).
     static __device__ __forceinline__ int swizzle(int r) { return XT == MX_X_MXFP4 ? (r >> 1) & 7 : r & 15; }
     static __device__ __forceinline__ int swap(int c) { return XT == MX_X_BF16 ? (c & 7) | (c & 8) << 1 | (c & 16) >> 1 : c; }
     static __device__ __forceinline__ int slot(int c, int r) { return swap(c) ^ swizzle(r); }
@@ -657,7 +658,9 @@ hipError_t launch(const Mxfp4GemmParams& p, hipStream_t st) {
 
 // Which kernel and tile.  Both split a call into workgroups of some weight rows
 // x some rows of x; small ones fill the GPU, large ones read less, and rows that
-// are short leave waves that split them idle.  In us, one call among others:
+// are short leave waves that split them idle.  In us, one call among others with
+// the weights in the caches, unless it says otherwise (from HBM 5 to 25% more, and
+// more for kernels that read the weights more than once):
 //   matrix, x in bf16, one round of workgroups of the smallest tile that gives no
 //     more than one a CU, with 8 waves: 576 x 7168, 96 tokens, 16 x 16 7.4, 32 x
 //     16 8.4; 1536 x 7168, 64 tokens, 32 x 16 8.5, 16 x 16 12.3; 2048 x 12608, 100
@@ -769,22 +772,27 @@ hipError_t launch_mxfp4_few(const Mxfp4GemmParams& p, int cus, hipStream_t st) {
 
 // Large tiles (mxfp4_gemm.hip), or none.  Those of 128 x 128 pay once they cover
 // the larger part of the GPU and the kernels of few rows would read W more than
-// once (us, 128 and few rows: bf16, 24576 x 1536, 65 tokens, 192 tiles, 14 and 17,
-// 64 tokens 14 and 11; 7168 x 16384, 300 tokens, 168 tiles, 107 and 135, 200
-// tokens, 112 tiles, 107 and 81; 16384 x 4096, 65 tokens, 128 tiles, 31 and 24;
-// MXFP4: there 15.5 and 16.6, 64 tokens 15.5 and 11.4; 24576 x 1536, 37 tokens,
-// 6.7 and 7.7; 4096 x 12608, 400 tokens, 128 tiles, 55 and 36), and for experts from some rows each (128 of 768 x 2048: bf16,
-// 62 rows, 45 and 46, 50 rows 44 and 38, 31 rows 42 and 31; 32 of 1536 x 7168, 88
-// rows, 85 and 98, 62 rows 82 and 76; MXFP4: 31 rows, 22.0 and 23.9, 19 rows 20.5
-// and 19.6).
+// once.  In us, one call among others, weights from HBM (from the caches 5 to 30%
+// less, with the same sides ahead except where noted), 128 and few rows:
+//   bf16: 24576 x 1536, 65 tokens, 192 tiles, 16.2 and 18.4, 64 tokens 16.1 and
+//     12.6; 7168 x 16384, 300 tokens, 168 tiles, 122 and 135, 200 tokens, 112 tiles,
+//     123 and 86; 16384 x 4096, 65 tokens, 128 tiles, 35 and 25
+//   MXFP4: 24576 x 1536, 64 tokens, 10.2 and 12.2, 37 tokens 9.9 and 10.5; 16384 x
+//     4096, 65 tokens, 19.8 and 17.5; 4096 x 12608, 400 tokens, 128 tiles, 68 and 42
+// and for experts from some rows each: bf16, 128 of 768 x 2048, 62 rows, 52 and 49,
+// 50 rows 52 and 44, 31 rows 50 and 38; 32 of 1536 x 7168, 88 rows, 99 and 110, 62
+// rows 96 and 89; MXFP4, 128 of 768 x 2048, 31 rows, 25.0 and 35.2, 19 rows 24.7 and
+// 26.1 (from the caches 20.4 and 19.4).  The border of 60 rows in bf16 is early by
+// about 10.
 // Between the tiles, by rounds of workgroups, in units of a sixth of the time of a
-// round of two a CU (bf16: a last round of at most one a CU takes 4):
-// three a CU 8, 256 x 256 12 (MXFP4) or 10.5 (bf16).  MXFP4, three, two, 256:
-// 24576 x 1536, 300 tokens, 13.5, 16.2 and 16.7 us, 4096 tokens 96, 107 and 103;
-// 16384 x 4096, 1000 tokens, 46, 44 and 38; 4096 tokens to 8 of 128 experts of 768
-// x 2048 45 and 50; 1024 to 8 of 32 of 1536 x 7168 77 and 69.  bf16, two and 256:
-// 24576 x 1536, 600 tokens, 45 and 72, 4096 tokens 260 and 247; 16384 x 4096, 1000
-// tokens, 116 and 101.
+// round of two a CU (bf16: a last round of at most one a CU takes 4): three a CU 8,
+// 256 x 256 12 (MXFP4) or 10.5 (bf16).
+//   MXFP4, three, two, 256: 24576 x 1536, 300 tokens, 16.1, 21.0 and 19.9, 4096
+//     tokens 121, 146 and 121; 16384 x 4096, 1000 tokens, 55, 52 and 41; 4096 tokens
+//     to 8 of 128 experts of 768 x 2048 54 and 62; 1024 to 8 of 32 of 1536 x 7168 98
+//     and 89; 7168 x 16384, 400 tokens, 72 and 64
+//   bf16, two and 256: 24576 x 1536, 600 tokens, 48 and 74, 4096 tokens 268 and 254;
+//     16384 x 4096, 1000 tokens, 120 and 102
 MxTiles tiles_of(const Mxfp4GemmParams& p, int cus) {
     if (p.x_kind == MX_X_F32) return MX_TILES_NONE;
     const bool mx = p.x_kind == MX_X_MXFP4;

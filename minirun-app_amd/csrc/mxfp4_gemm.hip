@@ -7,14 +7,14 @@
 // workgroup of 4 waves computes a tile, each wave a quarter of it in 32x32 MFMA
 // tiles; each operand fragment serves MI or JN of them.  With 256 x 256 (the
 // accumulators are half of the registers, one workgroup a CU) a prompt of 4096
-// tokens runs at 1.2 PFLOP/s in bf16 (24576 x 1536, 255 us) and 3.9 PFLOP/s in
-// MXFP4 (7168 x 16384, 245 us; 4.3 with the weights in the caches).  128 x 128
-// reads twice as much per operation, but two or three workgroups a CU cover each
-// other's waits, ends of tiles and starts: 4096 tokens to 8 of 128 experts of 768 x
-// 2048, MXFP4, three 62 us, two 67, with 128 x 256 and one workgroup 78 (31 us is
-// the time of the bytes; eight stages a tile leave latency in view: of the 30000
-// clocks of a tile with two workgroups 19000 were its stages', whose matrix
-// instructions take 5800, 7500 its start and 3500 its end).
+// tokens runs at 1.2 PFLOP/s in bf16 (24576 x 1536, 254 us) and 4.1 PFLOP/s in
+// MXFP4 (7168 x 16384, 232 us; 217 with the operands in the caches; 230 to 255 from
+// card to card).  128 x 128 reads twice as much per operation, but two or three
+// workgroups a CU cover each other's waits, ends of tiles and starts: 4096 tokens to
+// 8 of 128 experts of 768 x 2048, MXFP4, three 54 us, two 62 (weights from HBM; from
+// the caches 47 and 54; 31 us is the time of the bytes; eight stages a tile leave
+// latency in view: of the 30000 clocks of a tile with two workgroups 19000 were its
+// stages', whose matrix instructions take 5800, 7500 its start and 3500 its end).
 // Operands come by global -> LDS DMA, issued between the MFMAs.  A load costs by
 // the lines it touches, about two clocks each, whether it takes 4 or 128 bytes of
 // a line, so rows come in whole lines of 128 bytes and scales 16 bytes of a row
@@ -33,7 +33,7 @@
 //     leave of its way is the other workgroups' time.  It takes less LDS and fewer
 //     registers, which makes room for a third workgroup; where there are not that
 //     many, or for bf16 (a third one gained nothing there: 112 and 111 us), the
-//     ring of two is faster (7168 x 16384, 400 tokens, 49 and 57 us).
+//     ring of two is faster (7168 x 16384, 400 tokens, 64 and 72 us).
 //   x in bf16: a stage is 64 k: a line of each row of x, in a ring of three; W's
 //     rows come 64 bytes (two stages) at a time, in a ring of two.  Lane half h
 //     has block h of the stage's two: the block's four words, one per 16-deep
