@@ -21,8 +21,8 @@
 //     values of x that belong to the word.
 //   x in f32: the same with x cut into three bf16 parts by truncation, whose
 //     sum is x exactly.  Against an infinite weight (scale bytes 253 and 254) a
-//     part that is zero makes the sum NaN: outputs that are NaN are computed
-//     again, x uncut.
+//     part that is zero makes the sum NaN: outputs that are NaN, of weight rows
+//     that have such bytes, are computed again, x uncut.
 //   x in MXFP4: v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands' codes
 //     and scale bytes as they are.
 // Chains start from zero per entry and are added to the running sums in f32.
@@ -95,16 +95,27 @@ __device__ __forceinline__ float mx_f32_again(const float* x, const uint32_t* pa
     return wave_sum(d);
 }
 
-// Those that are NaN of a wave's outputs again: of lane l, bit i of `again`, in
-// row m of the tile from m0 on and weight row n of the expert, m and n from
-// at(l, i); stored by that lane through store(m, n, value).
+// Those that are NaN of a wave's outputs again, if any of the weight rows that they
+// are of may hold infinite weights: `words` has those rows' scale bytes, n of them
+// words.  Of lane l, bit i of `again` is an output in row m of the tile from m0 on and
+// weight row n of the expert, m and n from at(l, i); stored by that lane through
+// store(m, n, value).
 template <typename At, typename Store>
-__device__ __forceinline__ void mx_f32_nans(const Mxfp4GemmParams& p, bool by_token, int64_t first_row, int m0, uint32_t again,
-                                            At at, Store store) {
+__device__ __forceinline__ void mx_f32_nans(const Mxfp4GemmParams& p, bool by_token, int64_t first_row, int m0,
+                                            const uint32_t* words, int n_words, uint32_t again, At at, Store store) {
     const int l = threadIdx.x & 63;
     uint64_t lanes = __ballot(again != 0);
+    if (__builtin_expect(lanes == 0, 1)) return;
+    bool mine = false;
+#pragma unroll 4
+    for (int i = l; i < n_words; i += 64) {
+        const uint32_t v = words[i];
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) mine |= ((v >> k) & 255u) - 253u < 2u;
+    }
+    if (!__ballot(mine)) return;
 #pragma unroll 1
-    while (__builtin_expect(lanes != 0, 0)) {
+    while (lanes) {
         const int from = __builtin_ctzll(lanes);
         lanes &= lanes - 1;
         uint32_t bits = __builtin_amdgcn_readlane(again, from);
@@ -345,12 +356,11 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_few_kernel(Mxfp4GemmParams p, i
             for (int e = 0; e < 4; ++e) {
                 const int m = 16 * t + 4 * (lane >> 4) + e;
                 if (nn >= rows || m >= toks) continue;
-                if (v[e] == v[e])
-                    store(m, n0 + nn, v[e]);
-                else
-                    again |= 1u << e;
+                store(m, n0 + nn, v[e]);
+                if (v[e] != v[e]) again |= 1u << e;
             }
-            mx_f32_nans(p, by_token, first_row, m0, again,
+            mx_f32_nans(p, by_token, first_row, m0, (const uint32_t*)(uintptr_t)(wsa & ~3ull),
+                        (int)((ws0 + (uint32_t)rows * srow + 3u) >> 2), again,
                         [&](int from, int e, int& m, int& n) {
                             m = 16 * t + 4 * (from >> 4) + e;
                             n = n0 + 16 * r + (from & 15);
@@ -609,7 +619,8 @@ __global__ void __launch_bounds__(64 * NW) mxfp4_mid_kernel(Mxfp4GemmParams p, i
         }
     }
     if constexpr (XT == MX_X_F32)
-        mx_f32_nans(p, by_token, first_row, m0, again,
+        mx_f32_nans(p, by_token, first_row, m0, (const uint32_t*)(uintptr_t)(wsa & ~3ull),
+                    (int)((ws0 + wrows * srow + 3u) >> 2), again,
                     [&](int from, int i, int& m, int& n) {
                         m = 16 * (i / (4 * RT)) + (from & 15);
                         n = n0 + 16 * (i / 4 % RT) + 4 * (from >> 4) + i % 4;
