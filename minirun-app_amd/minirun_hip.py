@@ -637,8 +637,10 @@ def _call_stream(device, stream):
     cuda = torch.cuda
     if stream is None:
         # current_stream(device).cuda_stream without the two Python objects
-        # between, which cost 2 of a small call's 10 us
-        handle = torch._C._cuda_getCurrentRawStream(device.index)
+        # between, which cost 2 of a small call's 10 us; not part of torch's public
+        # interface, so not relied on
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        handle = raw(device.index) if raw else cuda.current_stream(device).cuda_stream
         return handle, _HERE if device.index == cuda.current_device() else cuda.device(device)
     if isinstance(stream, cuda.Stream):
         if stream.device != device:
