@@ -643,6 +643,158 @@ size_t mr_mla_prefill_block_workspace_size(const mr_mla_prefill_block_args *args
 mr_status mr_mla_prefill_block(const mr_mla_prefill_block_args *args, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Grouped-query attention over a paged cache: the part of QwenAttention.forward
+ * (Sources/ModelAdapters/Model/QwenMoEModel.swift:193-264) between its
+ * projections, for many sequences at once.  Norms of the heads of queries and
+ * keys with the rotation, keys and values into pages of bf16 or MXFP4, attention
+ * over the pages.  (The reference keeps one sequence's keys and values whole.)
+ * ------------------------------------------------------------------------ */
+
+/* A rotation of heads by their tokens' positions: columns [col0, col0 + dim) of
+ * a head, as pairs (2 i, 2 i + 1) (DeepSeekV4Rotary.apply,
+ * DeepSeekV4Attention.swift:108-165) or (i, i + dim / 2)
+ * (QwenMoEModel.swift:223-228), pair i of token t by the angle whose cosine and
+ * sine are cos_t[r][i], sin_t[r][i] with r = positions[t] (NULL: r = t), device
+ * f32 [table_rows][dim / 2] (mr_rope_table).  A position outside the tables gives
+ * NaN.  dim 0: no rotation, nothing else is read. */
+typedef enum mr_rope_pairs { MR_ROPE_ADJACENT = 0, MR_ROPE_HALVES = 1 } mr_rope_pairs;
+typedef struct mr_rotary {
+    const float *cos_t, *sin_t;
+    const int32_t *positions; /* device [tokens], or NULL */
+    int64_t table_rows;
+    int32_t dim, col0;
+    mr_rope_pairs pairs;
+} mr_rotary;
+
+/* The queries' or the keys' heads [tokens][heads][dim], strides in elements; no
+ * heads: heads 0.  `out` may be x (backward: x or d_out) itself, of the same
+ * strides and type; it overlaps no input otherwise, and its rows are apart. */
+typedef struct mr_head_rows {
+    int32_t heads;
+    const void *x;
+    int64_t x_token_stride, x_head_stride;
+    const void *weight; /* [dim], or NULL for ones */
+    void *out;          /* backward: the gradient of x */
+    int64_t out_token_stride, out_head_stride;
+    const void *d_out;  /* backward only: the gradient of the output */
+    int64_t d_out_token_stride, d_out_head_stride;
+    float *d_weight;    /* backward only: f32 [dim], or NULL */
+} mr_head_rows;
+
+/* For every head x of q and k, in f32, rounded once to out_dtype:
+ *   out = rotate(weight * (x * 1 / sqrt(mean(x^2) + eps)))
+ * (K3Norm.rms per head, Normalization.swift:15-19; the query norm without a
+ * weight and the rotated tail of DeepSeekV4CompressedAttention.swift:676-694).
+ * dim is 1 to 512; tokens * (q.heads + k.heads) * the lanes of a row (dim / 8,
+ * rounded up to a power of two) less than 2^32, and rows at most 2^31 - 1. */
+typedef struct mr_head_norm_args {
+    int32_t tokens, dim;
+    mr_head_rows q, k;
+    mr_dtype x_dtype;      /* of x and d_out: bf16 or f32 */
+    mr_dtype weight_dtype; /* bf16 or f32 */
+    mr_dtype out_dtype;    /* bf16 or f32 */
+    float eps;
+    mr_rotary rope;
+    void *workspace; /* backward, where a d_weight is asked for */
+    size_t workspace_bytes;
+} mr_head_norm_args;
+mr_status mr_head_norm_rope(const mr_head_norm_args *args, void *stream);
+
+/* Its gradients: with g = d_out turned back and r = 1 / sqrt(mean(x^2) + eps),
+ *   out = r * (g * weight - x * r * mean(g * weight * x * r)),
+ *   d_weight = the sum over tokens and heads of g * x * r, in f32
+ * (written, not added to; the order of the sums is fixed). */
+size_t mr_head_norm_rope_backward_workspace_size(const mr_head_norm_args *args);
+mr_status mr_head_norm_rope_backward(const mr_head_norm_args *args, void *stream);
+
+/* A layer's cache of keys and values in pages of `page_size` rows, a multiple of
+ * 16, of kv_heads heads each: k and v [pages][kv_heads][page_size][head_dim] bf16,
+ * or (k_scales and v_scales given) MXFP4: uint32 words
+ * [pages][kv_heads][page_size][head_dim / 8] and E8M0 bytes
+ * [pages][kv_heads][page_size][head_dim / 32].  No gaps inside a page; pages lie
+ * page_stride elements (words) and scale_page_stride bytes apart, the same for k
+ * and v.  head_dim is a multiple of 32 up to 256; page_size * kv_heads * head_dim
+ * at most 2^28; pages * page_size less than 2^31; k and v 16-byte aligned, page_stride
+ * a multiple of 16 bytes. */
+typedef struct mr_kv_cache {
+    void *k, *v;
+    uint8_t *k_scales, *v_scales;
+    int32_t pages, page_size, kv_heads, head_dim;
+    int64_t page_stride, scale_page_stride;
+} mr_kv_cache;
+
+/* Each token's keys and values into row slots[t] % page_size of page slots[t] /
+ * page_size, for every head; slots outside [0, pages * page_size) (padding) are
+ * passed over, and no other row is touched.  Where two tokens name one slot, which
+ * of them is written is not defined.  k, v [tokens][kv_heads][head_dim] bf16 or f32.
+ * Keys are normalised first where `normalize` is set (norm_w [head_dim], or NULL
+ * for ones, and eps as in mr_head_norm_rope), then rotated.  What is stored is
+ * rounded once from the exact value (computed in f64), MXFP4 by
+ * mr_mxfp4_quantize's rule.  tokens * kv_heads * the lanes of a row (head_dim / 8,
+ * rounded up to a power of two) less than 2^31. */
+typedef struct mr_kv_append_args {
+    mr_kv_cache cache;
+    int32_t tokens;
+    const void *k, *v;
+    mr_dtype dtype; /* of k and v */
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int32_t *slots; /* device [tokens] */
+    int32_t normalize;
+    const void *norm_w;
+    mr_dtype norm_w_dtype; /* bf16 or f32 */
+    float eps;
+    mr_rotary rope;
+} mr_kv_append_args;
+mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
+
+/* Causal attention of each sequence's queries over its cached keys and values:
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j]) v[j],  key head
+ *   h / (heads / kv_heads)
+ * Sequence b has kv_lens[b] keys (0: none; more than its table row holds: as many
+ * as it holds), key j in row j % page_size of page page_table[b][j / page_size]; entries
+ * past its keys are not read, one outside [0, pages) hides its keys.  Its queries
+ * are tokens q_offsets[b] .. q_offsets[b + 1] - 1 (NULL: token b, batch tokens in
+ * all), the last of them at position kv_lens[b] - 1.  A query sees the keys up to
+ * its position, or the last `window` of them (0: all).  A key that a query does not
+ * see has no part in its output, whatever it holds.  A sink (f32 [heads], or NULL)
+ * is one more score without a value.  A query that sees no key gets zeros.  Tokens
+ * of no sequence are left as they were.  q_offsets ascends from 0 or more to at most
+ * `tokens`; a sequence whose offsets do not is passed over.
+ *   q bf16; MXFP4 keys and values as mr_mxfp4_dequantize gives them in bf16; scores,
+ * softmax and sums in f32 but for the probabilities, which enter the second product as
+ * bf16 (out in f32 has that error too); out is rounded once.
+ * lse (or NULL): f32 [tokens][heads], the logarithm of the sum of exp of the scores
+ * (and sink); -inf where there is none.  With f32 out it joins parts of a context
+ * attended elsewhere.
+ *   q and out are 16-byte aligned, their strides multiples of 8.  heads a multiple of
+ * cache.kv_heads; tokens * heads less than 2^31.  max_kv_len: about the most keys of
+ * a sequence (0: what a table row holds); it decides how the work is split, so it is
+ * part of the workspace's size, and a longer sequence is right but slow.  Which kernel
+ * runs, and so a result's last bits, depends on the sizes of the call alone. */
+typedef struct mr_kv_attention_args {
+    mr_kv_cache cache;
+    int32_t batch, tokens, heads;
+    const void *q; /* bf16 [tokens][heads][head_dim] */
+    int64_t q_token_stride, q_head_stride;
+    const int32_t *page_table; /* device [batch][max_pages] */
+    int64_t page_table_stride;
+    int32_t max_pages;
+    const int32_t *kv_lens;   /* device [batch] */
+    const int32_t *q_offsets; /* device [batch + 1], or NULL */
+    int32_t max_kv_len, window;
+    float scale;
+    const float *sinks;
+    void *out; /* [tokens][heads][head_dim] */
+    mr_dtype out_dtype; /* bf16 or f32 */
+    int64_t out_token_stride, out_head_stride;
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+} mr_kv_attention_args;
+size_t mr_kv_attention_workspace_size(const mr_kv_attention_args *args);
+mr_status mr_kv_attention(const mr_kv_attention_args *args, void *stream);
+
+/* ------------------------------------------------------------------------
  * Index tables of DeepSeek V4 attention (DeepSeekV4Attention.swift:169-237),
  * host side, -1 = invalid entry.  `out` must hold rows*cols entries:
  * window: seq_len*min(seq_len, window) (or window when start_pos > 0);

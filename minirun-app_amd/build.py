@@ -34,11 +34,13 @@ FLAGS = [
 LIB_SOURCES = ["capi.cpp", "capi_adopt.cpp", "capi_block.cpp", "capi_prefill.cpp", "capi_topk.cpp", "decode.hip", "affine.hip",
                "mla_block.hip", "prefill.hip", "topk.hip", "indexer.hip", "linear.hip", "gemm.hip", "affine_gemm.hip",
                "skinny.hip", "generic.hip", "capi_experts.cpp", "mxfp4.hip",
-               "mxfp4_few.hip", "mxfp4_gemm.hip", "experts.hip"]
+               "mxfp4_few.hip", "mxfp4_gemm.hip", "experts.hip", "capi_kv.cpp", "head_norm.hip", "kv_append.hip",
+               "kv_attention.hip", "kv_prompt.hip"]
 # Per-source flags.  The decode kernel keeps its MFMA accumulators in VGPRs
 # (VGPR-form MFMA): with the AGPR form the compiler shuttles all 64 of them
-# through v_accvgpr moves on every 32-row step.
-EXTRA = {"decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# through v_accvgpr moves on every 32-row step.  The same for attention over a
+# paged cache (few queries of 128 dims: 4 waves a CU more).
+EXTRA = {"decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 SELFTEST_SOURCES = ["selftest.hip"]
 
 

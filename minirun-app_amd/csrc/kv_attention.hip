@@ -1,0 +1,459 @@
+// Attention of a few queries of each sequence over a paged cache of keys and
+// values, in bf16 or MXFP4, and the joining of partial results.
+//
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j   over the keys j that i sees
+//
+// with the softmax in one pass: a running maximum m, l = sum 2^(s_j - m) and
+// o = sum 2^(s_j - m) v_j, in f32; a sink enters l at the end.
+//
+// What bounds it: the cache's bytes from HBM (a key head's rows are read once
+// for all of its query heads), and for short sequences the chain of loads.
+// So a wave works alone: it walks keys of its own in steps of 32, has the next
+// step's loads in flight, and never meets a barrier before the end.  A step:
+//   - the packed rows arrive in registers, whole neighbouring rows a load;
+//     keys go to the wave's part of LDS as stored, values as bf16;
+//   - S^T = K . Q^T on 16x16x32 MFMA.  Lane (n, g) holds dims DP/4 g .. of
+//     key n, so that an MXFP4 key is one 16-byte read (of 128 dims) and its
+//     scale one byte; q's registers hold the same dims;
+//   - the lane that has query n's scores keeps its maximum and sum;
+//   - O^T += V^T . P^T: the scores' registers are the second operand as they
+//     are, V^T comes by transposed reads.  P is rounded to bf16 (2^-9 of each
+//     term, whose errors average out); sums stay in f32.
+// The waves of a workgroup split its keys and meet once, in LDS.  A tile's keys
+// are split over workgroups where that fills the GPU (kv_attention_route),
+// which leave (m, l, o) in the workspace for kv_join_kernel.
+//
+// Keys that no row may see are zeros where they are loaded.  Where some rows of
+// a step see a key and others do not, 0 times an infinity or a NaN of its value
+// would reach the others, so such a step with such values takes its keys one by
+// one (kv_step_apart).
+#include <algorithm>
+
+#include "kv_tiles.hpp"
+
+namespace mr {
+
+namespace {
+
+constexpr int KD_WAVES = 4, KD_STEP = 32;
+
+template <int DP, bool MX>
+struct KvDecodeLds {
+    // rows apart by an odd number of 16-byte (K) and 32-byte (V) pieces, so that 16
+    // rows read at one column, and 8 rows read by transposed reads, meet all banks
+    static constexpr int K_STRIDE = MX ? DP / 2 + 16 : DP * 2 + 16;  // bytes
+    static constexpr int V_STRIDE = DP + 16;                         // values
+    static constexpr int V_BYTES = KD_STEP * V_STRIDE * 2, K_BYTES = KD_STEP * K_STRIDE;
+    static constexpr int S_BYTES = MX ? KD_STEP * DP / 32 : 0;  // the keys' scales
+    static constexpr int O_STRIDE = DP + 4;                     // f32, the end's sums of 16 rows
+    static constexpr int WAVE = (V_BYTES + K_BYTES + S_BYTES + 15) / 16 * 16;
+    static_assert(16 * O_STRIDE * 4 <= WAVE, "the sums of 16 rows fit");
+};
+
+template <int DP, int R, bool MX>
+__global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p) {
+    using L = KvDecodeLds<DP, MX>;
+    constexpr int ROWS = 16 * R, KS = DP / 32, DT = DP / 16, CPL = DP / 4;
+    __shared__ __attribute__((aligned(16))) char lds[KD_WAVES * L::WAVE];
+    __shared__ float sm[KD_WAVES][ROWS], sl[KD_WAVES][ROWS];
+    const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int heads_splits = p.kv_heads * p.splits;
+    const int tile_id = blockIdx.x / heads_splits, rest = blockIdx.x - tile_id * heads_splits;
+    const int split = rest / p.kv_heads, kv_head = rest - split * p.kv_heads;
+    KvTile t;
+    if (!kv_find<ROWS>(p, tile_id, t)) return;
+
+    // this workgroup's keys, and this wave's
+    int kb = t.kbeg, ke = t.kend;
+    if (p.splits > 1) {
+        const int64_t at = (int64_t)t.kbeg + (int64_t)split * p.chunk;
+        kb = (int)min(at, (int64_t)t.kend);
+        if (split + 1 < p.splits) ke = (int)min(at + p.chunk, (int64_t)t.kend);
+    }
+    const int per = ((max(ke - kb, 0) + KD_WAVES - 1) / KD_WAVES + KD_STEP - 1) / KD_STEP * KD_STEP;
+    const int wb = min(kb + w * per, ke), we = min(wb + per, ke);
+
+    char* mine = lds + w * L::WAVE;
+    uint16_t* vt = (uint16_t*)mine;
+    char* kt = mine + L::V_BYTES;
+    uint8_t* ksc = (uint8_t*)(kt + L::K_BYTES);
+
+    KvRow row[R];
+    bf16x8 q[R][KS];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        row[r] = kv_row(p, t, kv_head, t.first_row + 16 * r + n);
+        const uint16_t* qp = p.q + row[r].token * p.q_ts + row[r].head * p.q_hs;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = CPL * g + 8 * s;
+            q[r][s] = row[r].ok && d < p.dim ? *(const bf16x8*)(qp + d) : bf16x8{};
+        }
+    }
+
+    float m[R], sum[R];
+    f32x4 o[R][DT];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        sum[r] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = f32x4{};
+    }
+
+    if (wb < we) {
+        KvWalk walk;
+        walk.start(p, t.b, wb);
+        // the two groups of a step: their pages, a step ahead of their loads
+        int id[2], off[2];
+        auto look = [&](int key) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                off[h] = walk.offset;
+                id[h] = key + 16 * h < we ? s_load(walk.entry) : -1;
+                walk.next(p.page_size);
+            }
+        };
+        KvGroup<DP, MX> k[2], v[2];
+        bool have[2];
+        auto load = [&](int key) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                have[h] = kv_page(p, id[h], key + 16 * h < we);
+                kv_load<DP, MX>(p, kv_head, id[h], off[h], have[h], l, k[h], v[h]);
+            }
+        };
+        look(wb);
+        load(wb);
+        look(wb + KD_STEP);
+        for (int k0 = wb; k0 < we; k0 += KD_STEP) {
+            const bool seen[2] = {have[0], have[1]};
+            const bool all = k0 >= t.all_lo && k0 + KD_STEP <= t.all_hi && k0 + KD_STEP <= we && seen[0] && seen[1];
+            bool apart = false;  // (wave-uniform)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (k0 + 16 * h + 16 > we) k[h].cut(we - k0 - 16 * h, l), v[h].cut(we - k0 - 16 * h, l);
+                if constexpr (MX) {
+#pragma unroll
+                    for (int i = 0; i < KvGroup<DP, MX>::N; ++i)
+                        if (k[h].active(l)) {
+                            const int rr = 16 * h + k[h].row(l, i);
+                            *(u32x4*)(kt + rr * L::K_STRIDE + 16 * k[h].piece(l)) = k[h].v[i];
+                            ksc[rr * (DP / 32) + k[h].piece(l)] = (uint8_t)k[h].scale[i];
+                        }
+                } else {
+                    k[h].put((uint16_t*)kt + 16 * h * (L::K_STRIDE / 2), L::K_STRIDE / 2, l);
+                }
+                v[h].put(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
+                if (!all) apart |= v[h].not_finite();
+            }
+            if (!all) apart = __builtin_amdgcn_ballot_w64(apart) != 0;
+            if (k0 + KD_STEP < we) {
+                load(k0 + KD_STEP);
+                look(k0 + 2 * KD_STEP);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+
+            f32x4 s[2][R];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) s[h][r] = f32x4{};
+                const char* kr = kt + (16 * h + n) * L::K_STRIDE + g * (MX ? CPL / 2 : CPL * 2);
+                bf16x8 a[KS];
+                if constexpr (MX) {
+                    uint32_t words[KS];
+                    if constexpr (KS == 2) {
+                        const u32x2 x = *(const u32x2*)kr;
+                        words[0] = x[0], words[1] = x[1];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < KS / 4; ++i) {
+                            const u32x4 x = *(const u32x4*)(kr + 16 * i);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) words[4 * i + e] = x[e];
+                        }
+                    }
+                    // the lane's dims lie in one block, or (DP 256) in two
+                    const uint8_t* sc = ksc + (16 * h + n) * (DP / 32) + CPL * g / 32;
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+                        a[i] = mxfp4_bf16(words[i], __uint_as_float((uint32_t)sc[DP == 256 ? i / 4 : 0] << 23));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) a[i] = *(const bf16x8*)(kr + 16 * i);
+                }
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) s[h][r] = mfma16(a[i], q[r][i], s[h][r]);
+            }
+
+            bf16x8 pb[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = k0 + 16 * h + 4 * g + i;
+                        float x = s[h][r][i] * p.scale_log2;
+                        if (!all && !(key >= row[r].lo && key < min(row[r].hi, we) && seen[h])) x = -INFINITY;
+                        s[h][r][i] = x;
+                        mx = fmaxf(mx, x);
+                    }
+                mx = xor32_max(xor16_max(mx));
+                const bool raise = mx > m[r] + KV_TAU;
+                if (__builtin_amdgcn_ballot_w64(raise)) {
+                    const float up = raise ? mx : m[r];
+                    const float alpha = raise ? __builtin_amdgcn_exp2f(m[r] - up) : 1.f;
+                    m[r] = up;
+                    sum[r] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[r][d] *= alpha;
+                }
+                const float ref = m[r] == -INFINITY ? 0.f : m[r];  // (no key yet: every score is -inf)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(s[h][r][i] - ref);
+                        sum[r] += e;
+                        pb[r][4 * h + i] = (__bf16)e;
+                    }
+            }
+
+            // key 4 g + e of group 0 and 4 g + e - 4 of group 1 are k-slot 8 g + e
+            auto values = [&](int d) {
+                const uint16_t* at = vt + (4 * g + (n >> 2)) * L::V_STRIDE + 16 * d + 4 * (n & 3);
+                const bf16x4 lo = ds_read_tr16(at), hi = ds_read_tr16(at + 16 * L::V_STRIDE);
+                return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            if (!apart) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const bf16x8 a = values(d);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) o[r][d] = mfma16(a, pb[r], o[r][d]);
+                }
+            } else {
+                // one key at a time, added where it is seen
+                for (int key = 0; key < KD_STEP; ++key) {
+                    if (!seen[key >> 4]) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        bf16x8 a = values(d);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (16 * (e >> 2) + 4 * g + (e & 3) != key) a[e] = (__bf16)0.f;
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            const f32x4 one = mfma16(a, pb[r], f32x4{});
+                            if (k0 + key >= row[r].lo && k0 + key < min(row[r].hi, we)) o[r][d] += one;
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+
+    // the waves' sums
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float all = xor32_sum(xor16_sum(sum[r]));
+        if (g == 0) {
+            sm[w][16 * r + n] = m[r];
+            sl[w][16 * r + n] = all;
+        }
+    }
+    __syncthreads();
+    const int rn = threadIdx.x >> 4, dn = 4 * (threadIdx.x & 15);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float* part = (float*)mine;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *(f32x4*)(part + n * L::O_STRIDE + 16 * d + 4 * g) = o[r][d];
+        __syncthreads();
+        // thread: row rn, dims dn + 64 i
+        float top = -INFINITY, total = 0.f, a[KD_WAVES];
+#pragma unroll
+        for (int x = 0; x < KD_WAVES; ++x) top = fmaxf(top, sm[x][16 * r + rn]);
+#pragma unroll
+        for (int x = 0; x < KD_WAVES; ++x) {
+            const float mw = sm[x][16 * r + rn];
+            a[x] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+            total = fmaf(sl[x][16 * r + rn], a[x], total);
+        }
+        const KvRow to = kv_row(p, t, kv_head, t.first_row + 16 * r + rn);
+        if (to.ok) {
+            const int64_t at = (int64_t)to.token * (p.kv_heads * p.group) + to.head;
+            float inv = 1.f;
+            if (p.splits == 1) {
+                if (p.sinks) {
+                    const float sink = p.sinks[to.head] * 1.4426950408889634f, up = fmaxf(top, sink);
+                    const float was = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - up);
+                    if (up != -INFINITY) total = fmaf(total, was, __builtin_amdgcn_exp2f(sink - up));
+#pragma unroll
+                    for (int x = 0; x < KD_WAVES; ++x) a[x] *= was;
+                    top = up;
+                }
+                inv = total == 0.f ? 0.f : 1.f / total;  // (no key is seen: zeros)
+                if (p.lse && dn == 0)
+                    p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+            } else if (dn == 0) {
+                float* ml = p.part_ml + 2 * (at * p.splits + split);
+                ml[0] = top;
+                ml[1] = total;
+            }
+            if (p.splits == 1 || total != 0.f) {
+#pragma unroll
+                for (int d = dn; d < DP; d += 64) {
+                    if (d >= p.dim) break;
+                    f32x4 x{};
+#pragma unroll
+                    for (int y = 0; y < KD_WAVES; ++y)
+                        x += a[y] * *(const f32x4*)((const float*)(lds + y * L::WAVE) + rn * L::O_STRIDE + d);
+                    if (p.splits > 1) {
+                        *(f32x4*)(p.part_o + (at * p.splits + split) * p.dim + d) = x;
+                    } else if (p.out_f32) {
+                        *(f32x4*)((float*)p.out + to.token * p.out_ts + to.head * p.out_hs + d) = x * inv;
+                    } else {
+                        *(u32x2*)((uint16_t*)p.out + to.token * p.out_ts + to.head * p.out_hs + d) =
+                            u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The parts of a row joined: a workgroup per (query, head), 4 dims a thread,
+// the threads that are left over share the parts.
+constexpr int KJ_MAX = 1024;  // parts
+
+__global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p) {
+    __shared__ float weight[KJ_MAX];
+    __shared__ __attribute__((aligned(16))) float add[256 * 4];
+    __shared__ float red[4];
+    const int heads = p.kv_heads * p.group;
+    const int64_t at = blockIdx.x;
+    const int token = (int)(at / heads), head = (int)(at - (int64_t)token * heads);
+    // tokens that no sequence has are left as they are
+    if (p.q_offsets && (token < s_load(p.q_offsets) || token >= s_load(p.q_offsets + p.batch))) return;
+    const float* ml = p.part_ml + 2 * at * p.splits;
+    const int w = threadIdx.x >> 6;
+    float top = -INFINITY;
+    for (int s = threadIdx.x; s < p.splits; s += 256) top = fmaxf(top, ml[2 * s]);
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) red[w] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    __syncthreads();
+    const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
+    top = fmaxf(top, sink);
+    float total = 0.f;
+    for (int s = threadIdx.x; s < p.splits; s += 256) {
+        const float ms = ml[2 * s], ls = ml[2 * s + 1];
+        const float a = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - top);
+        total = fmaf(ls, a, total);
+        weight[s] = ls == 0.f ? -1.f : a;  // (no sums were left: not read)
+    }
+    total = wave_sum(total);
+    if ((threadIdx.x & 63) == 0) red[w] = total;
+    __syncthreads();
+    total = (red[0] + red[1]) + (red[2] + red[3]);
+    if (sink != -INFINITY) total += __builtin_amdgcn_exp2f(sink - top);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (p.lse && threadIdx.x == 0)
+        p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    const int cols = p.dim / 4, shares = 256 / cols, share = threadIdx.x / cols, c = threadIdx.x - share * cols;
+    f32x4 x{};
+    if (share < shares) {
+        const float* o = p.part_o + at * p.splits * p.dim + 4 * c;
+        for (int s = share; s < p.splits; s += shares)
+            if (weight[s] >= 0.f || weight[s] != weight[s]) x += weight[s] * *(const f32x4*)(o + (int64_t)s * p.dim);
+    }
+    *(f32x4*)(add + 4 * threadIdx.x) = x;
+    __syncthreads();
+    if (share) return;
+    for (int s = 1; s < shares; ++s) x += *(const f32x4*)(add + 4 * (s * cols + c));
+    const int64_t to = token * p.out_ts + head * p.out_hs + 4 * c;
+    if (p.out_f32)
+        *(f32x4*)((float*)p.out + to) = x * inv;
+    else
+        *(u32x2*)((uint16_t*)p.out + to) =
+            u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
+}
+
+template <int DP, bool MX>
+hipError_t decode_rows(const KvAttnParams& p, int rows, unsigned grid, hipStream_t st) {
+    const dim3 block(64 * KD_WAVES);
+    if (rows == 16)
+        hipLaunchKernelGGL((kv_decode_kernel<DP, 1, MX>), dim3(grid), block, 0, st, p);
+    else if (rows == 32)
+        hipLaunchKernelGGL((kv_decode_kernel<DP, 2, MX>), dim3(grid), block, 0, st, p);
+    else if constexpr (DP <= 128)
+        hipLaunchKernelGGL((kv_decode_kernel<DP, 4, MX>), dim3(grid), block, 0, st, p);
+    else
+        return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+template <bool MX>
+hipError_t decode_dim(const KvAttnParams& p, int rows, unsigned grid, hipStream_t st) {
+    if (p.dim <= 64) return decode_rows<64, MX>(p, rows, grid, st);
+    if (p.dim <= 128) return decode_rows<128, MX>(p, rows, grid, st);
+    return decode_rows<256, MX>(p, rows, grid, st);
+}
+
+}  // namespace
+
+// `keys`: the most that a sequence has (an estimate is enough: a longer one's last
+// part takes what is left)
+KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_heads, int group, int dim, int window,
+                               int64_t keys, int cu_count) {
+    KvAttnRoute r;
+    const int64_t rows = ragged ? (tokens * group + batch - 1) / batch : group;  // of a sequence, on average
+    r.prompt = rows > (dim > 128 ? 32 : 64);  // (64 rows of 256 dims do not fit the registers)
+    // tiles of as few rows as hold a sequence's
+    r.rows = r.prompt ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    r.tiles = ragged ? (tokens * group + r.rows - 1) / r.rows + batch : int64_t(batch) * ((group + r.rows - 1) / r.rows);
+    const int64_t groups = r.tiles * kv_heads;  // workgroups without a split
+    // a tile's queries span at most its rows' positions
+    if (window) keys = std::min<int64_t>(keys, (int64_t)window + r.rows + 16);
+    // parts of equal length, so that long sequences weigh no more than their keys: about
+    // eight workgroups a CU in all, at least 512 keys each
+    const int64_t target = int64_t(cu_count) * (r.prompt ? 4 : 8), least = 512;
+    int64_t chunk = (groups * std::max<int64_t>(keys, 1) + target - 1) / target;
+    chunk = std::max(least, (chunk + 63) / 64 * 64);
+    chunk = std::max(chunk, ((keys + KJ_MAX - 1) / KJ_MAX + 63) / 64 * 64);
+    r.splits = (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk);
+    if (tokens * kv_heads * group > (1 << 20)) r.splits = 1;  // (the join has a workgroup per row)
+    r.chunk = (int)std::min<int64_t>(chunk, INT32_MAX - 63);
+    return r;
+}
+
+size_t kv_attention_workspace(const KvAttnRoute& r, int64_t tokens, int heads, int dim) {
+    return r.splits == 1 ? 0 : size_t(tokens) * heads * r.splits * (size_t(dim) + 2) * 4;
+}
+
+hipError_t launch_kv_attention(const KvAttnParams& p, const KvAttnRoute& r, hipStream_t st) {
+    const unsigned grid = (unsigned)(r.tiles * p.kv_heads * r.splits);
+    hipError_t e;
+    if (r.prompt)
+        e = launch_kv_prompt(p, grid, st);
+    else
+        e = p.k_scales ? decode_dim<true>(p, r.rows, grid, st) : decode_dim<false>(p, r.rows, grid, st);
+    if (e != hipSuccess || r.splits == 1) return e;
+    hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)((int64_t)p.tokens * p.kv_heads * p.group)), dim3(256), 0, st, p);
+    return hipGetLastError();
+}
+
+}  // namespace mr

@@ -1,0 +1,207 @@
+// What the two kernels of attention over a paged cache share: which rows and
+// keys a workgroup has, and the way of 16 keys of a page into its registers.
+//
+// A tile's rows are (query, head) pairs of one sequence and one key head: row
+// r is query r / group and the group's head r % group.  Query i of a sequence
+// of n queries and `len` keys sits at position len - n + i and sees the keys
+// up to there, or the last `window` of them.
+#pragma once
+
+#include "mr_kernels.hpp"
+
+namespace mr {
+
+constexpr float KV_TAU = 8.f;  // log2 headroom of the running maximum: sums are rescaled when a score passes it
+
+struct KvTile {
+    int b, q0, qn, len;  // sequence, its first query, queries and keys
+    int first_row;
+    int kbeg, kend;      // keys that some row sees (kbeg a multiple of 16); none: kbeg >= kend
+    int all_lo, all_hi;  // keys that every row sees
+};
+
+// int32 read through the scalar cache (nothing in these kernels writes them)
+__device__ __forceinline__ int s_load(const int32_t* p) {
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+
+__device__ __forceinline__ int kv_queries(const KvAttnParams& p, int b, int& q0) {
+    q0 = p.q_offsets[b];
+    const int q1 = p.q_offsets[b + 1];
+    return q0 >= 0 && q1 <= p.tokens && q1 > q0 ? q1 - q0 : 0;
+}
+
+// The tile `tile` of all sequences' tiles of ROWS rows; false: there is no such.
+template <int ROWS>
+__device__ __forceinline__ bool kv_find(const KvAttnParams& p, int tile, KvTile& t) {
+    if (!p.q_offsets) {
+        const int per = (p.group + ROWS - 1) / ROWS;
+        t.b = tile / per;
+        t.first_row = (tile - t.b * per) * ROWS;
+        t.q0 = t.b;
+        t.qn = 1;
+    } else {
+        // lanes count the tiles of 64 sequences, a scan finds the one that has this tile
+        const int l = threadIdx.x & 63;
+        uint32_t left = (uint32_t)tile;
+        int at = -1;
+        for (int b0 = 0; b0 < p.batch; b0 += 64) {
+            uint32_t n = 0;
+            int q0;
+            if (b0 + l < p.batch) n = ((uint32_t)kv_queries(p, b0 + l, q0) * (uint32_t)p.group + ROWS - 1) / ROWS;
+            const uint32_t end = wave_scan_incl(n), all = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+            if (left < all) {
+                const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end > left));
+                left -= (uint32_t)__builtin_amdgcn_readlane((int)(end - n), i);
+                at = b0 + i;
+                break;
+            }
+            left -= all;
+        }
+        if (at < 0) return false;
+        t.b = at;
+        const int q0 = s_load(p.q_offsets + at), q1 = s_load(p.q_offsets + at + 1);
+        t.q0 = q0;
+        t.qn = q1 - q0;
+        if (left >= ((uint32_t)t.qn * (uint32_t)p.group + ROWS - 1) / ROWS) return false;
+        t.first_row = (int)left * ROWS;
+    }
+    t.len = min(max(s_load(p.lens + t.b), 0), p.max_keys);
+    const int i0 = t.first_row / p.group, i1 = min((t.first_row + ROWS - 1) / p.group, t.qn - 1);
+    const int p0 = t.len - t.qn + i0, p1 = t.len - t.qn + i1;  // positions of the first and the last query
+    t.kend = max(p1 + 1, 0);
+    t.all_hi = max(p0 + 1, 0);
+    t.kbeg = p.window ? max(p0 + 1 - p.window, 0) & ~15 : 0;
+    t.all_lo = p.window ? max(p1 + 1 - p.window, 0) : 0;
+    return true;
+}
+
+// A row's keys [lo, hi), and where its query, output and sink are
+struct KvRow {
+    bool ok;
+    int token, head, lo, hi;
+};
+__device__ __forceinline__ KvRow kv_row(const KvAttnParams& p, const KvTile& t, int kv_head, int row) {
+    KvRow r;
+    const int i = row / p.group;
+    r.ok = i < t.qn;
+    r.token = t.q0 + min(i, t.qn - 1);
+    r.head = kv_head * p.group + row - i * p.group;
+    const int pos = t.len - t.qn + i;
+    r.hi = r.ok ? max(pos + 1, 0) : 0;
+    r.lo = p.window ? max(pos + 1 - p.window, 0) : 0;
+    return r;
+}
+
+// The groups of 16 keys of a sequence, one after another: a page holds a whole
+// number of them.  Wave-uniform.
+struct KvWalk {
+    const int32_t* entry;  // of the page table
+    int offset;            // of the group in its page
+    __device__ __forceinline__ void start(const KvAttnParams& p, int b, int key) {
+        const int page = key / p.page_size;
+        entry = p.table + b * p.table_stride + page;
+        offset = key - page * p.page_size;
+    }
+    __device__ __forceinline__ void next(int page_size) {
+        offset += 16;
+        if (offset == page_size) {
+            offset = 0;
+            ++entry;
+        }
+    }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_buffer(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
+}
+
+// 16 keys (or values) of one head as a wave loads them: 16-byte pieces, RPL
+// rows a load, so that a load covers whole neighbouring rows; MXFP4: a piece is
+// a block of 32 values, and its scale comes with it.  A group that does not
+// exist reads nothing and is zeros.
+template <int DP, bool MX>
+struct KvGroup {
+    static constexpr int LPR = MX ? DP / 32 : DP / 8;          // pieces of a row
+    static constexpr int RPL = 64 / LPR < 16 ? 64 / LPR : 16;  // rows of a load
+    static constexpr int N = 16 / RPL;
+    u32x4 v[N];
+    uint32_t scale[MX ? N : 1];
+
+    __device__ __forceinline__ static int row(int l, int i) { return i * RPL + l / LPR; }
+    __device__ __forceinline__ static int piece(int l) { return l % LPR; }
+    __device__ __forceinline__ static bool active(int l) { return RPL * LPR == 64 || l < RPL * LPR; }
+
+    // base, scales: the group's first row; row_bytes: of the stored row
+    __device__ __forceinline__ void load(const char* base, const uint8_t* scales, int dim, bool exists, int l) {
+        const int row_bytes = MX ? dim / 2 : dim * 2, blocks = dim / 32;
+        const bool mine = active(l) && piece(l) * (MX ? 32 : 8) < dim;
+        const __amdgpu_buffer_rsrc_t rows = kv_buffer(base, exists ? 16 * row_bytes : 0);
+        const int none = 0x40000000;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                 rows, mine ? row(l, i) * row_bytes + 16 * piece(l) : none, 0, 0));
+        if constexpr (MX) {
+            const __amdgpu_buffer_rsrc_t bytes = kv_buffer(scales, exists ? 16 * blocks : 0);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                scale[i] = __builtin_amdgcn_raw_buffer_load_b8(bytes, mine ? row(l, i) * blocks + piece(l) : none, 0, 0);
+        }
+    }
+    // rows from `n` on become zeros
+    __device__ __forceinline__ void cut(int n, int l) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (row(l, i) >= n) {
+                v[i] = u32x4{};
+                if constexpr (MX) scale[i] = 0;
+            }
+    }
+    // a value of this lane may be infinite or NaN (MXFP4: its block's scale says so)
+    __device__ __forceinline__ bool not_finite() const {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (MX) {
+                bad |= scale[i] >= 253;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    bad |= (v[i][k] & 0x7f80u) == 0x7f80u || (v[i][k] & 0x7f800000u) == 0x7f800000u;
+            }
+        }
+        return bad;
+    }
+    // into bf16 rows of `stride` values
+    __device__ __forceinline__ void put(uint16_t* rows, int stride, int l) const {
+        if (!active(l)) return;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (MX) {
+                uint16_t* to = rows + row(l, i) * stride + 32 * piece(l);
+                const float s = __uint_as_float(scale[i] << 23);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) *(bf16x8*)(to + 8 * k) = mxfp4_bf16(v[i][k], s);
+            } else {
+                *(u32x4*)(rows + row(l, i) * stride + 8 * piece(l)) = v[i];
+            }
+        }
+    }
+};
+
+// Key and value rows of the group at a walk's place
+__device__ __forceinline__ bool kv_page(const KvAttnParams& p, int id, bool in) { return in && (uint32_t)id < (uint32_t)p.pages; }
+
+template <int DP, bool MX>
+__device__ __forceinline__ void kv_load(const KvAttnParams& p, int kv_head, int id, int offset, bool exists, int l,
+                                        KvGroup<DP, MX>& k, KvGroup<DP, MX>& v) {
+    const int64_t page = exists ? id : 0;
+    const int64_t row = (int64_t)kv_head * p.page_size + offset;
+    const int64_t at = page * p.page_bytes + row * (MX ? p.dim / 2 : p.dim * 2);
+    const int64_t sc = MX ? page * p.scale_bytes + row * (p.dim / 32) : 0;
+    k.load(p.k + at, p.k_scales + sc, p.dim, exists, l);
+    v.load(p.v + at, p.v_scales + sc, p.dim, exists, l);
+}
+
+}  // namespace mr

@@ -597,4 +597,94 @@ hipError_t launch_expert_dispatch(const ExpertRowsParams& p, int cu_count, hipSt
 hipError_t launch_expert_combine(const ExpertRowsParams& p, int cu_count, hipStream_t st);
 hipError_t launch_expert_combine_backward(const ExpertRowsParams& p, int cu_count, hipStream_t st);
 
+// ---------------------------------------------------------------- attention heads: norms, rotation, paged cache
+// Angle tables of a rotation: f32 [rows][half], row positions[token] (or the
+// token itself); columns [col0, col0 + 2 half) of a head, adjacent pairs or
+// column i with column i + half.  half 0: no rotation.
+struct HeadRope {
+    const float *cos_t, *sin_t;
+    const int32_t* positions;
+    int64_t rows;
+    int32_t half, col0, halves;
+};
+// How a rotation's columns lie in lanes of eight (head_rows.hpp)
+enum RopeKind { ROPE_ADJACENT, ROPE_HALVES, ROPE_ANY };
+RopeKind head_rope_kind(const HeadRope& r);
+
+struct HeadSegment {  // the queries or the keys
+    int32_t heads;
+    const void* x;
+    int64_t x_ts, x_hs;
+    const void* w;   // null: ones
+    const void* dy;  // backward
+    int64_t dy_ts, dy_hs;
+    void* out;       // y, or dx
+    int64_t out_ts, out_hs;
+    float* dw;       // backward, or null
+};
+struct HeadNormParams {
+    HeadSegment seg[2];
+    int64_t tokens;
+    int32_t dim, x_f32, w_f32, out_f32;
+    float eps;
+    HeadRope rope;
+    float* partial;    // backward: [blocks[0] + blocks[1]][dim]
+    int32_t blocks[2];
+    int32_t lpr, lpr_log2;  // lanes of a row (set by the launcher)
+};
+void head_norm_blocks(int64_t tokens, const int (&heads)[2], int dim, int (&blocks)[2]);
+hipError_t launch_head_norm(HeadNormParams p, bool backward, hipStream_t st);
+
+struct KvAppendParams {
+    const void *k, *v;
+    int64_t k_ts, k_hs, v_ts, v_hs;
+    int64_t tokens;
+    int32_t heads, dim, f32;
+    const int32_t* slots;
+    int32_t slot_end, page_size;
+    int32_t norm, w_f32;
+    const void* w;  // null: ones
+    float eps;
+    HeadRope rope;
+    void *k_pages, *v_pages;        // bf16 values, or MXFP4 words
+    uint8_t *k_scales, *v_scales;   // null: bf16
+    int64_t page_stride, scale_stride;  // values or words; bytes
+    int32_t turn, lpr, lpr_log2;    // set by the launcher
+};
+hipError_t launch_kv_append(KvAppendParams p, hipStream_t st);
+
+struct KvAttnParams {
+    const uint16_t* q;
+    int64_t q_ts, q_hs;
+    const char *k, *v;              // pages [kv_heads][page_size][dim]: bf16, or MXFP4 words
+    const uint8_t *k_scales, *v_scales;  // null: bf16
+    int64_t page_bytes, scale_bytes;     // from page to page
+    int32_t pages, page_size, kv_heads, group, dim;  // group: query heads of a key head
+    const int32_t* table;
+    int64_t table_stride;
+    int32_t max_keys;               // positions a table row holds
+    const int32_t *lens, *q_offsets;
+    int32_t batch, tokens, window;  // window 0: none
+    float scale_log2;
+    const float* sinks;
+    void* out;
+    int64_t out_ts, out_hs;
+    int32_t out_f32;
+    float* lse;                     // [tokens][heads] or null
+    int32_t splits, chunk;          // parts of a tile's keys, `chunk` (a multiple of 64) keys each
+    float *part_o, *part_ml;        // splits > 1: [tokens * heads][splits][dim] and [..][2]
+};
+// Which kernel, its rows of a tile, and into how many parts its keys are cut
+struct KvAttnRoute {
+    bool prompt;
+    int rows;  // of a tile: (query, head of the group) pairs
+    int64_t tiles;
+    int splits, chunk;
+};
+KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_heads, int group, int dim, int window,
+                               int64_t keys, int cu_count);
+size_t kv_attention_workspace(const KvAttnRoute& r, int64_t tokens, int heads, int dim);
+hipError_t launch_kv_attention(const KvAttnParams& p, const KvAttnRoute& r, hipStream_t st);
+hipError_t launch_kv_prompt(const KvAttnParams& p, unsigned grid, hipStream_t st);
+
 }  // namespace mr

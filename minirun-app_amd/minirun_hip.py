@@ -12,6 +12,10 @@ Names follow the reference operators they stand in for:
                         mxfp4_dequantize, mxfp4_mm, mxfp4_expert_mm
   expert_sort           tokens by expert and back, for QwenExpertBackends.swift:77-260;
                         expert_dispatch, expert_combine and their gradients
+  head_norm_rope        norms of query and key heads with the rotation, of
+                        QwenAttention.forward (QwenMoEModel.swift:193-264), and
+                        head_norm_rope_backward; KVCache, kv_append, kv_attention:
+                        its keys, values and attention, in pages
 """
 from __future__ import annotations
 
@@ -157,6 +161,55 @@ class MXFP4ExpertArgs(C.Structure):
     ]
 
 
+class Rotary(C.Structure):
+    _fields_ = [("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("positions", C.c_void_p), ("table_rows", C.c_int64),
+                ("dim", C.c_int32), ("col0", C.c_int32), ("pairs", C.c_int)]
+
+
+class HeadRows(C.Structure):
+    _fields_ = [
+        ("heads", C.c_int32), ("x", C.c_void_p), ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64),
+        ("weight", C.c_void_p), ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("d_out", C.c_void_p), ("d_out_token_stride", C.c_int64), ("d_out_head_stride", C.c_int64), ("d_weight", C.c_void_p),
+    ]
+
+
+class HeadNormArgs(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int32), ("dim", C.c_int32), ("q", HeadRows), ("k", HeadRows), ("x_dtype", C.c_int),
+        ("weight_dtype", C.c_int), ("out_dtype", C.c_int), ("eps", C.c_float), ("rope", Rotary), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class KVCacheDesc(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("pages", C.c_int32),
+        ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_stride", C.c_int64),
+        ("scale_page_stride", C.c_int64),
+    ]
+
+
+class KVAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", KVCacheDesc), ("tokens", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int),
+        ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64), ("slots", C.c_void_p), ("normalize", C.c_int32), ("norm_w", C.c_void_p),
+        ("norm_w_dtype", C.c_int), ("eps", C.c_float), ("rope", Rotary),
+    ]
+
+
+class KVAttentionArgs(C.Structure):
+    _fields_ = [
+        ("cache", KVCacheDesc), ("batch", C.c_int32), ("tokens", C.c_int32), ("heads", C.c_int32), ("q", C.c_void_p),
+        ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_int64), ("max_pages", C.c_int32), ("kv_lens", C.c_void_p), ("q_offsets", C.c_void_p),
+        ("max_kv_len", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("sinks", C.c_void_p), ("out", C.c_void_p),
+        ("out_dtype", C.c_int), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 TOPK_CHECK = 1
 TOPK_UNCHECKED = 2
 
@@ -228,6 +281,12 @@ SIGNATURES = {
                                     _P]),
     "mr_expert_combine_backward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, _P, C.c_int64, _P, _P, C.c_int32,
                                              C.c_int32, _P, C.c_int64, _P, _P]),
+    "mr_head_norm_rope": (C.c_int, [C.POINTER(HeadNormArgs), _P]),
+    "mr_head_norm_rope_backward_workspace_size": (C.c_size_t, [C.POINTER(HeadNormArgs)]),
+    "mr_head_norm_rope_backward": (C.c_int, [C.POINTER(HeadNormArgs), _P]),
+    "mr_kv_append": (C.c_int, [C.POINTER(KVAppendArgs), _P]),
+    "mr_kv_attention_workspace_size": (C.c_size_t, [C.POINTER(KVAttentionArgs)]),
+    "mr_kv_attention": (C.c_int, [C.POINTER(KVAttentionArgs), _P]),
     "mr_attention_indices_window": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _P, _I32P, _I32P]),
     "mr_attention_indices_compressed": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _I32P, _I32P]),
 }
@@ -948,6 +1007,283 @@ def expert_combine_backward(d_out, rows, order: ExpertOrder, weights=None, out=N
 def expert_dispatch_backward(d_rows, order: ExpertOrder, stream=None):
     """Gradient of expert_dispatch: per token the sum of its rows' gradients."""
     return expert_combine(d_rows, order, None, stream)
+
+
+# ------------------------------------------------------------------ attention heads and the paged cache
+def _heads3d(t, name, shape=None, dtype=None):
+    """Token and head strides of a GPU tensor [tokens, heads, dim] with contiguous heads."""
+    if not isinstance(t, _torch().Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA (HIP) tensor")
+    if t.dim() != 3 or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name} must be {'[tokens, heads, dim]' if shape is None else list(shape)}, got {list(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    ts, hs, step = t.stride()
+    if step != 1 and t.shape[2] != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return ts, hs
+
+
+def _vector(t, name, n, dtype=None):
+    _need_whole(t, name, dtype)
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be [{n}], got {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _type_code(t, name):
+    if t.dtype not in (_torch().bfloat16, _torch().float32):
+        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
+    return _dtype_code(t.dtype)
+
+
+def _rotary(first, tokens, cos_t, sin_t, positions, col0, halves):
+    """The rotation of `tokens` tokens' heads; no tables: none."""
+    r = Rotary()
+    if cos_t is None and sin_t is None:
+        return r
+    torch = _torch()
+    if cos_t is None or sin_t is None or cos_t.dim() != 2 or cos_t.shape != sin_t.shape:
+        raise ValueError("cos_t and sin_t must both be [rows, pairs]")
+    _need_whole(cos_t, "cos_t", torch.float32)
+    _need_whole(sin_t, "sin_t", torch.float32)
+    _same_device(first, cos_t, sin_t, positions)
+    r.cos_t, r.sin_t, r.table_rows, r.dim = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0], 2 * cos_t.shape[1]
+    r.col0, r.pairs = col0, 1 if halves else 0
+    if positions is not None:
+        r.positions = _vector(positions, "positions", tokens, torch.int32)
+    return r
+
+
+def _head_norm_args(q, k, q_weight, k_weight, eps, cos_t, sin_t, positions, col0, halves):
+    a = HeadNormArgs()
+    _heads3d(q, "q")
+    a.tokens, a.dim, a.eps = q.shape[0], q.shape[2], eps
+    a.x_dtype = _type_code(q, "q")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    a.weight_dtype = _type_code(weights[0], "a weight") if weights else F32
+    for t, w, rows, name in ((q, q_weight, a.q, "q"), (k, k_weight, a.k, "k")):
+        if t is None:
+            if w is not None:
+                raise ValueError("k_weight without k")
+            continue
+        _same_device(q, t, w)
+        rows.x_token_stride, rows.x_head_stride = _heads3d(t, name, (q.shape[0], t.shape[1] if t.dim() == 3 else 0, q.shape[2]),
+                                                           q.dtype)
+        rows.heads, rows.x = t.shape[1], t.data_ptr()
+        if w is not None:
+            rows.weight = _vector(w, f"{name}_weight", q.shape[2], weights[0].dtype)
+    a.rope = _rotary(q, q.shape[0], cos_t, sin_t, positions, col0, halves)
+    return a
+
+
+def _put_out(rows, out, name, like, dtype):
+    _same_device(like, out)
+    rows.out_token_stride, rows.out_head_stride = _heads3d(out, name, like.shape, dtype)
+    rows.out = out.data_ptr()
+
+
+def head_norm_rope(q, k=None, *, q_weight=None, k_weight=None, eps=1e-6, cos_t=None, sin_t=None, positions=None, col0=0,
+                   halves=False, out_dtype=None, q_out=None, k_out=None, stream=None):
+    """RMSNorm of every head of q [tokens, heads, dim] and k [tokens, kv_heads,
+    dim] (bf16 or f32) with the rotation by the tokens' positions: (q, k), or q
+    alone without k.  q_weight, k_weight [dim], or None for ones.  cos_t, sin_t
+    [rows, n] f32 rotate columns col0 .. col0 + 2 n - 1, token t by row
+    positions[t] (int32; None: t), as adjacent pairs or (halves) column i with
+    i + n.  q_out, k_out: where to (q and k themselves, for one).  Records nothing
+    for autograd: head_norm_rope_backward is the gradient."""
+    torch = _torch()
+    a = _head_norm_args(q, k, q_weight, k_weight, eps, cos_t, sin_t, positions, col0, halves)
+    dtype = out_dtype or (q_out.dtype if q_out is not None else q.dtype)
+    handle, ctx = _call_stream(q.device, stream)
+    with ctx:
+        y = torch.empty(q.shape, dtype=dtype, device=q.device) if q_out is None else q_out
+        a.out_dtype = _type_code(y, "the output")
+        _put_out(a.q, y, "q_out", q, dtype)
+        if k is not None:
+            z = torch.empty(k.shape, dtype=dtype, device=q.device) if k_out is None else k_out
+            _put_out(a.k, z, "k_out", k, dtype)
+        _check(load().mr_head_norm_rope(C.byref(a), handle))
+    return y if k is None else (y, z)
+
+
+def head_norm_rope_backward(d_q, q, d_k=None, k=None, *, q_weight=None, k_weight=None, eps=1e-6, cos_t=None, sin_t=None,
+                            positions=None, col0=0, halves=False, stream=None):
+    """Gradients of head_norm_rope for d_q, d_k, those of its outputs (in q's
+    dtype): (dq, dk, d_q_weight, d_k_weight), the inputs' in their dtype, the
+    weights' f32 [dim] or None without a weight; (dq, d_q_weight) without k."""
+    torch = _torch()
+    if (d_k is None) != (k is None):
+        raise ValueError("d_k and k go together")
+    a = _head_norm_args(q, k, q_weight, k_weight, eps, cos_t, sin_t, positions, col0, halves)
+    a.out_dtype = a.x_dtype
+    lib = load()
+    handle, ctx = _call_stream(q.device, stream)
+    with ctx:
+        made = []
+        for t, d, w, rows, name in ((q, d_q, q_weight, a.q, "d_q"), (k, d_k, k_weight, a.k, "d_k")):
+            if t is None:
+                continue
+            _same_device(q, d)
+            rows.d_out_token_stride, rows.d_out_head_stride = _heads3d(d, name, t.shape, q.dtype)
+            rows.d_out = d.data_ptr()
+            dx = torch.empty(t.shape, dtype=t.dtype, device=q.device)
+            dw = None if w is None else torch.empty(q.shape[2], dtype=torch.float32, device=q.device)
+            _put_out(rows, dx, name, t, t.dtype)
+            if w is not None:
+                rows.d_weight = dw.data_ptr()
+            made.append((dx, dw))
+        if q_weight is not None or k_weight is not None:
+            a.workspace_bytes = lib.mr_head_norm_rope_backward_workspace_size(C.byref(a))
+            ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=q.device)
+            a.workspace = ws.data_ptr()
+        _check(lib.mr_head_norm_rope_backward(C.byref(a), handle))
+    return made[0] if k is None else (made[0][0], made[1][0], made[0][1], made[1][1])
+
+
+class KVCache:
+    """One layer's keys and values in pages: k, v [pages, kv_heads, page_size,
+    head_dim] bf16, or MXFP4: int32 (or uint32) words [..., head_dim / 8] with
+    k_scales, v_scales uint8 [..., head_dim / 32].  page_size is a multiple of 16,
+    head_dim one of 32 up to 256; pages may lie apart (their stride, the same for
+    k and v), what is inside one may not."""
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
+        torch = _torch()
+        mx = k_scales is not None
+        if mx != (v_scales is not None):
+            raise ValueError("k_scales and v_scales go together")
+        for t, n in ((k, "k"), (v, "v")):
+            if t.dim() != 4 or not t.is_cuda:
+                raise ValueError(f"{n} must be a CUDA (HIP) tensor [pages, kv_heads, page_size, head_dim], got {list(t.shape)}")
+            if t.dtype not in ((torch.int32, torch.uint32) if mx else (torch.bfloat16,)):
+                raise TypeError(f"{n} must be {'int32 or uint32 words' if mx else 'bfloat16'}, got {t.dtype}")
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.pages, self.kv_heads, self.page_size, last = k.shape
+        self.head_dim = 8 * last if mx else last
+        d = self.desc = KVCacheDesc()
+        d.pages, d.page_size, d.kv_heads, d.head_dim = self.pages, self.page_size, self.kv_heads, self.head_dim
+        d.page_stride = self._pages(k, v, "v", k.shape)
+        d.k, d.v = k.data_ptr(), v.data_ptr()
+        if mx:
+            for t, n in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+                if not t.is_cuda or t.dtype != torch.uint8:
+                    raise TypeError(f"{n} must be a uint8 CUDA (HIP) tensor, got {t.dtype}")
+            d.scale_page_stride = self._pages(k_scales, v_scales, "v_scales", (*k.shape[:3], self.head_dim // 32))
+            d.k_scales, d.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
+        _same_device(k, v, k_scales, v_scales)
+
+    @staticmethod
+    def _pages(a, b, name, shape):
+        """The two tensors' common page stride."""
+        for t in (a, b):
+            if tuple(t.shape) != tuple(shape):
+                raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+            if t.shape[0] and not t[0].is_contiguous():
+                raise ValueError("a page must be contiguous")
+        if a.shape[0] > 1 and a.stride(0) != b.stride(0):
+            raise ValueError(f"{name} must have the page stride of its counterpart, {a.stride(0)}, got {b.stride(0)}")
+        return a.stride(0)
+
+    @classmethod
+    def zeros(cls, pages, kv_heads, page_size, head_dim, mxfp4=False, device="cuda"):
+        torch = _torch()
+        made = lambda last, dt: [torch.zeros(pages, kv_heads, page_size, last, dtype=dt, device=device) for _ in range(2)]
+        if not mxfp4:
+            return cls(*made(head_dim, torch.bfloat16))
+        return cls(*made(head_dim // 8, torch.int32), *made(head_dim // 32, torch.uint8))
+
+    def values(self, dtype=None, stream=None):
+        """(keys, values) of all pages [pages, kv_heads, page_size, head_dim], f32 by default or bf16."""
+        torch = _torch()
+        dtype = dtype or torch.float32
+        if self.k_scales is None:
+            with _call_stream(self.k.device, stream)[1]:
+                return self.k.to(dtype, copy=True), self.v.to(dtype, copy=True)
+        rows = lambda t: t.contiguous().view(-1, t.shape[-1])
+        if not self.pages:
+            empty = lambda: torch.empty(*self.k.shape[:3], self.head_dim, dtype=dtype, device=self.k.device)
+            return empty(), empty()
+        return tuple(mxfp4_dequantize(MXFP4Weights(rows(w), rows(s)), dtype, stream).view(*w.shape[:3], self.head_dim)
+                     for w, s in ((self.k, self.k_scales), (self.v, self.v_scales)))
+
+
+def kv_append(cache: KVCache, k, v, slots, *, normalize=False, norm_weight=None, eps=1e-6, cos_t=None, sin_t=None,
+              positions=None, col0=0, halves=False, stream=None):
+    """Writes k, v [tokens, kv_heads, head_dim] (bf16 or f32) into the cache's rows
+    slots int32 [tokens] (page * page_size + row; outside the pages: passed over),
+    the keys normalised first (normalize; norm_weight [head_dim] or None for ones)
+    and rotated (as head_norm_rope).  Values are rounded once, to what the cache
+    holds.  No two tokens may name one slot."""
+    torch = _torch()
+    a = KVAppendArgs()
+    a.cache = cache.desc
+    _heads3d(k, "k")
+    shape = (k.shape[0], cache.kv_heads, cache.head_dim)
+    a.k_token_stride, a.k_head_stride = _heads3d(k, "k", shape)
+    a.v_token_stride, a.v_head_stride = _heads3d(v, "v", shape, k.dtype)
+    _same_device(cache.k, k, v, slots, norm_weight)
+    a.tokens, a.k, a.v, a.dtype = k.shape[0], k.data_ptr(), v.data_ptr(), _type_code(k, "k")
+    a.slots = _vector(slots, "slots", k.shape[0], torch.int32)
+    a.eps = eps
+    if normalize:
+        a.normalize, a.norm_w_dtype = 1, F32
+        if norm_weight is not None:
+            a.norm_w, a.norm_w_dtype = _vector(norm_weight, "norm_weight", cache.head_dim), _type_code(norm_weight, "norm_weight")
+    elif norm_weight is not None:
+        raise ValueError("norm_weight needs normalize=True")
+    a.rope = _rotary(k, k.shape[0], cos_t, sin_t, positions, col0, halves)
+    handle, ctx = _call_stream(k.device, stream)
+    with ctx:
+        _check(load().mr_kv_append(C.byref(a), handle))
+
+
+def kv_attention(q, cache: KVCache, page_table, kv_lens, *, scale, q_offsets=None, max_kv_len=0, window=0, sinks=None,
+                 out=None, out_dtype=None, return_lse=False, stream=None):
+    """Causal attention of q [tokens, heads, head_dim] bf16 over a paged cache:
+    page_table int32 [batch, max_pages], kv_lens int32 [batch]; one token a
+    sequence, or sequence b's are q_offsets[b] .. q_offsets[b + 1] - 1 (int32
+    [batch + 1]), the last of them at its last key.  window: the last so many keys
+    only; sinks f32 [heads]; max_kv_len: about the most keys of a sequence (0: what
+    a table row holds).  out [tokens, heads, head_dim] bf16 (or f32); tokens of no
+    sequence are not written (give `out` to keep what they hold).  return_lse: also
+    the log of the sum of exp, f32 [tokens, heads]."""
+    torch = _torch()
+    a = KVAttentionArgs()
+    a.cache = cache.desc
+    a.q_token_stride, a.q_head_stride = _heads3d(q, "q", (q.shape[0], q.shape[1] if q.dim() == 3 else 0, cache.head_dim),
+                                                 torch.bfloat16)
+    _need(page_table, "page_table", torch.int32)
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be [batch, max_pages], got {list(page_table.shape)}")
+    a.batch, a.max_pages = page_table.shape
+    a.tokens, a.heads, a.q, a.scale = q.shape[0], q.shape[1], q.data_ptr(), scale
+    _same_device(cache.k, q, page_table, kv_lens, q_offsets, sinks, out)
+    a.page_table, a.page_table_stride = page_table.data_ptr(), page_table.stride(0)
+    a.kv_lens = _vector(kv_lens, "kv_lens", a.batch, torch.int32)
+    if q_offsets is not None:
+        a.q_offsets = _vector(q_offsets, "q_offsets", a.batch + 1, torch.int32)
+    if sinks is not None:
+        a.sinks = _vector(sinks, "sinks", a.heads, torch.float32)
+    a.max_kv_len, a.window = max_kv_len, window
+    lib = load()
+    handle, ctx = _call_stream(q.device, stream)
+    with ctx:
+        if out is None:
+            out = torch.empty(q.shape, dtype=out_dtype or torch.bfloat16, device=q.device)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError(f"out must be {out_dtype}, got {out.dtype}")
+        a.out_token_stride, a.out_head_stride = _heads3d(out, "out", q.shape)
+        a.out, a.out_dtype = out.data_ptr(), _type_code(out, "out")
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+        if return_lse:
+            a.lse = lse.data_ptr()
+        n = lib.mr_kv_attention_workspace_size(C.byref(a))
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+        _check(lib.mr_kv_attention(C.byref(a), handle))
+    return (out, lse) if return_lse else out
 
 
 def rms_norm(x, weight, eps=1e-6, out_dtype=None, stream=None):

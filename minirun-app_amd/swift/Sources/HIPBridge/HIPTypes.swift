@@ -62,6 +62,27 @@ extension HIPTensor {
         try needType(name, want)
     }
 
+    /// [tokens, heads, dim] (nil: any) with the values of a head next to each other.
+    func needHeads(_ name: String, _ tokens: Int?, _ heads: Int?, _ dim: Int?, dtype want: mr_dtype? = nil) throws {
+        guard shape.count == 3, strides.count == 3, shape[0] == tokens ?? shape[0], shape[1] == heads ?? shape[1],
+              shape[2] == dim ?? shape[2] else {
+            throw HIPError(status: MR_INVALID_SHAPE, description: "\(name) must be [tokens, heads, dim] of the call, got \(shape)")
+        }
+        guard strides[2] == 1 || shape[2] == 1 else {
+            throw HIPError(status: MR_INVALID_ARGUMENT, description: "\(name) must be contiguous in its last dimension")
+        }
+        try needType(name, want)
+    }
+
+    /// Of this shape, without gaps inside a page (the first axis may have any stride).
+    func needPages(_ name: String, _ size: [Int], dtype want: mr_dtype) throws {
+        guard shape == size, strides.count == shape.count else {
+            throw HIPError(status: MR_INVALID_SHAPE, description: "\(name) must be \(size), got \(shape)")
+        }
+        let page = HIPTensor(pointer: pointer, shape: Array(shape.dropFirst()), strides: Array(strides.dropFirst()), dtype: dtype)
+        try page.needWhole(name, nil, dtype: want)
+    }
+
     private func needType(_ name: String, _ want: mr_dtype?) throws {
         guard dtype == want ?? dtype else {
             throw HIPError(status: MR_INVALID_DTYPE,
