@@ -301,7 +301,7 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     p.dim = c.head_dim;
     p.table = a->page_table;
     p.table_stride = a->page_table_stride;
-    p.max_keys = a->max_pages * c.page_size;
+    p.max_keys = c.pages ? a->max_pages * c.page_size : 0;  // (without pages nothing is read)
     p.lens = a->kv_lens;
     p.q_offsets = a->q_offsets;
     p.batch = a->batch;

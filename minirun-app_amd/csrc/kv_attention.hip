@@ -23,10 +23,9 @@
 // are split over workgroups where that fills the GPU (kv_attention_route),
 // which leave (m, l, o) in the workspace for kv_join_kernel.
 //
-// Keys that no row may see are zeros where they are loaded.  Where some rows of
-// a step see a key and others do not, 0 times an infinity or a NaN of its value
-// would reach the others, so such a step with such values takes its keys one by
-// one (kv_step_apart).
+// Keys that no row may see are zeros where they are loaded.  Infinities and NaN of
+// values that some rows of a step see and others do not take a way of their own
+// (kv_add_infinite).
 #include <algorithm>
 
 #include "kv_tiles.hpp"
@@ -37,6 +36,9 @@ namespace {
 
 constexpr int KD_WAVES = 4, KD_STEP = 32;
 
+// Workgroups a CU that registers are kept for
+constexpr int KD_PER_CU(int dp, int r, bool mx) { return dp == 128 && r == 1 ? (mx ? 4 : 3) : 1; }
+
 template <int DP, bool MX>
 struct KvDecodeLds {
     // rows apart by an odd number of 16-byte (K) and 32-byte (V) pieces, so that 16
@@ -46,12 +48,21 @@ struct KvDecodeLds {
     static constexpr int V_BYTES = KD_STEP * V_STRIDE * 2, K_BYTES = KD_STEP * K_STRIDE;
     static constexpr int S_BYTES = MX ? KD_STEP * DP / 32 : 0;  // the keys' scales
     static constexpr int O_STRIDE = DP + 4;                     // f32, the end's sums of 16 rows
-    static constexpr int WAVE = (V_BYTES + K_BYTES + S_BYTES + 15) / 16 * 16;
+    // the keys are in registers again before the values take their place
+    static constexpr int ALL_K = K_BYTES + S_BYTES, WAVE = ((V_BYTES > ALL_K ? V_BYTES : ALL_K) + 15) / 16 * 16;
     static_assert(16 * O_STRIDE * 4 <= WAVE, "the sums of 16 rows fit");
 };
 
+// A wave's LDS operations are done in order; the compiler has to keep them so
+// where lanes hand values over.
+__device__ __forceinline__ void kd_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int DP, int R, bool MX>
-__global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p) {
+__global__ void __launch_bounds__(64 * KD_WAVES, KD_PER_CU(DP, R, MX)) kv_decode_kernel(KvAttnParams p) {
     using L = KvDecodeLds<DP, MX>;
     constexpr int ROWS = 16 * R, KS = DP / 32, DT = DP / 16, CPL = DP / 4;
     __shared__ __attribute__((aligned(16))) char lds[KD_WAVES * L::WAVE];
@@ -76,7 +87,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 
     char* mine = lds + w * L::WAVE;
     uint16_t* vt = (uint16_t*)mine;
-    char* kt = mine + L::V_BYTES;
+    char* kt = mine;
     uint8_t* ksc = (uint8_t*)(kt + L::K_BYTES);
 
     KvRow row[R];
@@ -102,6 +113,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
         for (int d = 0; d < DT; ++d) o[r][d] = f32x4{};
     }
 
+    int apart_from = we, apart_to = 0;  // keys whose infinite values were left out
     if (wb < we) {
         KvWalk walk;
         walk.start(p, t.b, wb);
@@ -115,81 +127,99 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
                 walk.next(p.page_size);
             }
         };
-        KvGroup<DP, MX> k[2], v[2];
+        using Group = KvGroup<DP, MX>;
+        const typename Group::At at = Group::at(p.dim, l);
+        Group k[2], v[2];
         bool have[2];
-        auto load = [&](int key) {
+        auto load = [&]() {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                have[h] = kv_page(p, id[h], key + 16 * h < we);
-                kv_load<DP, MX>(p, kv_head, id[h], off[h], have[h], l, k[h], v[h]);
+                have[h] = kv_page(p, id[h]);
+                kv_load<DP, MX>(p, kv_head, id[h], off[h], at, k[h], v[h]);
             }
         };
         look(wb);
-        load(wb);
+        load();
         look(wb + KD_STEP);
         for (int k0 = wb; k0 < we; k0 += KD_STEP) {
             const bool seen[2] = {have[0], have[1]};
-            const bool all = k0 >= t.all_lo && k0 + KD_STEP <= t.all_hi && k0 + KD_STEP <= we && seen[0] && seen[1];
+            const bool all = k0 >= t.all_lo && k0 + KD_STEP <= min(t.all_hi, we) && seen[0] && seen[1];
             bool apart = false;  // (wave-uniform)
+            if (!all) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)  // (of a page that does not exist, all rows)
+                    if (k0 + 16 * h + 16 > we || !seen[h]) v[h].cut(seen[h] ? we - k0 - 16 * h : 0, l);
+                apart = __builtin_amdgcn_ballot_w64(v[0].not_finite() || v[1].not_finite()) != 0;
+                if (apart) apart_to = k0 + KD_STEP, apart_from = min(apart_from, k0);
+            }
+            if (p.dim < DP) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) k[h].narrow(at), v[h].narrow(at);
+            }
+            // keys through LDS, as they are stored, into the operands' registers
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (k0 + 16 * h + 16 > we) k[h].cut(we - k0 - 16 * h, l), v[h].cut(we - k0 - 16 * h, l);
                 if constexpr (MX) {
 #pragma unroll
-                    for (int i = 0; i < KvGroup<DP, MX>::N; ++i)
-                        if (k[h].active(l)) {
-                            const int rr = 16 * h + k[h].row(l, i);
-                            *(u32x4*)(kt + rr * L::K_STRIDE + 16 * k[h].piece(l)) = k[h].v[i];
-                            ksc[rr * (DP / 32) + k[h].piece(l)] = (uint8_t)k[h].scale[i];
+                    for (int i = 0; i < Group::N; ++i)
+                        if (Group::active(l)) {
+                            const int rr = 16 * h + Group::row(l, i);
+                            *(u32x4*)(kt + rr * L::K_STRIDE + 16 * Group::piece(l)) = k[h].v[i];
+                            ksc[rr * (DP / 32) + Group::piece(l)] = (uint8_t)k[h].scale[i];
                         }
                 } else {
                     k[h].put((uint16_t*)kt + 16 * h * (L::K_STRIDE / 2), L::K_STRIDE / 2, l);
                 }
-                v[h].put(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
-                if (!all) apart |= v[h].not_finite();
             }
-            if (!all) apart = __builtin_amdgcn_ballot_w64(apart) != 0;
+            kd_fence();
+            constexpr int KW = MX ? KS / 4 + (KS < 4) : KS;  // 16-byte pieces of a lane (DP 64 in MXFP4: half of one)
+            u32x4 kw[2][KW];
+            uint32_t ks[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char* kr = kt + (16 * h + n) * L::K_STRIDE + g * (MX ? CPL / 2 : CPL * 2);
+                if constexpr (MX && KS == 2) {
+                    const u32x2 x = *(const u32x2*)kr;
+                    kw[h][0] = u32x4{x[0], x[1], 0, 0};
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KW; ++i) kw[h][i] = *(const u32x4*)(kr + 16 * i);
+                }
+                if constexpr (MX) {  // the lane's dims lie in one block, or (DP 256) in two
+                    const uint8_t* sc = ksc + (16 * h + n) * (DP / 32) + CPL * g / 32;
+                    ks[h][0] = sc[0];
+                    ks[h][1] = DP == 256 ? sc[1] : 0;
+                }
+            }
+            kd_fence();
+            // values to where the keys were
+            if (apart) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[h].template put<true>(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[h].put(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
+            }
             if (k0 + KD_STEP < we) {
-                load(k0 + KD_STEP);
+                load();
                 look(k0 + 2 * KD_STEP);
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 
             f32x4 s[2][R];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) s[h][r] = f32x4{};
-                const char* kr = kt + (16 * h + n) * L::K_STRIDE + g * (MX ? CPL / 2 : CPL * 2);
-                bf16x8 a[KS];
-                if constexpr (MX) {
-                    uint32_t words[KS];
-                    if constexpr (KS == 2) {
-                        const u32x2 x = *(const u32x2*)kr;
-                        words[0] = x[0], words[1] = x[1];
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < KS / 4; ++i) {
-                            const u32x4 x = *(const u32x4*)(kr + 16 * i);
+                for (int i = 0; i < KS; ++i) {
+                    bf16x8 a;
+                    if constexpr (MX)
+                        a = mxfp4_bf16(kw[h][i / 4][i % 4], __uint_as_float(ks[h][i / 4] << 23));
+                    else
+                        a = __builtin_bit_cast(bf16x8, kw[h][i]);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) words[4 * i + e] = x[e];
-                        }
-                    }
-                    // the lane's dims lie in one block, or (DP 256) in two
-                    const uint8_t* sc = ksc + (16 * h + n) * (DP / 32) + CPL * g / 32;
-#pragma unroll
-                    for (int i = 0; i < KS; ++i)
-                        a[i] = mxfp4_bf16(words[i], __uint_as_float((uint32_t)sc[DP == 256 ? i / 4 : 0] << 23));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) a[i] = *(const bf16x8*)(kr + 16 * i);
+                    for (int r = 0; r < R; ++r) s[h][r] = mfma16(a, q[r][i], s[h][r]);
                 }
-#pragma unroll
-                for (int i = 0; i < KS; ++i)
-#pragma unroll
-                    for (int r = 0; r < R; ++r) s[h][r] = mfma16(a[i], q[r][i], s[h][r]);
             }
 
             bf16x8 pb[R];
@@ -227,41 +257,30 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
                     }
             }
 
+            kd_fence();
             // key 4 g + e of group 0 and 4 g + e - 4 of group 1 are k-slot 8 g + e
             auto values = [&](int d) {
                 const uint16_t* at = vt + (4 * g + (n >> 2)) * L::V_STRIDE + 16 * d + 4 * (n & 3);
                 const bf16x4 lo = ds_read_tr16(at), hi = ds_read_tr16(at + 16 * L::V_STRIDE);
                 return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             };
-            if (!apart) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const bf16x8 a = values(d);
+            for (int d = 0; d < DT; ++d) {
+                const bf16x8 a = values(d);
 #pragma unroll
-                    for (int r = 0; r < R; ++r) o[r][d] = mfma16(a, pb[r], o[r][d]);
-                }
-            } else {
-                // one key at a time, added where it is seen
-                for (int key = 0; key < KD_STEP; ++key) {
-                    if (!seen[key >> 4]) continue;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        bf16x8 a = values(d);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (16 * (e >> 2) + 4 * g + (e & 3) != key) a[e] = (__bf16)0.f;
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            const f32x4 one = mfma16(a, pb[r], f32x4{});
-                            if (k0 + key >= row[r].lo && k0 + key < min(row[r].hi, we)) o[r][d] += one;
-                        }
-                    }
-                }
+                for (int r = 0; r < R; ++r) o[r][d] = mfma16(a, pb[r], o[r][d]);
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            kd_fence();
         }
     }
+
+    for (int key = apart_from; key < min(apart_to, we); ++key)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                kv_add_infinite<MX>(p, t.b, kv_head, key, key >= row[r].lo && key < row[r].hi, 16 * d + 4 * g,
+                                    [&](int j, float v) { o[r][d][j] += v; });
 
     // the waves' sums
 #pragma unroll

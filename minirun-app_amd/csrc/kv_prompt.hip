@@ -12,8 +12,6 @@
 // the wave.
 // What bounds it: the products (4 dim flops a pair of query and key) with the
 // softmax on the vector units beside them.
-#include <type_traits>
-
 #include "kv_tiles.hpp"
 
 namespace mr {
@@ -31,6 +29,13 @@ struct KvPromptLds {
     static constexpr int BYTES = 2 * BUF * 2 + 64;
     static_assert(KP_ROWS * DP * 2 <= BYTES, "the output's tile fits");
 };
+
+// Every wave's LDS traffic is done; loads into registers stay in flight.  (The
+// builtin tells the compiler that earlier LDS reads have landed.)
+__device__ __forceinline__ void kp_barrier() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    lds_barrier();
+}
 
 // keys of tile index kb * 32 + 8 * (i / 4) + 4 * half + i % 4 are score i of block kb
 
@@ -79,7 +84,9 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
 
     // wave w brings keys 16 w .. of each tile
     const int steps = (max(ke - kb, 0) + KP_KEYS - 1) / KP_KEYS;
-    KvGroup<DP, MX> kreg, vreg;
+    using Group = KvGroup<DP, MX>;
+    const typename Group::At at = Group::at(p.dim, l);
+    Group kreg, vreg;
     KvWalk walk;
     walk.start(p, t.b, steps ? kb + 16 * w : 0);
     int id = -1, off = 0, ahead = kb + 16 * w;  // the next group to load, its page
@@ -93,55 +100,67 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
     int from = 0;
     auto load = [&]() {
         from = ahead;
-        have = kv_page(p, id, ahead < ke);
-        kv_load<DP, MX>(p, kv_head, id, off, have, l, kreg, vreg);
+        have = kv_page(p, id);
+        kv_load<DP, MX>(p, kv_head, id, off, at, kreg, vreg);
         ahead += KP_KEYS;
     };
-    // what was loaded goes to buffer `to`
+    // what was loaded goes to buffer `to`; flags say of the wave's 16 rows, in bit 0,
+    // that infinities or NaN among their values were left out (where not every row of the
+    // workgroup sees the tile), in bit 1 that their page does not exist
     auto put = [&](int to) {
-        if (from + 16 > ke) kreg.cut(ke - from, l), vreg.cut(ke - from, l);
+        if (from + 16 > ke || !have) vreg.cut(have ? ke - from : 0, l);
+        if (p.dim < DP) kreg.narrow(at), vreg.narrow(at);
         uint16_t* kt = lds + to * L::BUF;
+        const int k0 = from - 16 * w;
+        const bool apart = (k0 < t.all_lo || k0 + KP_KEYS > t.all_hi) && __builtin_amdgcn_ballot_w64(vreg.not_finite()) != 0;
         kreg.put(kt + 16 * w * L::K_STRIDE, L::K_STRIDE, l);
-        vreg.put(kt + L::K_SIZE + 16 * w * L::V_STRIDE, L::V_STRIDE, l);
-        // bit 0: infinities or NaN; bit 1: the rows do not exist
-        const int bad = (__builtin_amdgcn_ballot_w64(vreg.not_finite()) ? 1 : 0) | (have ? 0 : 2);
-        if (l == 0) flags[4 * to + w] = bad;
+        if (apart)
+            vreg.template put<true>(kt + L::K_SIZE + 16 * w * L::V_STRIDE, L::V_STRIDE, l);
+        else
+            vreg.put(kt + L::K_SIZE + 16 * w * L::V_STRIDE, L::V_STRIDE, l);
+        if (l == 0) flags[4 * to + w] = (apart ? 1 : 0) | (have ? 0 : 2);
     };
 
     const int tr_key = 4 * hh + ((l & 15) >> 2), tr_d = 16 * ((l >> 4) & 1) + 4 * (l & 3);
-    auto tile = [&](auto masked_tag, const uint16_t* kt, const int* fl, int k0) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
+    // one tile for this wave's 32 rows; masked: not every row sees every key (a branch
+    // around the masking alone: two forms of the whole cost 40 spilled registers)
+    auto tile = [&](bool masked, const uint16_t* kt, int gone, int k0) {
         const uint16_t* vt = kt + L::K_SIZE;
         f32x16 s[2] = {f32x16{}, f32x16{}};
+        // operands come in two sets, so that one's reads overlap the other's products
+        // (the fences keep the scheduler from reading them all at once)
+        bf16x8 ka[2][4];
+        auto keys = [&](int x, bf16x8(&a)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                a[e] = *(const bf16x8*)(kt + (32 * (e & 1) + lq) * L::K_STRIDE + 32 * x + 16 * (e >> 1) + 8 * hh);
+        };
+        keys(0, ka[0]);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int x = 0; x < KS; ++x)
+        for (int x = 0; x < KS / 2; ++x) {
+            if (x + 1 < KS / 2) keys(x + 1, ka[(x + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const bf16x8 a = *(const bf16x8*)(kt + (32 * b + lq) * L::K_STRIDE + 16 * x + 8 * hh);
-                s[b] = mfma32(a, qf[x], s[b]);
-            }
+            for (int e = 0; e < 4; ++e) s[e & 1] = mfma32(ka[x & 1][e], qf[2 * x + (e >> 1)], s[e & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         __builtin_amdgcn_s_setprio(0);
         float mx = -INFINITY;
-        bool apart = false;
-        uint32_t gone = 0;  // bit per group of 16 keys
-        if constexpr (MASKED) {
+        if (masked) {
+            const int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int f = __builtin_amdgcn_readfirstlane(fl[i]);
-                apart |= (f & 1) != 0;
-                gone |= (f & 2 ? 1u : 0u) << i;
-            }
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at = 32 * b + 8 * (i >> 2) + (i & 3);  // + 4 hh
+                    if (at >= hi || at < lo || (gone >> (at >> 4) & 1)) s[b][i] = -INFINITY;
+                }
         }
-        const int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int at = 32 * b + 8 * (i >> 2) + (i & 3);  // + 4 hh
-                if (MASKED && (at >= hi || at < lo || (gone >> (at >> 4) & 1))) s[b][i] = -INFINITY;
-                mx = fmaxf(mx, s[b][i]);
-            }
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
         mx = xor32_max(mx) * p.scale_log2;  // (the scale is positive)
         const bool raise = mx > m_run + KV_TAU;
         if (__builtin_amdgcn_ballot_w64(raise)) {
@@ -163,41 +182,34 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
                 ls[i & 3] += e;
             }
         l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        auto values = [&](int x, int d) {
-            const uint16_t* at = vt + (16 * x + tr_key) * L::V_STRIDE + 32 * d + tr_d;
-            const bf16x4 a = ds_read_tr16(at), b = ds_read_tr16(at + 8 * L::V_STRIDE);
-            return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        };
         __builtin_amdgcn_s_setprio(1);
+        // DB blocks of 32 dims of 16 keys, in two sets of at most four
+        constexpr int VB = DB < 4 ? DB : 4, VN = 4 * (DB / VB);
+        bf16x8 va[2][VB];
+        auto values = [&](int x, bf16x8(&a)[VB]) {
+            const uint16_t* at = vt + (16 * (x & 3) + tr_key) * L::V_STRIDE + 32 * VB * (x >> 2) + tr_d;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+            for (int d = 0; d < VB; ++d) {
+                const bf16x4 u = ds_read_tr16(at + 32 * d), v = ds_read_tr16(at + 32 * d + 8 * L::V_STRIDE);
+                a[d] = bf16x8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+            }
+        };
+        values(0, va[0]);
+#pragma unroll
+        for (int x = 0; x < VN; ++x) {
+            if (x + 1 < VN) values(x + 1, va[(x + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
             bf16x8 pb;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pb[e] = (__bf16)s[x >> 1][8 * (x & 1) + e];
-            if (!MASKED || !apart) {
+            for (int e = 0; e < 8; ++e) pb[e] = (__bf16)s[(x & 3) >> 1][8 * (x & 1) + e];
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = mfma32(values(x, d), pb, o[d]);
-            } else {
-                // one key at a time, added where it is seen
-                if (gone >> x & 1) continue;
-                for (int key = 0; key < 16; ++key) {
-                    const int at = 16 * x + key - 4 * hh;
-                    const bool mine = at < hi && at >= lo;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        bf16x8 a = values(x, d);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (8 * (e >> 2) + 4 * hh + (e & 3) != key) a[e] = (__bf16)0.f;
-                        const f32x16 one = mfma32(a, pb, f32x16{});
-                        if (mine) o[d] += one;
-                    }
-                }
-            }
+            for (int d = 0; d < VB; ++d) o[VB * (x >> 2) + d] = mfma32(va[x & 1][d], pb, o[VB * (x >> 2) + d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
     };
 
+    int apart_from = ke, apart_to = 0;  // keys whose infinite values were left out
     if (steps > 0) {
         look();
         load();
@@ -207,7 +219,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
             load();
             look();
         }
-        __syncthreads();
+        kp_barrier();
         for (int i = 0; i < steps; ++i) {
             if (i + 1 < steps) put((i + 1) & 1);
             if (i + 2 < steps) {
@@ -216,29 +228,37 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
             }
             const int k0 = kb + KP_KEYS * i;
             const uint16_t* kt = lds + (i & 1) * L::BUF;
-            const int* fl = flags + 4 * (i & 1);
             if (k0 < wave_hi && k0 + KP_KEYS > wave_lo) {
-                const bool whole = (__builtin_amdgcn_readfirstlane((fl[0] | fl[1]) | (fl[2] | fl[3])) & 2) == 0;
-                if (whole && k0 >= all_lo && k0 + KP_KEYS <= min(all_hi, ke))
-                    tile(std::false_type{}, kt, fl, k0);
-                else
-                    tile(std::true_type{}, kt, fl, k0);
+                // (four flags of two bits)
+                const u32x4 f = *(const u32x4*)(flags + 4 * (i & 1));
+                const int fl = __builtin_amdgcn_readfirstlane((int)(f[0] | f[1] << 2 | f[2] << 4 | f[3] << 6));
+                const int gone = (fl >> 1 & 1) | (fl >> 2 & 2) | (fl >> 3 & 4) | (fl >> 4 & 8);
+                tile(gone || k0 < all_lo || k0 + KP_KEYS > min(all_hi, ke), kt, gone, k0);
+                if (fl & 0x55) apart_to = k0 + KP_KEYS, apart_from = min(apart_from, k0);
             }
-            __syncthreads();
+            kp_barrier();
         }
     }
 
+    for (int key = apart_from; key < min(apart_to, ke); ++key)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                kv_add_infinite<MX>(p, t.b, kv_head, key, key >= row.lo && key < row.hi, 32 * d + 8 * c + 4 * hh,
+                                    [&](int j, float v) { o[d][4 * c + j] += v; });
+
     float total = xor32_sum(l_part);
-    const int64_t at = (int64_t)row.token * (p.kv_heads * p.group) + row.head;
+    const int64_t place = (int64_t)row.token * (p.kv_heads * p.group) + row.head;
     if (p.splits > 1) {
         if (!row.ok) return;
         if (hh == 0) {
-            float* ml = p.part_ml + 2 * (at * p.splits + split);
+            float* ml = p.part_ml + 2 * (place * p.splits + split);
             ml[0] = m_run;
             ml[1] = total;
         }
         if (total == 0.f) return;
-        float* to = p.part_o + (at * p.splits + split) * p.dim;
+        float* to = p.part_o + (place * p.splits + split) * p.dim;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -257,7 +277,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
     }
     const float inv = total == 0.f ? 0.f : was / total;  // (no key is seen: zeros)
     if (p.lse && row.ok && hh == 0)
-        p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+        p.lse[place] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
     if (p.out_f32) {
         if (!row.ok) return;
         float* to = (float*)p.out + row.token * p.out_ts + row.head * p.out_hs;

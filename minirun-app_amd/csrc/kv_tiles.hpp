@@ -112,14 +112,20 @@ struct KvWalk {
     }
 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_buffer(const void* p, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
+// Pairs of bf16 with zeros for infinities and NaN
+__device__ __forceinline__ u32x4 kv_finite(u32x4 x) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if ((x[k] & 0x7f80u) == 0x7f80u) x[k] &= 0xffff0000u;
+        if ((x[k] & 0x7f800000u) == 0x7f800000u) x[k] &= 0xffffu;
+    }
+    return x;
 }
 
 // 16 keys (or values) of one head as a wave loads them: 16-byte pieces, RPL
 // rows a load, so that a load covers whole neighbouring rows; MXFP4: a piece is
-// a block of 32 values, and its scale comes with it.  A group that does not
-// exist reads nothing and is zeros.
+// a block of 32 values, and its scale comes with it.  Lanes without a piece of
+// their own (heads of fewer dims than DP) read the row's first.
 template <int DP, bool MX>
 struct KvGroup {
     static constexpr int LPR = MX ? DP / 32 : DP / 8;          // pieces of a row
@@ -132,31 +138,45 @@ struct KvGroup {
     __device__ __forceinline__ static int piece(int l) { return l % LPR; }
     __device__ __forceinline__ static bool active(int l) { return RPL * LPR == 64 || l < RPL * LPR; }
 
-    // base, scales: the group's first row; row_bytes: of the stored row
-    __device__ __forceinline__ void load(const char* base, const uint8_t* scales, int dim, bool exists, int l) {
-        const int row_bytes = MX ? dim / 2 : dim * 2, blocks = dim / 32;
-        const bool mine = active(l) && piece(l) * (MX ? 32 : 8) < dim;
-        const __amdgpu_buffer_rsrc_t rows = kv_buffer(base, exists ? 16 * row_bytes : 0);
-        const int none = 0x40000000;
+    // A lane's byte offsets in a group's rows and scales; the next load's rows follow
+    struct At {
+        uint32_t bytes, scale, step, scale_step;
+        bool mine;
+    };
+    __device__ __forceinline__ static At at(int dim, int l) {
+        const uint32_t row_bytes = MX ? dim / 2 : dim * 2, blocks = dim / 32, r = active(l) ? l / LPR : 0;
+        At a;
+        a.mine = piece(l) * (MX ? 32 : 8) < dim;
+        a.bytes = r * row_bytes + (a.mine ? 16 * piece(l) : 0);
+        a.scale = r * blocks + (a.mine ? piece(l) : 0);
+        a.step = RPL * row_bytes;
+        a.scale_step = RPL * blocks;
+        return a;
+    }
+    // base, scales: the group's first row (wave-uniform)
+    __device__ __forceinline__ void load(const char* base, const uint8_t* scales, const At& a) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                 rows, mine ? row(l, i) * row_bytes + 16 * piece(l) : none, 0, 0));
+        for (int i = 0; i < N; ++i) v[i] = *(const u32x4*)(base + (a.bytes + i * a.step));
         if constexpr (MX) {
-            const __amdgpu_buffer_rsrc_t bytes = kv_buffer(scales, exists ? 16 * blocks : 0);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                scale[i] = __builtin_amdgcn_raw_buffer_load_b8(bytes, mine ? row(l, i) * blocks + piece(l) : none, 0, 0);
+            for (int i = 0; i < N; ++i) scale[i] = scales[a.scale + i * a.scale_step];
         }
+    }
+    __device__ __forceinline__ void clear(int i) {
+        v[i] = u32x4{};
+        if constexpr (MX) scale[i] = 0;
     }
     // rows from `n` on become zeros
     __device__ __forceinline__ void cut(int n, int l) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (row(l, i) >= n) {
-                v[i] = u32x4{};
-                if constexpr (MX) scale[i] = 0;
-            }
+            if (row(l, i) >= n) clear(i);
+    }
+    // dims past a head's become zeros
+    __device__ __forceinline__ void narrow(const At& a) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!a.mine) clear(i);
     }
     // a value of this lane may be infinite or NaN (MXFP4: its block's scale says so)
     __device__ __forceinline__ bool not_finite() const {
@@ -173,7 +193,8 @@ struct KvGroup {
         }
         return bad;
     }
-    // into bf16 rows of `stride` values
+    // into bf16 rows of `stride` values; CLEAN: zeros for infinities and NaN
+    template <bool CLEAN = false>
     __device__ __forceinline__ void put(uint16_t* rows, int stride, int l) const {
         if (!active(l)) return;
 #pragma unroll
@@ -182,26 +203,57 @@ struct KvGroup {
                 uint16_t* to = rows + row(l, i) * stride + 32 * piece(l);
                 const float s = __uint_as_float(scale[i] << 23);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) *(bf16x8*)(to + 8 * k) = mxfp4_bf16(v[i][k], s);
+                for (int k = 0; k < 4; ++k) {
+                    const u32x4 x = __builtin_bit_cast(u32x4, mxfp4_bf16(v[i][k], s));
+                    *(u32x4*)(to + 8 * k) = CLEAN ? kv_finite(x) : x;
+                }
             } else {
-                *(u32x4*)(rows + row(l, i) * stride + 8 * piece(l)) = v[i];
+                *(u32x4*)(rows + row(l, i) * stride + 8 * piece(l)) = CLEAN ? kv_finite(v[i]) : v[i];
             }
         }
     }
 };
 
-// Key and value rows of the group at a walk's place
-__device__ __forceinline__ bool kv_page(const KvAttnParams& p, int id, bool in) { return in && (uint32_t)id < (uint32_t)p.pages; }
+// Where some rows of a tile see a key and others do not, 0 times an infinity or a NaN
+// of its value would reach the others through the product.  Such values are zeros in
+// LDS (KvGroup::put), and this adds at the end what they come to: to each dim of a row
+// that sees the key, the infinity or NaN itself (again where the product had it, which
+// changes nothing).  add(j, v): to dims d0 + j (j < 4) of the lane's row.  `key` and
+// the sequence are wave-uniform, d0 is the lane's.
+template <bool MX, typename F>
+__device__ __forceinline__ void kv_add_infinite(const KvAttnParams& p, int b, int kv_head, int key, bool sees, int d0, F&& add) {
+    const int page = key / p.page_size, id = s_load(p.table + b * p.table_stride + page);
+    if ((uint32_t)id >= (uint32_t)p.pages || !sees || d0 >= p.dim) return;
+    const int64_t row = (int64_t)kv_head * p.page_size + (key - page * p.page_size);
+    uint32_t lo, hi;
+    if constexpr (MX) {
+        const uint16_t w = *(const uint16_t*)(p.v + id * p.page_bytes + (row * p.dim + d0) / 2);
+        const uint8_t e = p.v_scales[id * p.scale_bytes + (row * p.dim + d0) / 32];
+        const u32x4 x = __builtin_bit_cast(u32x4, mxfp4_bf16(w, __uint_as_float((uint32_t)e << 23)));
+        lo = x[0], hi = x[1];
+    } else {
+        const u32x2 x = *(const u32x2*)(p.v + id * p.page_bytes + (row * p.dim + d0) * 2);
+        lo = x[0], hi = x[1];
+    }
+    const uint32_t v[4] = {lo << 16, lo & 0xffff0000u, hi << 16, hi & 0xffff0000u};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if ((v[j] & 0x7f800000u) == 0x7f800000u) add(j, __uint_as_float(v[j]));
+}
 
+__device__ __forceinline__ bool kv_page(const KvAttnParams& p, int id) { return (uint32_t)id < (uint32_t)p.pages; }
+
+// Keys and values of the group at `offset` of page `id` (of page 0 where there is no
+// such page: whoever loads it hides the keys and clears the values)
 template <int DP, bool MX>
-__device__ __forceinline__ void kv_load(const KvAttnParams& p, int kv_head, int id, int offset, bool exists, int l,
-                                        KvGroup<DP, MX>& k, KvGroup<DP, MX>& v) {
-    const int64_t page = exists ? id : 0;
-    const int64_t row = (int64_t)kv_head * p.page_size + offset;
-    const int64_t at = page * p.page_bytes + row * (MX ? p.dim / 2 : p.dim * 2);
-    const int64_t sc = MX ? page * p.scale_bytes + row * (p.dim / 32) : 0;
-    k.load(p.k + at, p.k_scales + sc, p.dim, exists, l);
-    v.load(p.v + at, p.v_scales + sc, p.dim, exists, l);
+__device__ __forceinline__ void kv_load(const KvAttnParams& p, int kv_head, int id, int offset,
+                                        const typename KvGroup<DP, MX>::At& at, KvGroup<DP, MX>& k, KvGroup<DP, MX>& v) {
+    const int64_t page = kv_page(p, id) ? id : 0;
+    const uint32_t row = (uint32_t)(kv_head * p.page_size + offset);  // (a page has at most 2^28 values)
+    const int64_t bytes = page * p.page_bytes + row * (uint32_t)(MX ? p.dim / 2 : p.dim * 2);
+    const int64_t sc = MX ? page * p.scale_bytes + row * (uint32_t)(p.dim / 32) : 0;
+    k.load(p.k + bytes, p.k_scales + sc, at);
+    v.load(p.v + bytes, p.v_scales + sc, at);
 }
 
 }  // namespace mr
