@@ -36,9 +36,6 @@ namespace {
 
 constexpr int KD_WAVES = 4, KD_STEP = 32;
 
-// Workgroups a CU that registers are kept for
-constexpr int KD_PER_CU(int dp, int r, bool mx) { return dp == 128 && r == 1 ? (mx ? 4 : 3) : 1; }
-
 template <int DP, bool MX>
 struct KvDecodeLds {
     // rows apart by an odd number of 16-byte (K) and 32-byte (V) pieces, so that 16
@@ -62,16 +59,17 @@ __device__ __forceinline__ void kd_fence() {
 }
 
 template <int DP, int R, bool MX>
-__global__ void __launch_bounds__(64 * KD_WAVES, KD_PER_CU(DP, R, MX)) kv_decode_kernel(KvAttnParams p) {
+__global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p) {
     using L = KvDecodeLds<DP, MX>;
     constexpr int ROWS = 16 * R, KS = DP / 32, DT = DP / 16, CPL = DP / 4;
     __shared__ __attribute__((aligned(16))) char lds[KD_WAVES * L::WAVE];
     __shared__ float sm[KD_WAVES][ROWS], sl[KD_WAVES][ROWS];
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int heads_splits = p.kv_heads * p.splits;
-    const int tile_id = blockIdx.x / heads_splits, rest = blockIdx.x - tile_id * heads_splits;
-    const int split = rest / p.kv_heads, kv_head = rest - split * p.kv_heads;
+    // first parts first: the parts that short sequences do not have are spread over the XCDs
+    const int unit = blockIdx.x / p.kv_heads, kv_head = blockIdx.x - unit * p.kv_heads;
+    const int tiles = gridDim.x / (p.kv_heads * p.splits);
+    const int split = unit / tiles, tile_id = unit - split * tiles;
     KvTile t;
     if (!kv_find<ROWS>(p, tile_id, t)) return;
 
@@ -165,7 +163,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES, KD_PER_CU(DP, R, MX)) kv_decode
                         if (Group::active(l)) {
                             const int rr = 16 * h + Group::row(l, i);
                             *(u32x4*)(kt + rr * L::K_STRIDE + 16 * Group::piece(l)) = k[h].v[i];
-                            ksc[rr * (DP / 32) + Group::piece(l)] = (uint8_t)k[h].scale[i];
+                            ksc[rr * (DP / 32) + Group::piece(l)] = k[h].scale[i];
                         }
                 } else {
                     k[h].put((uint16_t*)kt + 16 * h * (L::K_STRIDE / 2), L::K_STRIDE / 2, l);
@@ -353,11 +351,11 @@ __global__ void __launch_bounds__(64 * KD_WAVES, KD_PER_CU(DP, R, MX)) kv_decode
     }
 }
 
-// The parts of a row joined: a workgroup per (query, head), 4 dims a thread,
-// the threads that are left over share the parts.
+// The parts of a row joined: blockIdx.x is the (query, head), blockIdx.y a span of
+// `cols` dims; 4 dims a thread, threads that are left over share the parts.
 constexpr int KJ_MAX = 1024;  // parts
 
-__global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p) {
+__global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) {
     __shared__ float weight[KJ_MAX];
     __shared__ __attribute__((aligned(16))) float add[256 * 4];
     __shared__ float red[4];
@@ -366,10 +364,17 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p) {
     const int token = (int)(at / heads), head = (int)(at - (int64_t)token * heads);
     // tokens that no sequence has are left as they are
     if (p.q_offsets && (token < s_load(p.q_offsets) || token >= s_load(p.q_offsets + p.batch))) return;
-    const float* ml = p.part_ml + 2 * at * p.splits;
+    const f32x2* ml = (const f32x2*)p.part_ml + at * p.splits;
     const int w = threadIdx.x >> 6;
     float top = -INFINITY;
-    for (int s = threadIdx.x; s < p.splits; s += 256) top = fmaxf(top, ml[2 * s]);
+    f32x2 mine[KJ_MAX / 256];
+#pragma unroll
+    for (int i = 0; i < KJ_MAX / 256; ++i) {
+        const int s = threadIdx.x + 256 * i;
+        mine[i] = s < p.splits ? ml[s] : f32x2{-INFINITY, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < KJ_MAX / 256; ++i) top = fmaxf(top, mine[i][0]);
     top = wave_max(top);
     if ((threadIdx.x & 63) == 0) red[w] = top;
     __syncthreads();
@@ -378,11 +383,11 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p) {
     const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
     top = fmaxf(top, sink);
     float total = 0.f;
-    for (int s = threadIdx.x; s < p.splits; s += 256) {
-        const float ms = ml[2 * s], ls = ml[2 * s + 1];
-        const float a = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - top);
-        total = fmaf(ls, a, total);
-        weight[s] = ls == 0.f ? -1.f : a;  // (no sums were left: not read)
+#pragma unroll
+    for (int i = 0; i < KJ_MAX / 256; ++i) {
+        const float a = mine[i][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine[i][0] - top);
+        total = fmaf(mine[i][1], a, total);
+        weight[threadIdx.x + 256 * i] = mine[i][1] == 0.f ? -1.f : a;  // (no sums were left: not read)
     }
     total = wave_sum(total);
     if ((threadIdx.x & 63) == 0) red[w] = total;
@@ -390,20 +395,22 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p) {
     total = (red[0] + red[1]) + (red[2] + red[3]);
     if (sink != -INFINITY) total += __builtin_amdgcn_exp2f(sink - top);
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (p.lse && threadIdx.x == 0)
+    if (p.lse && threadIdx.x == 0 && blockIdx.y == 0)
         p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
-    const int cols = p.dim / 4, shares = 256 / cols, share = threadIdx.x / cols, c = threadIdx.x - share * cols;
+    const int d0 = blockIdx.y * span, cols = min(span, p.dim - d0) / 4;
+    const int shares = 256 / cols, share = threadIdx.x / cols, c = threadIdx.x - share * cols;
     f32x4 x{};
     if (share < shares) {
-        const float* o = p.part_o + at * p.splits * p.dim + 4 * c;
+        const float* o = p.part_o + at * p.splits * p.dim + d0 + 4 * c;
+#pragma unroll 8
         for (int s = share; s < p.splits; s += shares)
-            if (weight[s] >= 0.f || weight[s] != weight[s]) x += weight[s] * *(const f32x4*)(o + (int64_t)s * p.dim);
+            if (!(weight[s] < 0.f)) x += weight[s] * *(const f32x4*)(o + (int64_t)s * p.dim);
     }
     *(f32x4*)(add + 4 * threadIdx.x) = x;
     __syncthreads();
     if (share) return;
     for (int s = 1; s < shares; ++s) x += *(const f32x4*)(add + 4 * (s * cols + c));
-    const int64_t to = token * p.out_ts + head * p.out_hs + 4 * c;
+    const int64_t to = token * p.out_ts + head * p.out_hs + d0 + 4 * c;
     if (p.out_f32)
         *(f32x4*)((float*)p.out + to) = x * inv;
     else
@@ -435,7 +442,20 @@ hipError_t decode_dim(const KvAttnParams& p, int rows, unsigned grid, hipStream_
 }  // namespace
 
 // `keys`: the most that a sequence has (an estimate is enough: a longer one's last
-// part takes what is left)
+// part takes what is left).  Parts of equal length, so that long sequences weigh no
+// more than their keys.  A workgroup costs about 4 us around its keys and 0.95 us per
+// 128 of them while HBM is not the bound, the join 3 to 5 us, more with many parts or
+// rows, so, measured at one query of 8 heads a key head (us):
+//   little work: one workgroup a CU, parts of 128 keys or more (4 key heads: 4000 keys
+//     in parts of 128 / 512 / whole 8.7 / 11.5 / 34.7; 32000 in 128 / 512 / 2048 17.8 /
+//     13.8 / 24.3), but no parts up to 512 keys (500 in 128 / whole 8.6 / 7.8)
+//   much: parts of 512 keys or more, four workgroups a CU (131072 keys, 8 key heads, in
+//     512 / 1024 / 2048 43 / 37 / 42), but of 1536 at most, since lengths differ (64
+//     sequences of 1000 to 12000, 4 key heads, in 1536 / 2048 / 3072 46 / 49 / 60)
+//   two workgroups a CU without parts: none (64 of 4000, 8 key heads, whole / in 2048
+//     55 / 64), unless sequences are long and may differ
+//   more rows a tile leave more sums: parts of 512 and 1024 keys at least for 32 and 64
+//     rows (4 x 8 queries over 8000 keys, 8 key heads, in 512 / 1024 40 / 32)
 KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_heads, int group, int dim, int window,
                                int64_t keys, int cu_count) {
     KvAttnRoute r;
@@ -444,15 +464,20 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     // tiles of as few rows as hold a sequence's
     r.rows = r.prompt ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     r.tiles = ragged ? (tokens * group + r.rows - 1) / r.rows + batch : int64_t(batch) * ((group + r.rows - 1) / r.rows);
-    const int64_t groups = r.tiles * kv_heads;  // workgroups without a split
+    const int64_t groups = batch * ((rows + r.rows - 1) / r.rows) * kv_heads;  // workgroups without parts
     // a tile's queries span at most its rows' positions
     if (window) keys = std::min<int64_t>(keys, (int64_t)window + r.rows + 16);
-    // parts of equal length, so that long sequences weigh no more than their keys: about
-    // eight workgroups a CU in all, at least 512 keys each
-    const int64_t target = int64_t(cu_count) * (r.prompt ? 4 : 8), least = 512;
-    int64_t chunk = (groups * std::max<int64_t>(keys, 1) + target - 1) / target;
-    chunk = std::max(least, (chunk + 63) / 64 * 64);
-    chunk = std::max(chunk, ((keys + KJ_MAX - 1) / KJ_MAX + 63) / 64 * 64);
+    const int64_t work = groups * std::max<int64_t>(keys, 1), cus = cu_count;
+    int64_t chunk;
+    if (r.prompt) {
+        chunk = std::max<int64_t>(512, work / (4 * cus));
+    } else {
+        chunk = std::max(std::min<int64_t>(work / cus, 512), work / (4 * cus));
+        chunk = std::min<int64_t>(std::max<int64_t>(chunk, r.rows == 16 ? 128 : 16 * r.rows), 1536);
+        if (keys <= 512 || (groups >= 2 * cus && keys <= 4096)) chunk = keys;
+    }
+    chunk = std::max(chunk, (keys + KJ_MAX - 1) / KJ_MAX);
+    chunk = std::max<int64_t>(64, (chunk + 63) / 64 * 64);
     r.splits = (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk);
     if (tokens * kv_heads * group > (1 << 20)) r.splits = 1;  // (the join has a workgroup per row)
     r.chunk = (int)std::min<int64_t>(chunk, INT32_MAX - 63);
@@ -471,7 +496,10 @@ hipError_t launch_kv_attention(const KvAttnParams& p, const KvAttnRoute& r, hipS
     else
         e = p.k_scales ? decode_dim<true>(p, r.rows, grid, st) : decode_dim<false>(p, r.rows, grid, st);
     if (e != hipSuccess || r.splits == 1) return e;
-    hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)((int64_t)p.tokens * p.kv_heads * p.group)), dim3(256), 0, st, p);
+    // few rows: 32 dims a workgroup, so that more of them read
+    const int64_t rows = (int64_t)p.tokens * p.kv_heads * p.group;
+    const int span = rows < 1024 ? 32 : p.dim;
+    hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)rows, (unsigned)((p.dim + span - 1) / span)), dim3(256), 0, st, p, span);
     return hipGetLastError();
 }
 

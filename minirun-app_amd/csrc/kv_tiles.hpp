@@ -132,7 +132,7 @@ struct KvGroup {
     static constexpr int RPL = 64 / LPR < 16 ? 64 / LPR : 16;  // rows of a load
     static constexpr int N = 16 / RPL;
     u32x4 v[N];
-    uint32_t scale[MX ? N : 1];
+    uint8_t scale[MX ? N : 1];  // (widened where it is used: sooner would wait for the load)
 
     __device__ __forceinline__ static int row(int l, int i) { return i * RPL + l / LPR; }
     __device__ __forceinline__ static int piece(int l) { return l % LPR; }
@@ -201,7 +201,7 @@ struct KvGroup {
         for (int i = 0; i < N; ++i) {
             if constexpr (MX) {
                 uint16_t* to = rows + row(l, i) * stride + 32 * piece(l);
-                const float s = __uint_as_float(scale[i] << 23);
+                const float s = __uint_as_float((uint32_t)scale[i] << 23);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const u32x4 x = __builtin_bit_cast(u32x4, mxfp4_bf16(v[i][k], s));

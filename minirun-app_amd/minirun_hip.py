@@ -1010,77 +1010,59 @@ def expert_dispatch_backward(d_rows, order: ExpertOrder, stream=None):
 
 
 # ------------------------------------------------------------------ attention heads and the paged cache
-def _heads3d(t, name, shape=None, dtype=None):
-    """Token and head strides of a GPU tensor [tokens, heads, dim] with contiguous heads."""
+# (Of a small call's 10 us most is Python, about 0.1 us a tensor's attribute and 0.4 a
+# nested call, so tensors are checked in one comparison each and structures filled at
+# once.)
+def _first_heads(t, name):
+    """Shape, device and type of a call's first tensor [tokens, heads, dim]."""
     if not isinstance(t, _torch().Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA (HIP) tensor")
-    if t.dim() != 3 or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name} must be {'[tokens, heads, dim]' if shape is None else list(shape)}, got {list(t.shape)}")
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, dim], got {list(shape)}")
+    return shape, t.device, t.dtype
+
+
+def _heads_like(t, name, shape, device, dtype):
+    """Token and head strides of a tensor of this shape (heads None: any), place and type."""
+    got = t.shape
+    if len(got) != 3 or got[0] != shape[0] or got[2] != shape[2] or (shape[1] is not None and got[1] != shape[1]):
+        raise ValueError(f"{name} must be {['any' if n is None else n for n in shape]}, got {list(got)}")
+    if t.dtype is not dtype or t.device != device:
+        raise TypeError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
     ts, hs, step = t.stride()
-    if step != 1 and t.shape[2] != 1:
+    if step != 1 and got[2] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
     return ts, hs
 
 
-def _vector(t, name, n, dtype=None):
-    _need_whole(t, name, dtype)
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name} must be [{n}], got {list(t.shape)}")
+def _vector(t, name, n, device, dtype):
+    """The address of a whole vector of n entries; None for None."""
+    if t is None:
+        return None
+    if t.shape != (n,) or t.dtype is not dtype or t.device != device or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a whole {dtype} [{n}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _type_code(t, name):
-    if t.dtype not in (_torch().bfloat16, _torch().float32):
-        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    return _dtype_code(t.dtype)
+def _code(dtype):
+    """An mr_dtype; the library refuses what has none."""
+    return _dtype_codes.get(dtype, 99) if _dtype_codes else (_dtype_code(_torch().float32), _code(dtype))[1]
 
 
-def _rotary(first, tokens, cos_t, sin_t, positions, col0, halves):
+def _rotary(device, tokens, cos_t, sin_t, positions, col0, halves):
     """The rotation of `tokens` tokens' heads; no tables: none."""
-    r = Rotary()
     if cos_t is None and sin_t is None:
-        return r
+        return Rotary()
     torch = _torch()
-    if cos_t is None or sin_t is None or cos_t.dim() != 2 or cos_t.shape != sin_t.shape:
-        raise ValueError("cos_t and sin_t must both be [rows, pairs]")
-    _need_whole(cos_t, "cos_t", torch.float32)
-    _need_whole(sin_t, "sin_t", torch.float32)
-    _same_device(first, cos_t, sin_t, positions)
-    r.cos_t, r.sin_t, r.table_rows, r.dim = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0], 2 * cos_t.shape[1]
-    r.col0, r.pairs = col0, 1 if halves else 0
-    if positions is not None:
-        r.positions = _vector(positions, "positions", tokens, torch.int32)
-    return r
-
-
-def _head_norm_args(q, k, q_weight, k_weight, eps, cos_t, sin_t, positions, col0, halves):
-    a = HeadNormArgs()
-    _heads3d(q, "q")
-    a.tokens, a.dim, a.eps = q.shape[0], q.shape[2], eps
-    a.x_dtype = _type_code(q, "q")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    a.weight_dtype = _type_code(weights[0], "a weight") if weights else F32
-    for t, w, rows, name in ((q, q_weight, a.q, "q"), (k, k_weight, a.k, "k")):
-        if t is None:
-            if w is not None:
-                raise ValueError("k_weight without k")
-            continue
-        _same_device(q, t, w)
-        rows.x_token_stride, rows.x_head_stride = _heads3d(t, name, (q.shape[0], t.shape[1] if t.dim() == 3 else 0, q.shape[2]),
-                                                           q.dtype)
-        rows.heads, rows.x = t.shape[1], t.data_ptr()
-        if w is not None:
-            rows.weight = _vector(w, f"{name}_weight", q.shape[2], weights[0].dtype)
-    a.rope = _rotary(q, q.shape[0], cos_t, sin_t, positions, col0, halves)
-    return a
-
-
-def _put_out(rows, out, name, like, dtype):
-    _same_device(like, out)
-    rows.out_token_stride, rows.out_head_stride = _heads3d(out, name, like.shape, dtype)
-    rows.out = out.data_ptr()
+    f32 = torch.float32
+    if (cos_t is None or sin_t is None or cos_t.dim() != 2 or cos_t.shape != sin_t.shape or cos_t.dtype is not f32
+            or sin_t.dtype is not f32 or cos_t.device != device or sin_t.device != device or not cos_t.is_contiguous()
+            or not sin_t.is_contiguous()):
+        raise ValueError(f"cos_t and sin_t must both be whole float32 [rows, pairs] on {device}")
+    rows, half = cos_t.shape
+    return Rotary(cos_t.data_ptr(), sin_t.data_ptr(), _vector(positions, "positions", tokens, device, torch.int32), rows,
+                  2 * half, col0, 1 if halves else 0)
 
 
 def head_norm_rope(q, k=None, *, q_weight=None, k_weight=None, eps=1e-6, cos_t=None, sin_t=None, positions=None, col0=0,
@@ -1093,16 +1075,28 @@ def head_norm_rope(q, k=None, *, q_weight=None, k_weight=None, eps=1e-6, cos_t=N
     i + n.  q_out, k_out: where to (q and k themselves, for one).  Records nothing
     for autograd: head_norm_rope_backward is the gradient."""
     torch = _torch()
-    a = _head_norm_args(q, k, q_weight, k_weight, eps, cos_t, sin_t, positions, col0, halves)
-    dtype = out_dtype or (q_out.dtype if q_out is not None else q.dtype)
-    handle, ctx = _call_stream(q.device, stream)
+    shape, device, dtype = _first_heads(q, "q")
+    T, H, D = shape
+    w = q_weight if q_weight is not None else k_weight
+    wtype = torch.float32 if w is None else w.dtype
+    otype = out_dtype or (dtype if q_out is None else q_out.dtype)
+    handle, ctx = _call_stream(device, stream)
     with ctx:
-        y = torch.empty(q.shape, dtype=dtype, device=q.device) if q_out is None else q_out
-        a.out_dtype = _type_code(y, "the output")
-        _put_out(a.q, y, "q_out", q, dtype)
-        if k is not None:
-            z = torch.empty(k.shape, dtype=dtype, device=q.device) if k_out is None else k_out
-            _put_out(a.k, z, "k_out", k, dtype)
+        y = torch.empty(shape, dtype=otype, device=device) if q_out is None else q_out
+        rows_q = HeadRows(H, q.data_ptr(), *_heads_like(q, "q", shape, device, dtype),
+                          _vector(q_weight, "q_weight", D, device, wtype), y.data_ptr(),
+                          *_heads_like(y, "q_out", shape, device, otype))
+        if k is None:
+            if k_weight is not None or k_out is not None:
+                raise ValueError("k_weight or k_out without k")
+            rows_k = HeadRows()
+        else:
+            strides = _heads_like(k, "k", (T, None, D), device, dtype)
+            z = torch.empty(k.shape, dtype=otype, device=device) if k_out is None else k_out
+            rows_k = HeadRows(k.shape[1], k.data_ptr(), *strides, _vector(k_weight, "k_weight", D, device, wtype),
+                              z.data_ptr(), *_heads_like(z, "k_out", k.shape, device, otype))
+        a = HeadNormArgs(T, D, rows_q, rows_k, _code(dtype), _code(wtype), _code(otype), eps,
+                         _rotary(device, T, cos_t, sin_t, positions, col0, halves))
         _check(load().mr_head_norm_rope(C.byref(a), handle))
     return y if k is None else (y, z)
 
@@ -1113,29 +1107,33 @@ def head_norm_rope_backward(d_q, q, d_k=None, k=None, *, q_weight=None, k_weight
     dtype): (dq, dk, d_q_weight, d_k_weight), the inputs' in their dtype, the
     weights' f32 [dim] or None without a weight; (dq, d_q_weight) without k."""
     torch = _torch()
-    if (d_k is None) != (k is None):
-        raise ValueError("d_k and k go together")
-    a = _head_norm_args(q, k, q_weight, k_weight, eps, cos_t, sin_t, positions, col0, halves)
-    a.out_dtype = a.x_dtype
+    if (d_k is None) != (k is None) or (k is None and k_weight is not None):
+        raise ValueError("d_k, k and k_weight go together")
+    shape, device, dtype = _first_heads(q, "q")
+    T, _, D = shape
+    w = q_weight if q_weight is not None else k_weight
+    wtype = torch.float32 if w is None else w.dtype
     lib = load()
-    handle, ctx = _call_stream(q.device, stream)
+    handle, ctx = _call_stream(device, stream)
     with ctx:
-        made = []
-        for t, d, w, rows, name in ((q, d_q, q_weight, a.q, "d_q"), (k, d_k, k_weight, a.k, "d_k")):
-            if t is None:
+        made, rows = [], []
+        for x, d, weight, name in ((q, d_q, q_weight, "q"), (k, d_k, k_weight, "k")):
+            if x is None:
+                rows.append(HeadRows())
                 continue
-            _same_device(q, d)
-            rows.d_out_token_stride, rows.d_out_head_stride = _heads3d(d, name, t.shape, q.dtype)
-            rows.d_out = d.data_ptr()
-            dx = torch.empty(t.shape, dtype=t.dtype, device=q.device)
-            dw = None if w is None else torch.empty(q.shape[2], dtype=torch.float32, device=q.device)
-            _put_out(rows, dx, name, t, t.dtype)
-            if w is not None:
-                rows.d_weight = dw.data_ptr()
+            strides = _heads_like(x, name, (T, None, D), device, dtype)
+            dx = torch.empty(x.shape, dtype=dtype, device=device)
+            dw = None if weight is None else torch.empty(D, dtype=torch.float32, device=device)
+            heads = x.shape[1]
+            rows.append(HeadRows(heads, x.data_ptr(), *strides, _vector(weight, f"{name}_weight", D, device, wtype),
+                                 dx.data_ptr(), heads * D, D, d.data_ptr(),
+                                 *_heads_like(d, f"d_{name}", x.shape, device, dtype), None if dw is None else dw.data_ptr()))
             made.append((dx, dw))
-        if q_weight is not None or k_weight is not None:
-            a.workspace_bytes = lib.mr_head_norm_rope_backward_workspace_size(C.byref(a))
-            ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=q.device)
+        a = HeadNormArgs(T, D, *rows, _code(dtype), _code(wtype), _code(dtype), eps,
+                         _rotary(device, T, cos_t, sin_t, positions, col0, halves))
+        if w is not None:
+            n = a.workspace_bytes = lib.mr_head_norm_rope_backward_workspace_size(C.byref(a))
+            ws = torch.empty(n, dtype=torch.uint8, device=device)
             a.workspace = ws.data_ptr()
         _check(lib.mr_head_norm_rope_backward(C.byref(a), handle))
     return made[0] if k is None else (made[0][0], made[1][0], made[0][1], made[1][1])
@@ -1159,6 +1157,7 @@ class KVCache:
             if t.dtype not in ((torch.int32, torch.uint32) if mx else (torch.bfloat16,)):
                 raise TypeError(f"{n} must be {'int32 or uint32 words' if mx else 'bfloat16'}, got {t.dtype}")
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.device = k.device
         self.pages, self.kv_heads, self.page_size, last = k.shape
         self.head_dim = 8 * last if mx else last
         d = self.desc = KVCacheDesc()
@@ -1200,12 +1199,16 @@ class KVCache:
         if self.k_scales is None:
             with _call_stream(self.k.device, stream)[1]:
                 return self.k.to(dtype, copy=True), self.v.to(dtype, copy=True)
-        rows = lambda t: t.contiguous().view(-1, t.shape[-1])
-        if not self.pages:
-            empty = lambda: torch.empty(*self.k.shape[:3], self.head_dim, dtype=dtype, device=self.k.device)
-            return empty(), empty()
-        return tuple(mxfp4_dequantize(MXFP4Weights(rows(w), rows(s)), dtype, stream).view(*w.shape[:3], self.head_dim)
-                     for w, s in ((self.k, self.k_scales), (self.v, self.v_scales)))
+        lib, device, n = load(), self.k.device, self.pages * self.kv_heads * self.page_size
+        handle, ctx = _call_stream(device, stream)
+        with ctx:
+            both = torch.empty(2, *self.k.shape[:3], self.head_dim, dtype=dtype, device=device)
+            for out, words, scales in zip(both, (self.k, self.v), (self.k_scales, self.v_scales)):
+                if not words.is_contiguous() or not scales.is_contiguous():
+                    words, scales = words.contiguous(), scales.contiguous()
+                d = MXFP4Desc(words.data_ptr(), scales.data_ptr(), n, self.head_dim)
+                _check(lib.mr_mxfp4_dequantize(C.byref(d), out.data_ptr(), _code(dtype), self.head_dim, handle))
+        return both[0], both[1]
 
 
 def kv_append(cache: KVCache, k, v, slots, *, normalize=False, norm_weight=None, eps=1e-6, cos_t=None, sin_t=None,
@@ -1216,24 +1219,22 @@ def kv_append(cache: KVCache, k, v, slots, *, normalize=False, norm_weight=None,
     and rotated (as head_norm_rope).  Values are rounded once, to what the cache
     holds.  No two tokens may name one slot."""
     torch = _torch()
-    a = KVAppendArgs()
-    a.cache = cache.desc
-    _heads3d(k, "k")
-    shape = (k.shape[0], cache.kv_heads, cache.head_dim)
-    a.k_token_stride, a.k_head_stride = _heads3d(k, "k", shape)
-    a.v_token_stride, a.v_head_stride = _heads3d(v, "v", shape, k.dtype)
-    _same_device(cache.k, k, v, slots, norm_weight)
-    a.tokens, a.k, a.v, a.dtype = k.shape[0], k.data_ptr(), v.data_ptr(), _type_code(k, "k")
-    a.slots = _vector(slots, "slots", k.shape[0], torch.int32)
-    a.eps = eps
-    if normalize:
-        a.normalize, a.norm_w_dtype = 1, F32
-        if norm_weight is not None:
-            a.norm_w, a.norm_w_dtype = _vector(norm_weight, "norm_weight", cache.head_dim), _type_code(norm_weight, "norm_weight")
-    elif norm_weight is not None:
-        raise ValueError("norm_weight needs normalize=True")
-    a.rope = _rotary(k, k.shape[0], cos_t, sin_t, positions, col0, halves)
-    handle, ctx = _call_stream(k.device, stream)
+    shape, device, dtype = _first_heads(k, "k")
+    if device != cache.device:
+        raise ValueError(f"k is on {device}, the cache on {cache.device}")
+    T = shape[0]
+    want = (T, cache.kv_heads, cache.head_dim)
+    wtype = torch.float32
+    if norm_weight is not None:
+        if not normalize:
+            raise ValueError("norm_weight needs normalize=True")
+        wtype = norm_weight.dtype
+    slots_at = _vector(slots, "slots", T, device, torch.int32)
+    a = KVAppendArgs(cache.desc, T, k.data_ptr(), v.data_ptr(), _code(dtype), *_heads_like(k, "k", want, device, dtype),
+                     *_heads_like(v, "v", want, device, dtype), slots_at, 1 if normalize else 0,
+                     _vector(norm_weight, "norm_weight", cache.head_dim, device, wtype), _code(wtype), eps,
+                     _rotary(device, T, cos_t, sin_t, positions, col0, halves))
+    handle, ctx = _call_stream(device, stream)
     with ctx:
         _check(load().mr_kv_append(C.byref(a), handle))
 
@@ -1249,38 +1250,34 @@ def kv_attention(q, cache: KVCache, page_table, kv_lens, *, scale, q_offsets=Non
     sequence are not written (give `out` to keep what they hold).  return_lse: also
     the log of the sum of exp, f32 [tokens, heads]."""
     torch = _torch()
-    a = KVAttentionArgs()
-    a.cache = cache.desc
-    a.q_token_stride, a.q_head_stride = _heads3d(q, "q", (q.shape[0], q.shape[1] if q.dim() == 3 else 0, cache.head_dim),
-                                                 torch.bfloat16)
-    _need(page_table, "page_table", torch.int32)
-    if page_table.dim() != 2:
-        raise ValueError(f"page_table must be [batch, max_pages], got {list(page_table.shape)}")
-    a.batch, a.max_pages = page_table.shape
-    a.tokens, a.heads, a.q, a.scale = q.shape[0], q.shape[1], q.data_ptr(), scale
-    _same_device(cache.k, q, page_table, kv_lens, q_offsets, sinks, out)
-    a.page_table, a.page_table_stride = page_table.data_ptr(), page_table.stride(0)
-    a.kv_lens = _vector(kv_lens, "kv_lens", a.batch, torch.int32)
-    if q_offsets is not None:
-        a.q_offsets = _vector(q_offsets, "q_offsets", a.batch + 1, torch.int32)
-    if sinks is not None:
-        a.sinks = _vector(sinks, "sinks", a.heads, torch.float32)
-    a.max_kv_len, a.window = max_kv_len, window
+    shape, device, dtype = _first_heads(q, "q")
+    if device != cache.device:
+        raise ValueError(f"q is on {device}, the cache on {cache.device}")
+    T, H, D = shape
+    i32 = torch.int32
+    if page_table.dim() != 2 or page_table.dtype is not i32 or page_table.device != device:
+        raise ValueError(f"page_table must be int32 [batch, max_pages] on {device}, got {page_table.dtype} "
+                         f"{list(page_table.shape)} on {page_table.device}")
+    B, most = page_table.shape
+    ld, step = page_table.stride()
+    if step != 1 and most > 1:
+        raise ValueError("page_table must be contiguous in its last dimension")
+    otype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
     lib = load()
-    handle, ctx = _call_stream(q.device, stream)
+    handle, ctx = _call_stream(device, stream)
     with ctx:
         if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or torch.bfloat16, device=q.device)
-        elif out_dtype is not None and out.dtype != out_dtype:
-            raise TypeError(f"out must be {out_dtype}, got {out.dtype}")
-        a.out_token_stride, a.out_head_stride = _heads3d(out, "out", q.shape)
-        a.out, a.out_dtype = out.data_ptr(), _type_code(out, "out")
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        if return_lse:
-            a.lse = lse.data_ptr()
+            out = torch.empty(shape, dtype=otype, device=device)
+        lse = torch.empty(T, H, dtype=torch.float32, device=device) if return_lse else None
+        a = KVAttentionArgs(cache.desc, B, T, H, q.data_ptr(),
+                            *_heads_like(q, "q", (T, H, cache.head_dim), device, torch.bfloat16), page_table.data_ptr(), ld,
+                            most, _vector(kv_lens, "kv_lens", B, device, i32),
+                            _vector(q_offsets, "q_offsets", B + 1, device, i32), max_kv_len, window, scale,
+                            _vector(sinks, "sinks", H, device, torch.float32), out.data_ptr(), _code(otype),
+                            *_heads_like(out, "out", shape, device, otype), None if lse is None else lse.data_ptr())
         n = lib.mr_kv_attention_workspace_size(C.byref(a))
         if n:
-            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            ws = torch.empty(n, dtype=torch.uint8, device=device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), n
         _check(lib.mr_kv_attention(C.byref(a), handle))
     return (out, lse) if return_lse else out

@@ -209,6 +209,39 @@ def test_strides_streams_and_graphs(M):
         assert torch.equal(got, want)
 
 
+def test_no_pages_and_no_keys(M):
+    import torch
+
+    q = torch.ones(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    lens = torch.tensor([5, 0, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    for mxfp4 in (False, True):
+        for pages, table in ((0, torch.zeros(3, 4, dtype=torch.int32, device="cuda")),
+                             (2, torch.zeros(3, 0, dtype=torch.int32, device="cuda")),
+                             (2, torch.full((3, 4), 2, dtype=torch.int32, device="cuda"))):
+            cache = M.KVCache.zeros(pages, 2, 16, 64, mxfp4=mxfp4)
+            for offsets in (None, torch.tensor([0, 1, 1, 3], dtype=torch.int32, device="cuda")):
+                out, lse = M.kv_attention(q, cache, table, lens, scale=1.0, q_offsets=offsets, return_lse=True)
+                assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_lengths_and_offsets_that_do_not_fit(M):
+    """A length past the table, or below zero; offsets that do not ascend or leave the tokens."""
+    import torch
+
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    cache = M.KVCache.zeros(4, 2, 16, 64)
+    cache.v.fill_(3)
+    q = torch.ones(6, 4, 64, device="cuda", dtype=torch.bfloat16)
+    table = i32([0, 1], [2, 3], [1, 2])
+    out, lse = M.kv_attention(q[:3], cache, table, i32(1000, -5, 32), scale=1.0, return_lse=True)
+    assert (out[0] == 3).all() and (out[1] == 0).all() and torch.allclose(lse[0], lse[2])
+    for bad in (i32(0, 5, 2, 6), i32(-1, 2, 4, 6), i32(0, 2, 4, 7), i32(2 ** 31 - 1, -2 ** 31, 0, 3)):
+        out = M.kv_attention(q, cache, table, i32(32, 32, 32), scale=1.0, q_offsets=bad, out=torch.full_like(q, 7))
+        assert ((out == 3) | (out == 7)).all()
+    out = M.kv_attention(q, cache, table, i32(32, 32, 32), scale=1.0, q_offsets=i32(0, 5, 2, 6), out=torch.full_like(q, 7))
+    assert (out[:5] == 3).all()
+
+
 def test_refusals(M):
     import torch
 
