@@ -7,31 +7,48 @@
 
 namespace mr {
 
-// Eight values of a row of n from column c as f32.  VEC: whole 16-byte loads
-// (c and n multiples of 8, the row aligned); else one by one, up to n.
+// Eight values of a row of n from column c, as stored: loaded first, widened where
+// they are used.  VEC: whole 16-byte loads (c and n multiples of 8, the row aligned);
+// else one by one, up to n.
+template <bool F32, bool VEC>
+struct HeadEight {
+    u32x4 raw[F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* base, int64_t at, int c, int n) {
+#pragma unroll
+        for (int k = 0; k < (F32 ? 2 : 1); ++k) raw[k] = u32x4{};
+        if constexpr (VEC) {
+            if (c < n) {
+                const u32x4* p = (const u32x4*)((const char*)base + (at + c) * (F32 ? 4 : 2));
+#pragma unroll
+                for (int k = 0; k < (F32 ? 2 : 1); ++k) raw[k] = p[k];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < n) {
+                    if constexpr (F32)
+                        raw[j >> 2][j & 3] = ((const uint32_t*)base)[at + c + j];
+                    else
+                        raw[0][j >> 1] |= (uint32_t)((const uint16_t*)base)[at + c + j] << (16 * (j & 1));
+                }
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (F32)
+                v[j] = __uint_as_float(raw[j >> 2][j & 3]);
+            else
+                v[j] = __uint_as_float(j & 1 ? raw[0][j >> 1] & 0xffff0000u : raw[0][j >> 1] << 16);
+        }
+    }
+};
+
 template <bool F32, bool VEC>
 __device__ __forceinline__ void head_load(const void* base, int64_t at, int c, int n, float (&v)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if constexpr (VEC) {
-        if (c < n) {
-            if constexpr (F32) {
-                const f32x4* p = (const f32x4*)((const float*)base + at + c);
-                const f32x4 a = p[0], b = p[1];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-            } else {
-                const u32x4 a = *(const u32x4*)((const uint16_t*)base + at + c);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(j & 1 ? a[j >> 1] & 0xffff0000u : a[j >> 1] << 16);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (c + j < n)
-                v[j] = F32 ? ((const float*)base)[at + c + j] : bf16_bits_to_f32(((const uint16_t*)base)[at + c + j]);
-    }
+    HeadEight<F32, VEC> e;
+    e.load(base, at, c, n);
+    e.values(v);
 }
 
 template <bool VEC>
@@ -66,6 +83,45 @@ __device__ __forceinline__ void head_store(void* base, int f32, int64_t at, int 
     }
 }
 
+// A row (token, head) of a tensor set and the offsets of its values, and the way to a
+// row `by` further: no division, and one 64-bit addition or two for each tensor.
+template <int N>
+struct HeadWalk {
+    struct Step {  // wave-uniform
+        uint32_t token, head, heads;
+        int64_t by[N], wrap[N];
+    };
+    uint32_t token, head;
+    int64_t at[N];
+
+    __device__ __forceinline__ static Step step(uint32_t by, uint32_t heads, const int64_t (&ts)[N], const int64_t (&hs)[N]) {
+        Step s;
+        s.token = by / heads;
+        s.head = by - s.token * heads;
+        s.heads = heads;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s.by[i] = s.token * ts[i] + s.head * hs[i];
+            s.wrap[i] = ts[i] - heads * hs[i];
+        }
+        return s;
+    }
+    __device__ __forceinline__ void start(uint32_t id, uint32_t heads, const int64_t (&ts)[N], const int64_t (&hs)[N]) {
+        token = id / heads;
+        head = id - token * heads;
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] = token * ts[i] + head * hs[i];
+    }
+    __device__ __forceinline__ void next(const Step& s) {
+        token += s.token;
+        head += s.head;
+        const bool wrap = head >= s.heads;
+        if (wrap) head -= s.heads, ++token;
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] += s.by[i] + (wrap ? s.wrap[i] : 0);
+    }
+};
+
 // This wave's LDS writes before its own LDS reads of other lanes' values (a
 // wave's LDS operations are done in order; the compiler has to keep them so).
 __device__ __forceinline__ void wave_lds_fence() {
@@ -81,66 +137,88 @@ __device__ __forceinline__ int64_t rope_row(const HeadRope& r, int64_t token) {
     return at >= 0 && at < r.rows ? at : -1;
 }
 
-// v (columns c .. c + 7 of a row) with columns [col0, col0 + 2 half) rotated by
-// the angles of table row `at` (INV: by the negated ones):
+// How far into the rotated columns a lane's eight are, as angles lie: KIND says how
+// the columns do.  ROPE_ADJACENT and ROPE_HALVES: col0 and half such that the eight
+// columns are four whole pairs, or all on one side with their partners in one other
+// lane, and table rows of whole 16-byte pieces; ROPE_ANY: anything.
+template <int KIND>
+struct HeadAngles {
+    static constexpr int N = KIND == ROPE_ADJACENT ? 4 : 8;
+    float co[N], si[N];
+    // table row `at` (rope_row), columns c .. c + 7
+    __device__ __forceinline__ void load(const HeadRope& r, int64_t at, int c) {
+        const int k = c - r.col0;
+        const int64_t table = max(at, (int64_t)0) * r.half;
+        if constexpr (KIND == ROPE_ANY) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int x = k + j;
+                if (x < 0 || x >= 2 * r.half) continue;
+                const int i = r.halves ? (x >= r.half ? x - r.half : x) : x >> 1;
+                co[j] = r.cos_t[table + i], si[j] = r.sin_t[table + i];
+            }
+        } else {
+            if (k < 0 || k >= 2 * r.half) return;
+            const int i = KIND == ROPE_ADJACENT ? k / 2 : (k >= r.half ? k - r.half : k);
+#pragma unroll
+            for (int x = 0; x < N; x += 4) {
+                const f32x4 a = *(const f32x4*)(r.cos_t + table + i + x), b = *(const f32x4*)(r.sin_t + table + i + x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) co[x + j] = a[j], si[x + j] = b[j];
+            }
+        }
+        if (at < 0) {  // the tables have no such row
+#pragma unroll
+            for (int j = 0; j < N; ++j) co[j] = si[j] = __builtin_nanf("");
+        }
+    }
+};
+
+// v (columns c .. c + 7 of a row) with columns [col0, col0 + 2 half) rotated (INV: by
+// the negated angles):
 //   (a, b) -> (a cos - b sin, a sin + b cos)
-// for adjacent pairs, or for column i and column i + half.  KIND: how the
-// columns lie.  ROPE_ADJACENT and ROPE_HALVES: col0 and half such that the
-// lane's eight columns are four whole pairs, or all on one side with their
-// partners in one other lane, and table rows of whole 16-byte pieces;
-// ROPE_ANY: anything.  `row` is the group's part of LDS (8 lpr values), which
-// ROPE_HALVES and ROPE_ANY use to hand partners over.  T: float rounds every
-// operation as written; double.
+// for adjacent pairs, or for column i and column i + half.  `row` is the group's part
+// of LDS (8 lpr values), through which ROPE_HALVES and ROPE_ANY hand partners over.
+// T: float rounds every operation as written; double.
 template <int KIND, bool INV, typename T>
-__device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, int64_t at, int c, T* row) {
+__device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, const HeadAngles<KIND>& g, int c, T* row) {
     if constexpr (KIND != ROPE_ADJACENT) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) row[c + j] = v[j];
         wave_lds_fence();
     }
-    const float nan = __builtin_nanf("");
     auto turn = [&](T a, T p, float co, float si, bool second) -> T {
-        const T cc = at < 0 ? nan : co, ss = at < 0 ? nan : (INV ? -si : si);
+        const T cc = co, ss = INV ? -si : si;
         if constexpr (sizeof(T) == 4)
             return second ? add_rn(mul_rn(p, ss), mul_rn(a, cc)) : sub_rn(mul_rn(a, cc), mul_rn(p, ss));
         else
             return second ? p * ss + a * cc : a * cc - p * ss;
     };
-    const int64_t table = max(at, (int64_t)0) * r.half;
+    const int k = c - r.col0;
     if constexpr (KIND == ROPE_ADJACENT) {
-        const int k = c - r.col0;
         if (k >= 0 && k < 2 * r.half) {
-            const f32x4 co = *(const f32x4*)(r.cos_t + table + k / 2), si = *(const f32x4*)(r.sin_t + table + k / 2);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const T a = v[2 * j], b = v[2 * j + 1];
-                v[2 * j] = turn(a, b, co[j], si[j], false);
-                v[2 * j + 1] = turn(b, a, co[j], si[j], true);
+                v[2 * j] = turn(a, b, g.co[j], g.si[j], false);
+                v[2 * j + 1] = turn(b, a, g.co[j], g.si[j], true);
             }
         }
     } else if constexpr (KIND == ROPE_HALVES) {
-        const int k = c - r.col0;
         if (k >= 0 && k < 2 * r.half) {
             const bool second = k >= r.half;
-            const int i = second ? k - r.half : k;
             const T* partner = row + (second ? c - r.half : c + r.half);
-            const f32x4 c0 = *(const f32x4*)(r.cos_t + table + i), c1 = *(const f32x4*)(r.cos_t + table + i + 4);
-            const f32x4 s0 = *(const f32x4*)(r.sin_t + table + i), s1 = *(const f32x4*)(r.sin_t + table + i + 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = turn(v[j], partner[j], c0[j], s0[j], second);
-                v[4 + j] = turn(v[4 + j], partner[4 + j], c1[j], s1[j], second);
-            }
+            for (int j = 0; j < 8; ++j) v[j] = turn(v[j], partner[j], g.co[j], g.si[j], second);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int k = c + j - r.col0;
-            if (k < 0 || k >= 2 * r.half) continue;
-            const bool second = r.halves ? k >= r.half : (k & 1);
-            const int i = r.halves ? (second ? k - r.half : k) : k >> 1;
+            const int x = k + j;
+            if (x < 0 || x >= 2 * r.half) continue;
+            const bool second = r.halves ? x >= r.half : (x & 1);
             const int d = r.halves ? r.half : 1;
-            v[j] = turn(v[j], row[second ? c + j - d : c + j + d], r.cos_t[table + i], r.sin_t[table + i], second);
+            v[j] = turn(v[j], row[second ? c + j - d : c + j + d], g.co[j], g.si[j], second);
         }
     }
     if constexpr (KIND != ROPE_ADJACENT) wave_lds_fence();  // the next row's values come after these reads

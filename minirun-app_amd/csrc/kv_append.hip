@@ -73,7 +73,11 @@ __global__ void __launch_bounds__(64 * KA_WAVES) kv_append_kernel(KvAppendParams
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = wt[j] * (y[j] * inv);
         }
-        if (p.rope.half) head_rotate<KIND, false>(y, p.rope, rope_row(p.rope, token), c, &sh[w][8 * (group << p.lpr_log2)]);
+        if (p.rope.half) {
+            HeadAngles<KIND> angles;
+            angles.load(p.rope, rope_row(p.rope, token), c);
+            head_rotate<KIND, false>(y, p.rope, angles, c, &sh[w][8 * (group << p.lpr_log2)]);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = to_odd(y[j]);
     }

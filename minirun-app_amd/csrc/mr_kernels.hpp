@@ -626,7 +626,7 @@ struct HeadNormParams {
     HeadSegment seg[2];
     int64_t tokens;
     int32_t dim, x_f32, w_f32, out_f32;
-    float eps;
+    float eps, inv_dim;  // (the latter set by the launcher)
     HeadRope rope;
     float* partial;    // backward: [blocks[0] + blocks[1]][dim]
     int32_t blocks[2];
