@@ -40,7 +40,8 @@ LIB_SOURCES = ["capi.cpp", "capi_adopt.cpp", "capi_block.cpp", "capi_prefill.cpp
 # (VGPR-form MFMA): with the AGPR form the compiler shuttles all 64 of them
 # through v_accvgpr moves on every 32-row step.  The same for attention over a
 # paged cache (few queries of 128 dims: 4 waves a CU more).
-EXTRA = {"decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+EXTRA = {"decode.hip": _VGPR_FORM, "kv_attention.hip": _VGPR_FORM, "kv_prompt.hip": _VGPR_FORM}
 SELFTEST_SOURCES = ["selftest.hip"]
 
 

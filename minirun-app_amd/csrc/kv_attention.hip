@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 have[h] = kv_page(p, id[h]);
-                kv_load<DP, MX>(p, kv_head, id[h], off[h], at, k[h], v[h]);
+                kv_load<DP, MX>(p, true, kv_head, id[h], off[h], at, k[h]);
+                kv_load<DP, MX>(p, false, kv_head, id[h], off[h], at, v[h]);
             }
         };
         look(wb);
@@ -142,13 +143,16 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
         for (int k0 = wb; k0 < we; k0 += KD_STEP) {
             const bool seen[2] = {have[0], have[1]};
             const bool all = k0 >= t.all_lo && k0 + KD_STEP <= min(t.all_hi, we) && seen[0] && seen[1];
-            bool apart = false;  // (wave-uniform)
             if (!all) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)  // (of a page that does not exist, all rows)
                     if (k0 + 16 * h + 16 > we || !seen[h]) v[h].cut(seen[h] ? we - k0 - 16 * h : 0, l);
-                apart = __builtin_amdgcn_ballot_w64(v[0].not_finite() || v[1].not_finite()) != 0;
-                if (apart) apart_to = k0 + KD_STEP, apart_from = min(apart_from, k0);
+                const bool apart = __builtin_amdgcn_ballot_w64(v[0].not_finite() || v[1].not_finite()) != 0;
+                if (apart) {
+                    apart_to = k0 + KD_STEP, apart_from = min(apart_from, k0);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) v[h].clean();
+                }
             }
             if (p.dim < DP) {
 #pragma unroll
@@ -191,13 +195,8 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             }
             kd_fence();
             // values to where the keys were
-            if (apart) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) v[h].template put<true>(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) v[h].put(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
-            }
+            for (int h = 0; h < 2; ++h) v[h].put(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
             if (k0 + KD_STEP < we) {
                 load();
                 look(k0 + 2 * KD_STEP);

@@ -4,14 +4,21 @@
 // A workgroup of four waves has 128 (query, head) rows of one sequence and key
 // head, heads of a query next to each other, so that a tile spans few positions
 // and all heads of a group share the keys.  Tiles of 64 keys come through two
-// LDS buffers as bf16 (MXFP4 values are converted once a workgroup): a tile's
-// rows are loaded into registers a whole tile ahead, 16 rows of one page a
-// wave, and written while the tile before is in use; one barrier a tile.
+// LDS buffers as bf16 (MXFP4 values are converted once a workgroup): rows are loaded
+// into registers a whole tile ahead of their way to LDS, 16 rows of one page a wave.
 //   S^T = K . Q^T and O^T = V^T . P^T on 32x32x16 MFMA: a lane owns one query,
 // whose maximum and sum stay in it but for one exchange between the halves of
 // the wave.
-// What bounds it: the products (4 dim flops a pair of query and key) with the
-// softmax on the vector units beside them.
+// What bounds it: the products (4 dim flops a pair of query and key) and, beside
+// them, the softmax and the conversions on the vector units, which take longer than
+// they do: 32 exp2 of 16 clocks, and about 150 instructions of 4, for 32 products of 32.
+// Two waves a SIMD alone ran them one after the other (2900 clocks a tile and wave), so
+// a wave's own products and vector instructions are interleaved: while the products of
+// the next tile's scores run, the scores of this one become probabilities, and while
+// its values are multiplied, the next scores' maximum is found and rows go to LDS.
+// So keys are a tile ahead of values, and one barrier ends a tile.
+#include <type_traits>
+
 #include "kv_tiles.hpp"
 
 namespace mr {
@@ -25,8 +32,9 @@ struct KvPromptLds {
     // rows read at one column (K) lie 16 bytes apart modulo all banks, the four rows
     // of a transposed read (V) 64 bytes
     static constexpr int K_STRIDE = DP + 8, V_STRIDE = DP + 32;
-    static constexpr int K_SIZE = KP_KEYS * K_STRIDE, V_SIZE = KP_KEYS * V_STRIDE, BUF = K_SIZE + V_SIZE;
-    static constexpr int BYTES = 2 * BUF * 2 + 64;
+    static constexpr int K_SIZE = KP_KEYS * K_STRIDE, V_SIZE = KP_KEYS * V_STRIDE;
+    static constexpr int V_AT = 2 * K_SIZE, FLAGS_AT = V_AT + 2 * V_SIZE;  // two buffers of each
+    static constexpr int BYTES = FLAGS_AT * 2 + 16;
     static_assert(KP_ROWS * DP * 2 <= BYTES, "the output's tile fits");
 };
 
@@ -37,14 +45,17 @@ __device__ __forceinline__ void kp_barrier() {
     lds_barrier();
 }
 
-// keys of tile index kb * 32 + 8 * (i / 4) + 4 * half + i % 4 are score i of block kb
+// score e of block b (32 keys) is key 32 b + 8 (e / 4) + 4 hh + e % 4 of its tile
 
 template <int DP, bool MX>
 __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAttnParams p) {
     using L = KvPromptLds<DP>;
     constexpr int KS = DP / 16, DB = DP / 32;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
-    int* flags = (int*)(lds + 2 * L::BUF);  // [2][4]: a wave's rows of the tile hold infinities or NaN
+    // a byte per wave and buffer: of the wave's 16 rows in it, that their page does not
+    // exist (keys), or that infinities or NaN were left out of them (values)
+    uint8_t* key_flags = (uint8_t*)(lds + L::FLAGS_AT);
+    uint8_t* value_flags = key_flags + 8;
     const int l = threadIdx.x & 63, lq = l & 31, hh = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads_splits = p.kv_heads * p.splits;
@@ -62,11 +73,10 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
     }
 
     const KvRow row = kv_row(p, t, kv_head, t.first_row + 32 * w + lq);
-    // keys that some, and that all of this wave's rows see
+    // keys that all of this wave's rows see
     const int w0 = t.first_row + 32 * w, i0 = min(w0 / p.group, t.qn - 1), i1 = min((w0 + 31) / p.group, t.qn - 1);
     const int pos0 = t.len - t.qn + i0, pos1 = t.len - t.qn + i1;
-    const int wave_hi = w0 < t.qn * p.group ? min(max(pos1 + 1, 0), ke) : 0, all_hi = max(pos0 + 1, 0);
-    const int wave_lo = p.window ? max(pos0 + 1 - p.window, 0) : 0, all_lo = p.window ? max(pos1 + 1 - p.window, 0) : 0;
+    const int all_hi = min(max(pos0 + 1, 0), ke), all_lo = p.window ? max(pos1 + 1 - p.window, 0) : 0;
 
     bf16x8 qf[KS];
     {
@@ -82,89 +92,99 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = f32x16{};
 
-    // wave w brings keys 16 w .. of each tile
-    const int steps = (max(ke - kb, 0) + KP_KEYS - 1) / KP_KEYS;
+    // wave w brings keys and values 16 w .. of each tile; tiles go by twos (a last one may
+    // have no keys), so that no branch divides the accumulators' way
+    const int steps = (max(ke - kb, 0) + 2 * KP_KEYS - 1) / (2 * KP_KEYS) * 2;
     using Group = KvGroup<DP, MX>;
     const typename Group::At at = Group::at(p.dim, l);
-    Group kreg, vreg;
+    struct Rows {  // 16 rows in registers: the first one's key, and whether their page exists
+        Group v;
+        int from;
+        bool have;
+    };
+    struct Source {
+        int from, id, offset;
+    };
+    Rows k, v;
     KvWalk walk;
     walk.start(p, t.b, steps ? kb + 16 * w : 0);
-    int id = -1, off = 0, ahead = kb + 16 * w;  // the next group to load, its page
-    auto look = [&]() {
-        off = walk.offset;
-        id = ahead < ke ? s_load(walk.entry) : -1;
+    int ahead = kb + 16 * w;
+    auto look = [&]() {  // where the next tile's rows are
+        const Source s = {ahead, ahead < ke ? s_load(walk.entry) : -1, walk.offset};
 #pragma unroll
         for (int i = 0; i < 4; ++i) walk.next(p.page_size);
-    };
-    bool have = false;
-    int from = 0;
-    auto load = [&]() {
-        from = ahead;
-        have = kv_page(p, id);
-        kv_load<DP, MX>(p, kv_head, id, off, at, kreg, vreg);
         ahead += KP_KEYS;
+        return s;
     };
-    // what was loaded goes to buffer `to`; flags say of the wave's 16 rows, in bit 0,
-    // that infinities or NaN among their values were left out (where not every row of the
-    // workgroup sees the tile), in bit 1 that their page does not exist
-    auto put = [&](int to) {
-        if (from + 16 > ke || !have) vreg.cut(have ? ke - from : 0, l);
-        if (p.dim < DP) kreg.narrow(at), vreg.narrow(at);
-        uint16_t* kt = lds + to * L::BUF;
-        const int k0 = from - 16 * w;
-        const bool apart = (k0 < t.all_lo || k0 + KP_KEYS > t.all_hi) && __builtin_amdgcn_ballot_w64(vreg.not_finite()) != 0;
-        kreg.put(kt + 16 * w * L::K_STRIDE, L::K_STRIDE, l);
-        if (apart)
-            vreg.template put<true>(kt + L::K_SIZE + 16 * w * L::V_STRIDE, L::V_STRIDE, l);
-        else
-            vreg.put(kt + L::K_SIZE + 16 * w * L::V_STRIDE, L::V_STRIDE, l);
-        if (l == 0) flags[4 * to + w] = (apart ? 1 : 0) | (have ? 0 : 2);
+    auto load = [&](bool keys, const Source& s, Rows& r) {
+        r.from = s.from;
+        r.have = kv_page(p, s.id);
+        kv_load<DP, MX>(p, keys, kv_head, s.id, s.offset, at, r.v);
     };
+    // what is left to do to loaded rows before they go to a buffer (rarely anything)
+    auto ready_keys = [&](int buffer) {
+        if (p.dim < DP) k.v.narrow(at);
+        if (l == 0) key_flags[4 * buffer + w] = k.have ? 0 : 1;
+    };
+    auto ready_values = [&](int buffer) {
+        if (v.from + 16 > ke || !v.have) v.v.cut(v.have ? ke - v.from : 0, l);
+        if (p.dim < DP) v.v.narrow(at);
+        const int k0 = v.from - 16 * w;
+        bool apart = false;  // where not every row of the workgroup sees the tile
+        if (k0 < t.all_lo || k0 + KP_KEYS > t.all_hi) {
+            apart = __builtin_amdgcn_ballot_w64(v.v.not_finite()) != 0;
+            if (apart) v.v.clean();
+        }
+        if (l == 0) value_flags[4 * buffer + w] = apart ? 1 : 0;
+    };
+    uint16_t* const k_mine = lds + 16 * w * L::K_STRIDE;
+    uint16_t* const v_mine = lds + L::V_AT + 16 * w * L::V_STRIDE;
 
+    // operands: keys 32 b + lq of a buffer, dims 16 x + 8 hh ..; values of 16 keys, four
+    // blocks (or all) of 32 dims
+    constexpr int VB = DB < 4 ? DB : 4, VN = 4 * (DB / VB);
     const int tr_key = 4 * hh + ((l & 15) >> 2), tr_d = 16 * ((l >> 4) & 1) + 4 * (l & 3);
-    // one tile for this wave's 32 rows; masked: not every row sees every key (a branch
-    // around the masking alone: two forms of the whole cost 40 spilled registers)
-    auto tile = [&](bool masked, const uint16_t* kt, int gone, int k0) {
-        const uint16_t* vt = kt + L::K_SIZE;
-        f32x16 s[2] = {f32x16{}, f32x16{}};
-        // operands come in two sets, so that one's reads overlap the other's products
-        // (the fences keep the scheduler from reading them all at once)
-        bf16x8 ka[2][4];
-        auto keys = [&](int x, bf16x8(&a)[4]) {
+    auto keys = [&](int buffer, int x, bf16x8(&a)[2]) {
+        const uint16_t* from = lds + buffer * L::K_SIZE + lq * L::K_STRIDE + 16 * x + 8 * hh;
+        a[0] = *(const bf16x8*)from;
+        a[1] = *(const bf16x8*)(from + 32 * L::K_STRIDE);
+    };
+    auto values = [&](int buffer, int x, bf16x8(&a)[VB]) {
+        const uint16_t* from = lds + L::V_AT + buffer * L::V_SIZE + (16 * (x & 3) + tr_key) * L::V_STRIDE +
+                               32 * VB * (x >> 2) + tr_d;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                a[e] = *(const bf16x8*)(kt + (32 * (e & 1) + lq) * L::K_STRIDE + 32 * x + 16 * (e >> 1) + 8 * hh);
-        };
-        keys(0, ka[0]);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int x = 0; x < KS / 2; ++x) {
-            if (x + 1 < KS / 2) keys(x + 1, ka[(x + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e & 1] = mfma32(ka[x & 1][e], qf[2 * x + (e >> 1)], s[e & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < VB; ++d) {
+            const bf16x4 lo = ds_read_tr16(from + 32 * d), hi = ds_read_tr16(from + 32 * d + 8 * L::V_STRIDE);
+            a[d] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
-        __builtin_amdgcn_s_setprio(0);
-        float mx = -INFINITY;
-        if (masked) {
-            const int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = 32 * b + 8 * (i >> 2) + (i & 3);  // + 4 hh
-                    if (at >= hi || at < lo || (gone >> (at >> 4) & 1)) s[b][i] = -INFINITY;
-                }
-        }
+    };
+    // scores that a row does not see become -inf; tile `i`, its keys in `buffer`
+    auto mask = [&](int i, int buffer, f32x16(&s)[2]) {
+        const int k0 = kb + KP_KEYS * i;
+        const uint32_t f = __builtin_amdgcn_readfirstlane(*(const int*)(key_flags + 4 * buffer));
+        if (!f && k0 >= all_lo && k0 + KP_KEYS <= all_hi) return;
+        const int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-        mx = xor32_max(mx) * p.scale_log2;  // (the scale is positive)
-        const bool raise = mx > m_run + KV_TAU;
+            for (int e = 0; e < 16; ++e) {
+                const int key = 32 * b + 8 * (e >> 2) + (e & 3);  // + 4 hh
+                if (key >= hi || key < lo || (f >> (8 * (key >> 4)) & 1)) s[b][e] = -INFINITY;
+            }
+    };
+
+    int apart_from = ke, apart_to = 0;  // keys whose infinite values were left out
+    float mx = -INFINITY;               // of the tile in turn, this lane's 32 scores
+    // Tile i: its scores are s, its values in buffer B, the next one's keys in B ^ 1.
+    // Leaves the next tile's scores in n and their maximum in mx, keys i + 2 and values
+    // i + 1 in LDS, keys i + 3 and values i + 2 under way.
+    Source next{}, after{};
+    auto tile = [&](auto buffer_tag, int i, f32x16(&s)[2], f32x16(&n)[2]) {
+        constexpr int B = decltype(buffer_tag)::value;
+        const float top = xor32_max(mx) * p.scale_log2;  // (the scale is positive)
+        const bool raise = top > m_run + KV_TAU;
         if (__builtin_amdgcn_ballot_w64(raise)) {
-            const float up = raise ? mx : m_run;
+            const float up = raise ? top : m_run;
             const float alpha = raise ? __builtin_amdgcn_exp2f(m_run - up) : 1.f;
             m_run = up;
             l_part *= alpha;
@@ -172,71 +192,92 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
             for (int d = 0; d < DB; ++d) o[d] *= alpha;
         }
         const float ref = m_run == -INFINITY ? 0.f : m_run;  // (no key yet: every score is -inf)
+        const uint32_t apart = __builtin_amdgcn_readfirstlane(*(const int*)(value_flags + 4 * B));
+        const int k0 = kb + KP_KEYS * i;
+        if (apart) apart_to = k0 + KP_KEYS, apart_from = min(apart_from, k0);
+
+        // (the fences keep each product's share of the other work beside it)
+        bf16x8 ka[2][2], pb[4];
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        n[0] = n[1] = f32x16{};
+        keys(B ^ 1, 0, ka[0]);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int x = 0; x < KS; ++x) {
+            if (x + 1 < KS) keys(B ^ 1, x + 1, ka[(x + 1) & 1]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.scale_log2, -ref));
-                s[b][i] = e;
-                ls[i & 3] += e;
+            for (int b = 0; b < 2; ++b) n[b] = mfma32(ka[x & 1][b], qf[x], n[b]);
+#pragma unroll
+            for (int e = 32 * x / KS; e < 32 * (x + 1) / KS; ++e) {
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], p.scale_log2, -ref));
+                ls[e & 3] += y;
+                pb[e >> 3][e & 7] = (__bf16)y;
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        __builtin_amdgcn_s_setprio(1);
-        // DB blocks of 32 dims of 16 keys, in two sets of at most four
-        constexpr int VB = DB < 4 ? DB : 4, VN = 4 * (DB / VB);
+        mask(i + 1, B ^ 1, n);
+        ready_keys(B);
+        ready_values(B ^ 1);
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         bf16x8 va[2][VB];
-        auto values = [&](int x, bf16x8(&a)[VB]) {
-            const uint16_t* at = vt + (16 * (x & 3) + tr_key) * L::V_STRIDE + 32 * VB * (x >> 2) + tr_d;
-#pragma unroll
-            for (int d = 0; d < VB; ++d) {
-                const bf16x4 u = ds_read_tr16(at + 32 * d), v = ds_read_tr16(at + 32 * d + 8 * L::V_STRIDE);
-                a[d] = bf16x8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-            }
-        };
-        values(0, va[0]);
+        values(B, 0, va[0]);
 #pragma unroll
         for (int x = 0; x < VN; ++x) {
-            if (x + 1 < VN) values(x + 1, va[(x + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-            bf16x8 pb;
+            if (x + 1 < VN) values(B, x + 1, va[(x + 1) & 1]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pb[e] = (__bf16)s[(x & 3) >> 1][8 * (x & 1) + e];
+            for (int d = 0; d < VB; ++d) o[VB * (x >> 2) + d] = mfma32(va[x & 1][d], pb[x & 3], o[VB * (x >> 2) + d]);
+            if (x < 4) {
+                k.v.put_part(k_mine + B * L::K_SIZE, L::K_STRIDE, l, x);
+                v.v.put_part(v_mine + (B ^ 1) * L::V_SIZE, L::V_STRIDE, l, x);
 #pragma unroll
-            for (int d = 0; d < VB; ++d) o[VB * (x >> 2) + d] = mfma32(va[x & 1][d], pb, o[VB * (x >> 2) + d]);
+                for (int e = 8 * x; e < 8 * x + 8; ++e) m4[e & 3] = fmaxf(m4[e & 3], n[e >> 4][e & 15]);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_s_setprio(0);
-    };
-
-    int apart_from = ke, apart_to = 0;  // keys whose infinite values were left out
-    if (steps > 0) {
-        look();
-        load();
-        look();
-        put(0);
-        if (steps > 1) {
-            load();
-            look();
+        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if (i + 2 < steps) load(false, next, v);
+        if (i + 3 < steps) {
+            next = after;
+            load(true, next, k);
+            after = look();
+        } else {
+            next = after;
         }
         kp_barrier();
-        for (int i = 0; i < steps; ++i) {
-            if (i + 1 < steps) put((i + 1) & 1);
-            if (i + 2 < steps) {
-                load();
-                look();
-            }
-            const int k0 = kb + KP_KEYS * i;
-            const uint16_t* kt = lds + (i & 1) * L::BUF;
-            if (k0 < wave_hi && k0 + KP_KEYS > wave_lo) {
-                // (four flags of two bits)
-                const u32x4 f = *(const u32x4*)(flags + 4 * (i & 1));
-                const int fl = __builtin_amdgcn_readfirstlane((int)(f[0] | f[1] << 2 | f[2] << 4 | f[3] << 6));
-                const int gone = (fl >> 1 & 1) | (fl >> 2 & 2) | (fl >> 3 & 4) | (fl >> 4 & 8);
-                tile(gone || k0 < all_lo || k0 + KP_KEYS > min(all_hi, ke), kt, gone, k0);
-                if (fl & 0x55) apart_to = k0 + KP_KEYS, apart_from = min(apart_from, k0);
-            }
-            kp_barrier();
+    };
+
+    if (steps > 0) {
+        Source first = look();
+        load(true, first, k);
+        load(false, first, v);
+        next = look();
+        ready_keys(0);
+        k.v.put(k_mine, L::K_STRIDE, l);
+        ready_values(0);
+        v.v.put(v_mine, L::V_STRIDE, l);
+        load(true, next, k);
+        ready_keys(1);
+        k.v.put(k_mine + L::K_SIZE, L::K_STRIDE, l);
+        load(false, next, v);
+        next = look();
+        load(true, next, k);
+        after = look();
+        kp_barrier();
+        f32x16 s[2] = {f32x16{}, f32x16{}}, n[2];
+        bf16x8 a[2];
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+            keys(0, x, a);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) s[b] = mfma32(a[b], qf[x], s[b]);
+        }
+        mask(0, 0, s);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+        kp_barrier();
+        for (int i = 0; i < steps; i += 2) {
+            tile(std::integral_constant<int, 0>{}, i, s, n);
+            tile(std::integral_constant<int, 1>{}, i + 1, n, s);
         }
     }
 

@@ -193,30 +193,46 @@ struct KvGroup {
         }
         return bad;
     }
-    // into bf16 rows of `stride` values; CLEAN: zeros for infinities and NaN
-    template <bool CLEAN = false>
-    __device__ __forceinline__ void put(uint16_t* rows, int stride, int l) const {
-        if (!active(l)) return;
+    // zeros for infinities and NaN (as bf16 values)
+    __device__ __forceinline__ void clean() {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if constexpr (MX) {
-                uint16_t* to = rows + row(l, i) * stride + 32 * piece(l);
-                const float s = __uint_as_float((uint32_t)scale[i] << 23);
+                // 2^126 and 2^127 leave the numbers below 4 and below 2 finite
+                const uint32_t e = scale[i];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const u32x4 x = __builtin_bit_cast(u32x4, mxfp4_bf16(v[i][k], s));
-                    *(u32x4*)(to + 8 * k) = CLEAN ? kv_finite(x) : x;
+                    const uint32_t w = v[i][k], two = w >> 2 & 0x11111111u, four = two & w >> 1;
+                    v[i][k] = e == 255 ? 0 : w & ~(15u * (e == 254 ? two : (e == 253 ? four : 0)));
                 }
+                if (e == 255) scale[i] = 0;
             } else {
-                *(u32x4*)(rows + row(l, i) * stride + 8 * piece(l)) = CLEAN ? kv_finite(v[i]) : v[i];
+                v[i] = kv_finite(v[i]);
             }
         }
+    }
+    // into bf16 rows of `stride` values; part: a quarter of it
+    __device__ __forceinline__ void put_part(uint16_t* rows, int stride, int l, int part) const {
+        if (!active(l)) return;
+        if constexpr (MX) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                *(bf16x8*)(rows + row(l, i) * stride + 32 * piece(l) + 8 * part) =
+                    mxfp4_bf16(v[i][part], __uint_as_float((uint32_t)scale[i] << 23));
+        } else {
+#pragma unroll
+            for (int i = part; i < N; i += 4) *(u32x4*)(rows + row(l, i) * stride + 8 * piece(l)) = v[i];
+        }
+    }
+    __device__ __forceinline__ void put(uint16_t* rows, int stride, int l) const {
+#pragma unroll
+        for (int part = 0; part < 4; ++part) put_part(rows, stride, l, part);
     }
 };
 
 // Where some rows of a tile see a key and others do not, 0 times an infinity or a NaN
 // of its value would reach the others through the product.  Such values are zeros in
-// LDS (KvGroup::put), and this adds at the end what they come to: to each dim of a row
+// LDS (KvGroup::clean), and this adds at the end what they come to: to each dim of a row
 // that sees the key, the infinity or NaN itself (again where the product had it, which
 // changes nothing).  add(j, v): to dims d0 + j (j < 4) of the lane's row.  `key` and
 // the sequence are wave-uniform, d0 is the lane's.
@@ -243,17 +259,16 @@ __device__ __forceinline__ void kv_add_infinite(const KvAttnParams& p, int b, in
 
 __device__ __forceinline__ bool kv_page(const KvAttnParams& p, int id) { return (uint32_t)id < (uint32_t)p.pages; }
 
-// Keys and values of the group at `offset` of page `id` (of page 0 where there is no
+// Keys, or values, of the group at `offset` of page `id` (of page 0 where there is no
 // such page: whoever loads it hides the keys and clears the values)
 template <int DP, bool MX>
-__device__ __forceinline__ void kv_load(const KvAttnParams& p, int kv_head, int id, int offset,
-                                        const typename KvGroup<DP, MX>::At& at, KvGroup<DP, MX>& k, KvGroup<DP, MX>& v) {
+__device__ __forceinline__ void kv_load(const KvAttnParams& p, bool keys, int kv_head, int id, int offset,
+                                        const typename KvGroup<DP, MX>::At& at, KvGroup<DP, MX>& group) {
     const int64_t page = kv_page(p, id) ? id : 0;
     const uint32_t row = (uint32_t)(kv_head * p.page_size + offset);  // (a page has at most 2^28 values)
     const int64_t bytes = page * p.page_bytes + row * (uint32_t)(MX ? p.dim / 2 : p.dim * 2);
     const int64_t sc = MX ? page * p.scale_bytes + row * (uint32_t)(p.dim / 32) : 0;
-    k.load(p.k + bytes, p.k_scales + sc, at);
-    v.load(p.v + bytes, p.v_scales + sc, at);
+    group.load((keys ? p.k : p.v) + bytes, (keys ? p.k_scales : p.v_scales) + sc, at);
 }
 
 }  // namespace mr
