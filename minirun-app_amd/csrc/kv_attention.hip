@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
     int apart_from = we, apart_to = 0;  // keys whose infinite values were left out
     if (wb < we) {
         KvWalk walk;
-        walk.start(p, t.b, wb);
+        walk.start(p, t.b, wb, 16);
         // the two groups of a step: their pages, a step ahead of their loads
         int id[2], off[2];
         auto look = [&](int key) {
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             for (int h = 0; h < 2; ++h) {
                 off[h] = walk.offset;
                 id[h] = key + 16 * h < we ? s_load(walk.entry) : -1;
-                walk.next(p.page_size);
+                walk.next();
             }
         };
         using Group = KvGroup<DP, MX>;
@@ -461,7 +461,7 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     const int64_t rows = ragged ? (tokens * group + batch - 1) / batch : group;  // of a sequence, on average
     r.prompt = rows > (dim > 128 ? 32 : 64);  // (64 rows of 256 dims do not fit the registers)
     // tiles of as few rows as hold a sequence's
-    r.rows = r.prompt ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    r.rows = r.prompt ? (dim > 128 ? 128 : 256) : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     r.tiles = ragged ? (tokens * group + r.rows - 1) / r.rows + batch : int64_t(batch) * ((group + r.rows - 1) / r.rows);
     const int64_t groups = batch * ((rows + r.rows - 1) / r.rows) * kv_heads;  // workgroups without parts
     // a tile's queries span at most its rows' positions
@@ -469,7 +469,7 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     const int64_t work = groups * std::max<int64_t>(keys, 1), cus = cu_count;
     int64_t chunk;
     if (r.prompt) {
-        chunk = std::max<int64_t>(512, work / (4 * cus));
+        chunk = std::max<int64_t>(512, work / (2 * cus));
     } else {
         chunk = std::max(std::min<int64_t>(work / cus, 512), work / (4 * cus));
         chunk = std::min<int64_t>(std::max<int64_t>(chunk, r.rows == 16 ? 128 : 16 * r.rows), 1536);

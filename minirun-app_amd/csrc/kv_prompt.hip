@@ -1,22 +1,25 @@
 // Attention of many queries of a sequence over a paged cache (kv_attention.hip
 // has the formula, the small form and what is shared).
 //
-// A workgroup of four waves has 128 (query, head) rows of one sequence and key
-// head, heads of a query next to each other, so that a tile spans few positions
-// and all heads of a group share the keys.  Tiles of 64 keys come through two
-// LDS buffers as bf16 (MXFP4 values are converted once a workgroup): rows are loaded
-// into registers a whole tile ahead of their way to LDS, 16 rows of one page a wave.
+// A workgroup of eight waves has 256 (query, head) rows of one sequence and key
+// head (four waves and 128 rows for heads of more than 128 dims, whose sums take
+// twice the registers), heads of a query next to each other, so that a tile spans few
+// positions and all heads of a group share the keys.  Tiles of 64 keys come through
+// two LDS buffers as bf16: rows are loaded into registers a whole tile ahead of their
+// way to LDS, 16 rows of keys or values of one page a wave.
 //   S^T = K . Q^T and O^T = V^T . P^T on 32x32x16 MFMA: a lane owns one query,
 // whose maximum and sum stay in it but for one exchange between the halves of
 // the wave.
 // What bounds it: the products (4 dim flops a pair of query and key) and, beside
-// them, the softmax and the conversions on the vector units, which take longer than
-// they do: 32 exp2 of 16 clocks, and about 150 instructions of 4, for 32 products of 32.
-// Two waves a SIMD alone ran them one after the other (2900 clocks a tile and wave), so
-// a wave's own products and vector instructions are interleaved: while the products of
-// the next tile's scores run, the scores of this one become probabilities, and while
-// its values are multiplied, the next scores' maximum is found and rows go to LDS.
-// So keys are a tile ahead of values, and one barrier ends a tile.
+// them, the softmax and the conversions on the vector units.  An exp2 and a conversion
+// of two MXFP4 values take 16 clocks of a wave's vector unit, other instructions 4: for
+// a wave's 32 products of 32 clocks a tile, 32 exp2, about 120 others and 16
+// conversions.  (With four waves a workgroup every wave has 32 of these: 44 of 230 us
+// of 4096 queries behind 1000 keys.)  Two waves a SIMD alone ran products and softmax
+// one after the other, so a wave's own are interleaved: while the products of the next
+// tile's scores run, the scores of this one become probabilities, and while its values
+// are multiplied, the next scores' maximum is found and rows go to LDS.  So keys are a
+// tile ahead of values, and one barrier ends a tile.
 #include <type_traits>
 
 #include "kv_tiles.hpp"
@@ -25,7 +28,8 @@ namespace mr {
 
 namespace {
 
-constexpr int KP_ROWS = 128, KP_KEYS = 64;
+constexpr int KP_KEYS = 64;
+constexpr int kp_waves(int dp) { return dp == 256 ? 4 : 8; }
 
 template <int DP>
 struct KvPromptLds {
@@ -35,7 +39,7 @@ struct KvPromptLds {
     static constexpr int K_SIZE = KP_KEYS * K_STRIDE, V_SIZE = KP_KEYS * V_STRIDE;
     static constexpr int V_AT = 2 * K_SIZE, FLAGS_AT = V_AT + 2 * V_SIZE;  // two buffers of each
     static constexpr int BYTES = FLAGS_AT * 2 + 16;
-    static_assert(KP_ROWS * DP * 2 <= BYTES, "the output's tile fits");
+    static_assert(32 * kp_waves(DP) * DP * 2 <= BYTES, "the output's tile fits");
 };
 
 // Every wave's LDS traffic is done; loads into registers stay in flight.  (The
@@ -48,14 +52,14 @@ __device__ __forceinline__ void kp_barrier() {
 // score e of block b (32 keys) is key 32 b + 8 (e / 4) + 4 hh + e % 4 of its tile
 
 template <int DP, bool MX>
-__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAttnParams p) {
+__global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt_kernel(KvAttnParams p) {
     using L = KvPromptLds<DP>;
-    constexpr int KS = DP / 16, DB = DP / 32;
+    constexpr int W = kp_waves(DP), KP_ROWS = 32 * W, KS = DP / 16, DB = DP / 32;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
-    // a byte per wave and buffer: of the wave's 16 rows in it, that their page does not
-    // exist (keys), or that infinities or NaN were left out of them (values)
-    uint8_t* key_flags = (uint8_t*)(lds + L::FLAGS_AT);
-    uint8_t* value_flags = key_flags + 8;
+    // a byte per 16 rows and buffer, of keys and of values: their page does not exist, or
+    // infinities or NaN were left out of them
+    uint8_t* const key_flags = (uint8_t*)(lds + L::FLAGS_AT);
+    uint8_t* const value_flags = key_flags + 8;
     const int l = threadIdx.x & 63, lq = l & 31, hh = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads_splits = p.kv_heads * p.splits;
@@ -92,53 +96,64 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = f32x16{};
 
-    // wave w brings keys and values 16 w .. of each tile; tiles go by twos (a last one may
-    // have no keys), so that no branch divides the accumulators' way
+    // Tiles go by twos (a last one may have no keys), so that no branch divides the
+    // accumulators' way.
     const int steps = (max(ke - kb, 0) + 2 * KP_KEYS - 1) / (2 * KP_KEYS) * 2;
+    // Wave w brings 16 keys, w % 4, of each tile: their keys or their values, or both in
+    // turn (TASKS).
+    constexpr int TASKS = 8 / W;
     using Group = KvGroup<DP, MX>;
     const typename Group::At at = Group::at(p.dim, l);
-    struct Rows {  // 16 rows in registers: the first one's key, and whether their page exists
+    const int part16 = w & 3;
+    struct Rows {
         Group v;
-        int from;
-        bool have;
+        int from;   // the first row's key
+        bool have;  // their page exists
+        KvWalk walk;
+        int ahead, id, offset;  // the next tile's, its page
     };
-    struct Source {
-        int from, id, offset;
+    Rows task[TASKS];
+    auto is_values = [&](int j) { return TASKS == 1 ? w >= 4 : j == 1; };  // (wave-uniform)
+    auto look = [&](Rows& r) {
+        r.id = r.ahead < ke ? s_load(r.walk.entry) : -1;
+        r.offset = r.walk.offset;
     };
-    Rows k, v;
-    KvWalk walk;
-    walk.start(p, t.b, steps ? kb + 16 * w : 0);
-    int ahead = kb + 16 * w;
-    auto look = [&]() {  // where the next tile's rows are
-        const Source s = {ahead, ahead < ke ? s_load(walk.entry) : -1, walk.offset};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) walk.next(p.page_size);
-        ahead += KP_KEYS;
-        return s;
-    };
-    auto load = [&](bool keys, const Source& s, Rows& r) {
-        r.from = s.from;
-        r.have = kv_page(p, s.id);
-        kv_load<DP, MX>(p, keys, kv_head, s.id, s.offset, at, r.v);
+    auto load = [&](int j) {  // the next tile's rows, and where those after it are
+        Rows& r = task[j];
+        r.from = r.ahead;
+        r.have = kv_page(p, r.id);
+        kv_load<DP, MX>(p, !is_values(j), kv_head, r.id, r.offset, at, r.v);
+        r.ahead += KP_KEYS;
+        r.walk.next();
+        look(r);
     };
     // what is left to do to loaded rows before they go to a buffer (rarely anything)
-    auto ready_keys = [&](int buffer) {
-        if (p.dim < DP) k.v.narrow(at);
-        if (l == 0) key_flags[4 * buffer + w] = k.have ? 0 : 1;
-    };
-    auto ready_values = [&](int buffer) {
-        if (v.from + 16 > ke || !v.have) v.v.cut(v.have ? ke - v.from : 0, l);
-        if (p.dim < DP) v.v.narrow(at);
-        const int k0 = v.from - 16 * w;
-        bool apart = false;  // where not every row of the workgroup sees the tile
-        if (k0 < t.all_lo || k0 + KP_KEYS > t.all_hi) {
-            apart = __builtin_amdgcn_ballot_w64(v.v.not_finite()) != 0;
-            if (apart) v.v.clean();
+    auto ready = [&](int j, int buffer) {
+        Rows& r = task[j];
+        if (p.dim < DP) r.v.narrow(at);
+        uint32_t flag = r.have ? 0 : 1;
+        if (is_values(j)) {
+            if (r.from + 16 > ke || !r.have) r.v.cut(r.have ? ke - r.from : 0, l);
+            const int k0 = r.from - 16 * part16;
+            flag = 0;
+            if (k0 < t.all_lo || k0 + KP_KEYS > t.all_hi) {  // not every row of the workgroup sees the tile
+                flag = __builtin_amdgcn_ballot_w64(r.v.not_finite()) != 0;
+                if (flag) r.v.clean();
+            }
         }
-        if (l == 0) value_flags[4 * buffer + w] = apart ? 1 : 0;
+        if (l == 0) (is_values(j) ? value_flags : key_flags)[4 * buffer + part16] = (uint8_t)flag;
     };
-    uint16_t* const k_mine = lds + 16 * w * L::K_STRIDE;
-    uint16_t* const v_mine = lds + L::V_AT + 16 * w * L::V_STRIDE;
+    // a quarter of them, or all, to the buffer
+    auto put = [&](int j, int buffer, int part) {
+        uint16_t* to = lds + (is_values(j) ? L::V_AT + buffer * L::V_SIZE + 16 * part16 * L::V_STRIDE
+                                           : buffer * L::K_SIZE + 16 * part16 * L::K_STRIDE);
+        task[j].v.put_part(to, is_values(j) ? L::V_STRIDE : L::K_STRIDE, l, part);
+    };
+    auto put_all = [&](int j, int buffer) {
+        ready(j, buffer);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) put(j, buffer, x);
+    };
 
     // operands: keys 32 b + lq of a buffer, dims 16 x + 8 hh ..; values of 16 keys, four
     // blocks (or all) of 32 dims
@@ -163,7 +178,8 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
         const int k0 = kb + KP_KEYS * i;
         const uint32_t f = __builtin_amdgcn_readfirstlane(*(const int*)(key_flags + 4 * buffer));
         if (!f && k0 >= all_lo && k0 + KP_KEYS <= all_hi) return;
-        const int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
+        int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
+        asm volatile("" : "+v"(hi), "+v"(lo));  // (behind the branch, not 64 compares a tile)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -178,7 +194,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
     // Tile i: its scores are s, its values in buffer B, the next one's keys in B ^ 1.
     // Leaves the next tile's scores in n and their maximum in mx, keys i + 2 and values
     // i + 1 in LDS, keys i + 3 and values i + 2 under way.
-    Source next{}, after{};
+    auto buffer_of = [&](int j, int B) { return is_values(j) ? B ^ 1 : B; };
+    auto load_next = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < TASKS; ++j)
+            if (i + (is_values(j) ? 2 : 3) < steps) load(j);
+    };
     auto tile = [&](auto buffer_tag, int i, f32x16(&s)[2], f32x16(&n)[2]) {
         constexpr int B = decltype(buffer_tag)::value;
         const float top = xor32_max(mx) * p.scale_log2;  // (the scale is positive)
@@ -197,87 +218,101 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(KvAtt
         if (apart) apart_to = k0 + KP_KEYS, apart_from = min(apart_from, k0);
 
         // (the fences keep each product's share of the other work beside it)
-        bf16x8 ka[2][2], pb[4];
+        bf16x8 ka[2][2];
+        u32x4 pb[4];  // probabilities as bf16: word e / 2 % 4 of the 16 keys e / 8
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
-        n[0] = n[1] = f32x16{};
         keys(B ^ 1, 0, ka[0]);
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
             if (x + 1 < KS) keys(B ^ 1, x + 1, ka[(x + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) n[b] = mfma32(ka[x & 1][b], qf[x], n[b]);
+            for (int b = 0; b < 2; ++b) n[b] = mfma32(ka[x & 1][b], qf[x], x ? n[b] : f32x16{});
 #pragma unroll
-            for (int e = 32 * x / KS; e < 32 * (x + 1) / KS; ++e) {
+            for (int e = 32 * x / KS; e < 32 * (x + 1) / KS; e += 2) {
                 const float y = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], p.scale_log2, -ref));
+                const float z = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][(e & 15) + 1], p.scale_log2, -ref));
                 ls[e & 3] += y;
-                pb[e >> 3][e & 7] = (__bf16)y;
+                ls[(e & 3) + 1] += z;
+                uint32_t two = pack_bf16x2_hw(y, z);
+                asm volatile("" : "+v"(two));  // (here, not where it is used)
+                pb[e >> 3][e >> 1 & 3] = two;
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         mask(i + 1, B ^ 1, n);
-        ready_keys(B);
-        ready_values(B ^ 1);
+#pragma unroll
+        for (int j = 0; j < TASKS; ++j) ready(j, buffer_of(j, B));
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         bf16x8 va[2][VB];
         values(B, 0, va[0]);
 #pragma unroll
         for (int x = 0; x < VN; ++x) {
             if (x + 1 < VN) values(B, x + 1, va[(x + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int d = 0; d < VB; ++d) o[VB * (x >> 2) + d] = mfma32(va[x & 1][d], pb[x & 3], o[VB * (x >> 2) + d]);
+            for (int d = 0; d < VB; ++d) o[VB * (x >> 2) + d] = mfma32(va[x & 1][d], __builtin_bit_cast(bf16x8, pb[x & 3]), o[VB * (x >> 2) + d]);
             if (x < 4) {
-                k.v.put_part(k_mine + B * L::K_SIZE, L::K_STRIDE, l, x);
-                v.v.put_part(v_mine + (B ^ 1) * L::V_SIZE, L::V_STRIDE, l, x);
+#pragma unroll
+                for (int j = 0; j < TASKS; ++j) put(j, buffer_of(j, B), x);
 #pragma unroll
                 for (int e = 8 * x; e < 8 * x + 8; ++e) m4[e & 3] = fmaxf(m4[e & 3], n[e >> 4][e & 15]);
+                asm volatile("" : "+v"(m4[0]), "+v"(m4[1]), "+v"(m4[2]), "+v"(m4[3]));
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        if (i + 2 < steps) load(false, next, v);
-        if (i + 3 < steps) {
-            next = after;
-            load(true, next, k);
-            after = look();
-        } else {
-            next = after;
-        }
+        load_next(i);
         kp_barrier();
     };
 
     if (steps > 0) {
-        Source first = look();
-        load(true, first, k);
-        load(false, first, v);
-        next = look();
-        ready_keys(0);
-        k.v.put(k_mine, L::K_STRIDE, l);
-        ready_values(0);
-        v.v.put(v_mine, L::V_STRIDE, l);
-        load(true, next, k);
-        ready_keys(1);
-        k.v.put(k_mine + L::K_SIZE, L::K_STRIDE, l);
-        load(false, next, v);
-        next = look();
-        load(true, next, k);
-        after = look();
-        kp_barrier();
-        f32x16 s[2] = {f32x16{}, f32x16{}}, n[2];
-        bf16x8 a[2];
+        // keys 0 and 1 and values 0 go to their buffers, keys 2 and values 1 are under way
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-            keys(0, x, a);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) s[b] = mfma32(a[b], qf[x], s[b]);
+        for (int j = 0; j < TASKS; ++j) {
+            Rows& r = task[j];
+            r.ahead = kb + 16 * part16;
+            r.walk.start(p, t.b, r.ahead, KP_KEYS);
+            look(r);
+            load(j);
         }
-        mask(0, 0, s);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+        for (int j = 0; j < TASKS; ++j) {
+            put_all(j, 0);
+            load(j);
+            if (!is_values(j)) {
+                put_all(j, 1);
+                load(j);
+            }
+        }
         kp_barrier();
-        for (int i = 0; i < steps; i += 2) {
-            tile(std::integral_constant<int, 0>{}, i, s, n);
-            tile(std::integral_constant<int, 1>{}, i + 1, n, s);
+        if (w0 >= t.qn * p.group) {
+            // a wave without rows of its own only brings the others' keys and values
+            kp_barrier();
+            for (int i = 0; i < steps; ++i) {
+#pragma unroll
+                for (int j = 0; j < TASKS; ++j) put_all(j, buffer_of(j, i & 1));
+                load_next(i);
+                kp_barrier();
+            }
+        } else {
+            f32x16 s[2] = {f32x16{}, f32x16{}}, n[2];
+            bf16x8 a[2];
+#pragma unroll
+            for (int x = 0; x < KS; ++x) {
+                keys(0, x, a);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) s[b] = mfma32(a[b], qf[x], s[b]);
+            }
+            mask(0, 0, s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+            kp_barrier();
+            for (int i = 0; i < steps; i += 2) {
+                tile(std::integral_constant<int, 0>{}, i, s, n);
+                tile(std::integral_constant<int, 1>{}, i + 1, n, s);
+            }
         }
     }
 
@@ -362,7 +397,7 @@ hipError_t prompt_launch(const KvAttnParams& p, unsigned grid, hipStream_t st) {
     constexpr int bytes = KvPromptLds<DP>::BYTES;
     const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((kv_prompt_kernel<DP, MX>), dim3(grid), dim3(256), bytes, st, p);
+    hipLaunchKernelGGL((kv_prompt_kernel<DP, MX>), dim3(grid), dim3(64 * kp_waves(DP)), bytes, st, p);
     return hipGetLastError();
 }
 

@@ -98,15 +98,20 @@ __device__ __forceinline__ KvRow kv_row(const KvAttnParams& p, const KvTile& t, 
 struct KvWalk {
     const int32_t* entry;  // of the page table
     int offset;            // of the group in its page
-    __device__ __forceinline__ void start(const KvAttnParams& p, int b, int key) {
+    int pages, rest, page_size;  // a step's whole pages and rows
+    __device__ __forceinline__ void start(const KvAttnParams& p, int b, int key, int step) {
         const int page = key / p.page_size;
         entry = p.table + b * p.table_stride + page;
         offset = key - page * p.page_size;
+        page_size = p.page_size;
+        pages = step / page_size;
+        rest = step - pages * page_size;
     }
-    __device__ __forceinline__ void next(int page_size) {
-        offset += 16;
-        if (offset == page_size) {
-            offset = 0;
+    __device__ __forceinline__ void next() {
+        entry += pages;
+        offset += rest;
+        if (offset >= page_size) {
+            offset -= page_size;
             ++entry;
         }
     }
