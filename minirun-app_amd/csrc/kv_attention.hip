@@ -133,8 +133,8 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 have[h] = kv_page(p, id[h]);
-                kv_load<DP, MX>(p, true, kv_head, id[h], off[h], at, k[h]);
-                kv_load<DP, MX>(p, false, kv_head, id[h], off[h], at, v[h]);
+                k[h].load(kv_from<MX>(p, true, kv_head, id[h], off[h]), at);
+                v[h].load(kv_from<MX>(p, false, kv_head, id[h], off[h]), at);
             }
         };
         look(wb);

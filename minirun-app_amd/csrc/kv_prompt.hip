@@ -110,22 +110,28 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
         int from;   // the first row's key
         bool have;  // their page exists
         KvWalk walk;
-        int ahead, id, offset;  // the next tile's, its page
+        int ahead, id;  // the next tile's first key, its page
+        KvFrom next;    // and where it is
+        bool next_have;
     };
     Rows task[TASKS];
     auto is_values = [&](int j) { return TASKS == 1 ? w >= 4 : j == 1; };  // (wave-uniform)
-    auto look = [&](Rows& r) {
-        r.id = r.ahead < ke ? s_load(r.walk.entry) : -1;
-        r.offset = r.walk.offset;
-    };
-    auto load = [&](int j) {  // the next tile's rows, and where those after it are
+    auto look = [&](Rows& r) { r.id = r.ahead < ke ? s_load(r.walk.entry) : -1; };
+    // the next tile's place, and a look at the one after it; then its rows.  (Tiles past
+    // the last read page 0.)
+    auto prepare = [&](int j) {
         Rows& r = task[j];
-        r.from = r.ahead;
-        r.have = kv_page(p, r.id);
-        kv_load<DP, MX>(p, !is_values(j), kv_head, r.id, r.offset, at, r.v);
+        r.next = kv_from<MX>(p, !is_values(j), kv_head, r.id, r.walk.offset);
+        r.next_have = kv_page(p, r.id);
         r.ahead += KP_KEYS;
         r.walk.next();
         look(r);
+    };
+    auto load = [&](int j) {
+        Rows& r = task[j];
+        r.from = r.ahead - KP_KEYS;
+        r.have = r.next_have;
+        r.v.load(r.next, at);
     };
     // what is left to do to loaded rows before they go to a buffer (rarely anything)
     auto ready = [&](int j, int buffer) {
@@ -173,10 +179,10 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             a[d] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
     };
-    // scores that a row does not see become -inf; tile `i`, its keys in `buffer`
-    auto mask = [&](int i, int buffer, f32x16(&s)[2]) {
+    // scores that a row does not see become -inf; tile `i`, its keys' flags
+    auto mask = [&](int i, int flags, f32x16(&s)[2]) {
         const int k0 = kb + KP_KEYS * i;
-        const uint32_t f = __builtin_amdgcn_readfirstlane(*(const int*)(key_flags + 4 * buffer));
+        const uint32_t f = __builtin_amdgcn_readfirstlane(flags);
         if (!f && k0 >= all_lo && k0 + KP_KEYS <= all_hi) return;
         int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
         asm volatile("" : "+v"(hi), "+v"(lo));  // (behind the branch, not 64 compares a tile)
@@ -195,11 +201,6 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
     // Leaves the next tile's scores in n and their maximum in mx, keys i + 2 and values
     // i + 1 in LDS, keys i + 3 and values i + 2 under way.
     auto buffer_of = [&](int j, int B) { return is_values(j) ? B ^ 1 : B; };
-    auto load_next = [&](int i) {
-#pragma unroll
-        for (int j = 0; j < TASKS; ++j)
-            if (i + (is_values(j) ? 2 : 3) < steps) load(j);
-    };
     auto tile = [&](auto buffer_tag, int i, f32x16(&s)[2], f32x16(&n)[2]) {
         constexpr int B = decltype(buffer_tag)::value;
         const float top = xor32_max(mx) * p.scale_log2;  // (the scale is positive)
@@ -213,9 +214,11 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             for (int d = 0; d < DB; ++d) o[d] *= alpha;
         }
         const float ref = m_run == -INFINITY ? 0.f : m_run;  // (no key yet: every score is -inf)
-        const uint32_t apart = __builtin_amdgcn_readfirstlane(*(const int*)(value_flags + 4 * B));
         const int k0 = kb + KP_KEYS * i;
-        if (apart) apart_to = k0 + KP_KEYS, apart_from = min(apart_from, k0);
+        if (k0 < t.all_lo || k0 + KP_KEYS > t.all_hi)  // (else no values were left out)
+            if (__builtin_amdgcn_readfirstlane(*(const int*)(value_flags + 4 * B)))
+                apart_to = k0 + KP_KEYS, apart_from = min(apart_from, k0);
+        const int flags = *(const int*)(key_flags + 4 * (B ^ 1));  // (used after the products)
 
         // (the fences keep each product's share of the other work beside it)
         bf16x8 ka[2][2];
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
             if (x + 1 < KS) keys(B ^ 1, x + 1, ka[(x + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+            if (x < TASKS) prepare(x);
 #pragma unroll
             for (int b = 0; b < 2; ++b) n[b] = mfma32(ka[x & 1][b], qf[x], x ? n[b] : f32x16{});
 #pragma unroll
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             __builtin_amdgcn_sched_barrier(0);
         }
         l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        mask(i + 1, B ^ 1, n);
+        mask(i + 1, flags, n);
 #pragma unroll
         for (int j = 0; j < TASKS; ++j) ready(j, buffer_of(j, B));
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -250,7 +253,6 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
 #pragma unroll
         for (int x = 0; x < VN; ++x) {
             if (x + 1 < VN) values(B, x + 1, va[(x + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < VB; ++d) o[VB * (x >> 2) + d] = mfma32(va[x & 1][d], __builtin_bit_cast(bf16x8, pb[x & 3]), o[VB * (x >> 2) + d]);
             if (x < 4) {
@@ -263,7 +265,8 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             __builtin_amdgcn_sched_barrier(0);
         }
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        load_next(i);
+#pragma unroll
+        for (int j = 0; j < TASKS; ++j) load(j);
         kp_barrier();
     };
 
@@ -275,14 +278,17 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             r.ahead = kb + 16 * part16;
             r.walk.start(p, t.b, r.ahead, KP_KEYS);
             look(r);
+            prepare(j);
             load(j);
         }
 #pragma unroll
         for (int j = 0; j < TASKS; ++j) {
             put_all(j, 0);
+            prepare(j);
             load(j);
             if (!is_values(j)) {
                 put_all(j, 1);
+                prepare(j);
                 load(j);
             }
         }
@@ -292,8 +298,11 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             kp_barrier();
             for (int i = 0; i < steps; ++i) {
 #pragma unroll
-                for (int j = 0; j < TASKS; ++j) put_all(j, buffer_of(j, i & 1));
-                load_next(i);
+                for (int j = 0; j < TASKS; ++j) {
+                    put_all(j, buffer_of(j, i & 1));
+                    prepare(j);
+                    load(j);
+                }
                 kp_barrier();
             }
         } else {
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
 #pragma unroll
                 for (int b = 0; b < 2; ++b) s[b] = mfma32(a[b], qf[x], s[b]);
             }
-            mask(0, 0, s);
+            mask(0, *(const int*)key_flags, s);
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
             kp_barrier();

@@ -117,6 +117,23 @@ struct KvWalk {
     }
 };
 
+__device__ __forceinline__ bool kv_page(const KvAttnParams& p, int id) { return (uint32_t)id < (uint32_t)p.pages; }
+
+// Where the group at `offset` of page `id` begins, its keys or its values (in page 0
+// where there is no such page: whoever loads it hides the keys and clears the values)
+struct KvFrom {
+    const char* rows;
+    const uint8_t* scales;
+};
+template <bool MX>
+__device__ __forceinline__ KvFrom kv_from(const KvAttnParams& p, bool keys, int kv_head, int id, int offset) {
+    const int64_t page = kv_page(p, id) ? id : 0;
+    const uint32_t row = (uint32_t)(kv_head * p.page_size + offset);  // (a page has at most 2^28 values)
+    const int64_t bytes = page * p.page_bytes + row * (uint32_t)(MX ? p.dim / 2 : p.dim * 2);
+    const int64_t sc = MX ? page * p.scale_bytes + row * (uint32_t)(p.dim / 32) : 0;
+    return KvFrom{(keys ? p.k : p.v) + bytes, (keys ? p.k_scales : p.v_scales) + sc};
+}
+
 // Pairs of bf16 with zeros for infinities and NaN
 __device__ __forceinline__ u32x4 kv_finite(u32x4 x) {
 #pragma unroll
@@ -158,13 +175,13 @@ struct KvGroup {
         a.scale_step = RPL * blocks;
         return a;
     }
-    // base, scales: the group's first row (wave-uniform)
-    __device__ __forceinline__ void load(const char* base, const uint8_t* scales, const At& a) {
+    // from: the group's first row (wave-uniform)
+    __device__ __forceinline__ void load(const KvFrom& from, const At& a) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = *(const u32x4*)(base + (a.bytes + i * a.step));
+        for (int i = 0; i < N; ++i) v[i] = *(const u32x4*)(from.rows + (a.bytes + i * a.step));
         if constexpr (MX) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) scale[i] = scales[a.scale + i * a.scale_step];
+            for (int i = 0; i < N; ++i) scale[i] = from.scales[a.scale + i * a.scale_step];
         }
     }
     __device__ __forceinline__ void clear(int i) {
@@ -260,20 +277,6 @@ __device__ __forceinline__ void kv_add_infinite(const KvAttnParams& p, int b, in
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if ((v[j] & 0x7f800000u) == 0x7f800000u) add(j, __uint_as_float(v[j]));
-}
-
-__device__ __forceinline__ bool kv_page(const KvAttnParams& p, int id) { return (uint32_t)id < (uint32_t)p.pages; }
-
-// Keys, or values, of the group at `offset` of page `id` (of page 0 where there is no
-// such page: whoever loads it hides the keys and clears the values)
-template <int DP, bool MX>
-__device__ __forceinline__ void kv_load(const KvAttnParams& p, bool keys, int kv_head, int id, int offset,
-                                        const typename KvGroup<DP, MX>::At& at, KvGroup<DP, MX>& group) {
-    const int64_t page = kv_page(p, id) ? id : 0;
-    const uint32_t row = (uint32_t)(kv_head * p.page_size + offset);  // (a page has at most 2^28 values)
-    const int64_t bytes = page * p.page_bytes + row * (uint32_t)(MX ? p.dim / 2 : p.dim * 2);
-    const int64_t sc = MX ? page * p.scale_bytes + row * (uint32_t)(p.dim / 32) : 0;
-    group.load((keys ? p.k : p.v) + bytes, (keys ? p.k_scales : p.v_scales) + sc, at);
 }
 
 }  // namespace mr
