@@ -133,7 +133,10 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
         r.have = r.next_have;
         r.v.load(r.next, at);
     };
-    // what is left to do to loaded rows before they go to a buffer (rarely anything)
+    // rows of values lie 64 bytes apart modulo all banks, as a lane's blocks do: four rows'
+    // lanes take other quarters of them (KvGroup::turn)
+    auto turned = [&](int j) { return is_values(j) ? Group::row(l, 0) & 3 : 0; };
+    // what is left to do to loaded rows before they go to a buffer (rarely more)
     auto ready = [&](int j, int buffer) {
         Rows& r = task[j];
         if (p.dim < DP) r.v.narrow(at);
@@ -148,12 +151,13 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             }
         }
         if (l == 0) (is_values(j) ? value_flags : key_flags)[4 * buffer + part16] = (uint8_t)flag;
+        r.v.turn(turned(j));
     };
     // a quarter of them, or all, to the buffer
     auto put = [&](int j, int buffer, int part) {
         uint16_t* to = lds + (is_values(j) ? L::V_AT + buffer * L::V_SIZE + 16 * part16 * L::V_STRIDE
                                            : buffer * L::K_SIZE + 16 * part16 * L::K_STRIDE);
-        task[j].v.put_part(to, is_values(j) ? L::V_STRIDE : L::K_STRIDE, l, part);
+        task[j].v.put_part(to, is_values(j) ? L::V_STRIDE : L::K_STRIDE, l, part, turned(j));
     };
     auto put_all = [&](int j, int buffer) {
         ready(j, buffer);

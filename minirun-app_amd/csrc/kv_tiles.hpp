@@ -233,13 +233,24 @@ struct KvGroup {
             }
         }
     }
-    // into bf16 rows of `stride` values; part: a quarter of it
-    __device__ __forceinline__ void put_part(uint16_t* rows, int stride, int l, int part) const {
+    // MXFP4: words k ^ turn in place of word k, so that lanes of neighbouring rows write
+    // other pieces of their blocks at a time
+    __device__ __forceinline__ void turn(int turn) {
+        if constexpr (MX) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const u32x4 a = v[i], b = turn & 1 ? u32x4{a[1], a[0], a[3], a[2]} : a;
+                v[i] = turn & 2 ? u32x4{b[2], b[3], b[0], b[1]} : b;
+            }
+        }
+    }
+    // into bf16 rows of `stride` values; part: a quarter of it; turned: by how much
+    __device__ __forceinline__ void put_part(uint16_t* rows, int stride, int l, int part, int turned = 0) const {
         if (!active(l)) return;
         if constexpr (MX) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                *(bf16x8*)(rows + row(l, i) * stride + 32 * piece(l) + 8 * part) =
+                *(bf16x8*)(rows + row(l, i) * stride + 32 * piece(l) + 8 * (part ^ turned)) =
                     mxfp4_bf16(v[i][part], __uint_as_float((uint32_t)scale[i] << 23));
         } else {
 #pragma unroll
