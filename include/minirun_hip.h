@@ -725,8 +725,8 @@ typedef struct mr_kv_cache {
 
 /* Each token's keys and values into row slots[t] % page_size of page slots[t] /
  * page_size, for every head; slots outside [0, pages * page_size) (padding) are
- * passed over, and no other row is touched.  Where two tokens name one slot, which
- * of them is written is not defined.  k, v [tokens][kv_heads][head_dim] bf16 or f32.
+ * passed over, and no other row is touched.  Where two tokens name one slot, what it
+ * holds is not defined.  k, v [tokens][kv_heads][head_dim] bf16 or f32.
  * Keys are normalised first where `normalize` is set (norm_w [head_dim], or NULL
  * for ones, and eps as in mr_head_norm_rope), then rotated.  What is stored is
  * rounded once from the exact value (computed in f64), MXFP4 by
@@ -758,8 +758,9 @@ mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
  * its position, or the last `window` of them (0: all).  A key that a query does not
  * see has no part in its output, whatever it holds.  A sink (f32 [heads], or NULL)
  * is one more score without a value.  A query that sees no key gets zeros.  Tokens
- * of no sequence are left as they were.  q_offsets ascends from 0 or more to at most
- * `tokens`; a sequence whose offsets do not is passed over.
+ * before the first sequence and behind the last are left as they were.  q_offsets
+ * ascends from 0 or more to at most `tokens`; where it does not, the outputs of all
+ * tokens are undefined.
  *   q bf16; MXFP4 keys and values as mr_mxfp4_dequantize gives them in bf16; scores,
  * softmax and sums in f32 but for the probabilities, which enter the second product as
  * bf16 (out in f32 has that error too); out is rounded once.
@@ -767,10 +768,11 @@ mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
  * (and sink); -inf where there is none.  With f32 out it joins parts of a context
  * attended elsewhere.
  *   q and out are 16-byte aligned, their strides multiples of 8.  heads a multiple of
- * cache.kv_heads; tokens * heads less than 2^31.  max_kv_len: about the most keys of
+ * cache.kv_heads; tokens * heads and max_pages * page_size at most 2^30.  max_kv_len: about the most keys of
  * a sequence (0: what a table row holds); it decides how the work is split, so it is
  * part of the workspace's size, and a longer sequence is right but slow.  Which kernel
- * runs, and so a result's last bits, depends on the sizes of the call alone. */
+ * runs, and so a result's last bits, depends on the sizes of the call alone: on the
+ * average of queries of a sequence, so prompts and single tokens run faster apart. */
 typedef struct mr_kv_attention_args {
     mr_kv_cache cache;
     int32_t batch, tokens, heads;

@@ -13,7 +13,8 @@ namespace {
 using mrc::fail;
 using mrc::hip_fail;
 
-constexpr int64_t FAR = int64_t(1) << 40;  // the longest stride, in elements
+constexpr int64_t FAR = int64_t(1) << 40;   // the longest stride, in elements
+constexpr int64_t MOST = int64_t(1) << 30;  // keys of a sequence, rows of queries: the kernels count past them in 32 bits
 
 bool act(mr_dtype d) { return d == MR_BF16 || d == MR_F32; }
 int size_of(mr_dtype d) { return d == MR_F32 ? 4 : 2; }
@@ -136,8 +137,7 @@ mr_status head_norm(const mr_head_norm_args* a, bool backward, void* stream) {
     return done(mr::launch_head_norm(p, backward, (hipStream_t)stream), backward ? "head norm backward launch" : "head norm launch");
 }
 
-// Sizes of a cache; bytes from page to page
-mr_status check_cache(const char* what, const mr_kv_cache& c, int64_t& page_bytes) {
+mr_status check_cache(const char* what, const mr_kv_cache& c) {
     if (c.pages < 0 || c.page_size <= 0 || c.page_size % 16 || c.kv_heads <= 0 || c.head_dim <= 0 || c.head_dim > 256 ||
         c.head_dim % 32)
         return fail(MR_INVALID_SHAPE,
@@ -147,13 +147,11 @@ mr_status check_cache(const char* what, const mr_kv_cache& c, int64_t& page_byte
         return fail(MR_INVALID_SHAPE, "%s: pages of more than 2^28 values, or 2^31 rows or more in all", what);
     const bool mx = c.k_scales || c.v_scales;
     const int64_t rows = int64_t(c.page_size) * c.kv_heads;
-    page_bytes = c.page_stride * (mx ? 4 : 2);
-    if (c.pages > 1 && (c.page_stride < rows * c.head_dim / (mx ? 8 : 1) || c.page_stride > FAR || page_bytes % 16 ||
+    if (c.pages > 1 && (c.page_stride < rows * c.head_dim / (mx ? 8 : 1) || c.page_stride > FAR || c.page_stride % (mx ? 4 : 8) ||
                         (mx && (c.scale_page_stride < rows * c.head_dim / 32 || c.scale_page_stride > FAR))))
         return fail(MR_INVALID_ARGUMENT, "%s: pages must be apart, by a multiple of 16 bytes", what);
     if (c.pages && (!c.k || !c.v || (mx && (!c.k_scales || !c.v_scales)) || !mrc::aligned16(c.k) || !mrc::aligned16(c.v)))
         return fail(MR_INVALID_ARGUMENT, "%s: NULL or misaligned cache (16 bytes)", what);
-    if (c.pages <= 1) page_bytes = 0;
     return MR_OK;
 }
 
@@ -161,15 +159,14 @@ mr_status check_cache(const char* what, const mr_kv_cache& c, int64_t& page_byte
 mr_status attention_route(const mr_kv_attention_args* a, mr::KvAttnRoute& r) {
     const char* what = "kv attention";
     const mr_kv_cache& c = a->cache;
-    int64_t page_bytes;
-    mr_status st = check_cache(what, c, page_bytes);
+    mr_status st = check_cache(what, c);
     if (st != MR_OK) return st;
-    if (a->batch < 0 || a->tokens < 0 || a->heads <= 0 || a->heads % c.kv_heads || int64_t(a->tokens) * a->heads > INT32_MAX)
+    if (a->batch < 0 || a->tokens < 0 || a->heads <= 0 || a->heads % c.kv_heads || int64_t(a->tokens) * a->heads > MOST)
         return fail(MR_INVALID_SHAPE, "%s: %d sequences, %d tokens of %d heads over %d key heads", what, a->batch, a->tokens,
                     a->heads, c.kv_heads);
     if (!a->q_offsets && a->tokens != a->batch)
         return fail(MR_INVALID_SHAPE, "%s: %d tokens of %d sequences need q_offsets", what, a->tokens, a->batch);
-    if (a->max_pages < 0 || int64_t(a->max_pages) * c.page_size > INT32_MAX || a->max_kv_len < 0 || a->window < 0)
+    if (a->max_pages < 0 || int64_t(a->max_pages) * c.page_size > MOST || a->max_kv_len < 0 || a->window < 0)
         return fail(MR_INVALID_SHAPE, "%s: %d pages a sequence, %d keys, window %d", what, a->max_pages, a->max_kv_len, a->window);
     const int64_t holds = int64_t(a->max_pages) * c.page_size;
     const int64_t keys = a->max_kv_len ? std::min<int64_t>(a->max_kv_len, holds) : holds;
@@ -204,8 +201,7 @@ mr_status mr_kv_append(const mr_kv_append_args* a, void* stream) {
     const char* what = "kv append";
     if (!a) return fail(MR_INVALID_ARGUMENT, "%s: args is NULL", what);
     const mr_kv_cache& c = a->cache;
-    int64_t page_bytes;
-    mr_status st = check_cache(what, c, page_bytes);
+    mr_status st = check_cache(what, c);
     if (st != MR_OK) return st;
     if (a->tokens < 0 || int64_t(a->tokens) * c.kv_heads > INT32_MAX / lanes_of(c.head_dim))
         return fail(MR_INVALID_SHAPE, "%s: %d tokens of %d heads are more than one launch takes", what, a->tokens, c.kv_heads);
@@ -245,8 +241,8 @@ mr_status mr_kv_append(const mr_kv_append_args* a, void* stream) {
     p.v_pages = c.v;
     p.k_scales = c.k_scales;
     p.v_scales = c.v_scales;
-    p.page_stride = c.page_stride;
-    p.scale_stride = c.scale_page_stride;
+    p.page_stride = c.pages > 1 ? c.page_stride : 0;
+    p.scale_stride = c.pages > 1 ? c.scale_page_stride : 0;
     return done(mr::launch_kv_append(p, (hipStream_t)stream), "kv append launch");
 }
 
@@ -292,8 +288,8 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     p.v = (const char*)c.v;
     p.k_scales = c.k_scales;
     p.v_scales = c.v_scales;
-    p.page_bytes = c.page_stride * (c.k_scales ? 4 : 2);
-    p.scale_bytes = c.scale_page_stride;
+    p.page_bytes = c.pages > 1 ? c.page_stride * (c.k_scales ? 4 : 2) : 0;
+    p.scale_bytes = c.pages > 1 ? c.scale_page_stride : 0;
     p.pages = c.pages;
     p.page_size = c.page_size;
     p.kv_heads = c.kv_heads;
@@ -306,7 +302,7 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     p.q_offsets = a->q_offsets;
     p.batch = a->batch;
     p.tokens = a->tokens;
-    p.window = a->window;
+    p.window = a->window < int64_t(a->max_pages) * c.page_size ? a->window : 0;  // (a longer one hides nothing)
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.sinks = a->sinks;
     p.out = a->out;

@@ -144,7 +144,7 @@ def attention(q, k, v, table, lens, offsets, scale, window=0, sinks=None):
     out, lse = np.full(q.shape, np.nan), np.full((T, H), np.nan)
     weight, terms = np.zeros(q.shape), np.zeros((T, H))
     for b, n in enumerate(lens):
-        q0, q1 = (b, b + 1) if offsets is None else (offsets[b], offsets[b + 1])
+        q0, q1 = (b, b + 1) if offsets is None else (int(offsets[b]), int(offsets[b + 1]))
         ids = table[b, :-(-n // ps)]
         there = np.repeat((ids >= 0) & (ids < pages), ps)[:n]
         rows = [np.moveaxis(a[np.clip(ids, 0, max(pages - 1, 0))], 1, 0).reshape(kvh, -1, D)[:, :n] for a in (k, v)]

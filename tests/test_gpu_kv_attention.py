@@ -54,8 +54,9 @@ def run(M, lens, queries=None, heads=8, kv_heads=2, dim=128, page=16, mxfp4=True
     score = (dim + 2) * K.MFMA * terms[..., None]
     tol = weight * (X.BF16_ROUND + 2 * score + (max(lens, default=0) + 8) * K.MFMA)
     tol = tol + (X.F32_ROUND if f32 else X.BF16_ROUND) * np.abs(want) + 1e-37
-    err = np.abs(got - want)
-    over = np.where(bad, 0, err - tol)
+    with np.errstate(invalid="ignore"):
+        err = np.abs(got - want)
+        over = np.where(bad | (got == want), 0, err - tol)  # (an infinity is met exactly)
     at = np.unravel_index(np.argmax(over), over.shape) if over.size else None
     assert (over <= 0).all(), (at, got[at], want[at], tol[at])
     empty = np.isneginf(lse64)
@@ -132,6 +133,39 @@ def test_splits_of_every_form(M, dim, mxfp4):
     run(M, [3000, 0, 700], heads=4, kv_heads=2, dim=dim, mxfp4=mxfp4, page=32, f32=True)
     run(M, [3000, 0, 700], [9, 2, 30], heads=16, kv_heads=2, dim=dim, mxfp4=mxfp4, page=32, window=1500)
     run(M, [3000, 0, 700], [50, 2, 120], heads=4, kv_heads=1, dim=dim, mxfp4=mxfp4, page=32, f32=dim == 128)
+
+
+# parts of many rows, which another kernel joins, some of them empty
+@pytest.mark.parametrize("dim,mxfp4", [(32, True), (96, False), (128, True), (256, True)])
+def test_joins_of_many_rows(M, dim, mxfp4):
+    run(M, [900, 0, 300], [200, 20, 60], dim=dim, mxfp4=mxfp4, sinks=True, first=1, behind=2)
+    run(M, [900], [300], dim=dim, mxfp4=mxfp4, window=100, f32=True)
+
+
+@pytest.mark.parametrize("queries", [None, [9, 3], [100, 130]])
+def test_windows_longer_than_any_sequence(M, queries):
+    for window in (2 ** 31 - 1, 128, 129):
+        run(M, [5, 100], queries, window=window)
+
+
+@pytest.mark.parametrize("queries", [None, [2, 7], [70, 20]])
+@pytest.mark.parametrize("mxfp4", [False, True])
+def test_infinite_and_nan_that_are_seen(M, mxfp4, queries):
+    """In keys: scores of either infinity, or NaN; in values: infinities of each dim's sign, or NaN."""
+    def poison(pages, table):
+        def put(x, scales, b, j, kv_head, bits):
+            page, row = table[b, j // 16], j % 16
+            if mxfp4:
+                scales[page, kv_head, row] = 255 if bits == 0x7FC0 else 254
+            else:
+                x[page, kv_head, row] = bits
+
+        put(pages.k, pages.ks, 0, 40, 0, 0x7F80)
+        put(pages.v, pages.vs, 0, 95, 1, 0xFF80)
+        put(pages.k, pages.ks, 1, 85, 0, 0x7FC0)
+        put(pages.v, pages.vs, 1, 70, 1, 0x7FC0)
+
+    run(M, [100, 90], queries, mxfp4=mxfp4, edit=poison)
 
 
 def test_one_key_is_its_value(M):

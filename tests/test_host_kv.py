@@ -164,6 +164,12 @@ def test_attention_refusals(lib):
     refused(call(**long, workspace=AT, workspace_bytes=need - 1), M.WORKSPACE_TOO_SMALL)
     refused(call(**long, workspace_bytes=need), M.INVALID_ARGUMENT, "workspace")
     refused(call(**long, workspace=AT + 4, workspace_bytes=need), M.INVALID_ARGUMENT, "workspace")
+    # counted in 32 bits, past the keys by a few tiles
+    most = dict(max_pages=2 ** 25, page_table_stride=2 ** 25, max_kv_len=100)
+    refused(call(**{**most, "max_pages": 2 ** 25 + 1}), M.INVALID_SHAPE, "pages")
+    refused(call(**most, out=None), M.INVALID_ARGUMENT)
+    refused(call(tokens=2 ** 27 + 1, q_offsets=AT), M.INVALID_SHAPE, "tokens")
+    refused(call(tokens=2 ** 27, q_offsets=AT, out=None), M.INVALID_ARGUMENT)
     # a hint or a window below the least part of a split: no workspace
     assert size(C.byref(attention_args(**long, max_kv_len=300))) == 0
     assert size(C.byref(attention_args(**long, window=300))) == 0
