@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 // The parts of a row joined: blockIdx.x is the (query, head), blockIdx.y a span of
 // `cols` dims; 4 dims a thread, threads that are left over share the parts.
 constexpr int KJ_MAX = 1024;  // parts
+constexpr int KJ_FEW = 32;
 
 __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) {
     __shared__ float weight[KJ_MAX];
@@ -417,6 +418,48 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
             u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
 }
 
+// The same for many rows of few parts: 2^lanes_log2 lanes have a row, 4 dims a lane, and
+// read its parts one after another (8192 rows of 8 parts of 128 dims, attention with its
+// join: 39 us, 50 with a workgroup a row; 1024 rows of 32 parts 47 and 43).
+__global__ void __launch_bounds__(256) kv_join_rows_kernel(KvAttnParams p, int lanes_log2) {
+    const int heads = p.kv_heads * p.group, c = 4 * (threadIdx.x & ((1 << lanes_log2) - 1));
+    const int64_t at = ((int64_t)blockIdx.x << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
+    if (at >= (int64_t)p.tokens * heads) return;
+    const int token = (int)(at / heads), head = (int)(at - (int64_t)token * heads);
+    // tokens that no sequence has are left as they are
+    if (p.q_offsets && (token < s_load(p.q_offsets) || token >= s_load(p.q_offsets + p.batch))) return;
+    const f32x2* ml = (const f32x2*)p.part_ml + at * p.splits;
+    float top = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
+    const float sink = top;
+    int first = p.splits, last = 0;  // the parts that left sums are among these
+    for (int s = 0; s < p.splits; ++s) {
+        const f32x2 x = ml[s];
+        top = fmaxf(top, x[0]);
+        if (x[1] != 0.f) first = min(first, s), last = s + 1;
+    }
+    float total = sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - top);
+    f32x4 x{};
+    const float* o = p.part_o + at * p.splits * p.dim + (c < p.dim ? c : 0);
+#pragma unroll 4
+    for (int s = first; s < last; ++s) {
+        const f32x2 y = ml[s];
+        const f32x4 v = *(const f32x4*)(o + (int64_t)s * p.dim);
+        const float a = y[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y[0] - top);
+        total = fmaf(y[1], a, total);
+        if (y[1] != 0.f) x += a * v;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (p.lse && c == 0)
+        p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    if (c >= p.dim) return;
+    const int64_t to = token * p.out_ts + head * p.out_hs + c;
+    if (p.out_f32)
+        *(f32x4*)((float*)p.out + to) = x * inv;
+    else
+        *(u32x2*)((uint16_t*)p.out + to) =
+            u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
+}
+
 template <int DP, bool MX>
 hipError_t decode_rows(const KvAttnParams& p, int rows, unsigned grid, hipStream_t st) {
     const dim3 block(64 * KD_WAVES);
@@ -444,22 +487,33 @@ hipError_t decode_dim(const KvAttnParams& p, int rows, unsigned grid, hipStream_
 // part takes what is left).  Parts of equal length, so that long sequences weigh no
 // more than their keys.  A workgroup costs about 4 us around its keys and 0.95 us per
 // 128 of them while HBM is not the bound, the join 3 to 5 us, more with many parts or
-// rows, so, measured at one query of 8 heads a key head (us):
-//   little work: one workgroup a CU, parts of 128 keys or more (4 key heads: 4000 keys
-//     in parts of 128 / 512 / whole 8.7 / 11.5 / 34.7; 32000 in 128 / 512 / 2048 17.8 /
-//     13.8 / 24.3), but no parts up to 512 keys (500 in 128 / whole 8.6 / 7.8)
-//   much: parts of 512 keys or more, four workgroups a CU (131072 keys, 8 key heads, in
-//     512 / 1024 / 2048 43 / 37 / 42), but of 1536 at most, since lengths differ (64
-//     sequences of 1000 to 12000, 4 key heads, in 1536 / 2048 / 3072 46 / 49 / 60)
-//   two workgroups a CU without parts: none (64 of 4000, 8 key heads, whole / in 2048
-//     55 / 64), unless sequences are long and may differ
-//   more rows a tile leave more sums: parts of 512 and 1024 keys at least for 32 and 64
-//     rows (4 x 8 queries over 8000 keys, 8 key heads, in 512 / 1024 40 / 32)
+// rows; measured with 8 heads a key head of 128 dims, MXFP4 (us):
+//   16 rows, little work: one workgroup a CU, parts of 128 keys or more (4 key heads: 4000
+//     keys in parts of 128 / 512 / whole 8.7 / 11.5 / 34.7; 32000 in 128 / 512 / 2048
+//     17.8 / 13.8 / 24.3)
+//   16 rows, much: parts of 512 keys or more, four workgroups a CU (131072 keys, 8 key
+//     heads, in 512 / 1024 / 2048 43 / 37 / 42), but of 1536 at most, since lengths differ
+//     (64 sequences of 1000 to 12000, 4 key heads, in 1024 / 1536 / 2048 49 / 45 / 48)
+//   32 and 64 rows leave more sums and fill a CU with two workgroups (24 rows, 32
+//     sequences of 1000 to 6000, in 512 / 1024 / 2048 38 / 32 / 36) or one (40 rows: 72 /
+//     57 / 48; 24 rows of 256 dims 77 / 64 / 52)
+//   no parts up to 512 keys (1 query of 500 in 128 / whole 8.6 / 7.8, 6 queries of 300
+//     14.5 / 13.4), nor for two workgroups a CU without them unless sequences are long and
+//     may differ (64 of 4000, 8 key heads, whole / in 2048 57 / 61; 8 queries of 64 x 3000
+//     113 / 137)
+//   prompts: one workgroup a CU, and sums of many rows are dear: parts where whole tiles
+//     leave half of the CUs idle (256 tiles, 100 queries of 16 x 600 keys, in 512 / whole
+//     68 / 33; 64 tiles, 512 queries behind 16000, in 1024 / 4096 / whole 185 / 144 / 411;
+//     4 tiles, 16 queries behind 2000, in 128 / 256 / 512 17.7 / 18.9 / 23.2), and few keys
+//     in one (16 queries of 250 in 128 / whole 16.1 / 12.1, of 400 16.7 / 17.2; 512 queries
+//     of 512, 64 tiles, 30 / 23)
+// A tile of the few-query kernel has at most 64 rows (32 of 256 dims: registers).  More
+// are prompts: 128 rows behind 16000 keys 27.8 us as such, 32.6 in tiles of 64.
 KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_heads, int group, int dim, int window,
                                int64_t keys, int cu_count) {
     KvAttnRoute r;
     const int64_t rows = ragged ? (tokens * group + batch - 1) / batch : group;  // of a sequence, on average
-    r.prompt = rows > (dim > 128 ? 32 : 64);  // (64 rows of 256 dims do not fit the registers)
+    r.prompt = rows > (dim > 128 ? 32 : 64);
     // tiles of as few rows as hold a sequence's
     r.rows = r.prompt ? (dim > 128 ? 128 : 256) : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     r.tiles = ragged ? (tokens * group + r.rows - 1) / r.rows + batch : int64_t(batch) * ((group + r.rows - 1) / r.rows);
@@ -469,10 +523,15 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     const int64_t work = groups * std::max<int64_t>(keys, 1), cus = cu_count;
     int64_t chunk;
     if (r.prompt) {
-        chunk = std::max<int64_t>(512, work / (2 * cus));
+        chunk = std::max<int64_t>(128, groups >= cus ? keys : (keys + cus / groups - 1) / (cus / groups));
+        if (keys <= 256 || (keys <= 512 && 8 * groups >= cus)) chunk = keys;
     } else {
-        chunk = std::max(std::min<int64_t>(work / cus, 512), work / (4 * cus));
-        chunk = std::min<int64_t>(std::max<int64_t>(chunk, r.rows == 16 ? 128 : 16 * r.rows), 1536);
+        const int fit = r.rows * dim > 32 * 128 ? 1 : 2;  // workgroups a CU
+        if (r.rows == 16)
+            chunk = std::max({std::min<int64_t>(work / cus, 512), work / (4 * cus), int64_t(128)});
+        else
+            chunk = std::max<int64_t>(256, work / (fit * cus));
+        chunk = std::min<int64_t>(chunk, r.rows > 16 && fit == 1 ? 2048 : 1536);
         if (keys <= 512 || (groups >= 2 * cus && keys <= 4096)) chunk = keys;
     }
     chunk = std::max(chunk, (keys + KJ_MAX - 1) / KJ_MAX);
@@ -495,8 +554,15 @@ hipError_t launch_kv_attention(const KvAttnParams& p, const KvAttnRoute& r, hipS
     else
         e = p.k_scales ? decode_dim<true>(p, r.rows, grid, st) : decode_dim<false>(p, r.rows, grid, st);
     if (e != hipSuccess || r.splits == 1) return e;
-    // few rows: 32 dims a workgroup, so that more of them read
     const int64_t rows = (int64_t)p.tokens * p.kv_heads * p.group;
+    if (r.splits <= KJ_FEW && rows >= 2048) {
+        int lanes_log2 = 3;
+        while ((4 << lanes_log2) < p.dim) ++lanes_log2;
+        const int64_t per = 256 >> lanes_log2;
+        hipLaunchKernelGGL(kv_join_rows_kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, p, lanes_log2);
+        return hipGetLastError();
+    }
+    // few rows: 32 dims a workgroup, so that more of them read
     const int span = rows < 1024 ? 32 : p.dim;
     hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)rows, (unsigned)((p.dim + span - 1) / span)), dim3(256), 0, st, p, span);
     return hipGetLastError();
