@@ -712,8 +712,8 @@ mr_status mr_head_norm_rope_backward(const mr_head_norm_args *args, void *stream
  * or (k_scales and v_scales given) MXFP4: uint32 words
  * [pages][kv_heads][page_size][head_dim / 8] and E8M0 bytes
  * [pages][kv_heads][page_size][head_dim / 32].  No gaps inside a page; pages lie
- * page_stride elements (words) and scale_page_stride bytes apart, the same for k
- * and v.  head_dim is a multiple of 32 up to 256; page_size * kv_heads * head_dim
+ * page_stride elements (words) and scale_page_stride bytes apart, less than 2^32
+ * bytes, the same for k and v.  head_dim is a multiple of 32 up to 256; page_size * kv_heads * head_dim
  * at most 2^28; pages * page_size less than 2^31; k and v 16-byte aligned, page_stride
  * a multiple of 16 bytes. */
 typedef struct mr_kv_cache {

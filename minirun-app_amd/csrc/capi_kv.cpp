@@ -14,6 +14,7 @@ using mrc::fail;
 using mrc::hip_fail;
 
 constexpr int64_t FAR = int64_t(1) << 40;   // the longest stride, in elements
+constexpr int64_t PITCH = int64_t(1) << 32;  // a cache's pages lie nearer, in bytes
 constexpr int64_t MOST = int64_t(1) << 30;  // keys of a sequence, rows of queries: the kernels count past them in 32 bits
 
 bool act(mr_dtype d) { return d == MR_BF16 || d == MR_F32; }
@@ -147,9 +148,10 @@ mr_status check_cache(const char* what, const mr_kv_cache& c) {
         return fail(MR_INVALID_SHAPE, "%s: pages of more than 2^28 values, or 2^31 rows or more in all", what);
     const bool mx = c.k_scales || c.v_scales;
     const int64_t rows = int64_t(c.page_size) * c.kv_heads;
-    if (c.pages > 1 && (c.page_stride < rows * c.head_dim / (mx ? 8 : 1) || c.page_stride > FAR || c.page_stride % (mx ? 4 : 8) ||
-                        (mx && (c.scale_page_stride < rows * c.head_dim / 32 || c.scale_page_stride > FAR))))
-        return fail(MR_INVALID_ARGUMENT, "%s: pages must be apart, by a multiple of 16 bytes", what);
+    if (c.pages > 1 && (c.page_stride < rows * c.head_dim / (mx ? 8 : 1) || c.page_stride >= (mx ? PITCH / 4 : PITCH / 2) ||
+                        c.page_stride % (mx ? 4 : 8) ||
+                        (mx && (c.scale_page_stride < rows * c.head_dim / 32 || c.scale_page_stride >= PITCH))))
+        return fail(MR_INVALID_ARGUMENT, "%s: pages must be apart, by a multiple of 16 bytes below 2^32", what);
     if (c.pages && (!c.k || !c.v || (mx && (!c.k_scales || !c.v_scales)) || !mrc::aligned16(c.k) || !mrc::aligned16(c.v)))
         return fail(MR_INVALID_ARGUMENT, "%s: NULL or misaligned cache (16 bytes)", what);
     return MR_OK;
@@ -288,8 +290,8 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     p.v = (const char*)c.v;
     p.k_scales = c.k_scales;
     p.v_scales = c.v_scales;
-    p.page_bytes = c.pages > 1 ? c.page_stride * (c.k_scales ? 4 : 2) : 0;
-    p.scale_bytes = c.pages > 1 ? c.scale_page_stride : 0;
+    p.page_bytes = c.pages > 1 ? (uint32_t)(c.page_stride * (c.k_scales ? 4 : 2)) : 0;
+    p.scale_bytes = c.pages > 1 ? (uint32_t)c.scale_page_stride : 0;
     p.pages = c.pages;
     p.page_size = c.page_size;
     p.kv_heads = c.kv_heads;

@@ -113,22 +113,28 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 
     int apart_from = we, apart_to = 0;  // keys whose infinite values were left out
     if (wb < we) {
-        KvWalk walk;
-        walk.start(p, t.b, wb, 16);
-        // the two groups of a step: their pages, a step ahead of their loads
+        // the two groups of a step: their pages, a step ahead of their loads (past the last
+        // key again its page, whose rows are cut and masked)
+        const char* table = (const char*)(p.table + t.b * p.table_stride);
+        const uint32_t last = 4u * ((uint32_t)(we - 1) / (uint32_t)p.page_size);
+        uint32_t entry = 4u * ((uint32_t)wb / (uint32_t)p.page_size);  // bytes
+        int offset = wb - (int)(entry / 4) * p.page_size;
         int id[2], off[2];
-        auto look = [&](int key) {
+        auto look = [&]() {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                off[h] = walk.offset;
-                id[h] = key + 16 * h < we ? s_load(walk.entry) : -1;
-                walk.next();
+                off[h] = offset;
+                id[h] = s_load((const int32_t*)(table + min(entry, last)));
+                offset += 16;
+                const int same = (offset - p.page_size) >> 31;  // -1, or 0 at a page's end
+                offset &= same;
+                entry += 4 + 4 * same;
             }
         };
         using Group = KvGroup<DP, MX>;
         const typename Group::At at = Group::at(p.dim, l);
         Group k[2], v[2];
-        bool have[2];
+        int have[2];
         auto load = [&]() {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -137,12 +143,12 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
                 v[h].load(kv_from<MX>(p, false, kv_head, id[h], off[h]), at);
             }
         };
-        look(wb);
+        look();
         load();
-        look(wb + KD_STEP);
+        look();
         for (int k0 = wb; k0 < we; k0 += KD_STEP) {
-            const bool seen[2] = {have[0], have[1]};
-            const bool all = k0 >= t.all_lo && k0 + KD_STEP <= min(t.all_hi, we) && seen[0] && seen[1];
+            const int seen[2] = {have[0], have[1]};
+            const bool all = k0 >= t.all_lo && k0 + KD_STEP <= min(t.all_hi, we) && (seen[0] & seen[1]);
             if (!all) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)  // (of a page that does not exist, all rows)
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             for (int h = 0; h < 2; ++h) v[h].put(vt + 16 * h * L::V_STRIDE, L::V_STRIDE, l);
             if (k0 + KD_STEP < we) {
                 load();
-                look(k0 + 2 * KD_STEP);
+                look();
             }
 
             f32x4 s[2][R];
@@ -222,18 +228,21 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             bf16x8 pb[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                if (!all) {
+                    int lo = row[r].lo - k0 - 4 * g, hi = min(row[r].hi, we) - k0 - 4 * g;
+                    asm volatile("" : "+v"(lo), "+v"(hi));  // (behind the branch)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)  // key 4 g + this of the step
+                            if (16 * h + i < lo || 16 * h + i >= hi || !seen[h]) s[h][r][i] = -INFINITY;
+                }
                 float mx = -INFINITY;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = k0 + 16 * h + 4 * g + i;
-                        float x = s[h][r][i] * p.scale_log2;
-                        if (!all && !(key >= row[r].lo && key < min(row[r].hi, we) && seen[h])) x = -INFINITY;
-                        s[h][r][i] = x;
-                        mx = fmaxf(mx, x);
-                    }
-                mx = xor32_max(xor16_max(mx));
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[h][r][i]);
+                mx = xor32_max(xor16_max(mx)) * p.scale_log2;  // (the scale is positive)
                 const bool raise = mx > m[r] + KV_TAU;
                 if (__builtin_amdgcn_ballot_w64(raise)) {
                     const float up = raise ? mx : m[r];
@@ -248,7 +257,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(s[h][r][i] - ref);
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[h][r][i], p.scale_log2, -ref));
                         sum[r] += e;
                         pb[r][4 * h + i] = (__bf16)e;
                     }

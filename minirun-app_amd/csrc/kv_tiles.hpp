@@ -127,10 +127,10 @@ struct KvFrom {
 };
 template <bool MX>
 __device__ __forceinline__ KvFrom kv_from(const KvAttnParams& p, bool keys, int kv_head, int id, int offset) {
-    const int64_t page = kv_page(p, id) ? id : 0;
+    const uint64_t page = kv_page(p, id) ? (uint32_t)id : 0u;
     const uint32_t row = (uint32_t)(kv_head * p.page_size + offset);  // (a page has at most 2^28 values)
-    const int64_t bytes = page * p.page_bytes + row * (uint32_t)(MX ? p.dim / 2 : p.dim * 2);
-    const int64_t sc = MX ? page * p.scale_bytes + row * (uint32_t)(p.dim / 32) : 0;
+    const uint64_t bytes = page * p.page_bytes + row * (uint32_t)(MX ? p.dim / 2 : p.dim * 2);
+    const uint64_t sc = MX ? page * p.scale_bytes + row * (uint32_t)(p.dim / 32) : 0;
     return KvFrom{(keys ? p.k : p.v) + bytes, (keys ? p.k_scales : p.v_scales) + sc};
 }
 
@@ -276,12 +276,12 @@ __device__ __forceinline__ void kv_add_infinite(const KvAttnParams& p, int b, in
     const int64_t row = (int64_t)kv_head * p.page_size + (key - page * p.page_size);
     uint32_t lo, hi;
     if constexpr (MX) {
-        const uint16_t w = *(const uint16_t*)(p.v + id * p.page_bytes + (row * p.dim + d0) / 2);
-        const uint8_t e = p.v_scales[id * p.scale_bytes + (row * p.dim + d0) / 32];
+        const uint16_t w = *(const uint16_t*)(p.v + (uint64_t)id * p.page_bytes + (row * p.dim + d0) / 2);
+        const uint8_t e = p.v_scales[(uint64_t)id * p.scale_bytes + (row * p.dim + d0) / 32];
         const u32x4 x = __builtin_bit_cast(u32x4, mxfp4_bf16(w, __uint_as_float((uint32_t)e << 23)));
         lo = x[0], hi = x[1];
     } else {
-        const u32x2 x = *(const u32x2*)(p.v + id * p.page_bytes + (row * p.dim + d0) * 2);
+        const u32x2 x = *(const u32x2*)(p.v + (uint64_t)id * p.page_bytes + (row * p.dim + d0) * 2);
         lo = x[0], hi = x[1];
     }
     const uint32_t v[4] = {lo << 16, lo & 0xffff0000u, hi << 16, hi & 0xffff0000u};

@@ -658,7 +658,7 @@ struct KvAttnParams {
     int64_t q_ts, q_hs;
     const char *k, *v;              // pages [kv_heads][page_size][dim]: bf16, or MXFP4 words
     const uint8_t *k_scales, *v_scales;  // null: bf16
-    int64_t page_bytes, scale_bytes;     // from page to page
+    uint32_t page_bytes, scale_bytes;    // from page to page
     int32_t pages, page_size, kv_heads, group, dim;  // group: query heads of a key head
     const int32_t* table;
     int64_t table_stride;
