@@ -11,15 +11,19 @@
 // whose maximum and sum stay in it but for one exchange between the halves of
 // the wave.
 // What bounds it: the products (4 dim flops a pair of query and key) and, beside
-// them, the softmax and the conversions on the vector units.  An exp2 and a conversion
-// of two MXFP4 values take 16 clocks of a wave's vector unit, other instructions 4: for
-// a wave's 32 products of 32 clocks a tile, 32 exp2, about 120 others and 16
-// conversions.  (With four waves a workgroup every wave has 32 of these: 44 of 230 us
-// of 4096 queries behind 1000 keys.)  Two waves a SIMD alone ran products and softmax
-// one after the other, so a wave's own are interleaved: while the products of the next
-// tile's scores run, the scores of this one become probabilities, and while its values
-// are multiplied, the next scores' maximum is found and rows go to LDS.  So keys are a
-// tile ahead of values, and one barrier ends a tile.
+// them, the softmax and the conversions on the vector units and the way of operands from
+// LDS, each of which is about half busy.  An exp2 and a conversion of two MXFP4 values
+// take 16 clocks of a wave's vector unit, other instructions 4: for a wave's 32 products
+// of 32 clocks a tile, 32 exp2, about 120 others and 16 conversions.  (With four waves a
+// workgroup every wave has 32 of these, which cost 44 us of 230.)  Two waves a SIMD alone
+// ran products and softmax one after the other, so a wave's own are interleaved: while the
+// products of the next tile's scores run, the scores of this one become probabilities, and
+// while its values are multiplied, the next scores' maximum is found and rows go to LDS.
+// So keys are a tile ahead of values, and one barrier ends a tile.
+//   Measured: 4096 queries of 32 heads behind 1000 keys, 4 key heads of 128 in MXFP4,
+// 199 us, 1.03 PFLOP/s (4-wave workgroups 245 without and 231 with the interleaving).  Keys
+// as codes on the scaled matrix instructions, a quarter of the LDS reads for keys and no
+// conversion of them, took 200.
 #include <type_traits>
 
 #include "kv_tiles.hpp"
