@@ -703,7 +703,7 @@ mr_status mr_head_norm_rope(const mr_head_norm_args *args, void *stream);
 /* Its gradients: with g = d_out turned back and r = 1 / sqrt(mean(x^2) + eps),
  *   out = r * (g * weight - x * r * mean(g * weight * x * r)),
  *   d_weight = the sum over tokens and heads of g * x * r, in f32
- * (written, not added to; the order of the sums is fixed). */
+ * (written, not added to, so not one for q and k; the order of the sums is fixed). */
 size_t mr_head_norm_rope_backward_workspace_size(const mr_head_norm_args *args);
 mr_status mr_head_norm_rope_backward(const mr_head_norm_args *args, void *stream);
 

@@ -117,6 +117,8 @@ mr_status head_norm(const mr_head_norm_args* a, bool backward, void* stream) {
             s.dy_hs = r.d_out_head_stride;
         }
     }
+    if (p.seg[0].dw && p.seg[0].dw == p.seg[1].dw)
+        return fail(MR_INVALID_ARGUMENT, "%s: one d_weight for queries and keys (it is written, not added to)", what);
     p.tokens = a->tokens;
     p.dim = a->dim;
     p.x_f32 = a->x_dtype == MR_F32;
@@ -263,7 +265,7 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     if (st != MR_OK) return st;
     if (!act(a->out_dtype))
         return fail(MR_INVALID_DTYPE, "%s: out must be bf16 or f32, got %s", what, mrc::dtype_name(a->out_dtype));
-    if (!(a->scale > 0) || !std::isfinite(a->scale)) return fail(MR_INVALID_SHAPE, "%s: scale must be finite, > 0", what);
+    if (!(a->scale > 0) || !std::isfinite(a->scale * 1.4426950408889634f)) return fail(MR_INVALID_SHAPE, "%s: scale must be finite, > 0", what);
     if (!a->tokens || !a->batch) return MR_OK;
     if (!a->q || !a->out || !a->kv_lens || (a->max_pages && !a->page_table))
         return fail(MR_INVALID_ARGUMENT, "%s: q, out, kv_lens and page_table must be non-NULL", what);

@@ -37,7 +37,7 @@ def norm_args(**fields):
     a = M.HeadNormArgs()
     put(a, tokens=5, dim=64, x_dtype=M.BF16, weight_dtype=M.F32, out_dtype=M.BF16, eps=1e-6)
     for rows, heads in ((a.q, 4), (a.k, 2)):
-        put(rows, heads=heads, x=AT, out=AT, weight=AT, d_out=AT, d_weight=AT, x_token_stride=64 * heads, x_head_stride=64,
+        put(rows, heads=heads, x=AT, out=AT, weight=AT, d_out=AT, d_weight=AT + 256 * heads, x_token_stride=64 * heads, x_head_stride=64,
             out_token_stride=64 * heads, out_head_stride=64, d_out_token_stride=64 * heads, d_out_head_stride=64)
     put(a.rope, cos_t=AT, sin_t=AT, positions=AT, table_rows=9, dim=32)
     return put(a, **fields)
@@ -64,6 +64,7 @@ def test_head_norm_refusals(lib):
             refused(call(**kw), M.INVALID_ARGUMENT)
     call = lambda **kw: lib.mr_head_norm_rope_backward(C.byref(norm_args(**kw)), None)
     refused(call(q__d_out=None), M.INVALID_ARGUMENT, "NULL")
+    refused(call(q__d_weight=AT, k__d_weight=AT), M.INVALID_ARGUMENT, "one d_weight")
     refused(call(q__d_out_token_stride=-1), M.INVALID_ARGUMENT, "stride")
     refused(call(), M.WORKSPACE_TOO_SMALL, "workspace")
     refused(call(workspace_bytes=1 << 20), M.INVALID_ARGUMENT, "workspace")
@@ -148,6 +149,7 @@ def test_attention_refusals(lib):
     for kw in (dict(batch=-1), dict(tokens=-1), dict(heads=0), dict(heads=7), dict(heads=-8), dict(tokens=4), dict(max_pages=-1),
                dict(max_pages=2 ** 27), dict(max_kv_len=-1), dict(window=-1), dict(tokens=2 ** 30, q_offsets=AT),
                dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+               dict(scale=3e38),
                dict(batch=2 ** 24, tokens=2 ** 24)):
         refused(call(**kw), M.INVALID_SHAPE)
     refused(call(out_dtype=M.F16), M.INVALID_DTYPE)
