@@ -179,16 +179,22 @@ struct HeadAngles {
 //   (a, b) -> (a cos - b sin, a sin + b cos)
 // for adjacent pairs, or for column i and column i + half.  `row` is the group's part
 // of LDS (8 lpr values), through which ROPE_HALVES and ROPE_ANY hand partners over.
-// T: float rounds every operation as written; double.
+// T: float rounds every operation as written; double.  sum: if given, the magnitudes of
+// the two terms of each result, added; of columns that stay, the value's.
 template <int KIND, bool INV, typename T>
-__device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, const HeadAngles<KIND>& g, int c, T* row) {
+__device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, const HeadAngles<KIND>& g, int c, T* row,
+                                            float* sum = nullptr) {
+    if (sum)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] = __builtin_fabsf((float)v[j]);
     if constexpr (KIND != ROPE_ADJACENT) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) row[c + j] = v[j];
         wave_lds_fence();
     }
-    auto turn = [&](T a, T p, float co, float si, bool second) -> T {
+    auto turn = [&](T a, T p, float co, float si, bool second, int j) -> T {
         const T cc = co, ss = INV ? -si : si;
+        if (sum) sum[j] = __builtin_fabsf((float)a * co) + __builtin_fabsf((float)p * si);
         if constexpr (sizeof(T) == 4)
             return second ? add_rn(mul_rn(p, ss), mul_rn(a, cc)) : sub_rn(mul_rn(a, cc), mul_rn(p, ss));
         else
@@ -200,8 +206,8 @@ __device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, const 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const T a = v[2 * j], b = v[2 * j + 1];
-                v[2 * j] = turn(a, b, g.co[j], g.si[j], false);
-                v[2 * j + 1] = turn(b, a, g.co[j], g.si[j], true);
+                v[2 * j] = turn(a, b, g.co[j], g.si[j], false, 2 * j);
+                v[2 * j + 1] = turn(b, a, g.co[j], g.si[j], true, 2 * j + 1);
             }
         }
     } else if constexpr (KIND == ROPE_HALVES) {
@@ -209,7 +215,7 @@ __device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, const 
             const bool second = k >= r.half;
             const T* partner = row + (second ? c - r.half : c + r.half);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = turn(v[j], partner[j], g.co[j], g.si[j], second);
+            for (int j = 0; j < 8; ++j) v[j] = turn(v[j], partner[j], g.co[j], g.si[j], second, j);
         }
     } else {
 #pragma unroll
@@ -218,7 +224,7 @@ __device__ __forceinline__ void head_rotate(T (&v)[8], const HeadRope& r, const 
             if (x < 0 || x >= 2 * r.half) continue;
             const bool second = r.halves ? x >= r.half : (x & 1);
             const int d = r.halves ? r.half : 1;
-            v[j] = turn(v[j], row[second ? c + j - d : c + j + d], g.co[j], g.si[j], second);
+            v[j] = turn(v[j], row[second ? c + j - d : c + j + d], g.co[j], g.si[j], second, j);
         }
     }
     if constexpr (KIND != ROPE_ADJACENT) wave_lds_fence();  // the next row's values come after these reads

@@ -644,7 +644,7 @@ struct KvAppendParams {
     int32_t slot_end, page_size;
     int32_t norm, w_f32;
     const void* w;  // null: ones
-    float eps;
+    float eps, inv_dim;
     HeadRope rope;
     void *k_pages, *v_pages;        // bf16 values, or MXFP4 words
     uint8_t *k_scales, *v_scales;   // null: bf16

@@ -65,7 +65,8 @@ def norm_backward(dy, x, w, eps, cos, sin, col0, halves):
 def round_bf16(x):
     """64 bits to bf16 (uint16), once, to nearest even."""
     m, e = np.frexp(np.where(np.isfinite(x), x, 0))
-    y = np.ldexp(np.rint(np.ldexp(m, 8)), e - 8).astype(np.float32)
+    step = np.maximum(e - 8, -133)  # (below 2^-126 a bf16's steps are 2^-133)
+    y = np.ldexp(np.rint(np.ldexp(m, e - step)), step).astype(np.float32)
     return X.to_bf16(np.where(np.isfinite(x), y, x).astype(np.float32))
 
 

@@ -90,6 +90,29 @@ def test_stored_rows(M, shape, f32, mxfp4):
 
 
 @pytest.mark.parametrize("mxfp4", [False, True])
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e-18, 1e-3, 1e3, 1e18, 1e30, 1e37])
+def test_rows_of_any_size(M, scale, mxfp4):
+    """Squares that leave f32's range, values near its ends, rows of zeros, and a large value in each third row:
+    what the stored values are does not depend on how they were found."""
+    rng = np.random.default_rng(5)
+    T, H, D = 48, 2, 128
+    x = (scale * rng.standard_normal((T, H, D))).astype(np.float32)
+    x[::3, :, 7] *= 1e3 if scale < 1e34 else 1.0
+    x[5] = 0
+    w = rng.uniform(0.5, 1.5, D).astype(np.float32)
+    cos, sin = K.tables(rng, T, D // 2)
+    for normalize in (True, False):
+        pages = K.Pages(rng, 4, H, 16, D, mxfp4)
+        cache = pages.device(M)
+        slots = rng.permutation(64)[:T].astype(np.int32)
+        k64 = K.norm(x.astype(np.float64), w.astype(np.float64), float(np.float32(EPS))) if normalize else x.astype(np.float64)
+        M.kv_append(cache, X.dev(x), X.dev(x), X.dev(slots), normalize=normalize, norm_weight=X.dev(w) if normalize else None,
+                    eps=EPS, cos_t=X.dev(cos), sin_t=X.dev(sin), halves=True)
+        for got, want in zip(stored(cache), expect(pages, K.turn(k64, cos, sin, 0, True), x.astype(np.float64), slots)):
+            assert np.array_equal(got, want), np.argwhere(got != want)[:3]
+
+
+@pytest.mark.parametrize("mxfp4", [False, True])
 def test_values_next_to_a_border(M, mxfp4):
     """Values that lie on a border of the 4-bit (or bf16) grid, or next to one by less than f32 resolves."""
     D, T = 64, 40
