@@ -1037,7 +1037,7 @@ def _heads_like(t, name, shape, device, dtype):
 
 
 def _room(t, dtype):
-    """A new tensor of t's shape and place without gaps.  (empty_like takes 1.1 us, empty 1.6.)"""
+    """A new tensor of t's shape and place without gaps.  (Where t has none, empty_like takes 1.1 us, empty 1.6.)"""
     if dtype is t.dtype and t.is_contiguous():
         return _torch().empty_like(t)
     return _torch().empty(t.shape, dtype=dtype, device=t.device)
@@ -1131,7 +1131,7 @@ def head_norm_rope_backward(d_q, q, d_k=None, k=None, *, q_weight=None, k_weight
                 continue
             strides = _heads_like(x, name, (T, None, D), device, dtype)
             dx = _room(x, dtype)
-            dw = None if weight is None else torch.empty(D, dtype=torch.float32, device=device)
+            dw = None if weight is None else _room(weight, torch.float32)
             heads = x.shape[1]
             rows.append(HeadRows(heads, x.data_ptr(), *strides, _vector(weight, f"{name}_weight", D, device, wtype),
                                  dx.data_ptr(), heads * D, D, d.data_ptr(),
