@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 // The parts of a row joined: blockIdx.x is the (query, head), blockIdx.y a span of
 // `cols` dims; 4 dims a thread, threads that are left over share the parts.
 constexpr int KJ_MAX = 1024;  // parts
-constexpr int KJ_FEW = 32;
+constexpr int KJ_FEW = 32;    // of them where a row has a group of lanes alone
+constexpr int KJ_EARLY = 4;
 
 __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) {
     __shared__ float weight[KJ_MAX];
@@ -383,8 +384,18 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
     if (p.q_offsets && (token < s_load(p.q_offsets) || token >= s_load(p.q_offsets + p.batch))) return;
     const f32x2* ml = (const f32x2*)p.part_ml + at * p.splits;
     const int w = threadIdx.x >> 6;
+    const int d0 = blockIdx.y * span, cols = min(span, p.dim - d0) / 4;
+    const int shares = 256 / cols, share = threadIdx.x / cols, c = threadIdx.x - share * cols;
     float top = -INFINITY;
     f32x2 mine[KJ_MAX / 256];
+    // the first sums of this thread's share are under way while the weights are found
+    const float* o = p.part_o + at * p.splits * p.dim + d0 + 4 * c;
+    f32x4 early[KJ_EARLY];
+#pragma unroll
+    for (int i = 0; i < KJ_EARLY; ++i) {
+        const int s = share + shares * i;
+        early[i] = share < shares && s < p.splits ? *(const f32x4*)(o + (int64_t)s * p.dim) : f32x4{};
+    }
 #pragma unroll
     for (int i = 0; i < KJ_MAX / 256; ++i) {
         const int s = threadIdx.x + 256 * i;
@@ -414,13 +425,15 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
     const float inv = total == 0.f ? 0.f : 1.f / total;
     if (p.lse && threadIdx.x == 0 && blockIdx.y == 0)
         p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
-    const int d0 = blockIdx.y * span, cols = min(span, p.dim - d0) / 4;
-    const int shares = 256 / cols, share = threadIdx.x / cols, c = threadIdx.x - share * cols;
     f32x4 x{};
     if (share < shares) {
-        const float* o = p.part_o + at * p.splits * p.dim + d0 + 4 * c;
+#pragma unroll
+        for (int i = 0; i < KJ_EARLY; ++i) {
+            const int s = share + shares * i;
+            if (s < p.splits && !(weight[s] < 0.f)) x += weight[s] * early[i];
+        }
 #pragma unroll 8
-        for (int s = share; s < p.splits; s += shares)
+        for (int s = share + KJ_EARLY * shares; s < p.splits; s += shares)
             if (!(weight[s] < 0.f)) x += weight[s] * *(const f32x4*)(o + (int64_t)s * p.dim);
     }
     *(f32x4*)(add + 4 * threadIdx.x) = x;
