@@ -521,9 +521,11 @@ hipError_t decode_dim(const KvAttnParams& p, int rows, unsigned grid, hipStream_
 //   16 rows, little work: one workgroup a CU, parts of 128 keys or more (4 key heads: 4000
 //     keys in parts of 128 / 512 / whole 8.7 / 11.5 / 34.7; 32000 in 128 / 512 / 2048
 //     17.8 / 13.8 / 24.3)
-//   16 rows, much: parts of 512 keys or more, four workgroups a CU (131072 keys, 8 key
-//     heads, in 512 / 1024 / 2048 43 / 37 / 42), but of 1536 at most, since lengths differ
-//     (64 sequences of 1000 to 12000, 4 key heads, in 1024 / 1536 / 2048 49 / 45 / 48)
+//   16 rows, much: parts of 512 keys or more, three workgroups a CU, all of a length (131072
+//     keys, 8 key heads, by 3 / 3.5 / 4 / 5 a CU 35.6 / 38.8 / 37.4 / 40.3; bf16, 32
+//     sequences of 2000 to 8000, by 3 / 4 59 / 67), four of up to 64 dims (27.3 / 28.2 /
+//     25.6 / 26.4), but of 1536 keys at most, since lengths differ (64 of 1000 to 12000, 4
+//     key heads, in 1024 / 1536 / 2048 49 / 45 / 48)
 //   32 and 64 rows leave more sums and fill a CU with two workgroups (24 rows, 32
 //     sequences of 1000 to 6000, in 512 / 1024 / 2048 38 / 32 / 36) or one (40 rows: 72 /
 //     57 / 48; 24 rows of 256 dims 77 / 64 / 52)
@@ -558,7 +560,7 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     } else {
         const int fit = r.rows * dim > 32 * 128 ? 1 : 2;  // workgroups a CU
         if (r.rows == 16)
-            chunk = std::max({std::min<int64_t>(work / cus, 512), work / (4 * cus), int64_t(128)});
+            chunk = std::max({std::min<int64_t>(work / cus, 512), work / ((dim > 64 ? 3 : 4) * cus), int64_t(128)});
         else
             chunk = std::max<int64_t>(256, work / (fit * cus));
         chunk = std::min<int64_t>(chunk, r.rows > 16 && fit == 1 ? 2048 : 1536);

@@ -43,7 +43,7 @@ def route(tmp_path_factory):
 # queries, keys, key heads, group, further sizes; many queries?, rows of a tile, parts, keys of a part
 TABLE = [
     ((None, 500, 4, 8), {}, (0, 16, 1, 512)), ((None, 4000, 4, 8), {}, (0, 16, 32, 128)),
-    ((None, 131072, 8, 8), {}, (0, 16, 128, 1024)), ((None, 12000, 4, 8), dict(batch=64), (0, 16, 8, 1536)),
+    ((None, 131072, 8, 8), {}, (0, 16, 94, 1408)), ((None, 131072, 8, 8), dict(dim=64), (0, 16, 128, 1024)), ((None, 12000, 4, 8), dict(batch=64), (0, 16, 8, 1536)),
     ((None, 4000, 8, 8), dict(batch=64), (0, 16, 1, 4032)), ((None, 10 ** 7, 1, 8), {}, (0, 16, 1022, 9792)),
     ((3, 6000, 4, 8), dict(batch=32), (0, 32, 4, 1536)), ((3, 6000, 4, 8), dict(batch=32, dim=256), (0, 32, 3, 2048)),
     ((8, 3000, 8, 8), dict(batch=64), (0, 64, 1, 3008)), ((5, 2000, 4, 8), dict(dim=256), (1, 128, 16, 128)),
