@@ -17,23 +17,24 @@
 //     scale one byte; q's registers hold the same dims;
 //   - the lane that has query n's scores keeps its maximum and sum;
 //   - O^T += V^T . P^T: the scores' registers are the second operand as they
-//     are, V^T comes by transposed reads.  P is rounded to bf16 (2^-9 of each
-//     term, whose errors average out); sums stay in f32.
+//     are, V^T comes by transposed reads.  P is rounded to bf16 (at most 2^-8 of
+//     each term, whose errors average out); sums stay in f32.
 // The waves of a workgroup split its keys and meet once, in LDS.  A tile's keys
 // are split over workgroups where that fills the GPU (kv_attention_route),
 // which leave (m, l, o) in the workspace for the join.
 //   Measured (8 query heads a key head of 128, MXFP4 unless said; us): 64 sequences of
 // 4000 keys, 8 key heads, 56, 4.9 TB/s, in bf16 186, 5.6 TB/s; one of 131072, 8 key heads,
-// 31 and the join 5; 64 of 1000 to 12000, 4 key heads, 39 and the join 4 (about 10 of them
+// 30 and the join 4; 64 of 1000 to 12000, 4 key heads, 39 and the join 4 (about 10 of them
 // while the last parts leave CUs idle).  A wave alone takes 0.9 a step, mostly the issue
 // of its instructions (150 vector, about 70 scalar, 32 LDS): the loads of a second step in
-// flight changed nothing (the last two, with their joins, became 43 and 51, since fewer
-// waves fit), nor did keys as codes on the scaled matrix instructions against q in two
-// e4m3 parts (38 and 45, and scores 100 times less exact).
+// flight changed nothing (the last two, with their joins, 43 and 51 for 38 and 44, since
+// fewer waves fit), nor did eight waves a workgroup (38 and 49), nor keys as codes on the
+// scaled matrix instructions against q in two e4m3 parts (38 and 45, and scores 100 times
+// less exact).
 //
-// Keys that no row may see are zeros where they are loaded.  Infinities and NaN of
-// values that some rows of a step see and others do not take a way of their own
-// (kv_add_infinite).
+// Scores of keys that a row does not see become -inf, values that no row may see zeros
+// where they are loaded.  Infinities and NaN of values that some rows of a step see and
+// others do not take a way of their own (kv_add_infinite).
 #include <algorithm>
 
 #include "kv_tiles.hpp"
