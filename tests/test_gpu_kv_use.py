@@ -148,6 +148,39 @@ def test_captured_steps_replay_with_other_inputs(M, hint):
         at += 1
 
 
+@pytest.mark.parametrize("hint", [0, 100])  # the keys in parts, joined, and whole
+def test_captured_prompts_replay_with_other_lengths(M, hint):
+    """A captured step of 300 tokens, replayed while they belong to other sequences of other lengths."""
+    import torch
+
+    layer = Layer(M, 12, True, pages=200, positions=1200)
+    table = np.stack([np.arange(70) + 70 * b for b in range(2)]).astype(np.int32)
+    q, k, v = (t.clone() for t in layer.rows(300))
+    pos, slots, lens, offsets = i32(np.zeros(300)), i32(np.full(300, -1)), i32([0, 0]), i32([0, 0, 0])
+    step = lambda: layer.step(q, k, v, pos, slots, i32_table, lens, offsets, max_kv_len=hint)
+    i32_table = i32(table)
+    g, (_, gout) = capture(step)
+    have = np.zeros(2, np.int64)
+    for counts in ([200, 100], [299, 0], [1, 250], [150, 150]):
+        at = np.concatenate([have[b] + np.arange(c) for b, c in enumerate(counts)])
+        owner = np.repeat([0, 1], counts)
+        pad = 300 - len(at)
+        have += counts
+        for dst, src in zip((q, k, v), layer.rows(300)):
+            dst.copy_(src)
+        pos.copy_(i32(np.append(at, np.zeros(pad))))
+        slots.copy_(i32(np.append(table[owner, at // PAGE] * PAGE + at % PAGE, np.full(pad, -1))))
+        lens.copy_(i32(have))
+        offsets.copy_(i32(np.cumsum([0] + counts)))
+        gout.fill_(7)
+        g.replay()
+        torch.cuda.synchronize()
+        got = gout.clone()
+        _, eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got[:len(at)], eager[:len(at)]) and (got[len(at):] == 7).all()
+
+
 def test_captured_backward_replays(M):
     import torch
 
