@@ -116,8 +116,11 @@ __global__ void __launch_bounds__(64 * KA_WAVES) kv_append_kernel(KvAppendParams
         // With u = 2^-24: the sum of squares is off by 14 u of it (8 and 6 roundings), the
         // mean and eps by 17, the root (1 ulp of the instruction) by 8.5 + 2, so y by 12.5;
         // a rotation's result by 12.5 + 1 and 1 of its two terms' magnitudes, and each end
-        // by one more: 15.5 u, 3 u without the norm.  Rows whose squares could leave f32's
-        // range, and results that could, are left to f64.
+        // by one more: 15.5 u, 3 u without the norm.  That holds for normal numbers: a product
+        // below them is off by 2^-150, which a large weight makes too much if it comes before
+        // it, so such rows (zeros too, which it may have become) are left to f64, like rows
+        // whose squares could leave f32's range and results that could; later ones are within
+        // 2^-140, with cosines.
         float y[8], sum[8], ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = x[j];
@@ -129,7 +132,11 @@ __global__ void __launch_bounds__(64 * KA_WAVES) kv_append_kernel(KvAppendParams
             sure = ss > 0x1p-100f && ss < 0x1p100f;
             const float inv = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_dim, p.eps));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = wt[j] * (y[j] * inv);
+            for (int j = 0; j < 8; ++j) {
+                y[j] *= inv;
+                sure = sure && !__builtin_amdgcn_classf(y[j], 0xF0);  // (zeros and subnormal numbers)
+                y[j] *= wt[j];
+            }
         }
         if (p.rope.half) {
             head_rotate<KIND, false>(y, p.rope, angles, c, (float*)&sh[w][0] + at, sum);
@@ -142,7 +149,7 @@ __global__ void __launch_bounds__(64 * KA_WAVES) kv_append_kernel(KvAppendParams
         uint32_t near = 0, far = 0;  // the largest magnitude is between these
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float off = sum[j] == 0.f ? 0.f : fmaf(sum[j], u, 0x1p-140f);
+            const float off = fmaf(sum[j], u, 0x1p-140f);
             ends[0][j] = y[j] - off, ends[1][j] = y[j] + off;
             near = max(near, min(magnitude(ends[0][j]), magnitude(ends[1][j])));
             far = max(far, max(magnitude(ends[0][j]), magnitude(ends[1][j])));
