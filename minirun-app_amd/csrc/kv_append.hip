@@ -45,6 +45,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {
 
 // Eight values as they are stored: bf16, or codes and the scale of the block that four
 // lanes have.  `most`: the largest magnitude of the eight, or more in the same binade.
+// The values of an MXFP4 block stand for 2^lift times as much (one lift for all of it).
 struct Stored {
     u32x4 bf16;
     uint32_t codes, byte;
@@ -52,7 +53,7 @@ struct Stored {
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-__device__ __forceinline__ Stored narrow(bool mx, const float (&v)[8], uint32_t most) {
+__device__ __forceinline__ Stored narrow(bool mx, const float (&v)[8], uint32_t most, uint32_t lift = 0) {
     Stored s{};
     if (!mx) {
         s.bf16 = u32x4{pack_bf16x2_hw(v[0], v[1]), pack_bf16x2_hw(v[2], v[3]), pack_bf16x2_hw(v[4], v[5]),
@@ -62,8 +63,8 @@ __device__ __forceinline__ Stored narrow(bool mx, const float (&v)[8], uint32_t 
     most = block_max(most);
     const bool finite = most < 0x7f800000u;
     const uint32_t e = most >> 23;
-    s.byte = finite ? (e > 2 ? e - 2 : 0) : 255u;
-    const float scale = __uint_as_float(finite ? s.byte << 23 : 0x3f800000u);
+    s.byte = finite ? min((e > 2 ? e - 2 : 0) + lift, 254u) : 255u;
+    const float scale = __uint_as_float(finite ? (s.byte - lift) << 23 : 0x3f800000u);
     uint32_t word = 0;
     word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], scale, 0);
     word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], scale, 1);
@@ -179,9 +180,20 @@ __global__ void __launch_bounds__(64 * KA_WAVES) kv_append_kernel(KvAppendParams
                 for (int j = 0; j < 8; ++j) z[j] = wt[j] * (z[j] * inv);
             }
             if (p.rope.half) head_rotate<KIND, false>(z, p.rope, angles, c, &sh[w][at]);
+            // A block of values of 2^126 or more, which may pass f32, takes part 2^-8 times as
+            // large (what that cuts off its small values has code 0 beside the large one).
+            uint32_t lift = 0;
+            if (mx) {
+                uint32_t top = 0;  // sign, exponent and first bits of an f64, without the sign
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = to_odd(z[j]);
-            s = narrow(mx, y, most_of(y));
+                for (int j = 0; j < 8; ++j) top = max(top, (uint32_t)(__builtin_bit_cast(uint64_t, z[j]) >> 32) & 0x7fffffffu);
+                top = block_max(top);
+                if (top >= 1149u << 20 && top < 0x7ff00000u) lift = 8;
+            }
+            const double by = lift ? 0x1p-8 : 1.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = to_odd(z[j] * by);
+            s = narrow(mx, y, most_of(y), lift);
         }
     } else {
         s = narrow(mx, x, most_of(x));
