@@ -678,7 +678,7 @@ typedef struct mr_head_rows {
     int64_t out_token_stride, out_head_stride;
     const void *d_out;  /* backward only: the gradient of the output */
     int64_t d_out_token_stride, d_out_head_stride;
-    float *d_weight;    /* backward only: f32 [dim], or NULL */
+    float *d_weight;    /* backward only: f32 [dim], or NULL (heads 0: zeros are written) */
 } mr_head_rows;
 
 /* For every head x of q and k, in f32, rounded once to out_dtype:

@@ -88,12 +88,12 @@ mr_status head_norm(const mr_head_norm_args* a, bool backward, void* stream) {
         const mr_head_rows& r = *rows[i];
         mr::HeadSegment& s = p.seg[i];
         s.heads = r.heads;
+        s.dw = backward ? r.d_weight : nullptr;  // (also without heads: zeros)
+        weights = weights || s.dw;
+        if (!mrc::aligned4(s.dw)) return fail(MR_INVALID_ARGUMENT, "%s: a misaligned weight", what);
         if (!r.heads) continue;
         s.w = r.weight;
-        s.dw = backward ? r.d_weight : nullptr;
-        weights = weights || s.dw;
-        if (!elem_aligned(r.weight, a->weight_dtype) || !mrc::aligned4(s.dw))
-            return fail(MR_INVALID_ARGUMENT, "%s: a misaligned weight", what);
+        if (!elem_aligned(r.weight, a->weight_dtype)) return fail(MR_INVALID_ARGUMENT, "%s: a misaligned weight", what);
         if (!a->tokens) continue;
         if (!r.x || !r.out || (backward && !r.d_out)) return fail(MR_INVALID_ARGUMENT, "%s: NULL rows", what);
         if (!elem_aligned(r.x, a->x_dtype) || !elem_aligned(r.out, a->out_dtype) ||

@@ -1,11 +1,10 @@
 """The gradients of head norms where a workgroup walks over many rows: values at sizes of
 several steps, with whole and partial last ones, heads that divide a step and heads that do not;
-and in place.
+in place; and the gradient of a weight whose side has no heads.
 
 The oracle is test_gpu_head_norm.py's formula in f64 on the GPU, with its tolerances."""
 import ctypes as C
 
-import numpy as np
 import pytest
 
 import kv_inputs as K
@@ -92,12 +91,14 @@ def test_gradients_of_many_rows(M, shape, f32):
     check(got[1], got[3], dk, k, wk, *at, col0, halves, f32)
 
 
-def args_of(M, q, dq, out, weight, d_weight):
+def args_of(M, q, dq, out, weight, d_weight, heads_k=0, k_weight=None, d_k_weight=None):
     T, H, D = q.shape
     rows = lambda t: (t.data_ptr(), *t.stride()[:2])
     a = M.HeadNormArgs(T, D, M.HeadRows(H, *rows(q), weight.data_ptr(), *rows(out), *rows(dq), d_weight.data_ptr()),
-                       M.HeadRows(), M.BF16 if q.element_size() == 2 else M.F32, M.F32,
+                       M.HeadRows(heads_k), M.BF16 if q.element_size() == 2 else M.F32, M.F32,
                        M.BF16 if out.element_size() == 2 else M.F32, EPS)
+    if k_weight is not None:
+        a.k.weight, a.k.d_weight = k_weight.data_ptr(), d_k_weight.data_ptr()
     return a
 
 
@@ -127,3 +128,23 @@ def test_gradients_in_place(M, where, f32, T, H, D):
     out = q if where == "x" else dq
     call(M, args_of(M, q, dq, out, w, dw))
     assert torch.equal(out, want) and torch.equal(dw, want_w)
+
+
+def test_a_side_without_heads_has_gradients_of_zero(M):
+    """A weight whose side has no heads: its gradient is written like one of no tokens."""
+    import torch
+
+    T, H, D = 9, 4, 40
+    q, dq, w = torch.randn(T, H, D, device="cuda"), torch.randn(T, H, D, device="cuda"), torch.ones(D, device="cuda")
+    want, want_w = M.head_norm_rope_backward(dq, q, q_weight=w, eps=EPS)
+    dw, dwk = (torch.full((D,), float("nan"), device="cuda") for _ in range(2))
+    out = torch.empty_like(q)
+    call(M, args_of(M, q, dq, out, w, dw, 0, w, dwk))
+    assert torch.equal(out, want) and torch.equal(dw, want_w) and (dwk == 0).all()
+    # and from Python
+    none = q[:, :0]
+    torch.full((D,), float("nan"), device="cuda")  # (what the next vector of D may be found to hold)
+    dx, dk, dw, dwk = M.head_norm_rope_backward(dq, q, none, none, q_weight=w, k_weight=w, eps=EPS)
+    assert torch.equal(dx, want) and dk.shape == (T, 0, D) and torch.equal(dw, want_w) and (dwk == 0).all()
+    dx, dk, dw, dwk = M.head_norm_rope_backward(none, none, dq, q, q_weight=w, k_weight=w, eps=EPS)
+    assert torch.equal(dk, want) and torch.equal(dwk, want_w) and (dw == 0).all()
