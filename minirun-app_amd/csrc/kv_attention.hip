@@ -329,17 +329,9 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             const int64_t at = (int64_t)to.token * (p.kv_heads * p.group) + to.head;
             float inv = 1.f;
             if (p.splits == 1) {
-                if (p.sinks) {
-                    const float sink = p.sinks[to.head] * 1.4426950408889634f, up = fmaxf(top, sink);
-                    const float was = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - up);
-                    if (up != -INFINITY) total = fmaf(total, was, __builtin_amdgcn_exp2f(sink - up));
-#pragma unroll
-                    for (int x = 0; x < KD_WAVES; ++x) a[x] *= was;
-                    top = up;
-                }
-                inv = total == 0.f ? 0.f : 1.f / total;  // (no key is seen: zeros)
-                if (p.lse && dn == 0)
-                    p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+                const KvEnd end = kv_end(top, total, p.sinks ? p.sinks[to.head] : -INFINITY);
+                inv = end.inv;
+                if (p.lse && dn == 0) p.lse[at] = end.lse;
             } else if (dn == 0) {
                 float* ml = p.part_ml + 2 * (at * p.splits + split);
                 ml[0] = top;
@@ -409,8 +401,6 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
     __syncthreads();
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     __syncthreads();
-    const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
-    top = fmaxf(top, sink);
     float total = 0.f;
 #pragma unroll
     for (int i = 0; i < KJ_MAX / 256; ++i) {
@@ -422,10 +412,9 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
     if ((threadIdx.x & 63) == 0) red[w] = total;
     __syncthreads();
     total = (red[0] + red[1]) + (red[2] + red[3]);
-    if (sink != -INFINITY) total += __builtin_amdgcn_exp2f(sink - top);
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (p.lse && threadIdx.x == 0 && blockIdx.y == 0)
-        p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    const KvEnd end = kv_end(top, total, p.sinks ? p.sinks[head] : -INFINITY);
+    const float inv = end.inv;
+    if (p.lse && threadIdx.x == 0 && blockIdx.y == 0) p.lse[at] = end.lse;
     f32x4 x{};
     if (share < shares) {
 #pragma unroll
@@ -460,15 +449,14 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(KvAttnParams p, int l
     // tokens that no sequence has are left as they are
     if (p.q_offsets && (token < s_load(p.q_offsets) || token >= s_load(p.q_offsets + p.batch))) return;
     const f32x2* ml = (const f32x2*)p.part_ml + at * p.splits;
-    float top = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
-    const float sink = top;
+    float top = -INFINITY;
     int first = p.splits, last = 0;  // the parts that left sums are among these
     for (int s = 0; s < p.splits; ++s) {
         const f32x2 x = ml[s];
         top = fmaxf(top, x[0]);
         if (x[1] != 0.f) first = min(first, s), last = s + 1;
     }
-    float total = sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - top);
+    float total = 0.f;
     f32x4 x{};
     const float* o = p.part_o + at * p.splits * p.dim + (c < p.dim ? c : 0);
 #pragma unroll 4
@@ -479,9 +467,9 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(KvAttnParams p, int l
         total = fmaf(y[1], a, total);
         if (y[1] != 0.f) x += a * v;
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (p.lse && c == 0)
-        p.lse[at] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    const KvEnd end = kv_end(top, total, p.sinks ? p.sinks[head] : -INFINITY);
+    const float inv = end.inv;
+    if (p.lse && c == 0) p.lse[at] = end.lse;
     if (c >= p.dim) return;
     const int64_t to = token * p.out_ts + head * p.out_hs + c;
     if (p.out_f32)

@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
                 kv_add_infinite<MX>(p, t.b, kv_head, key, key >= row.lo && key < row.hi, 32 * d + 8 * c + 4 * hh,
                                     [&](int j, float v) { o[d][4 * c + j] += v; });
 
-    float total = xor32_sum(l_part);
+    const float total = xor32_sum(l_part);
     const int64_t place = (int64_t)row.token * (p.kv_heads * p.group) + row.head;
     if (p.splits > 1) {
         if (!row.ok) return;
@@ -361,16 +361,9 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             }
         return;
     }
-    float top = m_run, was = 1.f;
-    if (p.sinks && row.ok) {
-        const float sink = p.sinks[row.head] * 1.4426950408889634f;
-        top = fmaxf(m_run, sink);
-        was = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - top);
-        if (top != -INFINITY) total = fmaf(total, was, __builtin_amdgcn_exp2f(sink - top));
-    }
-    const float inv = total == 0.f ? 0.f : was / total;  // (no key is seen: zeros)
-    if (p.lse && row.ok && hh == 0)
-        p.lse[place] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    const KvEnd end = kv_end(m_run, total, p.sinks && row.ok ? p.sinks[row.head] : -INFINITY);
+    const float inv = end.inv;
+    if (p.lse && row.ok && hh == 0) p.lse[place] = end.lse;
     if (p.out_f32) {
         if (!row.ok) return;
         float* to = (float*)p.out + row.token * p.out_ts + row.head * p.out_hs;

@@ -96,6 +96,20 @@ __device__ __forceinline__ KvRow kv_row(const KvAttnParams& p, const KvTile& t, 
     return r;
 }
 
+// What a row's sums come to with its sink (-inf: none): the factor of its output and the
+// logarithm, from the running maximum of its scores in base 2 and their sum.  In natural units,
+// since a sink may be any f32 and many would leave f32 in base 2.
+struct KvEnd {
+    float inv, lse;
+};
+__device__ __forceinline__ KvEnd kv_end(float top, float total, float sink) {
+    if (total == 0.f) return KvEnd{0.f, sink};  // no key is seen: zeros
+    const float m = top * 0.6931471805599453f, up = fmaxf(m, sink);
+    const float was = __builtin_amdgcn_exp2f((m - up) * 1.4426950408889634f);
+    const float all = fmaf(total, was, __builtin_amdgcn_exp2f((sink - up) * 1.4426950408889634f));
+    return KvEnd{was / all, up + __builtin_amdgcn_logf(all) * 0.6931471805599453f};
+}
+
 // The groups of 16 keys of a sequence, one after another: a page holds a whole
 // number of them.  Wave-uniform.
 struct KvWalk {

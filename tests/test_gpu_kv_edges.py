@@ -1,0 +1,91 @@
+"""Ends of the softmax of attention over a paged cache, in every form (whole and in parts, one
+query and many, both joins): sinks of any f32.  Tolerances as in test_gpu_kv_attention.py."""
+import numpy as np
+import pytest
+
+import kv_inputs as K
+import mxfp4_inputs as X
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def M():
+    import minirun_hip as M
+
+    M.load()
+    return M
+
+
+# lengths, queries (None: one each, no offsets), heads, kv_heads: which form and join each takes is
+# what tests/test_routes_kv_edges.py asks
+FORMS = {
+    "one": ([77, 0, 200], None, 8, 2),
+    "one in parts": ([3000, 0, 700], None, 8, 2),
+    "few": ([77, 9, 40], [3, 6, 0], 8, 2),
+    "few in parts": ([3000, 0, 700], [7, 2, 9], 8, 2),
+    "many": ([120, 130], [70, 60], 8, 2),
+    "many in parts": ([900, 20, 0], [55, 17, 9], 8, 2),
+    "many rows joined": ([900, 0, 300], [200, 20, 62], 8, 2),
+}
+
+
+def case(form, dim, mxfp4, seed=0):
+    lens, queries, heads, kv_heads = FORMS[form]
+    rng = np.random.default_rng([len(form), dim, mxfp4, seed])
+    table, n = K.page_tables(rng, lens, 32)
+    pages = K.Pages(rng, n, kv_heads, 32, dim, mxfp4)
+    offsets = None if queries is None else np.cumsum([0] + list(queries)).astype(np.int32)
+    T = len(lens) if queries is None else int(offsets[-1])
+    q64 = X.from_bf16(X.to_bf16((1.5 * rng.standard_normal((T, heads, dim))).astype(np.float32))).astype(np.float64)
+    return rng, table, pages, lens, offsets, q64
+
+
+def attend(M, q64, pages, table, lens, offsets, scale, sinks=None, f32=True):
+    """(out, lse) as 64-bit arrays."""
+    import torch
+
+    out, lse = M.kv_attention(X.dev(X.to_bf16(q64.astype(np.float32))), pages.device(M), X.dev(table),
+                              X.dev(np.array(lens, np.int32)), scale=scale, sinks=None if sinks is None else X.dev(sinks),
+                              q_offsets=None if offsets is None else X.dev(offsets), return_lse=True,
+                              out_dtype=torch.float32 if f32 else torch.bfloat16)
+    return X.host(out), X.host(lse)
+
+
+def keys_seen(lens, offsets, tokens):
+    """Of each token: [first, last) of its sequence's keys, and the sequence."""
+    owner = np.arange(tokens) if offsets is None else np.searchsorted(offsets, np.arange(tokens), side="right") - 1
+    end = np.arange(tokens) + 1 if offsets is None else offsets[owner + 1]
+    return owner, np.maximum(np.array(lens)[owner] - (end - 1 - np.arange(tokens)), 0)
+
+
+def compare(got, lse, want, lse64, weight, terms, dim, longest, f32):
+    score = (dim + 2) * K.MFMA * terms[..., None]
+    tol = weight * (X.BF16_ROUND + 2 * score + (longest + 8) * K.MFMA) + (X.F32_ROUND if f32 else X.BF16_ROUND) * np.abs(want) + 1e-37
+    assert np.array_equal(np.isnan(got), np.isnan(want)), np.argwhere(np.isnan(got) != np.isnan(want))[:3]
+    with np.errstate(invalid="ignore"):
+        over = np.where(np.isnan(want) | (got == want), 0, np.abs(got - want) - tol)
+        assert (over <= 0).all(), np.argwhere(over > 0)[:3]
+        off = np.abs(lse - lse64) > score[..., 0] + 2.0 ** -21 * (1 + np.abs(lse64)) + longest * K.MFMA
+    assert np.array_equal(np.isnan(lse), np.isnan(lse64)), np.argwhere(np.isnan(lse) != np.isnan(lse64))[:3]
+    assert np.array_equal(lse[np.isinf(lse64)], lse64[np.isinf(lse64)])
+    assert not (off & np.isfinite(lse64)).any(), np.argwhere(off & np.isfinite(lse64))[:3]
+
+
+SINKS = np.array([3.4028235e38, -3.4028235e38, 3e38, np.nan, -np.inf, np.inf, 40.0, -40.0], np.float32)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("mxfp4,dim", [(True, 128), (False, 64), (True, 256)])
+@pytest.mark.parametrize("form", FORMS)
+def test_sinks_of_any_size(M, form, dim, mxfp4, f32):
+    """The largest and the least f32 ("no sink" of a mask's convention), both infinities, NaN.  A query
+    without keys gets zeros and its sink as lse."""
+    _, table, pages, lens, offsets, q64 = case(form, dim, mxfp4)
+    scale = dim ** -0.5
+    with np.errstate(invalid="ignore"):
+        want, lse64, weight, terms = K.attention(q64, *pages.values(), table, lens, offsets, scale, 0, SINKS.astype(np.float64))
+    none = keys_seen(lens, offsets, len(q64))[1] == 0
+    want[none], lse64[none], weight[none] = 0, SINKS, 0
+    got, lse = attend(M, q64, pages, table, lens, offsets, scale, SINKS, f32)
+    compare(got, lse, want, lse64, weight, terms, dim, max(lens), f32)
