@@ -757,10 +757,11 @@ mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
  * all), the last of them at position kv_lens[b] - 1.  A query sees the keys up to
  * its position, or the last `window` of them (0: all).  A key that a query does not
  * see has no part in its output, whatever it holds.  A sink (f32 [heads], or NULL)
- * is one more score without a value.  A query that sees no key gets zeros.  Tokens
- * before the first sequence and behind the last are left as they were.  q_offsets
- * ascends from 0 or more to at most `tokens`; where it does not, the outputs of all
- * tokens are undefined.
+ * is one more score without a value.  A query that sees no key gets zeros, and so does
+ * one whose scores are all -inf (infinite keys): a part of a context that has nothing
+ * else weighs nothing where parts are joined by their lse.  Tokens before the first
+ * sequence and behind the last are left as they were.  q_offsets ascends from 0 or more
+ * to at most `tokens`; where it does not, the outputs of all tokens are undefined.
  *   q bf16; MXFP4 keys and values as mr_mxfp4_dequantize gives them in bf16; scores,
  * softmax and sums in f32 but for the probabilities, which enter the second product as
  * bf16 (out in f32 has that error too); out is rounded once.

@@ -345,6 +345,7 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
 #pragma unroll
                     for (int y = 0; y < KD_WAVES; ++y)
                         x += a[y] * *(const f32x4*)((const float*)(lds + y * L::WAVE) + rn * L::O_STRIDE + d);
+                    if (total == 0.f) x = f32x4{};  // (0 times an infinity is not)
                     if (p.splits > 1) {
                         *(f32x4*)(p.part_o + (at * p.splits + split) * p.dim + d) = x;
                     } else if (p.out_f32) {

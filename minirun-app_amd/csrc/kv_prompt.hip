@@ -363,6 +363,9 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
     }
     const KvEnd end = kv_end(m_run, total, p.sinks && row.ok ? p.sinks[row.head] : -INFINITY);
     const float inv = end.inv;
+    if (total == 0.f)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = f32x16{};  // (0 times an infinity is not)
     if (p.lse && row.ok && hh == 0) p.lse[place] = end.lse;
     if (p.out_f32) {
         if (!row.ok) return;

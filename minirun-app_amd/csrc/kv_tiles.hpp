@@ -103,7 +103,7 @@ struct KvEnd {
     float inv, lse;
 };
 __device__ __forceinline__ KvEnd kv_end(float top, float total, float sink) {
-    if (total == 0.f) return KvEnd{0.f, sink};  // no key is seen: zeros
+    if (total == 0.f) return KvEnd{0.f, sink};  // no key is seen, or none with a score above -inf: zeros
     const float m = top * 0.6931471805599453f, up = fmaxf(m, sink);
     const float was = __builtin_amdgcn_exp2f((m - up) * 1.4426950408889634f);
     const float all = fmaf(total, was, __builtin_amdgcn_exp2f((sink - up) * 1.4426950408889634f));

@@ -1,5 +1,6 @@
 """Ends of the softmax of attention over a paged cache, in every form (whole and in parts, one
-query and many, both joins): sinks of any f32.  Tolerances as in test_gpu_kv_attention.py."""
+query and many, both joins): sinks of any f32, and keys whose scores are all -inf.  Tolerances
+as in test_gpu_kv_attention.py."""
 import numpy as np
 import pytest
 
@@ -7,6 +8,7 @@ import kv_inputs as K
 import mxfp4_inputs as X
 
 pytestmark = pytest.mark.gpu
+PLUS, MINUS = 0x7F80, 0xFF80  # bf16
 
 
 @pytest.fixture(scope="module")
@@ -89,3 +91,32 @@ def test_sinks_of_any_size(M, form, dim, mxfp4, f32):
     want[none], lse64[none], weight[none] = 0, SINKS, 0
     got, lse = attend(M, q64, pages, table, lens, offsets, scale, SINKS, f32)
     compare(got, lse, want, lse64, weight, terms, dim, max(lens), f32)
+
+
+@pytest.mark.parametrize("mxfp4,dim", [(True, 128), (False, 64), (False, 256)])
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_that_are_all_minus_infinity(M, form, sinks, dim, mxfp4):
+    """As without keys, also where the values are infinite; other heads and sequences have none of it."""
+    _, table, pages, lens, offsets, q64 = case(form, dim, mxfp4)
+    q64 = X.from_bf16(X.to_bf16((np.abs(q64) + 0.5).astype(np.float32))).astype(np.float64)
+    hidden = table[0, :-(-lens[0] // 32)]  # the first sequence's keys, of key head 0
+    if mxfp4:
+        pages.k[hidden, 0, :, :4], pages.ks[hidden, 0, :, 0] = 0xFFFFFFFF, 254  # -6 2^127
+        pages.v[hidden[-1:], 0, :, 4:8], pages.vs[hidden[-1:], 0, :, 1] = 0x77777777, 254
+    else:
+        pages.k[hidden, 0, :, 3] = MINUS
+        pages.v[hidden[-1:], 0, :, 9] = PLUS
+    s = np.linspace(-3, 3, 8).astype(np.float32) if sinks else None
+    scale = dim ** -0.5
+    with np.errstate(invalid="ignore"):
+        want, lse64, weight, terms = K.attention(q64, *pages.values(), table, lens, offsets, scale, 0,
+                                                 None if s is None else s.astype(np.float64))
+    owner, seen = keys_seen(lens, offsets, len(q64))
+    for t in range(len(q64)):
+        if owner[t] == 0 or seen[t] == 0:
+            heads = slice(0, 4) if seen[t] else slice(0, 8)
+            want[t, heads], weight[t, heads], terms[t, heads] = 0, 0, 0
+            lse64[t, heads] = -np.inf if s is None else s[heads]
+    got, lse = attend(M, q64, pages, table, lens, offsets, scale, s)
+    compare(got, lse, want, lse64, weight, terms, dim, max(lens), True)
