@@ -756,7 +756,8 @@ mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
  * are tokens q_offsets[b] .. q_offsets[b + 1] - 1 (NULL: token b, batch tokens in
  * all), the last of them at position kv_lens[b] - 1.  A query sees the keys up to
  * its position, or the last `window` of them (0: all).  A key that a query does not
- * see has no part in its output, whatever it holds.  A sink (f32 [heads], or NULL)
+ * see has no part in its output, whatever it holds; an infinite or NaN value of one that
+ * it sees, with a score above -inf, is in its output however small its probability.  A sink (f32 [heads], or NULL)
  * is one more score without a value.  A query that sees no key gets zeros, and so does
  * one whose scores are all -inf (infinite keys): a part of a context that has nothing
  * else weighs nothing where parts are joined by their lse.  Tokens before the first

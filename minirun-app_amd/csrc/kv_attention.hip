@@ -34,7 +34,8 @@
 //
 // Scores of keys that a row does not see become -inf, values that no row may see zeros
 // where they are loaded.  Infinities and NaN of values that some rows of a step see and
-// others do not take a way of their own (kv_add_infinite).
+// others do not, or whose probability left f32's range, take a way of their own
+// (kv_add_infinite).
 #include <algorithm>
 
 #include "kv_tiles.hpp"
@@ -70,7 +71,7 @@ __device__ __forceinline__ void kd_fence() {
 template <int DP, int R, bool MX>
 __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p) {
     using L = KvDecodeLds<DP, MX>;
-    constexpr int ROWS = 16 * R, KS = DP / 32, DT = DP / 16, CPL = DP / 4;
+    constexpr int ROWS = 16 * R, KS = DP / 32, DT = DP / 16, CPL = DP / 4, DN = DP / 64;
     __shared__ __attribute__((aligned(16))) char lds[KD_WAVES * L::WAVE];
     __shared__ float sm[KD_WAVES][ROWS], sl[KD_WAVES][ROWS];
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
@@ -289,13 +290,18 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
         }
     }
 
-    for (int key = apart_from; key < min(apart_to, we); ++key)
+    // infinite values that were left out (kv_add_infinite)
+    kv_each_infinite<DP, MX>(
+        p, t.b, kv_head, apart_from, min(apart_to, we), l, [](int) { return true; },
+        [&](int first, int last) {
+            for (int key = first; key < last; ++key)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+                for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-                kv_add_infinite<MX>(p, t.b, kv_head, key, key >= row[r].lo && key < row[r].hi, 16 * d + 4 * g,
-                                    [&](int j, float v) { o[r][d][j] += v; });
+                    for (int d = 0; d < DT; ++d)
+                        kv_add_infinite<MX>(p, t.b, kv_head, key, key >= row[r].lo && key < row[r].hi, 16 * d + 4 * g,
+                                            [&](int j, float v) { o[r][d][j] += v; });
+        });
 
     // the waves' sums
 #pragma unroll
@@ -325,11 +331,45 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             total = fmaf(sl[x][16 * r + rn], a[x], total);
         }
         const KvRow to = kv_row(p, t, kv_head, t.first_row + 16 * r + rn);
+        f32x4 x[DN];
+#pragma unroll
+        for (int i = 0; i < DN; ++i) {
+            x[i] = f32x4{};
+#pragma unroll
+            for (int y = 0; y < KD_WAVES; ++y)
+                x[i] += a[y] * *(const f32x4*)((const float*)(lds + y * L::WAVE) + rn * L::O_STRIDE + dn + 64 * i);
+        }
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < DN; ++i) nan |= kv_nan(x[i]);
+        nan &= to.ok & (total == total);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(nan) != 0, 0)) {  // (kv_add_infinite)
+            f32x4 y[DN];
+#pragma unroll
+            for (int i = 0; i < DN; ++i) y[i] = f32x4{};
+            bool left = true;
+            kv_each_infinite<DP, MX>(
+                p, t.b, kv_head, kb, ke, l, [&](int) { return left; },
+                [&](int first, int last) {
+                    for (int key = first; key < last; ++key)
+#pragma unroll
+                        for (int i = 0; i < DN; ++i)
+                            kv_add_infinite<MX>(p, t.b, kv_head, key, nan && key >= to.lo && key < to.hi, dn + 64 * i,
+                                                [&](int j, float v) { y[i][j] += v; });
+                    bool more = false;
+#pragma unroll
+                    for (int i = 0; i < 4 * DN; ++i) more |= (x[i / 4][i % 4] != x[i / 4][i % 4]) & (y[i / 4][i % 4] == y[i / 4][i % 4]);
+                    left = __builtin_amdgcn_ballot_w64(nan && more) != 0;
+                });
+#pragma unroll
+            for (int i = 0; i < 4 * DN; ++i)  // (none: sums of finite values have left f32's range)
+                if (nan && x[i / 4][i % 4] != x[i / 4][i % 4] && !(__builtin_fabsf(y[i / 4][i % 4]) < INFINITY)) x[i / 4][i % 4] = y[i / 4][i % 4];
+        }
         if (to.ok) {
             const int64_t at = (int64_t)to.token * (p.kv_heads * p.group) + to.head;
             float inv = 1.f;
             if (p.splits == 1) {
-                const KvEnd end = kv_end(top, total, p.sinks ? p.sinks[to.head] : -INFINITY);
+                const KvEnd end = kv_end(top, total, p.sinks, to.head);
                 inv = end.inv;
                 if (p.lse && dn == 0) p.lse[at] = end.lse;
             } else if (dn == 0) {
@@ -339,21 +379,19 @@ __global__ void __launch_bounds__(64 * KD_WAVES) kv_decode_kernel(KvAttnParams p
             }
             if (p.splits == 1 || total != 0.f) {
 #pragma unroll
-                for (int d = dn; d < DP; d += 64) {
+                for (int i = 0; i < DN; ++i) {
+                    const int d = dn + 64 * i;
                     if (d >= p.dim) break;
-                    f32x4 x{};
-#pragma unroll
-                    for (int y = 0; y < KD_WAVES; ++y)
-                        x += a[y] * *(const f32x4*)((const float*)(lds + y * L::WAVE) + rn * L::O_STRIDE + d);
-                    if (total == 0.f) x = f32x4{};  // (0 times an infinity is not)
                     if (p.splits > 1) {
-                        *(f32x4*)(p.part_o + (at * p.splits + split) * p.dim + d) = x;
-                    } else if (p.out_f32) {
-                        *(f32x4*)((float*)p.out + to.token * p.out_ts + to.head * p.out_hs + d) = x * inv;
-                    } else {
-                        *(u32x2*)((uint16_t*)p.out + to.token * p.out_ts + to.head * p.out_hs + d) =
-                            u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
+                        *(f32x4*)(p.part_o + (at * p.splits + split) * p.dim + d) = x[i];
+                        continue;
                     }
+                    const f32x4 y = total == 0.f ? f32x4{} : kv_weighted(x[i], inv);  // (0 times an infinity is not)
+                    if (p.out_f32)
+                        *(f32x4*)((float*)p.out + to.token * p.out_ts + to.head * p.out_hs + d) = y;
+                    else
+                        *(u32x2*)((uint16_t*)p.out + to.token * p.out_ts + to.head * p.out_hs + d) =
+                            u32x2{pack_bf16x2_hw(y[0], y[1]), pack_bf16x2_hw(y[2], y[3])};
                 }
             }
         }
@@ -413,7 +451,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
     if ((threadIdx.x & 63) == 0) red[w] = total;
     __syncthreads();
     total = (red[0] + red[1]) + (red[2] + red[3]);
-    const KvEnd end = kv_end(top, total, p.sinks ? p.sinks[head] : -INFINITY);
+    const KvEnd end = kv_end(top, total, p.sinks, head);
     const float inv = end.inv;
     if (p.lse && threadIdx.x == 0 && blockIdx.y == 0) p.lse[at] = end.lse;
     f32x4 x{};
@@ -426,17 +464,22 @@ __global__ void __launch_bounds__(256) kv_join_kernel(KvAttnParams p, int span) 
 #pragma unroll 8
         for (int s = share + KJ_EARLY * shares; s < p.splits; s += shares)
             if (!(weight[s] < 0.f)) x += weight[s] * *(const f32x4*)(o + (int64_t)s * p.dim);
+        if (__builtin_expect(kv_nan(x) && total == total, 0)) {  // (an infinity of a part whose weight is 0)
+            x = f32x4{};
+            for (int s = share; s < p.splits; s += shares)
+                if (!(weight[s] < 0.f)) x += kv_weighted(*(const f32x4*)(o + (int64_t)s * p.dim), weight[s]);
+        }
     }
     *(f32x4*)(add + 4 * threadIdx.x) = x;
     __syncthreads();
     if (share) return;
     for (int s = 1; s < shares; ++s) x += *(const f32x4*)(add + 4 * (s * cols + c));
     const int64_t to = token * p.out_ts + head * p.out_hs + d0 + 4 * c;
+    x = kv_weighted(x, inv);
     if (p.out_f32)
-        *(f32x4*)((float*)p.out + to) = x * inv;
+        *(f32x4*)((float*)p.out + to) = x;
     else
-        *(u32x2*)((uint16_t*)p.out + to) =
-            u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
+        *(u32x2*)((uint16_t*)p.out + to) = u32x2{pack_bf16x2_hw(x[0], x[1]), pack_bf16x2_hw(x[2], x[3])};
 }
 
 // The same for many rows of few parts: 2^lanes_log2 lanes have a row, 4 dims a lane, and
@@ -468,16 +511,24 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(KvAttnParams p, int l
         total = fmaf(y[1], a, total);
         if (y[1] != 0.f) x += a * v;
     }
-    const KvEnd end = kv_end(top, total, p.sinks ? p.sinks[head] : -INFINITY);
+    if (__builtin_expect(kv_nan(x) && total == total, 0)) {  // (an infinity of a part whose weight is 0)
+        x = f32x4{};
+        for (int s = first; s < last; ++s) {
+            const f32x2 y = ml[s];
+            if (y[1] != 0.f)
+                x += kv_weighted(*(const f32x4*)(o + (int64_t)s * p.dim), __builtin_amdgcn_exp2f(y[0] - top));
+        }
+    }
+    const KvEnd end = kv_end(top, total, p.sinks, head);
     const float inv = end.inv;
     if (p.lse && c == 0) p.lse[at] = end.lse;
     if (c >= p.dim) return;
     const int64_t to = token * p.out_ts + head * p.out_hs + c;
+    x = kv_weighted(x, inv);
     if (p.out_f32)
-        *(f32x4*)((float*)p.out + to) = x * inv;
+        *(f32x4*)((float*)p.out + to) = x;
     else
-        *(u32x2*)((uint16_t*)p.out + to) =
-            u32x2{pack_bf16x2_hw(x[0] * inv, x[1] * inv), pack_bf16x2_hw(x[2] * inv, x[3] * inv)};
+        *(u32x2*)((uint16_t*)p.out + to) = u32x2{pack_bf16x2_hw(x[0], x[1]), pack_bf16x2_hw(x[2], x[3])};
 }
 
 template <int DP, bool MX>

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
         if (split + 1 < p.splits) ke = (int)min(at + p.chunk, (int64_t)t.kend);
     }
 
-    const KvRow row = kv_row(p, t, kv_head, t.first_row + 32 * w + lq);
+    const KvRow own = kv_row(p, t, kv_head, t.first_row + 32 * w + lq);
     // keys that all of this wave's rows see
     const int w0 = t.first_row + 32 * w, i0 = min(w0 / p.group, t.qn - 1), i1 = min((w0 + 31) / p.group, t.qn - 1);
     const int pos0 = t.len - t.qn + i0, pos1 = t.len - t.qn + i1;
@@ -88,11 +88,11 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
 
     bf16x8 qf[KS];
     {
-        const uint16_t* qp = p.q + row.token * p.q_ts + row.head * p.q_hs;
+        const uint16_t* qp = p.q + own.token * p.q_ts + own.head * p.q_hs;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = 16 * s + 8 * hh;
-            qf[s] = row.ok && d < p.dim ? *(const bf16x8*)(qp + d) : bf16x8{};
+            qf[s] = own.ok && d < p.dim ? *(const bf16x8*)(qp + d) : bf16x8{};
         }
     }
     float m_run = -INFINITY, l_part = 0.f;
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
         const int k0 = kb + KP_KEYS * i;
         const uint32_t f = __builtin_amdgcn_readfirstlane(flags);
         if (!f && k0 >= all_lo && k0 + KP_KEYS <= all_hi) return;
-        int hi = min(row.hi, ke) - k0 - 4 * hh, lo = row.lo - k0 - 4 * hh;
+        int hi = min(own.hi, ke) - k0 - 4 * hh, lo = own.lo - k0 - 4 * hh;
         asm volatile("" : "+v"(hi), "+v"(lo));  // (behind the branch, not 64 compares a tile)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -333,18 +333,61 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
         }
     }
 
-    for (int key = apart_from; key < min(apart_to, ke); ++key)
+    const float total = xor32_sum(l_part);
+    // infinities and NaN (kv_add_infinite): dims that are NaN begin again from 0
+    float any[4] = {};  // (NaN if a dim is, or if some are infinities of both signs)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) any[e & 3] += o[d][e];
+    const float z = (any[0] + any[1]) + (any[2] + any[3]);
+    const bool nan = z != z && own.hi > 0 && total == total;
+    const bool again = __builtin_amdgcn_ballot_w64(nan) != 0;
+    bool left = again;
+    uint32_t lost[DB] = {};  // these dims, a bit each
+    if (__builtin_expect(again, 0)) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                kv_add_infinite<MX>(p, t.b, kv_head, key, key >= row.lo && key < row.hi, 32 * d + 8 * c + 4 * hh,
-                                    [&](int j, float v) { o[d][4 * c + j] += v; });
+            for (int e = 0; e < 16; ++e)
+                if (nan && o[d][e] != o[d][e]) lost[d] |= 1u << e, o[d][e] = 0.f;
+    }
+    kv_each_infinite<DP, MX>(
+        p, t.b, kv_head, again ? kb : apart_from, again ? ke : min(apart_to, ke), l,
+        [&](int k0) { return left || (k0 >= apart_from && k0 < apart_to); },
+        [&](int first, int last) {
+            for (int key = first; key < last; ++key)
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        kv_add_infinite<MX>(p, t.b, kv_head, key, key >= own.lo && key < own.hi, 32 * d + 8 * c + 4 * hh,
+                                            [&](int j, float v) { o[d][4 * c + j] += v; });
+            if (!left) return;
+            bool more = false;  // dims that are not NaN again
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) more = more || ((lost[d] >> e & 1) && o[d][e] == o[d][e]);
+            left = __builtin_amdgcn_ballot_w64(more) != 0;
+        });
+    if (__builtin_expect(again, 0)) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)  // (sums of finite values that left f32's range)
+                if ((lost[d] >> e & 1) && __builtin_fabsf(o[d][e]) < INFINITY) o[d][e] = __builtin_nanf("");
+    }
 
-    const float total = xor32_sum(l_part);
-    const int64_t place = (int64_t)row.token * (p.kv_heads * p.group) + row.head;
+    auto mine = [&]() {  // this lane's row, found again rather than kept in registers
+        int at = lq;
+        asm volatile("" : "+v"(at));
+        return kv_row(p, t, kv_head, t.first_row + 32 * w + at);
+    };
     if (p.splits > 1) {
+        const KvRow row = mine();
         if (!row.ok) return;
+        const int64_t place = (int64_t)row.token * (p.kv_heads * p.group) + row.head;
         if (hh == 0) {
             float* ml = p.part_ml + 2 * (place * p.splits + split);
             ml[0] = m_run;
@@ -361,13 +404,31 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             }
         return;
     }
-    const KvEnd end = kv_end(m_run, total, p.sinks && row.ok ? p.sinks[row.head] : -INFINITY);
+    int head = 0;
+    if (p.sinks) {
+        const KvRow row = mine();
+        head = row.ok ? row.head : 0;
+    }
+    const KvEnd end = kv_end(m_run, total, p.sinks, head);
     const float inv = end.inv;
     if (total == 0.f)
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = f32x16{};  // (0 times an infinity is not)
-    if (p.lse && row.ok && hh == 0) p.lse[place] = end.lse;
+    if (__builtin_expect(inv != 0.f, 1)) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] *= inv;
+    } else {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = kv_weighted(o[d][e], inv);
+    }
+    if (p.lse && hh == 0) {
+        const KvRow row = mine();
+        if (row.ok) p.lse[(int64_t)row.token * (p.kv_heads * p.group) + row.head] = end.lse;
+    }
     if (p.out_f32) {
+        const KvRow row = mine();
         if (!row.ok) return;
         float* to = (float*)p.out + row.token * p.out_ts + row.head * p.out_hs;
 #pragma unroll
@@ -376,7 +437,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
             for (int i = 0; i < 4; ++i) {
                 const int c = 32 * d + 8 * i + 4 * hh;
                 if (c < p.dim)
-                    *(f32x4*)(to + c) = f32x4{o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv};
+                    *(f32x4*)(to + c) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             }
         return;
     }
@@ -388,8 +449,7 @@ __global__ void __launch_bounds__(64 * kp_waves(DP), kp_waves(DP) / 4) kv_prompt
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             *(u32x2*)(st + lq * DP + (((4 * d + i) ^ (lq & 7)) << 3) + 4 * hh) =
-                u32x2{pack_bf16x2_hw(o[d][4 * i] * inv, o[d][4 * i + 1] * inv),
-                      pack_bf16x2_hw(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv)};
+                u32x2{pack_bf16x2_hw(o[d][4 * i], o[d][4 * i + 1]), pack_bf16x2_hw(o[d][4 * i + 2], o[d][4 * i + 3])};
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");

@@ -96,18 +96,21 @@ __device__ __forceinline__ KvRow kv_row(const KvAttnParams& p, const KvTile& t, 
     return r;
 }
 
-// What a row's sums come to with its sink (-inf: none): the factor of its output and the
-// logarithm, from the running maximum of its scores in base 2 and their sum.  In natural units,
-// since a sink may be any f32 and many would leave f32 in base 2.
+// What a row's sums come to with its head's sink (sinks null: none): the factor of its output
+// and the logarithm, from the running maximum of its scores in base 2 and their sum.  The sink
+// is met in natural units, since it may be any f32 and many would leave f32 in base 2.
 struct KvEnd {
     float inv, lse;
 };
-__device__ __forceinline__ KvEnd kv_end(float top, float total, float sink) {
+__device__ __forceinline__ KvEnd kv_end(float top, float total, const float* sinks, int head) {
+    constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
+    if (!sinks) return total == 0.f ? KvEnd{0.f, -INFINITY} : KvEnd{1.f / total, (top + __builtin_amdgcn_logf(total)) * LN2};
+    const float sink = sinks[head];
     if (total == 0.f) return KvEnd{0.f, sink};  // no key is seen, or none with a score above -inf: zeros
-    const float m = top * 0.6931471805599453f, up = fmaxf(m, sink);
-    const float was = __builtin_amdgcn_exp2f((m - up) * 1.4426950408889634f);
-    const float all = fmaf(total, was, __builtin_amdgcn_exp2f((sink - up) * 1.4426950408889634f));
-    return KvEnd{was / all, up + __builtin_amdgcn_logf(all) * 0.6931471805599453f};
+    const float m = top * LN2, up = fmaxf(m, sink);
+    const float was = __builtin_amdgcn_exp2f((m - up) * LOG2E);
+    const float all = fmaf(total, was, __builtin_amdgcn_exp2f((sink - up) * LOG2E));
+    return KvEnd{was / all, up + __builtin_amdgcn_logf(all) * LN2};
 }
 
 // The groups of 16 keys of a sequence, one after another: a page holds a whole
@@ -280,12 +283,16 @@ struct KvGroup {
     }
 };
 
-// Where some rows of a tile see a key and others do not, 0 times an infinity or a NaN
-// of its value would reach the others through the product.  Such values are zeros in
-// LDS (KvGroup::clean), and this adds at the end what they come to: to each dim of a row
-// that sees the key, the infinity or NaN itself (again where the product had it, which
-// changes nothing).  add(j, v): to dims d0 + j (j < 4) of the lane's row.  `key` and
-// the sequence are wave-uniform, d0 is the lane's.
+// An infinite or NaN value of a key that a row sees makes its dim of the row so, however
+// small the key's probability.  A product does not always say that:
+//   - where some rows of a tile see a key and others do not, 0 times such a value would
+//     reach the others: it is a zero in LDS (KvGroup::clean);
+//   - where a probability, or a factor that sums are rescaled by, has left f32's range, 0
+//     times an infinity is NaN for the row that sees it too.
+// So at the end the keys of the former, and all of a row's keys where a dim is NaN, are
+// looked through again, and what they hold is added: the infinity or NaN itself.  (Again
+// where the product had it, which changes nothing.)  add(j, v): to dims d0 + j (j < 4) of
+// the lane's row.  `key` and the sequence are wave-uniform, d0 is the lane's.
 template <bool MX, typename F>
 __device__ __forceinline__ void kv_add_infinite(const KvAttnParams& p, int b, int kv_head, int key, bool sees, int d0, F&& add) {
     const int page = key / p.page_size, id = s_load(p.table + b * p.table_stride + page);
@@ -305,6 +312,36 @@ __device__ __forceinline__ void kv_add_infinite(const KvAttnParams& p, int b, in
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if ((v[j] & 0x7f800000u) == 0x7f800000u) add(j, __uint_as_float(v[j]));
+}
+
+// Groups of 16 keys (`from` a multiple of 16) with values of this head that are infinite or
+// NaN: each(first, last).  wanted(first): whether to look at a group.  A wave together.
+template <int DP, bool MX, typename W, typename F>
+__device__ __forceinline__ void kv_each_infinite(const KvAttnParams& p, int b, int kv_head, int from, int to, int l, W&& wanted,
+                                                 F&& each) {
+    using Group = KvGroup<DP, MX>;
+    const typename Group::At at = Group::at(p.dim, l);
+    if (__builtin_expect(from >= to, 1)) return;
+    for (int k0 = from; k0 < to; k0 += 16) {
+        if (!wanted(k0)) continue;
+        const int page = k0 / p.page_size, id = s_load(p.table + b * p.table_stride + page);
+        if (!kv_page(p, id)) continue;
+        Group v;
+        v.load(kv_from<MX>(p, false, kv_head, id, k0 - page * p.page_size), at);
+        if (__builtin_amdgcn_ballot_w64(v.not_finite())) each(k0, min(k0 + 16, to));
+    }
+}
+
+// v times a weight or factor that may have left f32's range
+__device__ __forceinline__ float kv_weighted(float v, float a) {
+    return a == 0.f && !(__builtin_fabsf(v) < INFINITY) ? v : a * v;
+}
+__device__ __forceinline__ f32x4 kv_weighted(f32x4 v, float a) {
+    if (__builtin_expect(a != 0.f, 1)) return a * v;
+    return f32x4{kv_weighted(v[0], a), kv_weighted(v[1], a), kv_weighted(v[2], a), kv_weighted(v[3], a)};
+}
+__device__ __forceinline__ bool kv_nan(f32x4 v) {
+    return __builtin_isunordered(v[0], v[1]) | __builtin_isunordered(v[2], v[3]);
 }
 
 }  // namespace mr

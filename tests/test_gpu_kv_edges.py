@@ -1,6 +1,7 @@
 """Ends of the softmax of attention over a paged cache, in every form (whole and in parts, one
-query and many, both joins): sinks of any f32, and keys whose scores are all -inf.  Tolerances
-as in test_gpu_kv_attention.py."""
+query and many, both joins): sinks of any f32, keys whose scores are all -inf, and infinite
+values of keys whose probability is less than f32 holds.  Tolerances as in
+test_gpu_kv_attention.py."""
 import numpy as np
 import pytest
 
@@ -8,7 +9,7 @@ import kv_inputs as K
 import mxfp4_inputs as X
 
 pytestmark = pytest.mark.gpu
-PLUS, MINUS = 0x7F80, 0xFF80  # bf16
+NAN, PLUS, MINUS = 0x7FC0, 0x7F80, 0xFF80  # bf16
 
 
 @pytest.fixture(scope="module")
@@ -120,3 +121,58 @@ def test_scores_that_are_all_minus_infinity(M, form, sinks, dim, mxfp4):
             lse64[t, heads] = -np.inf if s is None else s[heads]
     got, lse = attend(M, q64, pages, table, lens, offsets, scale, s)
     compare(got, lse, want, lse64, weight, terms, dim, max(lens), True)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("mxfp4,dim", [(True, 64), (True, 128), (False, 128), (True, 256), (False, 96)])
+@pytest.mark.parametrize("sink", [None, 2000.0])
+@pytest.mark.parametrize("form", FORMS)
+def test_infinite_values_of_any_probability(M, form, sink, dim, mxfp4, f32):
+    """Scores of +-150 and more, so that most probabilities are less than f32 holds (with the sink: all).
+    Infinite values reach every query that sees them, whichever tile or part they are in."""
+    rng, table, pages, lens, offsets, q64 = case(form, dim, mxfp4, 1)
+    scale, kv_heads = 3.0, pages.shape[1]
+    cols = 32 if mxfp4 else 1
+    odd = {}  # (sequence, key, key head) -> {dim: value}
+    for b, n in enumerate(lens):
+        for j in {0, 1, n // 2, n - 1, n - 2, *rng.integers(0, max(n, 1), 6).tolist()}:
+            if not 0 <= j < n:
+                continue
+            page, row, h = table[b, j // 32], j % 32, int(rng.integers(kv_heads))
+            block, value = int(rng.integers(dim // cols)), [np.inf, -np.inf, np.nan][int(rng.choice(3, p=[0.45, 0.45, 0.1]))]
+            odd[b, j, h] = {d: value for d in range(block * cols, (block + 1) * cols)}
+            if not mxfp4:
+                pages.v[page, h, row, block] = {np.inf: PLUS, -np.inf: MINUS}.get(value, NAN)
+            elif np.isnan(value):
+                pages.vs[page, h, row, block] = 255
+            else:
+                pages.vs[page, h, row, block] = 254
+                pages.v[page, h, row, 4 * block:4 * block + 4] = 0x77777777 if value > 0 else 0xFFFFFFFF
+    s = None if sink is None else np.full(q64.shape[1], sink, np.float32)
+    k64, v64 = pages.values()
+    want, lse64, weight, terms = K.attention(q64, k64, np.where(np.isfinite(v64), v64, 0), table, lens, offsets, scale, 0,
+                                             None if s is None else s.astype(np.float64))
+    owner, seen = keys_seen(lens, offsets, len(q64))
+    none = seen == 0
+    want[none], weight[none] = 0, 0
+    lse64[none] = -np.inf if s is None else sink
+    with np.errstate(invalid="ignore"):
+        for (b, j, h), dims in odd.items():
+            rows = np.flatnonzero((owner == b) & (seen > j))
+            for d, value in dims.items():
+                want[rows[:, None], np.arange(4 * h, 4 * h + 4)[None], d] += value
+    got, lse = attend(M, q64, pages, table, lens, offsets, scale, s, f32)
+    compare(got, lse, want, lse64, weight, terms, dim, max(lens), f32)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("mxfp4", [False, True])
+def test_values_that_are_all_nan(M, form, mxfp4):
+    _, table, pages, lens, offsets, q64 = case(form, 128, mxfp4)
+    if mxfp4:
+        pages.vs[:] = 255
+    else:
+        pages.v[:] = NAN
+    got, lse = attend(M, q64, pages, table, lens, offsets, 0.1)
+    none = keys_seen(lens, offsets, len(q64))[1] == 0
+    assert np.isnan(got[~none]).all() and (got[none] == 0).all() and np.array_equal(np.isneginf(lse).all(1), none)
