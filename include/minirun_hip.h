@@ -666,8 +666,8 @@ typedef struct mr_rotary {
     mr_rope_pairs pairs;
 } mr_rotary;
 
-/* The queries' or the keys' heads [tokens][heads][dim], strides in elements; no
- * heads: heads 0.  `out` may be x (backward: x or d_out) itself, of the same
+/* The queries' or the keys' heads [tokens][heads][dim], strides in elements (here and
+ * below, that of an axis of one entry is not read); no heads: heads 0.  `out` may be x (backward: x or d_out) itself, of the same
  * strides and type; it overlaps no input otherwise, and its rows are apart. */
 typedef struct mr_head_rows {
     int32_t heads;

@@ -21,6 +21,8 @@ bool act(mr_dtype d) { return d == MR_BF16 || d == MR_F32; }
 int size_of(mr_dtype d) { return d == MR_F32 ? 4 : 2; }
 bool elem_aligned(const void* p, mr_dtype d) { return reinterpret_cast<uintptr_t>(p) % size_of(d) == 0; }
 mr_status done(hipError_t e, const char* what) { return e == hipSuccess ? MR_OK : hip_fail(e, what); }
+// nothing lies a stride away along an axis of one entry
+int64_t stride_of(int64_t entries, int64_t stride) { return entries > 1 ? stride : 0; }
 bool stride_in(int64_t s) { return s >= 0 && s <= FAR; }
 
 int64_t lanes_of(int dim) {
@@ -99,23 +101,22 @@ mr_status head_norm(const mr_head_norm_args* a, bool backward, void* stream) {
         if (!elem_aligned(r.x, a->x_dtype) || !elem_aligned(r.out, a->out_dtype) ||
             (backward && !elem_aligned(r.d_out, a->x_dtype)))
             return fail(MR_INVALID_ARGUMENT, "%s: misaligned rows", what);
-        if (!stride_in(r.x_token_stride) || !stride_in(r.x_head_stride) ||
-            (backward && (!stride_in(r.d_out_token_stride) || !stride_in(r.d_out_head_stride))))
-            return fail(MR_INVALID_ARGUMENT, "%s: strides must be 0 to 2^40", what);
-        if (!rows_apart(a->tokens, r.heads, a->dim, r.out_token_stride, r.out_head_stride))
-            return fail(MR_INVALID_ARGUMENT, "%s: strides %lld and %lld of the output make rows of %d meet", what,
-                        (long long)r.out_token_stride, (long long)r.out_head_stride, a->dim);
         s.x = r.x;
-        s.x_ts = r.x_token_stride;
-        s.x_hs = r.x_head_stride;
+        s.x_ts = stride_of(a->tokens, r.x_token_stride);
+        s.x_hs = stride_of(r.heads, r.x_head_stride);
         s.out = r.out;
-        s.out_ts = r.out_token_stride;
-        s.out_hs = r.out_head_stride;
+        s.out_ts = stride_of(a->tokens, r.out_token_stride);
+        s.out_hs = stride_of(r.heads, r.out_head_stride);
         if (backward) {
             s.dy = r.d_out;
-            s.dy_ts = r.d_out_token_stride;
-            s.dy_hs = r.d_out_head_stride;
+            s.dy_ts = stride_of(a->tokens, r.d_out_token_stride);
+            s.dy_hs = stride_of(r.heads, r.d_out_head_stride);
         }
+        if (!stride_in(s.x_ts) || !stride_in(s.x_hs) || !stride_in(s.dy_ts) || !stride_in(s.dy_hs))
+            return fail(MR_INVALID_ARGUMENT, "%s: strides must be 0 to 2^40", what);
+        if (!rows_apart(a->tokens, r.heads, a->dim, s.out_ts, s.out_hs))
+            return fail(MR_INVALID_ARGUMENT, "%s: strides %lld and %lld of the output make rows of %d meet", what,
+                        (long long)r.out_token_stride, (long long)r.out_head_stride, a->dim);
     }
     if (p.seg[0].dw && p.seg[0].dw == p.seg[1].dw)
         return fail(MR_INVALID_ARGUMENT, "%s: one d_weight for queries and keys (it is written, not added to)", what);
@@ -220,16 +221,15 @@ mr_status mr_kv_append(const mr_kv_append_args* a, void* stream) {
     if (!elem_aligned(a->k, a->dtype) || !elem_aligned(a->v, a->dtype) || !mrc::aligned4(a->slots) ||
         (a->normalize && !elem_aligned(a->norm_w, a->norm_w_dtype)))
         return fail(MR_INVALID_ARGUMENT, "%s: a misaligned pointer", what);
-    if (!stride_in(a->k_token_stride) || !stride_in(a->k_head_stride) || !stride_in(a->v_token_stride) ||
-        !stride_in(a->v_head_stride))
+    p.k_ts = stride_of(a->tokens, a->k_token_stride);
+    p.k_hs = stride_of(c.kv_heads, a->k_head_stride);
+    p.v_ts = stride_of(a->tokens, a->v_token_stride);
+    p.v_hs = stride_of(c.kv_heads, a->v_head_stride);
+    if (!stride_in(p.k_ts) || !stride_in(p.k_hs) || !stride_in(p.v_ts) || !stride_in(p.v_hs))
         return fail(MR_INVALID_ARGUMENT, "%s: strides must be 0 to 2^40", what);
     if (!c.pages) return MR_OK;
     p.k = a->k;
     p.v = a->v;
-    p.k_ts = a->k_token_stride;
-    p.k_hs = a->k_head_stride;
-    p.v_ts = a->v_token_stride;
-    p.v_hs = a->v_head_stride;
     p.tokens = a->tokens;
     p.heads = c.kv_heads;
     p.dim = c.head_dim;
@@ -269,11 +269,11 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     if (!a->tokens || !a->batch) return MR_OK;
     if (!a->q || !a->out || !a->kv_lens || (a->max_pages && !a->page_table))
         return fail(MR_INVALID_ARGUMENT, "%s: q, out, kv_lens and page_table must be non-NULL", what);
-    if (!mrc::aligned16(a->q) || !mrc::aligned16(a->out) || a->q_token_stride % 8 || a->q_head_stride % 8 ||
-        a->out_token_stride % 8 || a->out_head_stride % 8)
+    const int64_t q_ts = stride_of(a->tokens, a->q_token_stride), q_hs = stride_of(a->heads, a->q_head_stride);
+    const int64_t out_ts = stride_of(a->tokens, a->out_token_stride), out_hs = stride_of(a->heads, a->out_head_stride);
+    if (!mrc::aligned16(a->q) || !mrc::aligned16(a->out) || q_ts % 8 || q_hs % 8 || out_ts % 8 || out_hs % 8)
         return fail(MR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned, their strides multiples of 8", what);
-    if (!stride_in(a->q_token_stride) || !stride_in(a->q_head_stride) ||
-        !rows_apart(a->tokens, a->heads, c.head_dim, a->out_token_stride, a->out_head_stride))
+    if (!stride_in(q_ts) || !stride_in(q_hs) || !rows_apart(a->tokens, a->heads, c.head_dim, out_ts, out_hs))
         return fail(MR_INVALID_ARGUMENT, "%s: strides of q must be 0 to 2^40, and rows of out apart", what);
     if (!mrc::aligned4(a->page_table) || !mrc::aligned4(a->kv_lens) || !mrc::aligned4(a->q_offsets) ||
         !mrc::aligned4(a->sinks) || !mrc::aligned4(a->lse) ||
@@ -286,8 +286,8 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
         return fail(MR_INVALID_ARGUMENT, "%s: NULL or misaligned workspace (16 bytes)", what);
     mr::KvAttnParams p{};
     p.q = (const uint16_t*)a->q;
-    p.q_ts = a->q_token_stride;
-    p.q_hs = a->q_head_stride;
+    p.q_ts = q_ts;
+    p.q_hs = q_hs;
     p.k = (const char*)c.k;
     p.v = (const char*)c.v;
     p.k_scales = c.k_scales;
@@ -310,8 +310,8 @@ mr_status mr_kv_attention(const mr_kv_attention_args* a, void* stream) {
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.sinks = a->sinks;
     p.out = a->out;
-    p.out_ts = a->out_token_stride;
-    p.out_hs = a->out_head_stride;
+    p.out_ts = out_ts;
+    p.out_hs = out_hs;
     p.out_f32 = a->out_dtype == MR_F32;
     p.lse = a->lse;
     p.splits = r.splits;
