@@ -1013,6 +1013,11 @@ def expert_dispatch_backward(d_rows, order: ExpertOrder, stream=None):
 # (Of a small call's 10 us most is Python, about 0.1 us a tensor's attribute and 0.4 a
 # nested call, so tensors are checked in one comparison each and structures filled at
 # once.)
+def _past_int32(what):
+    """For numbers that the library takes in 32 bits: ctypes would keep their low half."""
+    raise ValueError(f"{what} must be 0 to 2^31 - 1")
+
+
 def _first_heads(t, name):
     """Shape, device and type of a call's first tensor [tokens, heads, dim]."""
     if not isinstance(t, _torch().Tensor) or not t.is_cuda:
@@ -1020,6 +1025,8 @@ def _first_heads(t, name):
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f"{name} must be [tokens, heads, dim], got {list(shape)}")
+    if (shape[0] | shape[1] | shape[2]) >> 31:
+        _past_int32("tokens, heads and dim")
     return shape, t.device, t.dtype
 
 
@@ -1068,6 +1075,8 @@ def _rotary(device, tokens, cos_t, sin_t, positions, col0, halves):
             or not sin_t.is_contiguous()):
         raise ValueError(f"cos_t and sin_t must both be whole float32 [rows, pairs] on {device}")
     rows, half = cos_t.shape
+    if (col0 | 2 * half) >> 31:
+        _past_int32("col0 and the rotated columns")
     return Rotary(cos_t.data_ptr(), sin_t.data_ptr(), _vector(positions, "positions", tokens, device, torch.int32), rows,
                   2 * half, col0, 1 if halves else 0)
 
@@ -1101,6 +1110,8 @@ def head_norm_rope(q, k=None, *, q_weight=None, k_weight=None, eps=1e-6, cos_t=N
             strides = _heads_like(k, "k", (T, None, D), device, dtype)
             z = _room(k, otype) if k_out is None else k_out
             heads = k.shape[1]
+            if heads >> 31:
+                _past_int32("k's heads")
             rows_k = HeadRows(heads, k.data_ptr(), *strides, _vector(k_weight, "k_weight", D, device, wtype), z.data_ptr(),
                               *((heads * D, D) if k_out is None else _heads_like(z, "k_out", k.shape, device, otype)))
         a = HeadNormArgs(T, D, rows_q, rows_k, _code(dtype), _code(wtype), _code(otype), eps,
@@ -1133,6 +1144,8 @@ def head_norm_rope_backward(d_q, q, d_k=None, k=None, *, q_weight=None, k_weight
             dx = _room(x, dtype)
             dw = None if weight is None else _room(weight, torch.float32)
             heads = x.shape[1]
+            if heads >> 31:
+                _past_int32(f"{name}'s heads")
             rows.append(HeadRows(heads, x.data_ptr(), *strides, _vector(weight, f"{name}_weight", D, device, wtype),
                                  dx.data_ptr(), heads * D, D, d.data_ptr(),
                                  *_heads_like(d, f"d_{name}", x.shape, device, dtype), None if dw is None else dw.data_ptr()))
@@ -1268,6 +1281,8 @@ def kv_attention(q, cache: KVCache, page_table, kv_lens, *, scale, q_offsets=Non
         raise ValueError(f"page_table must be int32 [batch, max_pages] on {device}, got {page_table.dtype} "
                          f"{list(page_table.shape)} on {page_table.device}")
     B, most = page_table.shape
+    if (B | most | window | max_kv_len) >> 31:
+        _past_int32("page_table's sizes, window and max_kv_len")
     ld, step = page_table.stride()
     if step != 1 and most > 1:
         raise ValueError("page_table must be contiguous in its last dimension")

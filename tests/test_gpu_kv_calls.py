@@ -1,4 +1,5 @@
-"""Calls of the paged cache from Python that its documentation allows: strides of axes of one entry."""
+"""Calls of the paged cache from Python that its documentation allows or refuses: strides of
+axes of one entry, numbers past 32 bits."""
 import numpy as np
 import pytest
 
@@ -50,3 +51,38 @@ def test_strides_of_axes_of_one_entry(M, tokens, heads):
         M.kv_append(a, q, q, slots)
         M.kv_append(b, strange, strange, slots)
         assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+
+
+def test_numbers_past_32_bits_are_refused(M):
+    """ctypes keeps the low 32 bits of a number, which would be another window or column."""
+    import torch
+
+    cache = M.KVCache.zeros(2, 1, 16, 64)
+    q = torch.zeros(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    table, lens = ints(0).reshape(1, 1), ints(5)
+    trig = torch.zeros(1, 4, device="cuda")
+    k = torch.zeros(1, 1, 64, device="cuda")
+    bad = [lambda n: M.kv_attention(q, cache, table, lens, scale=1.0, window=n),
+           lambda n: M.kv_attention(q, cache, table, lens, scale=1.0, max_kv_len=n),
+           lambda n: M.head_norm_rope(q, cos_t=trig, sin_t=trig, col0=n),
+           lambda n: M.head_norm_rope_backward(q, q, cos_t=trig, sin_t=trig, col0=n),
+           lambda n: M.kv_append(cache, k, k, ints(0), cos_t=trig, sin_t=trig, col0=n)]
+    for i, call in enumerate(bad):
+        for n in (2 ** 32, 2 ** 32 + 3, 2 ** 31, -2 ** 32, 2 ** 70):
+            with pytest.raises((M.MRError, TypeError, ValueError)):
+                call(n)
+                print("accepted", i, n)
+
+
+def test_sizes_past_32_bits_are_refused(M):
+    """2^32 + 1 tokens or heads (of one row in memory) are not one."""
+    import torch
+
+    many = 2 ** 32 + 1
+    one = torch.ones(1, 1, 8, device="cuda", dtype=torch.bfloat16)
+    out = torch.zeros(1, 1, 8, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises((M.MRError, ValueError)):
+        M.head_norm_rope(one.expand(many, 1, 8), q_out=out.expand(many, 1, 8))
+    with pytest.raises((M.MRError, ValueError)):
+        M.head_norm_rope(one, one.expand(1, many, 8), k_out=out.expand(1, many, 8))
+    assert (out == 0).all()
