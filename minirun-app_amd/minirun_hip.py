@@ -1165,7 +1165,13 @@ class KVCache:
     head_dim] bf16, or MXFP4: int32 (or uint32) words [..., head_dim / 8] with
     k_scales, v_scales uint8 [..., head_dim / 32].  page_size is a multiple of 16,
     head_dim one of 32 up to 256; pages may lie apart (their stride, the same for
-    k and v), what is inside one may not."""
+    k and v), what is inside one may not.  Its attributes stay as they are: calls take
+    the tensors' addresses from here, so other tensors are another KVCache."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{name} of a KVCache stays as it is; make another one of other tensors")
+        super().__setattr__(name, value)
 
     def __init__(self, k, v, k_scales=None, v_scales=None):
         torch = _torch()

@@ -1,5 +1,5 @@
 """Calls of the paged cache from Python that its documentation allows or refuses: strides of
-axes of one entry, numbers past 32 bits."""
+axes of one entry, numbers past 32 bits, a cache whose tensors would be exchanged."""
 import numpy as np
 import pytest
 
@@ -86,3 +86,15 @@ def test_sizes_past_32_bits_are_refused(M):
     with pytest.raises((M.MRError, ValueError)):
         M.head_norm_rope(one, one.expand(1, many, 8), k_out=out.expand(1, many, 8))
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("mxfp4", [False, True])
+def test_a_cache_keeps_its_tensors(M, mxfp4):
+    """What calls take lies behind the addresses that the cache was made with."""
+    import torch
+
+    cache = M.KVCache.zeros(2, 1, 16, 64, mxfp4=mxfp4)
+    for name in ("k", "v", "k_scales", "v_scales", "pages", "page_size", "kv_heads", "head_dim", "device"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros(4, 1, 16, 64, device="cuda"))
+    assert cache.k.shape[0] == cache.pages == 2 and cache.head_dim == 64 and (cache.k_scales is not None) == mxfp4
