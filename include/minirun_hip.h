@@ -770,9 +770,11 @@ mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
  * (and sink); -inf where there is none.  With f32 out it joins parts of a context
  * attended elsewhere.
  *   q and out are 16-byte aligned, their strides multiples of 8.  heads a multiple of
- * cache.kv_heads; tokens * heads and max_pages * page_size at most 2^30.  max_kv_len: about the most keys of
- * a sequence (0: what a table row holds); it decides how the work is split, so it is
- * part of the workspace's size, and a longer sequence is right but slow.  Which kernel
+ * cache.kv_heads; tokens * heads and max_pages * page_size at most 2^30.  max_kv_len:
+ * about the most keys of a sequence (0: what a table row holds); it decides how the work
+ * is split, so it is part of the workspace's size, a longer sequence is right but slow,
+ * and parts that no sequence is long enough for are launched all the same: give it where
+ * table rows hold much more than the sequences have.  A workspace has 0.3 GB at most.  Which kernel
  * runs, and so a result's last bits, depends on the sizes of the call alone: on the
  * average of queries of a sequence, so prompts and single tokens run faster apart. */
 typedef struct mr_kv_attention_args {

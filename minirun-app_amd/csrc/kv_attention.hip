@@ -580,8 +580,14 @@ hipError_t decode_dim(const KvAttnParams& p, int rows, unsigned grid, hipStream_
 //     4 tiles, 16 queries behind 2000, in 128 / 256 / 512 17.7 / 18.9 / 23.2), and few keys
 //     in one (16 queries of 250 in 128 / whole 16.1 / 12.1, of 400 16.7 / 17.2; 512 queries
 //     of 512, 64 tiles, 30 / 23)
+//   at most 32 workgroups a CU in parts: more of them cost more than what unequal lengths leave
+//     idle, and workspace without end (64 sequences, 8 key heads, of 8000 to 65536 keys, by
+//     8 / 16 / 32 / 64 / any 395 / 378 / 383 / 401 / 423; of 1 to 65536, each 1.25 times the
+//     next, 202 / 131 / 115 / 122 / 138; 256 of 4000 to 32768 662 / 727 / 713 / 741 / 818)
 // A tile of the few-query kernel has at most 64 rows (32 of 256 dims: registers).  More
 // are prompts: 128 rows behind 16000 keys 27.8 us as such, 32.6 in tiles of 64.
+constexpr int KV_PARTS = 32;  // workgroups a CU, where there are parts
+
 KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_heads, int group, int dim, int window,
                                int64_t keys, int cu_count) {
     KvAttnRoute r;
@@ -593,7 +599,7 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     const int64_t groups = batch * ((rows + r.rows - 1) / r.rows) * kv_heads;  // workgroups without parts
     // a tile's queries span at most its rows' positions
     if (window) keys = std::min<int64_t>(keys, (int64_t)window + r.rows + 16);
-    const int64_t work = groups * std::max<int64_t>(keys, 1), cus = cu_count;
+    const int64_t cus = cu_count, work = std::min(groups, KV_PARTS * cus) * std::max<int64_t>(keys, 1);
     int64_t chunk;
     if (r.prompt) {
         chunk = std::max<int64_t>(128, groups >= cus ? keys : (keys + cus / groups - 1) / (cus / groups));
@@ -607,7 +613,8 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
         chunk = std::min<int64_t>(chunk, r.rows > 16 && fit == 1 ? 2048 : 1536);
         if (keys <= 512 || (groups >= 2 * cus && keys <= 4096)) chunk = keys;
     }
-    chunk = std::max(chunk, (keys + KJ_MAX - 1) / KJ_MAX);
+    const int64_t most = std::min<int64_t>(KJ_MAX, std::max<int64_t>(1, KV_PARTS * cus / groups));
+    chunk = std::max(chunk, (keys + most - 1) / most);
     chunk = std::max<int64_t>(64, (chunk + 63) / 64 * 64);
     r.splits = (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk);
     if (tokens * kv_heads * group > (1 << 20)) r.splits = 1;  // (the join has a workgroup per row)

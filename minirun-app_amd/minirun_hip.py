@@ -1274,7 +1274,7 @@ def kv_attention(q, cache: KVCache, page_table, kv_lens, *, scale, q_offsets=Non
     sequence, or sequence b's are q_offsets[b] .. q_offsets[b + 1] - 1 (int32
     [batch + 1]), the last of them at its last key.  window: the last so many keys
     only; sinks f32 [heads]; max_kv_len: about the most keys of a sequence (0: what
-    a table row holds).  out [tokens, heads, head_dim] bf16 (or f32); tokens of no
+    a table row holds, which is slower where that is much more).  out [tokens, heads, head_dim] bf16 (or f32); tokens of no
     sequence are not written (give `out` to keep what they hold).  return_lse: also
     the log of the sum of exp, f32 [tokens, heads]."""
     torch = _torch()
