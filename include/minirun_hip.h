@@ -770,7 +770,10 @@ mr_status mr_kv_append(const mr_kv_append_args *args, void *stream);
  * (and sink); -inf where there is none.  With f32 out it joins parts of a context
  * attended elsewhere.
  *   q and out are 16-byte aligned, their strides multiples of 8.  heads a multiple of
- * cache.kv_heads; tokens * heads and max_pages * page_size at most 2^30.  max_kv_len:
+ * cache.kv_heads; tokens * heads and max_pages * page_size at most 2^30.  A launch takes
+ * less than 2^24 workgroups, for prompts of heads up to 128 less than 2^23: one for each key
+ * head and each 16, 32, 64 (few queries) or 256 (128 for longer heads) rows (query, head of
+ * the group) of a sequence, the sequences rounded up; larger calls are refused.  max_kv_len:
  * about the most keys of a sequence (0: what a table row holds); it decides how the work
  * is split, so it is part of the workspace's size, a longer sequence is right but slow,
  * and parts that no sequence is long enough for are launched all the same: give it where

@@ -176,12 +176,12 @@ mr_status attention_route(const mr_kv_attention_args* a, mr::KvAttnRoute& r) {
     const int64_t holds = int64_t(a->max_pages) * c.page_size;
     const int64_t keys = a->max_kv_len ? std::min<int64_t>(a->max_kv_len, holds) : holds;
     if (!a->batch || !a->tokens) {
-        r = mr::KvAttnRoute{false, 16, 0, 1, 64};
+        r = mr::KvAttnRoute{false, 16, 0, 1, 64, 256};
         return MR_OK;
     }
     r = mr::kv_attention_route(a->tokens, a->batch, a->q_offsets != nullptr, c.kv_heads, a->heads / c.kv_heads, c.head_dim,
                                a->window, keys, mrc::cu_count());
-    if (r.tiles * c.kv_heads * r.splits >= (int64_t(1) << 24))
+    if (r.tiles * c.kv_heads * r.splits >= (int64_t(1) << 32) / r.threads)
         return fail(MR_INVALID_SHAPE, "%s: %lld tiles of %d key heads are more than one launch takes", what, (long long)r.tiles,
                     c.kv_heads);
     return MR_OK;

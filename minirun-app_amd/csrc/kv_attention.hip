@@ -595,6 +595,7 @@ KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_he
     r.prompt = rows > (dim > 128 ? 32 : 64);
     // tiles of as few rows as hold a sequence's
     r.rows = r.prompt ? (dim > 128 ? 128 : 256) : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    r.threads = r.prompt ? 2 * r.rows : 64 * KD_WAVES;  // (a wave has 32 rows of a prompt)
     r.tiles = ragged ? (tokens * group + r.rows - 1) / r.rows + batch : int64_t(batch) * ((group + r.rows - 1) / r.rows);
     const int64_t groups = batch * ((rows + r.rows - 1) / r.rows) * kv_heads;  // workgroups without parts
     // a tile's queries span at most its rows' positions

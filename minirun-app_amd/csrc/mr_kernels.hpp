@@ -680,6 +680,7 @@ struct KvAttnRoute {
     int rows;  // of a tile: (query, head of the group) pairs
     int64_t tiles;
     int splits, chunk;
+    int threads;  // of a workgroup
 };
 KvAttnRoute kv_attention_route(int64_t tokens, int batch, bool ragged, int kv_heads, int group, int dim, int window,
                                int64_t keys, int cu_count);

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 import minirun_hip as M
-from test_host_kv import FAR, append_args, attention_args, norm_args, refused
+from test_host_kv import AT, FAR, append_args, attention_args, norm_args, refused
 
 
 @pytest.fixture(scope="module")
@@ -32,3 +32,20 @@ def test_strides_of_axes_of_one_entry_are_not_read(lib):
                     dict(cache=dict(kv_heads=1, pages=0, k=None, v=None), k_head_stride=s, v_head_stride=s)):
             args = append_args(**{"cache": dict(pages=0, k=None, v=None), **one})
             assert lib.mr_kv_append(C.byref(args), None) == M.OK
+
+
+def test_more_workgroups_than_a_launch_takes(lib):
+    """A launch has fewer than 2^32 threads: 2^24 workgroups of few queries, 2^23 of prompts.  (Without
+    `out` nothing is launched: what passes the sizes is refused for that.)"""
+    call = lambda **kw: lib.mr_kv_attention(C.byref(attention_args(**kw, out=None, q_offsets=AT)), None)
+    heads = dict(heads=8, cache=dict(kv_heads=8, page_stride=8 * 32 * 64))
+    # 65 rows of a sequence and key head: a tile for each, one more for the average
+    for batch, ok in ((10 ** 6, False), (830000, True)):
+        refused(call(batch=batch, tokens=65 * batch, **heads), *((M.INVALID_ARGUMENT, "non-NULL") if ok else (M.INVALID_SHAPE, "launch")))
+    wide = dict(heads=8, cache=dict(kv_heads=8, head_dim=160, page_stride=8 * 32 * 160))
+    refused(call(batch=10 ** 6, tokens=65 * 10 ** 6, **wide), M.INVALID_ARGUMENT, "non-NULL")
+    for batch, ok in ((2 ** 21, False), (10 ** 6, True)):
+        refused(call(batch=batch, tokens=batch, **heads), *((M.INVALID_ARGUMENT, "non-NULL") if ok else (M.INVALID_SHAPE, "launch")))
+    # parts do not count: a call that they would take past a launch has fewer of them
+    long = dict(heads=32, cache=dict(kv_heads=32, page_stride=32 * 32 * 64), max_pages=2 ** 15)
+    refused(lib.mr_kv_attention(C.byref(attention_args(batch=1024, tokens=1024, **long, out=None)), None), M.INVALID_ARGUMENT, "non-NULL")
