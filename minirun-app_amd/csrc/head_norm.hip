@@ -30,6 +30,7 @@ namespace {
 
 constexpr int HN_WAVES = 4;
 constexpr int HN_PARTIALS = 1024;  // partial rows of a segment at most
+constexpr int HN_ROWS = 2;         // that a group of the backward pass takes a step
 
 // A row, (token, head) in order, a group of lanes: the keys' workgroups follow the
 // queries'.  (4096 tokens of 32 + 4 heads of 128, bf16: 20.5 us, 3.8 TB/s; two, four and
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(64 * HN_WAVES) head_norm_kernel(HeadNormParams
 // partial[workgroup][dim].
 template <bool F32, bool VEC, int KIND>
 __global__ void __launch_bounds__(64 * HN_WAVES) head_norm_backward_kernel(HeadNormParams p) {
-    constexpr int U = 2;
+    constexpr int U = HN_ROWS;
     __shared__ __attribute__((aligned(16))) float sh[HN_WAVES][512];
     const int l = threadIdx.x & 63, group = l >> p.lpr_log2, c = 8 * (l & (p.lpr - 1));
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -214,10 +215,10 @@ RopeKind head_rope_kind(const HeadRope& r) {
     return ROPE_ANY;
 }
 
-// Partial rows for the weights' gradients: workgroups of both segments by their rows,
-// about HN_PARTIALS in all.
+// Partial rows for the weights' gradients: workgroups of both segments by their rows (none
+// without), about HN_PARTIALS in all.
 void head_norm_blocks(int64_t tokens, const int (&heads)[2], int dim, int (&blocks)[2]) {
-    const int64_t per_block = int64_t(HN_WAVES) * (64 >> lanes_log2(dim)), all = tokens * (int64_t(heads[0]) + heads[1]);
+    const int64_t per_block = int64_t(HN_WAVES) * (64 >> lanes_log2(dim)) * HN_ROWS, all = tokens * (int64_t(heads[0]) + heads[1]);
     for (int i = 0; i < 2; ++i) {
         const int64_t rows = tokens * heads[i];
         const int64_t full = (rows + per_block - 1) / per_block, share = all ? HN_PARTIALS * rows / all : 0;

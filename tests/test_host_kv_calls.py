@@ -49,3 +49,13 @@ def test_more_workgroups_than_a_launch_takes(lib):
     # parts do not count: a call that they would take past a launch has fewer of them
     long = dict(heads=32, cache=dict(kv_heads=32, page_stride=32 * 32 * 64), max_pages=2 ** 15)
     refused(lib.mr_kv_attention(C.byref(attention_args(batch=1024, tokens=1024, **long, out=None)), None), M.INVALID_ARGUMENT, "non-NULL")
+
+
+def test_every_workgroup_of_the_gradients_has_rows(lib):
+    """A workgroup, whose sums take a row of the workspace, has 4 waves of 64 / lanes groups that take 2 rows a step."""
+    for dim, lanes in ((128, 16), (64, 8), (33, 8), (512, 64), (8, 1)):
+        step = 4 * (64 // lanes) * 2
+        for tokens, q, k in ((1, 1, 0), (1, 32, 4), (300, 6, 2), (777, 12, 2), (5000, 3, 1), (100000, 32, 8)):
+            a = M.HeadNormArgs(tokens, dim, M.HeadRows(q), M.HeadRows(k))
+            rows = lib.mr_head_norm_rope_backward_workspace_size(C.byref(a)) // (4 * dim)
+            assert 0 < rows <= min(-(-tokens * q // step) + -(-tokens * k // step), 1026), (dim, tokens, q, k, rows)
