@@ -1169,7 +1169,7 @@ class KVCache:
     the tensors' addresses from here, so other tensors are another KVCache."""
 
     def __setattr__(self, name, value):
-        if name in self.__dict__:
+        if self.__dict__.get(name, value) is not value:  # (the same one comes back from `cache.k += 1`)
             raise AttributeError(f"{name} of a KVCache stays as it is; make another one of other tensors")
         super().__setattr__(name, value)
 

@@ -97,4 +97,6 @@ def test_a_cache_keeps_its_tensors(M, mxfp4):
     for name in ("k", "v", "k_scales", "v_scales", "pages", "page_size", "kv_heads", "head_dim", "device"):
         with pytest.raises(AttributeError):
             setattr(cache, name, torch.zeros(4, 1, 16, 64, device="cuda"))
+    cache.k += 1  # (in place: the same tensor)
+    assert (cache.k == 1).all()
     assert cache.k.shape[0] == cache.pages == 2 and cache.head_dim == 64 and (cache.k_scales is not None) == mxfp4
