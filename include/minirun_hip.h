@@ -683,6 +683,7 @@ typedef struct mr_head_rows {
 
 /* For every head x of q and k, in f32, rounded once to out_dtype:
  *   out = rotate(weight * (x * 1 / sqrt(mean(x^2) + eps)))
+ * (a row whose squares' sum passes f32 gives zeros).
  * (K3Norm.rms per head, Normalization.swift:15-19; the query norm without a
  * weight and the rotated tail of DeepSeekV4CompressedAttention.swift:676-694).
  * dim is 1 to 512; tokens * (q.heads + k.heads) * the lanes of a row (dim / 8,
@@ -729,7 +730,7 @@ typedef struct mr_kv_cache {
  * holds is not defined.  k, v [tokens][kv_heads][head_dim] bf16 or f32.
  * Keys are normalised first where `normalize` is set (norm_w [head_dim], or NULL
  * for ones, and eps as in mr_head_norm_rope), then rotated.  What is stored is
- * rounded once from the exact value (computed in f64), MXFP4 by
+ * rounded once from the exact value (that of f64 arithmetic), MXFP4 by
  * mr_mxfp4_quantize's rule.  tokens * kv_heads * the lanes of a row (head_dim / 8,
  * rounded up to a power of two) less than 2^31. */
 typedef struct mr_kv_append_args {

@@ -16,10 +16,10 @@
 //
 // The weights' gradients are sums over all rows: a workgroup of the backward
 // pass walks rows of the queries or of the keys with the next ones in flight (8192
-// tokens of 32 + 8 heads of 128, bf16: 54 us, 4.7 TB/s, 50 of them here; one row at a
-// time, nothing in flight, 76), keeps its sums in registers and leaves one partial
-// row; a second launch adds the partial rows in their order, so the result does not
-// depend on timing.
+// tokens of 32 + 8 heads of 128, bf16: 57 us a call among others, 49 of them here, 5.2
+// TB/s; where the two took 54, one row at a time with nothing in flight took 76), keeps
+// its sums in registers and leaves one partial row; a second launch adds the partial rows
+// in their order, so the result does not depend on timing.
 #include <algorithm>
 
 #include "head_rows.hpp"
@@ -33,10 +33,10 @@ constexpr int HN_PARTIALS = 1024;  // partial rows of a segment at most
 constexpr int HN_ROWS = 2;         // that a group of the backward pass takes a step
 
 // A row, (token, head) in order, a group of lanes: the keys' workgroups follow the
-// queries'.  (4096 tokens of 32 + 4 heads of 128, bf16: 20.5 us, 3.8 TB/s; two, four and
-// eight rows a group loaded together 21.2, 22.0 and 24.4, waves that walk rows with the
-// next ones in flight 23.3, stores past the caches 20.9.  A copy of these bytes takes
-// 16.2.)
+// queries'.  (4096 tokens of 32 + 4 heads of 128, bf16: 18.9 us a call among others, 4.1
+// TB/s; 20.2 in a profiler's trace.  A copy of these bytes takes 16.2.  Where this form
+// took 20.5, two, four and eight rows a group loaded together took 21.2, 22.0 and 24.4,
+// waves that walk rows with the next ones in flight 23.3, stores past the caches 20.9.)
 template <bool F32, bool VEC, int KIND>
 __global__ void __launch_bounds__(64 * HN_WAVES) head_norm_kernel(HeadNormParams p, uint32_t q_blocks) {
     __shared__ __attribute__((aligned(16))) float sh[HN_WAVES][512];

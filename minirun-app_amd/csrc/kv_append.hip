@@ -15,12 +15,17 @@
 // off, the last bit set if that lost anything, which no later rounding to fewer bits
 // can tell from the f64 value.
 //
-// What bounds it: HBM (8192 tokens of 8 heads of 128 as they are, bf16: 15.1 us, 4.7
-// TB/s) and the registers that keep more rows from being under way: with norm and
-// rotation in MXFP4 18.6 us (all keys in f64 22.2, f32's terms kept for it 20.5), in bf16
-// 27.2 (25.9 in f64 alone; with the rotation alone 20.4 and 22.1).  A group of dim / 8
-// lanes has one head's row, as in head_norm.hip; the four lanes of a block find its
-// largest magnitude by two DPP steps.  Everything a row needs is asked for at once.
+// What bounds it, by 8192 tokens of 8 heads of 128 in bf16, not in the caches: HBM where
+// they are stored as they are (in bf16 15.1 us, 4.4 TB/s); with norm and rotation the
+// vector units (in MXFP4 19.4 to 20.5 us, 15 of them the issue of 9.2 million
+// instructions; where it took 18.6, all keys in f64 22.2, f32's terms kept for it 20.5; in
+// bf16, half of the waves in f64, 25.7 to 27, f64 alone 0.5 less).  The rotation alone in
+// bf16, 20.2 to 21.1, is held by neither: 3.3 TB/s, and half of the time instructions; the
+// registers (67) keep more rows from being under way.
+//
+// A group of dim / 8 lanes has one head's row, as in head_norm.hip; the four lanes of a
+// block find its largest magnitude by two DPP steps.  Everything a row needs is asked for
+// at once.
 #include "head_rows.hpp"
 
 namespace mr {
