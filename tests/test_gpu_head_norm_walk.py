@@ -148,3 +148,16 @@ def test_a_side_without_heads_has_gradients_of_zero(M):
     assert torch.equal(dx, want) and dk.shape == (T, 0, D) and torch.equal(dw, want_w) and (dwk == 0).all()
     dx, dk, dw, dwk = M.head_norm_rope_backward(none, none, dq, q, q_weight=w, k_weight=w, eps=EPS)
     assert torch.equal(dk, want) and torch.equal(dwk, want_w) and (dw == 0).all()
+
+
+@pytest.mark.parametrize("dim", [96, 33])
+def test_rows_whose_squares_pass_f32(M, dim):
+    """Zeros, as the header says, and gradients of zeros; the other rows are as without them."""
+    import torch
+
+    x, dy = torch.randn(5, 2, dim, device="cuda"), torch.randn(5, 2, dim, device="cuda")
+    want, (dx, _) = M.head_norm_rope(x, eps=EPS), M.head_norm_rope_backward(dy, x, eps=EPS)
+    x[2, 1] *= 1e20
+    got, (gx, _) = M.head_norm_rope(x, eps=EPS), M.head_norm_rope_backward(dy, x, eps=EPS)
+    want[2, 1], dx[2, 1] = 0, 0
+    assert torch.equal(got, want) and torch.equal(gx, dx)
